@@ -401,8 +401,8 @@ def _own(s):
                                   s["free_blocks"], s["free_start"], s["block"], s["max_tokens"])
         return {"tables": s["tables"], "query_starts": plan.query_starts,
                 "context_tokens": plan.context_tokens, "slots": plan.slots,
-                "positions": plan.positions, "free_next": plan.free_next[0],
-                "lacking": plan.lacking[0]}
+                "positions": plan.positions, "free_next": plan.free_next,
+                "lacking": plan.lacking}
     if kind == "write":
         sz.write_kv_paged(s["k"], s["v"], s["kv"], s["slots"])
         return s["kv"]
