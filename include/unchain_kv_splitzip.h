@@ -510,6 +510,93 @@ long long kvq_splitzip_top16_decode_attention(
     unsigned long long workspace_ptr, unsigned long long workspace_bytes, float scale,
     unsigned long long stream_ptr);
 
+/* ------------------------------------------------------------------------------
+ * A serving step over a paged layer (no counterpart in the reference, whose engine does
+ * this around it): tables and slots from the requests' lengths, the new tokens' K and V
+ * rows into the layer, and attention of chunks (single tokens among them) and of whole
+ * prompts. Lengths, row ranges and tables are DEVICE arrays of 32-bit integers; a call
+ * captured in a HIP graph follows their values.
+ * ---------------------------------------------------------------------------- */
+
+/* Request r has cached_tokens[r] tokens in its blocks and gets new_tokens[r] (negative: 0).
+ * Its blocks ceil(cached / block_tokens) .. ceil((cached + new) / block_tokens) are taken
+ * from free_blocks (free_count entries), in request order from entry free_start[0] on, and
+ * written to its row of tables (row r at tables + r * table_stride, table_width entries);
+ * other entries are only read. Written: query_starts[r] (requests + 1), the first packed
+ * row of request r's new tokens; context_tokens[r] = cached + new; for each of max_tokens
+ * rows slots[t] = block * block_tokens + place in the block (i64; -1 without a block) and
+ * positions[t] (i64), -1 and 0 behind the last row; free_next[0], the first free entry
+ * left; lacking[0], blocks that were wanted beyond the free list or the table's width
+ * (entries and slots -1). Tokens past max_tokens get no row. Results must overlap neither
+ * the inputs nor each other. Returns requests, 0 on a failed precondition. */
+long long kvq_splitzip_plan_step_paged(
+    unsigned long long new_tokens_ptr, unsigned long long cached_tokens_ptr,
+    unsigned long long requests, unsigned long long tables_ptr, unsigned long long table_stride,
+    unsigned long long table_width, unsigned long long free_blocks_ptr,
+    unsigned long long free_count, unsigned long long free_start_ptr,
+    unsigned long long block_tokens, unsigned long long max_tokens,
+    unsigned long long query_starts_ptr, unsigned long long context_tokens_ptr,
+    unsigned long long slots_ptr, unsigned long long positions_ptr,
+    unsigned long long free_next_ptr, unsigned long long lacking_ptr,
+    unsigned long long stream_ptr);
+
+/* K and V rows of `tokens` tokens into a layer by slot: head h of row t is head_bytes
+ * bytes at k + t * k_row_bytes + h * k_head_bytes (v likewise) and goes to
+ * kv + slots[t] * heads * head_bytes + h * head_bytes, V plane_bytes later. Rows whose slot
+ * is not in [0, slot_count) are not written. The rows must not overlap the layer; of two
+ * rows with one slot it is not said whose values stay. Any alignment (16-byte aligned rows,
+ * heads and planes are the fast case). Returns the rows' bytes, 0 on a failed
+ * precondition. */
+long long kvq_splitzip_write_kv_paged(
+    unsigned long long k_ptr, unsigned long long v_ptr, unsigned long long tokens,
+    unsigned long long heads, unsigned long long head_bytes, unsigned long long k_row_bytes,
+    unsigned long long k_head_bytes, unsigned long long v_row_bytes,
+    unsigned long long v_head_bytes, unsigned long long kv_ptr, unsigned long long plane_bytes,
+    unsigned long long slot_count, unsigned long long slots_ptr, unsigned long long stream_ptr);
+
+/* Workspace bytes of the two attention calls; max_context = table_width * block_tokens. */
+unsigned long long kvq_splitzip_chunk_attention_workspace_bytes(
+    unsigned long long tokens, unsigned long long requests, unsigned long long q_heads,
+    unsigned long long kv_heads, unsigned long long head_dim, unsigned long long max_context,
+    unsigned long long max_query);
+unsigned long long kvq_splitzip_prompt_attention_workspace_bytes(
+    unsigned long long tokens, unsigned long long requests, unsigned long long q_heads,
+    unsigned long long kv_heads, unsigned long long head_dim, unsigned long long max_query);
+
+/* Causal attention of packed rows over a layer kv (2, blocks, block_tokens, kv_heads,
+ * head_dim), contiguous: request r's rows are query_starts[r] .. query_starts[r + 1] of q
+ * (`tokens` rows; head h of row t at q + t * q_row_bytes + h * q_head_bytes, multiples of 16),
+ * the last of its context_tokens[r] tokens, so row i of n sees tokens 0 .. context - n + i.
+ * Query head h reads KV head h / (q_heads / kv_heads). dtype 0: bf16, 1: fp16; head_dim 64 or
+ * 128; scale positive and finite. out: [tokens][q_heads][head_dim]; lse_ptr: 0, or f32
+ * [tokens][q_heads] for the rows' log-sum-exps. max_query (at most tokens) bounds a request's
+ * rows: longer ones are left out. Rows that see nothing are 0 (lse -inf); rows of no request,
+ * or of a range that is not inside q, stay; a context past its table's row, or an entry that is
+ * no block, gives NaN rows. workspace: 16-byte aligned, of the size above, for one call at a
+ * time. Returns the bytes of out, 0 on a failed precondition (out must not overlap an input). */
+long long kvq_splitzip_chunk_attention_paged(
+    unsigned long long q_ptr, unsigned long long q_row_bytes, unsigned long long q_head_bytes,
+    unsigned long long tokens, unsigned long long q_heads, unsigned long long kv_heads,
+    unsigned long long head_dim, unsigned long long dtype, unsigned long long kv_ptr,
+    unsigned long long blocks, unsigned long long block_tokens, unsigned long long tables_ptr,
+    unsigned long long table_stride, unsigned long long table_width,
+    unsigned long long query_starts_ptr, unsigned long long context_tokens_ptr,
+    unsigned long long requests, unsigned long long max_query, unsigned long long out_ptr,
+    unsigned long long lse_ptr, unsigned long long workspace_ptr,
+    unsigned long long workspace_bytes, float scale, unsigned long long stream_ptr);
+
+/* The same for whole prompts over their own packed K and V rows (`tokens` rows as q; strides
+ * multiples of 16): row i of a prompt sees the prompt's rows 0 .. i. */
+long long kvq_splitzip_prompt_attention(
+    unsigned long long q_ptr, unsigned long long q_row_bytes, unsigned long long q_head_bytes,
+    unsigned long long k_ptr, unsigned long long k_row_bytes, unsigned long long k_head_bytes,
+    unsigned long long v_ptr, unsigned long long v_row_bytes, unsigned long long v_head_bytes,
+    unsigned long long tokens, unsigned long long q_heads, unsigned long long kv_heads,
+    unsigned long long head_dim, unsigned long long dtype, unsigned long long query_starts_ptr,
+    unsigned long long requests, unsigned long long max_query, unsigned long long out_ptr,
+    unsigned long long lse_ptr, unsigned long long workspace_ptr,
+    unsigned long long workspace_bytes, float scale, unsigned long long stream_ptr);
+
 #ifdef __cplusplus
 }
 #endif

@@ -13,6 +13,12 @@ namespace unchainkv {
 long long fail(const char* what, hipError_t status);
 long long fail_msg(const std::string& msg);
 
+// Whether two byte ranges meet.
+inline bool overlap(unsigned long long a, unsigned long long a_bytes, unsigned long long b,
+                    unsigned long long b_bytes) {
+  return a_bytes != 0 && b_bytes != 0 && a < b + b_bytes && b < a + a_bytes;
+}
+
 constexpr int kThreads = 256;                         // 4 waves of 64
 constexpr int kWave = 64;
 // Lane-run kernels: each lane owns 16 consecutive words (any alignment).

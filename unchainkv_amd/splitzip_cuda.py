@@ -26,9 +26,11 @@ from __future__ import annotations
 
 import array
 import ctypes
+import functools
 import operator
 import os
 from pathlib import Path
+from typing import NamedTuple
 
 from . import codec_format
 
@@ -160,6 +162,14 @@ _SIGNATURES = (
         ctypes.c_longlong,
         False,
     ),
+    ("kvq_splitzip_plan_step_paged", [_U64] * 18, ctypes.c_longlong, False),
+    ("kvq_splitzip_write_kv_paged", [_U64] * 14, ctypes.c_longlong, False),
+    ("kvq_splitzip_chunk_attention_workspace_bytes", [_U64] * 7, _U64, False),
+    ("kvq_splitzip_prompt_attention_workspace_bytes", [_U64] * 6, _U64, False),
+    ("kvq_splitzip_chunk_attention_paged", [_U64] * 22 + [ctypes.c_float, _U64],
+     ctypes.c_longlong, False),
+    ("kvq_splitzip_prompt_attention", [_U64] * 21 + [ctypes.c_float, _U64],
+     ctypes.c_longlong, False),
     (
         "kvq_splitzip_bf16_decode_mode_paged",
         [_U64, _U64P, _U64P, _U64, _U64, _U64, _U64, _U64, _U64, _U64P, _U64, ctypes.c_int],
@@ -1209,6 +1219,337 @@ def decode_attention_top16(q, payloads, payload_offsets, context_tokens, kv_head
                  int(workspace.data_ptr()), int(workspace.numel()), float(scale), int(stream))
     if got < 0:
         _raise_last(lib, "splitzip top16 decode attention failed")
+    return out if got else None
+
+
+# ---------------------------------------------------------------------------
+# a step over a paged layer: tables and slots, the K/V write, attention of chunks and prompts
+
+# element types of the layers and rows that these calls take, as the C entries number them
+_ROW_DTYPES: dict = {}
+
+
+def _row_dtype(dtype, torch):
+    if not _ROW_DTYPES:
+        _ROW_DTYPES.update({torch.bfloat16: 0, torch.float16: 1})
+    return _ROW_DTYPES.get(dtype)
+
+
+def _call_on(device, torch, fn, *args):
+    """``fn(*args, stream)`` with ``device`` current and its current stream."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return fn(*args, _stream_handle(device, torch))
+    with torch.cuda.device(device):
+        return fn(*args, _stream_handle(device, torch))
+
+
+def _index_vector_ok(t, device, count: int, dtype) -> bool:
+    """A contiguous vector of at least ``count`` indexes on ``device``."""
+    return t.dtype == dtype and t.dim() == 1 and t.is_contiguous() and t.device == device and \
+        t.numel() >= count
+
+
+class StepPlan(NamedTuple):
+    """What ``plan_step_paged`` gives of a step, on the device.
+
+    ``query_starts`` (requests + 1) int32: request r's new tokens are rows
+    query_starts[r] .. query_starts[r + 1] of the step's packed rows. ``context_tokens``
+    (requests) int32: its tokens with the new ones. ``slots`` and ``positions``
+    (max_tokens) int64: each row's place in the layer (block * block_tokens + place in the
+    block; -1 without one) and in its sequence; -1 and 0 behind the last row.
+    ``free_next`` (1) int32: the first entry of the free list that is still free.
+    ``lacking`` (1) int32: blocks that the step wanted and did not get (their table entries
+    and slots are -1)."""
+
+    query_starts: object
+    context_tokens: object
+    slots: object
+    positions: object
+    free_next: object
+    lacking: object
+
+
+def new_step_plan(requests: int, max_tokens: int, device, torch=None) -> StepPlan:
+    """Buffers for ``plan_step_paged(..., plan=)``, which a captured step keeps."""
+    if torch is None:
+        import torch
+    small = torch.empty(2 * requests + 3, dtype=torch.int32, device=device)
+    starts, contexts, free_next, lacking = small.split_with_sizes((requests + 1, requests, 1, 1))
+    slots, positions = torch.empty((2, max_tokens), dtype=torch.int64, device=device).unbind(0)
+    return StepPlan(starts, contexts, slots, positions, free_next, lacking)
+
+
+def plan_step_paged(new_tokens, cached_tokens, tables, free_blocks, free_start,
+                    block_tokens: int, max_tokens: int, *, plan: StepPlan | None = None):
+    """Tables of one serving step from its requests' lengths, on the GPU and without a host
+    read, so that a captured step follows new lengths.
+
+    Request r has ``cached_tokens[r]`` tokens in its blocks and gets ``new_tokens[r]`` (0:
+    none; negative lengths count as 0) behind them. ``tables`` (requests, width) lists each
+    request's blocks in token order; its entries for the blocks that the new tokens need and
+    the request does not hold yet are filled IN PLACE, in request order, from
+    ``free_blocks`` starting at ``free_start[0]``; no other entry is written. All are int32
+    tensors on one GPU (the rows of ``tables`` may be strided). ``max_tokens`` is the row
+    count of the step's packed tensors; tokens past it get no row (query_starts still
+    counts them). A block past the free list or the table's width is not given: its entry
+    and its tokens' slots are -1, and ``lacking`` counts it.
+
+    Returns a ``StepPlan`` (``plan``, when given: from ``new_step_plan`` or an earlier call
+    of the same sizes, and overlapping none of the inputs; a step whose ``cached_tokens``
+    are the last plan's ``context_tokens`` needs another plan to write to), or ``None``
+    when the kernel declines."""
+    lib = _load()
+    make = getattr(lib, "kvq_splitzip_plan_step_paged", None) if lib else None
+    if make is None or not _is_cuda(new_tokens):
+        return None
+    import torch
+
+    device, i32 = new_tokens.device, torch.int32
+    requests, block_tokens, max_tokens = new_tokens.numel(), int(block_tokens), int(max_tokens)
+    if not (_index_vector_ok(new_tokens, device, 1, i32)
+            and _index_vector_ok(cached_tokens, device, requests, i32)
+            and _index_vector_ok(free_blocks, device, 0, i32)
+            and _index_vector_ok(free_start, device, 1, i32)):
+        return None
+    if tables.dtype != i32 or tables.dim() != 2 or tables.device != device or \
+            cached_tokens.numel() != requests or tables.shape[0] != requests or \
+            (tables.shape[1] != 1 and tables.stride(1) != 1) or block_tokens <= 0 or max_tokens < 0:
+        return None
+    if plan is None:
+        plan = new_step_plan(requests, max_tokens, device, torch)
+    elif not (_index_vector_ok(plan.query_starts, device, requests + 1, i32)
+              and _index_vector_ok(plan.context_tokens, device, requests, i32)
+              and _index_vector_ok(plan.slots, device, max_tokens, torch.int64)
+              and _index_vector_ok(plan.positions, device, max_tokens, torch.int64)
+              and _index_vector_ok(plan.free_next, device, 1, i32)
+              and _index_vector_ok(plan.lacking, device, 1, i32)):
+        return None
+    width = tables.shape[1]
+    got = _call_on(device, torch, make, new_tokens.data_ptr(), cached_tokens.data_ptr(), requests,
+                   tables.data_ptr(), tables.stride(0) if requests > 1 else width, width,
+                   free_blocks.data_ptr(), free_blocks.numel(), free_start.data_ptr(),
+                   block_tokens, max_tokens, plan.query_starts.data_ptr(),
+                   plan.context_tokens.data_ptr(), plan.slots.data_ptr(),
+                   plan.positions.data_ptr(), plan.free_next.data_ptr(),
+                   plan.lacking.data_ptr())
+    if got < 0:
+        _raise_last(lib, "splitzip step plan failed")
+    return plan if got else None
+
+
+def _kv_layer_ok(kv_layer, dtype, device) -> bool:
+    """A contiguous (2, num_blocks, block_tokens, kv_heads, head_dim) layer."""
+    return kv_layer.dtype == dtype and kv_layer.device == device and kv_layer.dim() == 5 and \
+        kv_layer.shape[0] == 2 and kv_layer.numel() > 0 and kv_layer.is_contiguous()
+
+
+def write_kv_paged(k, v, kv_layer, slots) -> int | None:
+    """K and V rows of a step's tokens into a paged layer: row t of ``k`` and ``v``
+    (tokens, kv_heads, head_dim) goes to slot ``slots[t]`` (block * block_tokens + place in
+    the block, int64; ``StepPlan.slots``) of ``kv_layer`` (2, num_blocks, block_tokens,
+    kv_heads, head_dim). Rows whose slot is negative or past the layer are not written.
+    bf16 or fp16; rows and heads may be strided (views of one projection). ``slots`` may
+    be longer than the rows. Of two rows with one slot it is not said whose values stay (a
+    plan's slots are distinct). Returns the rows' bytes (0 without rows), or ``None`` when the kernel
+    declines (other types or layouts, rows that overlap the layer)."""
+    lib = _load()
+    write = getattr(lib, "kvq_splitzip_write_kv_paged", None) if lib else None
+    if write is None or not _is_cuda(k):
+        return None
+    import torch
+
+    device = k.device
+    if _row_dtype(k.dtype, torch) is None or k.dim() != 3 or v.shape != k.shape or \
+            v.dtype != k.dtype or v.device != device or not _kv_layer_ok(kv_layer, k.dtype, device):
+        return None
+    tokens, heads, head_dim = k.shape
+    if kv_layer.shape[3] != heads or kv_layer.shape[4] != head_dim or \
+            (head_dim != 1 and (k.stride(2) != 1 or v.stride(2) != 1)) or \
+            not _index_vector_ok(slots, device, tokens, torch.int64):
+        return None
+    if tokens == 0:
+        return 0
+    got = _call_on(device, torch, write, k.data_ptr(), v.data_ptr(), tokens, heads, 2 * head_dim,
+                   2 * k.stride(0), 2 * k.stride(1), 2 * v.stride(0), 2 * v.stride(1),
+                   kv_layer.data_ptr(), 2 * kv_layer.stride(0),
+                   kv_layer.shape[1] * kv_layer.shape[2], slots.data_ptr())
+    if got < 0:
+        _raise_last(lib, "splitzip K/V write failed")
+    return int(got) or None
+
+
+@functools.lru_cache(maxsize=1024)
+def _attention_workspace(name: str, device, sizes: tuple) -> int:
+    import torch
+
+    with torch.cuda.device(device):
+        return int(getattr(_load(), name)(*sizes))
+
+
+def chunk_attention_workspace_bytes(tokens: int, requests: int, q_heads: int, kv_heads: int,
+                                    head_dim: int, max_context: int,
+                                    max_query: int | None = None) -> int:
+    """Workspace of ``chunk_attention_paged`` for ``tokens`` rows of q, with ``max_context`` the
+    tokens that a row of the block tables can hold (its width in blocks * block_tokens)."""
+    lib = _load()
+    if lib is None or not hasattr(lib, "kvq_splitzip_chunk_attention_workspace_bytes"):
+        raise RuntimeError(f"HIP codec library not loaded: {load_error()}")
+    return int(lib.kvq_splitzip_chunk_attention_workspace_bytes(
+        tokens, requests, q_heads, kv_heads, head_dim, max_context, max_query or tokens))
+
+
+def prompt_attention_workspace_bytes(tokens: int, requests: int, q_heads: int, kv_heads: int,
+                                     head_dim: int, max_query: int | None = None) -> int:
+    """Workspace of ``prompt_attention`` for ``tokens`` packed rows."""
+    lib = _load()
+    if lib is None or not hasattr(lib, "kvq_splitzip_prompt_attention_workspace_bytes"):
+        raise RuntimeError(f"HIP codec library not loaded: {load_error()}")
+    return int(lib.kvq_splitzip_prompt_attention_workspace_bytes(
+        tokens, requests, q_heads, kv_heads, head_dim, max_query or tokens))
+
+
+def _rows_ok(t, dtype, device) -> bool:
+    """(rows, heads, head_dim) with whole head rows; the last dim contiguous."""
+    return t.dim() == 3 and t.dtype == dtype and t.device == device and \
+        (t.shape[2] == 1 or t.stride(2) == 1) and t.stride(0) >= 0 and t.stride(1) >= 0
+
+
+def _attention_buffers(q, out, lse, torch):
+    """(ok, out) of an attention call's results."""
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    elif out.dtype != q.dtype or out.shape != q.shape or out.device != q.device or \
+            not out.is_contiguous():
+        return False, None
+    if lse is not None and (lse.dtype != torch.float32 or lse.shape != q.shape[:2]
+                            or lse.device != q.device or not lse.is_contiguous()):
+        return False, None
+    return True, out
+
+
+def chunk_attention_paged(q, kv_layer, tables, query_starts, context_tokens, *,
+                          max_query: int | None = None, scale: float | None = None, out=None,
+                          lse=None, workspace=None):
+    """Causal attention of a step's new tokens over a paged layer that holds their own K and V
+    already (``write_kv_paged``); single tokens (decode), chunks of prompts and drafted
+    tokens mixed in any way.
+
+    ``q`` (tokens, q_heads, head_dim) are the packed rows; request r's are rows
+    ``query_starts[r]`` .. ``query_starts[r + 1]``, the last of its ``context_tokens[r]``
+    tokens, so row i of its n sees tokens 0 .. context - n + i. Query head h reads KV head
+    h // (q_heads / kv_heads). ``tables`` (requests, width) int32 lists each request's blocks in
+    token order, ``query_starts`` (requests + 1) and ``context_tokens`` (requests) are int32;
+    all stay on the device (``StepPlan``), and a captured call follows their values.
+    ``max_query`` bounds the new tokens of a request (default: the rows of q); a smaller bound
+    spares a decode step the kernel for long chunks. ``scale`` (positive) defaults to head_dim
+    ** -0.5. ``lse`` (tokens, q_heads) float32 receives each row's log-sum-exp, for joining
+    with attention over other tokens. bf16 or fp16, head_dim 64 or 128; rows and heads of q
+    may be strided by multiples of 16 bytes.
+
+    A row that sees no token (context_tokens[r] less than its new tokens) is zero, its lse
+    -inf. Rows of no request, of one with more new tokens than max_query, and of one whose
+    row range is not inside q stay as they are. A context longer than its table, or a table
+    entry that is no block of the layer, makes the rows that read there NaN (every row of
+    the same 128 or 16, at least).
+    No gradient: inputs that require one are declined while gradients are recorded.
+
+    Returns ``out`` (tokens, q_heads, head_dim), or ``None`` when the kernel declines."""
+    lib = _load()
+    attend = getattr(lib, "kvq_splitzip_chunk_attention_paged", None) if lib else None
+    if attend is None or not _is_cuda(q):
+        return None
+    import torch
+
+    device = q.device
+    dtype = _row_dtype(q.dtype, torch)
+    if dtype is None or not _rows_ok(q, q.dtype, device) or \
+            not _kv_layer_ok(kv_layer, q.dtype, device):
+        return None
+    if (q.requires_grad or kv_layer.requires_grad) and torch.is_grad_enabled():
+        return None
+    tokens, q_heads, head_dim = q.shape
+    _, blocks, block_tokens, kv_heads, kv_dim = kv_layer.shape
+    if tables.dtype != torch.int32 or tables.dim() != 2 or tables.device != device:
+        return None
+    requests, width = tables.shape
+    if kv_dim != head_dim or (width != 1 and tables.stride(1) != 1) or \
+            not _index_vector_ok(query_starts, device, requests + 1, torch.int32) or \
+            not _index_vector_ok(context_tokens, device, requests, torch.int32):
+        return None
+    max_query = tokens if max_query is None else min(int(max_query), tokens)
+    ok, out = _attention_buffers(q, out, lse, torch)
+    if not ok:
+        return None
+    if tokens == 0:
+        return out
+    if max_query <= 0 or width == 0:
+        return None
+    need = _attention_workspace(
+        "kvq_splitzip_chunk_attention_workspace_bytes", device,
+        (tokens, requests, q_heads, kv_heads, head_dim, width * block_tokens, max_query))
+    if not _byte_buffer_ok(workspace, device, need, torch):
+        workspace = torch.empty(max(need, 16), dtype=torch.uint8, device=device)
+    got = _call_on(device, torch, attend, q.data_ptr(), 2 * q.stride(0), 2 * q.stride(1), tokens,
+                   q_heads, kv_heads, head_dim, dtype, kv_layer.data_ptr(), blocks, block_tokens,
+                   tables.data_ptr(), tables.stride(0) if requests > 1 else width, width,
+                   query_starts.data_ptr(), context_tokens.data_ptr(), requests, max_query,
+                   out.data_ptr(), 0 if lse is None else lse.data_ptr(), workspace.data_ptr(),
+                   workspace.numel(), head_dim ** -0.5 if scale is None else float(scale))
+    if got < 0:
+        _raise_last(lib, "splitzip chunk attention failed")
+    return out if got else None
+
+
+def prompt_attention(q, k, v, query_starts, *, max_query: int | None = None,
+                     scale: float | None = None, out=None, lse=None, workspace=None):
+    """Causal attention of whole prompts packed one behind the other, over their own K and V
+    rows (before any of them is in a layer): row i of prompt r, which is row
+    ``query_starts[r]`` + i of ``q`` (tokens, q_heads, head_dim), ``k`` and ``v`` (tokens,
+    kv_heads, head_dim), sees the prompt's rows 0 .. i. ``query_starts`` (prompts + 1) is
+    int32 on the device. Types, strides (of k and v too), heads, ``max_query`` (of a prompt's
+    tokens, here a bound for the workspace alone), ``scale``, ``lse``, the rows outside any
+    prompt and gradients as in ``chunk_attention_paged``. Returns ``out`` (tokens, q_heads, head_dim),
+    or ``None`` when the kernel declines."""
+    lib = _load()
+    attend = getattr(lib, "kvq_splitzip_prompt_attention", None) if lib else None
+    if attend is None or not _is_cuda(q):
+        return None
+    import torch
+
+    device = q.device
+    dtype = _row_dtype(q.dtype, torch)
+    if dtype is None or not _rows_ok(q, q.dtype, device) or not _rows_ok(k, q.dtype, device) or \
+            not _rows_ok(v, q.dtype, device):
+        return None
+    if (q.requires_grad or k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
+        return None
+    tokens, q_heads, head_dim = q.shape
+    kv_heads = k.shape[1]
+    if k.shape != v.shape or k.shape[0] != tokens or k.shape[2] != head_dim or \
+            not _index_vector_ok(query_starts, device, 1, torch.int32):
+        return None
+    requests = query_starts.numel() - 1
+    max_query = tokens if max_query is None else min(int(max_query), tokens)
+    ok, out = _attention_buffers(q, out, lse, torch)
+    if not ok:
+        return None
+    if tokens == 0 or requests == 0:
+        return out
+    if max_query <= 0:
+        return None
+    need = _attention_workspace(
+        "kvq_splitzip_prompt_attention_workspace_bytes", device,
+        (tokens, requests, q_heads, kv_heads, head_dim, max_query))
+    if not _byte_buffer_ok(workspace, device, need, torch):
+        workspace = torch.empty(max(need, 16), dtype=torch.uint8, device=device)
+    got = _call_on(device, torch, attend, q.data_ptr(), 2 * q.stride(0), 2 * q.stride(1),
+                   k.data_ptr(), 2 * k.stride(0), 2 * k.stride(1), v.data_ptr(),
+                   2 * v.stride(0), 2 * v.stride(1), tokens, q_heads, kv_heads, head_dim, dtype,
+                   query_starts.data_ptr(), requests, max_query, out.data_ptr(),
+                   0 if lse is None else lse.data_ptr(), workspace.data_ptr(), workspace.numel(),
+                   head_dim ** -0.5 if scale is None else float(scale))
+    if got < 0:
+        _raise_last(lib, "splitzip prompt attention failed")
     return out if got else None
 
 
