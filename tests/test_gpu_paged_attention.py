@@ -222,9 +222,9 @@ def test_row_ranges_that_do_not_hold(sz):
     case.starts = i32([0, 2, 5, 1 << 20])
     out, _ = case.run(sz)
     assert torch.equal(out[:5], whole[:5]) and (out[5:] == MARK).all()
-    case.starts = i32([0, 2, 1, 41])
+    case.starts = i32([0, 2, 1, 41])  # (row 1 is in two ranges: either's)
     out, _ = case.run(sz)
-    assert torch.equal(out[:2], whole[:2]) and (out[41:] == MARK).all()
+    assert torch.equal(out[:1], whole[:1]) and (out[41:] == MARK).all()
     case.starts = i32([-1, -1, -1, -1])
     out, _ = case.run(sz)
     assert (out == MARK).all()

@@ -101,6 +101,16 @@ __device__ __forceinline__ typename Elem<E>::x8 pack8(const float* p) {
   return __builtin_bit_cast(typename Elem<E>::x8, v);
 }
 
+// What attention_merge has to know of a slot that holds the first split of some rows: rows first ..
+// first + rows of the request whose rows start at `start`, row m's last token at shift + m / group,
+// in the slots slot, slot + kv_heads, ... (`splits` of them). splits == 0: nothing to join.
+struct Job {
+  unsigned int start, first;
+  int shift;
+  unsigned short rows, splits;
+};
+static_assert(sizeof(Job) == 16, "one load");
+
 struct AttendArgs {
   const unsigned char* q;
   unsigned char* out;        // [tokens][q_heads][D]
@@ -110,15 +120,17 @@ struct AttendArgs {
   const int* starts;         // [requests + 1]
   const int* contexts;       // [requests]; null: a request's own rows (prompts)
   const int* tables;         // [requests][table_stride]; null for prompts
-  float* partial;
+  float* partial;            // slots of the tiles, then of the few
+  struct Job* jobs;          // one for each slot
   unsigned long long q_row, q_head;  // bytes from token to token, from head to head
   unsigned long long k_row, k_head, v_row, v_head;
   unsigned long long table_stride;
   unsigned int table_width, blocks, block_tokens;
   Divider by_block;
   unsigned int tokens, requests, q_heads, kv_heads, group;
-  unsigned int few_rows;      // most rows of a request that goes to attention_few; 0: none
-  unsigned int tiles_too;     // whether attention_tiles runs (else longer requests are left out)
+  unsigned int few_rows;      // most rows of a request that goes to the streaming path; 0: none
+  unsigned int tiles_too;     // whether tiles are taken (else longer requests are left out)
+  unsigned int tile_groups, few_groups;  // workgroups of the two paths
   unsigned int few_target, tile_target;   // workgroups to split for
   unsigned int max_query;     // requests with more new tokens are left out
   unsigned int tile_slots, few_slots;  // partial slots: of the tiles, then of the few
@@ -160,8 +172,7 @@ __device__ __forceinline__ int kind_of(const AttendArgs& a, const Request& q) {
   return a.tiles_too ? 2 : 0;
 }
 
-template <typename T>
-__device__ __forceinline__ T wave_sum(T v) {
+__device__ __forceinline__ float wave_sum(float v) {
 #pragma unroll
   for (int d = 1; d < kWave; d *= 2) v += __shfl_xor(v, d, kWave);
   return v;
@@ -173,45 +184,70 @@ __device__ __forceinline__ float wave_max(float v) {
   return v;
 }
 
+// Inclusive sum over the wave's lanes, on the VALU: shifts by 1, 2, 4, 8 within each row of 16
+// lanes, then the rows' ends into the rows behind them.
+__device__ __forceinline__ unsigned int wave_scan(unsigned int v) {
+  v += __builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xA, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xC, 0xF, false);
+  return v;
+}
+__device__ __forceinline__ unsigned int lane_value(unsigned int v, int lane) {
+  return (unsigned int)__builtin_amdgcn_readlane((int)v, lane);
+}
+
 __device__ __forceinline__ unsigned int steps_of(unsigned int tokens, unsigned int step) {
-  return (tokens + step - 1) / step;
+  return tokens / step + (tokens % step != 0 ? 1u : 0u);
 }
 
 __device__ __forceinline__ unsigned int tiles_of(const AttendArgs& a, unsigned int n) {
-  return (unsigned int)(((unsigned long long)n * a.group + kTileRows - 1) / kTileRows);
+  return (n * a.group + kTileRows - 1) / kTileRows;
 }
 
-// Steps of a split (of attention_few and of attention_tiles), from the sums over all requests.
-// Few: the even share of all rounds over few_target workgroups. Tiles: no split (0) once there
-// are tile_target tiles, else the even share of all tiles' steps, a tile of a request counted
-// with the request's mean context.
+// Steps of a split on the streaming path and of a tile's, from the sums over all requests (each
+// lane a request, 64 at a time; `head` holds the first 64, which most launches end with). Few:
+// the even share of all rounds over few_target workgroups. Tiles: no split (0) once there are
+// tile_target tiles, else the even share of all tiles' steps, a tile of a request counted with
+// the request's mean context (a request's sum beyond kMostSteps, which the 32-bit sums do not
+// take, is not split either).
 struct SplitSteps {
   unsigned int few, tiles;
 };
+constexpr unsigned int kMostSteps = 1u << 25;
 
-__device__ __forceinline__ SplitSteps split_steps(const AttendArgs& a) {
+// ceil(sum / parts), by a 32-bit division where it serves.
+__device__ __forceinline__ unsigned int share_of(unsigned long long sum, unsigned int parts) {
+  sum += parts - 1;
+  return (sum >> 32) == 0 ? (unsigned int)sum / parts : (unsigned int)(sum / parts);
+}
+
+__device__ __forceinline__ SplitSteps split_steps(const AttendArgs& a, const Request& head) {
   unsigned long long few = 0, tiles = 0, tile_steps = 0;
+  bool large = false;
   for (unsigned int r0 = 0; r0 < a.requests; r0 += kWave) {
-    const Request q = load_request(a, r0 + __lane_id());
+    const Request q = r0 == 0 ? head : load_request(a, r0 + __lane_id());
     const int kind = kind_of(a, q);
-    if (kind == 1) few += steps_of(q.ctx, kFewRound);
-    if (kind == 2) {
-      const unsigned long long t = tiles_of(a, q.n);
-      tiles += t;
-      tile_steps += t * steps_of(q.ctx - min(q.ctx, q.n) / 2, kTileTokens);
+    if (a.few_rows != 0)
+      few += lane_value(wave_scan(kind == 1 ? steps_of(q.ctx, kFewRound) : 0u), 63);
+    if (a.tiles_too != 0) {
+      const unsigned int t = kind == 2 ? tiles_of(a, q.n) : 0u;
+      const unsigned long long all =
+          (unsigned long long)t * steps_of(q.ctx - min(q.ctx, q.n) / 2, kTileTokens);
+      large |= __ballot(all > kMostSteps) != 0;
+      tiles += lane_value(wave_scan(t), 63);
+      tile_steps += lane_value(wave_scan((unsigned int)min(all, (unsigned long long)kMostSteps)), 63);
     }
   }
-  few = wave_sum(few) * a.kv_heads;
-  tiles = wave_sum(tiles) * a.kv_heads;
-  tile_steps = wave_sum(tile_steps) * a.kv_heads;
+  few *= a.kv_heads;
+  tiles *= a.kv_heads;
+  tile_steps *= a.kv_heads;
   SplitSteps s;
-  s.few = (unsigned int)max(1ull, (few + a.few_target - 1) / a.few_target);
-  s.tiles = tiles >= a.tile_target
-                ? 0u
-                : max(kLeastTileSteps,
-                      (unsigned int)((tile_steps + a.tile_target - 1) / a.tile_target));
-  s.few = uniform(s.few);
-  s.tiles = uniform(s.tiles);
+  s.few = max(1u, share_of(few, a.few_target));
+  s.tiles = tiles >= a.tile_target || large ? 0u
+                                            : max(kLeastTileSteps, share_of(tile_steps, a.tile_target));
   return s;
 }
 
@@ -226,34 +262,25 @@ __device__ __forceinline__ unsigned int tile_splits(unsigned int ctx, unsigned i
 // last one. All wave-uniform.
 struct Place {
   Request q;
-  unsigned int r, index, first;  // index within the request; items before the request
+  unsigned int r, index;  // index within the request
 };
 
 template <typename Count>
-__device__ __forceinline__ bool find_item(const AttendArgs& a, unsigned long long item, Count count,
-                                          Place& p) {
+__device__ __forceinline__ bool find_item(const AttendArgs& a, const Request& head,
+                                          unsigned int item, Count count, Place& p) {
   unsigned long long before = 0;
-  const unsigned int lane = __lane_id();
   for (unsigned int r0 = 0; r0 < a.requests; r0 += kWave) {
-    const Request q = load_request(a, r0 + lane);
-    const unsigned long long own = count(q);
-    unsigned long long sum = own;
-#pragma unroll
-    for (int d = 1; d < kWave; d *= 2) {
-      const unsigned long long o = __shfl_up(sum, d, kWave);
-      if (lane >= (unsigned int)d) sum += o;
-    }
-    const unsigned long long all = __shfl(sum, kWave - 1, kWave);
+    const Request q = r0 == 0 ? head : load_request(a, r0 + __lane_id());
+    const unsigned int own = count(q), sum = wave_scan(own), all = lane_value(sum, 63);
     if (item < before + all) {
-      const unsigned long long in = __ballot(before + sum > item);
-      const int at = __ffsll((long long)in) - 1;
-      p.r = uniform(r0 + (unsigned int)at);
-      p.first = uniform((unsigned int)(before + __shfl(sum - own, at, kWave)));
-      p.index = uniform((unsigned int)(item - p.first));
-      p.q.start = uniform(__shfl(q.start, at, kWave));
-      p.q.n = uniform(__shfl(q.n, at, kWave));
-      p.q.ctx = uniform(__shfl(q.ctx, at, kWave));
-      p.q.bad = uniform(__shfl((unsigned int)q.bad, at, kWave)) != 0;
+      const unsigned int in = item - (unsigned int)before;
+      const int at = __ffsll((long long)__ballot(sum > in)) - 1;
+      p.r = r0 + (unsigned int)at;
+      p.index = in - lane_value(sum - own, at);
+      p.q.start = lane_value(q.start, at);
+      p.q.n = lane_value(q.n, at);
+      p.q.ctx = lane_value(q.ctx, at);
+      p.q.bad = lane_value(q.bad ? 1u : 0u, at) != 0;
       return true;
     }
     before += all;
@@ -387,6 +414,15 @@ __device__ __forceinline__ void store_slow(const AttendArgs& a, bool split, bool
   }
 }
 
+// A slot's job, by one thread of its workgroup. (Row ranges that overlap each other can ask for
+// more slots than there are: their rows stay as they were.)
+__device__ __forceinline__ void store_job(const AttendArgs& a, bool few, unsigned int slot, Job j) {
+  const unsigned int slots = few ? a.few_slots : a.tile_slots;
+  if (threadIdx.x != 0 || slot >= slots) return;
+  if (j.splits != 0 && slot + (unsigned long long)(j.splits - 1) * a.kv_heads >= slots) j.splits = 0;
+  a.jobs[(few ? a.tile_slots : 0u) + slot] = j;
+}
+
 // ---------------------------------------------------------------------------
 // 128 rows by 64 tokens a step
 
@@ -397,41 +433,40 @@ __device__ __forceinline__ void store_slow(const AttendArgs& a, bool split, bool
 // rows; V's 64-byte quarters q at q ^ (t % 4), read transposed 8 bytes a lane, 4 tokens by 32 dims
 // per half wave.
 template <typename E, int D, bool kPaged>
-__global__ __launch_bounds__(kT, 2) void attention_tiles(AttendArgs a) {
+__device__ __forceinline__ void tile_path(const AttendArgs& a, const Request& first_requests,
+                                          const SplitSteps& steps, unsigned int block,
+                                          unsigned char* s0, unsigned char* s1) {
   typedef typename Elem<E>::x8 x8;
   constexpr int kRowBytes = 2 * D, kPieces = kRowBytes / 16;  // pieces of a row
   constexpr int kRowsPerLoad = kWave / kPieces, kLoads = 16 / kRowsPerLoad;
   constexpr int kTileBytes = kTileTokens * kRowBytes;
   constexpr int kSlabs = D / 16, kDimTiles = D / 32;
-  // (a variable for each buffer: the compiler orders a read of one behind the loads into it,
-  // and not behind those into the others)
-  __shared__ __align__(1024) unsigned char sK0[kTileBytes];
-  __shared__ __align__(1024) unsigned char sV0[kTileBytes];
-  __shared__ __align__(1024) unsigned char sK1[kTileBytes];
-  __shared__ __align__(1024) unsigned char sV1[kTileBytes];
 
   const unsigned int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
   const unsigned int half = lane / 32, col = lane % 32;
-  const unsigned int head = blockIdx.x % a.kv_heads, item = blockIdx.x / a.kv_heads;
-  const SplitSteps steps = split_steps(a);
+  const unsigned int head = block % a.kv_heads, item = block / a.kv_heads, slot = block;
   Place p;
-  if (!find_item(a, item, [&](const Request& q) -> unsigned long long {
-        return kind_of(a, q) == 2 ? (unsigned long long)tiles_of(a, q.n) * tile_splits(q.ctx, steps.tiles)
-                                  : 0ull;
-      }, p))
+  if (!find_item(a, first_requests, item, [&](const Request& q) -> unsigned int {
+        return kind_of(a, q) == 2 ? tiles_of(a, q.n) * tile_splits(q.ctx, steps.tiles) : 0u;
+      }, p)) {
+    store_job(a, false, slot, Job{});
     return;
-  const unsigned int splits = tile_splits(p.q.ctx, steps.tiles);
+  }
+  const unsigned int all = tile_splits(p.q.ctx, steps.tiles);
   // the tiles with the longest contexts first
-  const unsigned int tile = tiles_of(a, p.q.n) - 1 - p.index / splits, split = p.index % splits;
-  const unsigned int slot = item * a.kv_heads + head;
+  const unsigned int tile = tiles_of(a, p.q.n) - 1 - p.index / all, split = p.index % all;
   const unsigned int rows = p.q.n * a.group;
   const unsigned int m0 = tile * kTileRows;
   // last visible token of a row (negative: none)
   const int shift = (int)p.q.ctx - (int)p.q.n;
   const int last_of_tile = shift + (int)((min(rows, m0 + kTileRows) - 1) / a.group);
   const unsigned int seen = last_of_tile < 0 ? 0u : (unsigned int)last_of_tile + 1;
+  const unsigned int splits = tile_splits(seen, steps.tiles);  // of this tile
+  store_job(a, false, slot,
+            Job{p.q.start, m0, shift, (unsigned short)min(rows - m0, (unsigned int)kTileRows),
+                (unsigned short)(split == 0 && splits > 1 ? splits : 0u)});
+  if (split >= splits) return;
   const unsigned int t_begin = split * steps.tiles * kTileTokens;
-  if (split != 0 && t_begin >= seen) return;
   const unsigned int t_end =
       splits == 1 ? seen : min(seen, t_begin + steps.tiles * kTileTokens);
   const unsigned int mw = m0 + wave * 32, m = mw + col;
@@ -562,24 +597,24 @@ __global__ __launch_bounds__(kT, 2) void attention_tiles(AttendArgs a) {
 
   if (t_begin < t_end) {
     fetch_ids(t_begin);
-    issue(t_begin, sK0, sV0);
+    issue(t_begin, s0, s0 + kTileBytes);
     if (t_begin + kTileTokens < t_end) fetch_ids(t_begin + kTileTokens);
     unsigned int base = t_begin;
-    auto turn = [&](unsigned char* bk, unsigned char* bv, unsigned char* nk, unsigned char* nv) {
+    auto turn = [&](unsigned char* now, unsigned char* next) {
       // this tile's loads have landed, and every wave is done with the other buffer
       wait_loads<0>();
       __syncthreads();
       if (base + kTileTokens < t_end) {
-        issue(base + kTileTokens, nk, nv);
+        issue(base + kTileTokens, next, next + kTileBytes);
         if (base + 2 * kTileTokens < t_end) fetch_ids(base + 2 * kTileTokens);
       }
-      if ((int)base <= last_limit) step(base, bk, bv);
+      if ((int)base <= last_limit) step(base, now, now + kTileBytes);
       base += kTileTokens;
     };
     while (base < t_end) {
-      turn(sK0, sV0, sK1, sV1);
+      turn(s0, s1);
       if (base >= t_end) break;
-      turn(sK1, sV1, sK0, sV0);
+      turn(s1, s0);
     }
   }
 
@@ -649,30 +684,33 @@ __global__ __launch_bounds__(kT, 2) void attention_tiles(AttendArgs a) {
 // pieces of row t at piece ^ (t % 8), so that the 16 tokens of a transposed read spread over the
 // banks. The waves of a workgroup take turns at 32 tokens of a split and join their sums in LDS.
 template <typename E, int D>
-__global__ __launch_bounds__(kT, 2) void attention_few(AttendArgs a) {
+__device__ __forceinline__ void few_path(const AttendArgs& a, const Request& first_requests,
+                                         const SplitSteps& steps, unsigned int block,
+                                         unsigned char* s0, unsigned char* s1) {
   typedef typename Elem<E>::x8 x8;
   constexpr int kRowBytes = 2 * D, kPieces = kRowBytes / 16;
   constexpr int kRowsPerLoad = kWave / kPieces, kLoads = kFewStep / kRowsPerLoad;
   constexpr int kStageBytes = kFewStep * kRowBytes;
   constexpr int kSlabs = D / 32, kDimTiles = D / 16;
-  __shared__ __align__(1024) unsigned char sV0[kWaves * kStageBytes];
-  __shared__ __align__(1024) unsigned char sV1[kWaves * kStageBytes];
   // the waves' sums, then their (m, l), once the stages are read
-  float* const s_acc = reinterpret_cast<float*>(sV0);
-  float* const s_ml = reinterpret_cast<float*>(sV1);
+  float* const s_acc = reinterpret_cast<float*>(s0);
+  float* const s_ml = reinterpret_cast<float*>(s1);
   static_assert(kStageBytes >= kFewRows * D * 4, "a wave's sums fit its stage");
 
   const unsigned int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
   const unsigned int col = lane % 16, grp = lane / 16;
-  const unsigned int head = blockIdx.x % a.kv_heads, item = blockIdx.x / a.kv_heads;
-  const SplitSteps steps = split_steps(a);
+  const unsigned int head = block % a.kv_heads, item = block / a.kv_heads, slot = block;
   Place p;
-  if (!find_item(a, item, [&](const Request& q) -> unsigned long long {
+  if (!find_item(a, first_requests, item, [&](const Request& q) -> unsigned int {
         return kind_of(a, q) == 1 ? few_splits(q.ctx, steps.few) : 0u;
-      }, p))
+      }, p)) {
+    store_job(a, true, slot, Job{});
     return;
+  }
   const unsigned int splits = few_splits(p.q.ctx, steps.few), split = p.index;
-  const unsigned int slot = item * a.kv_heads + head;
+  store_job(a, true, slot,
+            Job{p.q.start, 0, (int)p.q.ctx - (int)p.q.n, (unsigned short)(p.q.n * a.group),
+                (unsigned short)(split == 0 && splits > 1 ? splits : 0u)});
   const unsigned int rows = p.q.n * a.group;
   const unsigned int t_begin = split * steps.few * kFewRound;
   const unsigned int t_end = min(p.q.ctx, t_begin + steps.few * kFewRound);
@@ -698,8 +736,8 @@ __global__ __launch_bounds__(kT, 2) void attention_few(AttendArgs a) {
   struct Keys {
     u32x4 v[2][kSlabs];
   };
-  unsigned char* const stage0 = sV0 + wave * kStageBytes;
-  unsigned char* const stage1 = sV1 + wave * kStageBytes;
+  unsigned char* const stage0 = s0 + wave * kStageBytes;
+  unsigned char* const stage1 = s1 + wave * kStageBytes;
   const unsigned int piece = lane % kPieces, sub = lane / kPieces;
   // lane l looks up token l % 32 of a step
   auto token_of = [&](unsigned int base) { return min(base + lane % 32, t_end - 1); };
@@ -875,96 +913,152 @@ __global__ __launch_bounds__(kT, 2) void attention_few(AttendArgs a) {
 }
 
 // ---------------------------------------------------------------------------
-// the splits of a row joined: a wave a row
+// both paths in one launch
+
+// Workgroups take the two paths in turns of 8 (one on each XCD, so that a KV head of eight stays
+// on its XCD's L2), so that streaming and matrix work run beside each other, then what is left of
+// the longer list.
+template <typename E, int D, bool kPaged, bool kTiles, bool kFew>
+__global__ __launch_bounds__(kT, 2) void attention_step(AttendArgs a) {
+  // (a variable for each buffer: the compiler orders a read of one behind the loads into it, and
+  // not behind those into the other)
+  constexpr int kBuffer = 2 * kTileTokens * 2 * D;
+  static_assert(kBuffer == kWaves * kFewStep * 2 * D, "both paths' stages");
+  __shared__ __align__(1024) unsigned char s0[kBuffer];
+  __shared__ __align__(1024) unsigned char s1[kBuffer];
+  const Request first_requests = load_request(a, __lane_id());
+  const SplitSteps steps = split_steps(a, first_requests);
+  unsigned int block = blockIdx.x;
+  bool few = kFew;
+  if constexpr (kTiles && kFew) {
+    const unsigned int turns = min(a.tile_groups, a.few_groups) / 8;
+    if (block < 16 * turns) {
+      few = (block / 8) % 2 != 0;
+      block = block / 16 * 8 + block % 8;
+    } else {
+      block -= 8 * turns;
+      few = block >= a.tile_groups;
+      if (few) block -= a.tile_groups - 8 * turns;
+    }
+  }
+  if (kFew && few) {
+    if constexpr (kFew) few_path<E, D>(a, first_requests, steps, block, s0, s1);
+  } else {
+    if constexpr (kTiles) tile_path<E, D, kPaged>(a, first_requests, steps, block, s0, s1);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// the splits of a row joined
+
+// A workgroup looks at its share of the slots' jobs with one load and takes those that have
+// something to join: 16 rows of a tile with a thread for 8 (D = 64: 4) sums of a row, or 4 rows of
+// the streaming path, which has more splits, with four threads that share a row's splits.
+constexpr int kTileParts = kTileRows / 16, kFewParts = kFewRows / 4;
 
 template <typename E, int D>
 __global__ __launch_bounds__(kT) void attention_merge(AttendArgs a) {
-  constexpr int kVals = D / 64;
+  constexpr int kVals = D / 16;
   constexpr int kBatch = 8;
-  const unsigned int lane = threadIdx.x & 63;
-  const unsigned int waves = gridDim.x * kWaves;
-  const SplitSteps steps = split_steps(a);
-#pragma unroll 1
-  for (int few = 0; few < 2; ++few) {
-    if (few ? a.few_rows == 0 : (a.tiles_too == 0 || steps.tiles == 0)) continue;
-    // (row, head) pairs of the requests with several splits
-    auto rows_of = [&](const Request& q) -> unsigned long long {
-      if (kind_of(a, q) != (few ? 1 : 2)) return 0;
-      const unsigned int splits = few ? few_splits(q.ctx, steps.few) : tile_splits(q.ctx, steps.tiles);
-      return splits > 1 ? (unsigned long long)q.n * a.q_heads : 0ull;
-    };
-    auto items_of = [&](const Request& q) -> unsigned long long {
-      if (kind_of(a, q) != (few ? 1 : 2)) return 0;
-      return few ? few_splits(q.ctx, steps.few)
-                 : (unsigned long long)tiles_of(a, q.n) * tile_splits(q.ctx, steps.tiles);
-    };
-    for (unsigned long long w = blockIdx.x * kWaves + uniform(threadIdx.x >> 6);; w += waves) {
-      Place p;
-      if (!find_item(a, w, rows_of, p)) break;
-      // items of the requests before this one
-      unsigned long long items = 0;
-      for (unsigned int r = lane; r < p.r; r += kWave) items += items_of(load_request(a, r));
-      items = wave_sum(items);
-      const unsigned int head = p.index / (p.q.n * a.group), m = p.index % (p.q.n * a.group);
-      const unsigned int tok = m / a.group, qh = head * a.group + m - tok * a.group;
-      unsigned int splits, slot_row;
-      if (few) {
-        splits = few_splits(p.q.ctx, steps.few);
-        slot_row = m;
-      } else {
-        const unsigned int all = tile_splits(p.q.ctx, steps.tiles), tile = m / kTileRows;
-        const unsigned int rows = p.q.n * a.group;
-        const int last = (int)p.q.ctx - (int)p.q.n +
-                         (int)((min(rows, (tile + 1) * kTileRows) - 1) / a.group);
-        // the tile's own splits
-        splits = max(1u, steps_of(steps_of(last < 0 ? 0u : (unsigned int)last + 1, kTileTokens), steps.tiles));
-        items += (unsigned long long)(tiles_of(a, p.q.n) - 1 - tile) * all;
-        slot_row = m % kTileRows;
-      }
-      // (row ranges that overlap each other can ask for more slots than there are)
-      if ((items + splits) * a.kv_heads > (few ? a.few_slots : a.tile_slots)) continue;
-      auto slot_of = [&](unsigned int s) { return (unsigned int)((items + s) * a.kv_heads + head); };
+  __shared__ float s_part[kT][kVals + 2];
+  const unsigned int tid = threadIdx.x, lane = tid & 63;
+  const unsigned int tile_jobs = a.tile_slots * kTileParts;
+  const unsigned int jobs = tile_jobs + a.few_slots * kFewParts;
+  auto slot_of = [&](unsigned int j) {
+    return j < tile_jobs ? j / kTileParts : a.tile_slots + (j - tile_jobs) / kFewParts;
+  };
+  for (unsigned int j0 = blockIdx.x; j0 < jobs; j0 += kWave * gridDim.x) {
+    const unsigned int mine = j0 + lane * gridDim.x;
+    unsigned long long todo = __ballot(mine < jobs && a.jobs[slot_of(min(mine, jobs - 1))].splits != 0);
+    while (todo != 0) {
+      const unsigned int j = j0 + ((unsigned int)__ffsll((long long)todo) - 1) * gridDim.x;
+      todo &= todo - 1;
+      const bool few = j >= tile_jobs;
+      const unsigned int job_slot = slot_of(j);
+      const Job job = a.jobs[job_slot];
+      const unsigned int slot = few ? job_slot - a.tile_slots : job_slot;
+      const unsigned int head = slot % a.kv_heads;
+      const unsigned int shares = few ? 4 : 1;  // threads that share a row's splits
+      const unsigned int share = (tid / 16) % shares, dims = (tid % 16) * kVals;
+      const unsigned int row = few ? (j - tile_jobs) % kFewParts * 4 + tid / 64
+                                   : j % kTileParts * 16 + tid / 16;
+      const bool in = row < job.rows;
+      const unsigned int use = in ? row : 0u;
       float big = kNoMax, l = 0.f, acc[kVals];
       bool bad = false;
 #pragma unroll
       for (int i = 0; i < kVals; ++i) acc[i] = 0.f;
-      for (unsigned int s0 = 0; s0 < splits; s0 += kWave) {
-        const unsigned int s = min(s0 + lane, splits - 1);
-        const f32x2 ml = *reinterpret_cast<const f32x2*>(slot_ml<D>(a, few, slot_of(s)) + 2 * slot_row);
-        const bool in = s0 + lane < splits;
-        bad |= in && ml.x != ml.x;
-        const float top = fmaxf(big, wave_max(in ? ml.x : kNoMax));
-        const float alpha = exp2f(big - top), f = in ? exp2f(ml.x - top) : 0.f;
+      for (unsigned int b = share; b < job.splits; b += shares * kBatch) {
+        f32x2 ml[kBatch];
+        f32x4 v[kBatch][kVals / 4];
+        // (past the last split the last one again, without weight: loads behind branches would
+        // wait for each other)
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+          const unsigned int at = slot + min(b + k * shares, job.splits - 1u) * a.kv_heads;
+          ml[k] = *reinterpret_cast<const f32x2*>(slot_ml<D>(a, few, at) + 2 * use);
+          const float* src = slot_acc<D>(a, few, at) + use * D + dims;
+#pragma unroll
+          for (int i = 0; i < kVals / 4; ++i) v[k][i] = *reinterpret_cast<const f32x4*>(src + 4 * i);
+        }
+        float top = big;
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+          if (b + k * shares >= job.splits) ml[k] = f32x2{kNoMax, 0.f};
+          bad |= ml[k].x != ml[k].x;
+          top = fmaxf(top, ml[k].x);
+        }
+        const float alpha = exp2f(big - top);
         big = top;
-        l = l * alpha + wave_sum(in ? ml.y * f : 0.f);
+        l *= alpha;
 #pragma unroll
         for (int i = 0; i < kVals; ++i) acc[i] *= alpha;
-        const unsigned int count = min(splits - s0, (unsigned int)kWave);
-        for (unsigned int j0 = 0; j0 < count; j0 += kBatch) {
-          float v[kBatch][kVals];
 #pragma unroll
-          for (int j = 0; j < kBatch; ++j) {
-            const unsigned int sj = s0 + min(j0 + j, count - 1);
-            const float* src = slot_acc<D>(a, few, slot_of(sj)) + slot_row * D + lane * kVals;
+        for (int k = 0; k < kBatch; ++k) {
+          const float f = b + k * shares < job.splits ? exp2f(ml[k].x - big) : 0.f;
+          l += ml[k].y * f;
 #pragma unroll
-            for (int i = 0; i < kVals; ++i) v[j][i] = src[i];
-          }
-#pragma unroll
-          for (int j = 0; j < kBatch; ++j) {
-            if (j0 + j >= count) break;
-            const float fj = __shfl(f, (int)(j0 + j), kWave);
-#pragma unroll
-            for (int i = 0; i < kVals; ++i) acc[i] = fmaf(v[j][i], fj, acc[i]);
-          }
+          for (int i = 0; i < kVals; ++i) acc[i] = f != 0.f ? fmaf(v[k][i / 4][i % 4], f, acc[i]) : acc[i];
         }
       }
-      bad = __ballot(bad) != 0;
-      const unsigned long long out_row = (unsigned long long)(p.q.start + tok) * a.q_heads + qh;
-      const bool none = (int)p.q.ctx - (int)p.q.n + (int)tok < 0 && !bad;
-      E* dst = reinterpret_cast<E*>(a.out) + out_row * D + lane * kVals;
+      if (few) {
+        __syncthreads();  // the job before this one is done with the LDS
+        float* own = s_part[tid];
+        own[0] = bad ? NAN : big;
+        own[1] = l;
 #pragma unroll
-      for (int i = 0; i < kVals; ++i) dst[i] = (E)(bad ? NAN : none ? 0.f : acc[i] / l);
-      if (a.lse != nullptr && lane == 0)
+        for (int i = 0; i < kVals; ++i) own[2 + i] = acc[i];
+        __syncthreads();
+        big = kNoMax;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float m = s_part[tid / 64 * 64 + 16 * k + tid % 16][0];
+          bad |= m != m;
+          big = fmaxf(big, m);
+        }
+        l = 0.f;
+#pragma unroll
+        for (int i = 0; i < kVals; ++i) acc[i] = 0.f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float* src = s_part[tid / 64 * 64 + 16 * k + tid % 16];
+          const float f = exp2f(src[0] - big);
+          l += src[1] * f;
+#pragma unroll
+          for (int i = 0; i < kVals; ++i) acc[i] += src[2 + i] * f;
+        }
+        if (share != 0) continue;
+      }
+      if (!in) continue;
+      const unsigned int m = job.first + row, tok = m / a.group;
+      const unsigned long long out_row =
+          (unsigned long long)(job.start + tok) * a.q_heads + head * a.group + (m - tok * a.group);
+      const bool none = job.shift + (int)tok < 0 && !bad;
+      const float inv = bad ? NAN : none ? 0.f : 1.f / l;
+      uint32_t* dst = reinterpret_cast<uint32_t*>(a.out + (out_row * D + dims) * 2);
+#pragma unroll
+      for (int i = 0; i < kVals; i += 2) dst[i / 2] = pack2<E>(acc[i] * inv, acc[i + 1] * inv);
+      if (a.lse != nullptr && dims == 0)
         a.lse[out_row] = bad ? NAN : none ? -INFINITY : (big + log2f(l)) * kLn2;
     }
   }
@@ -1031,43 +1125,42 @@ unsigned long long tile_slots_of(const Bounds& b, unsigned long long kv_heads) {
   return b.tiles ? std::min(b.tile_items * kv_heads, 3 * b.tile_target + kv_heads) : 0;
 }
 
+// The slots' partials, then their jobs.
 unsigned long long partial_bytes(const Bounds& b, unsigned long long kv_heads,
                                  unsigned long long head_dim) {
-  return ((b.few ? b.few_items * kv_heads * kFewRows : 0) + tile_slots_of(b, kv_heads) * kTileRows) *
+  return (b.few_items * kv_heads * kFewRows + tile_slots_of(b, kv_heads) * kTileRows) *
          (head_dim + 2) * sizeof(float);
+}
+unsigned long long workspace_of(const Bounds& b, unsigned long long kv_heads,
+                                unsigned long long head_dim) {
+  return partial_bytes(b, kv_heads, head_dim) +
+         (b.few_items * kv_heads + tile_slots_of(b, kv_heads)) * sizeof(Job);
 }
 
 template <typename E, int D, bool kPaged>
-long long launch(const AttendArgs& a, const Bounds& b, hipStream_t stream) {
-  if (b.tiles) {
-    hipLaunchKernelGGL((attention_tiles<E, D, kPaged>),
-                       dim3((unsigned int)(b.tile_items * a.kv_heads)), dim3(kT), 0, stream, a);
-    const hipError_t st = hipGetLastError();
-    if (st != hipSuccess) return fail("attention_tiles", st);
-  }
-  if constexpr (kPaged) {
-    if (b.few) {
-      hipLaunchKernelGGL((attention_few<E, D>), dim3((unsigned int)(b.few_items * a.kv_heads)),
-                         dim3(kT), 0, stream, a);
-      const hipError_t st = hipGetLastError();
-      if (st != hipSuccess) return fail("attention_few", st);
-    }
-  }
-  const unsigned long long rows = (unsigned long long)a.tokens * a.q_heads;
-  hipLaunchKernelGGL((attention_merge<E, D>),
-                     dim3((unsigned int)std::min<unsigned long long>((rows + kWaves - 1) / kWaves, 1024)),
-                     dim3(kT), 0, stream, a);
-  const hipError_t st = hipGetLastError();
+long long launch(const AttendArgs& a, hipStream_t stream) {
+  const dim3 grid(a.tile_groups + a.few_groups), threads(kT);
+  if constexpr (!kPaged)
+    hipLaunchKernelGGL((attention_step<E, D, false, true, false>), grid, threads, 0, stream, a);
+  else if (a.tile_groups != 0)
+    hipLaunchKernelGGL((attention_step<E, D, true, true, true>), grid, threads, 0, stream, a);
+  else
+    hipLaunchKernelGGL((attention_step<E, D, true, false, true>), grid, threads, 0, stream, a);
+  hipError_t st = hipGetLastError();
+  if (st != hipSuccess) return fail("attention_step", st);
+  const unsigned int jobs = a.tile_slots * kTileParts + a.few_slots * kFewParts;
+  hipLaunchKernelGGL((attention_merge<E, D>), dim3(std::min(jobs, 1024u)), threads, 0, stream, a);
+  st = hipGetLastError();
   if (st != hipSuccess) return fail("attention_merge", st);
-  return (long long)(rows * D * 2);
+  return (long long)((unsigned long long)a.tokens * a.q_heads * D * 2);
 }
 
 template <bool kPaged>
-long long launch_typed(const AttendArgs& a, const Bounds& b, unsigned long long head_dim,
-                       unsigned long long dtype, hipStream_t stream) {
+long long launch_typed(const AttendArgs& a, unsigned long long head_dim, unsigned long long dtype,
+                       hipStream_t stream) {
   if (head_dim == 128)
-    return dtype ? launch<_Float16, 128, kPaged>(a, b, stream) : launch<__bf16, 128, kPaged>(a, b, stream);
-  return dtype ? launch<_Float16, 64, kPaged>(a, b, stream) : launch<__bf16, 64, kPaged>(a, b, stream);
+    return dtype ? launch<_Float16, 128, kPaged>(a, stream) : launch<__bf16, 128, kPaged>(a, stream);
+  return dtype ? launch<_Float16, 64, kPaged>(a, stream) : launch<__bf16, 64, kPaged>(a, stream);
 }
 
 constexpr unsigned long long kMostRows = 0x7FFFFFFFull;
@@ -1094,7 +1187,7 @@ extern "C" unsigned long long kvq_splitzip_chunk_attention_workspace_bytes(
     unsigned long long kv_heads, unsigned long long head_dim, unsigned long long max_context,
     unsigned long long max_query) {
   if (!sizes_ok(tokens, requests, q_heads, kv_heads, head_dim, max_query)) return 0;
-  return partial_bytes(bounds_of(tokens, requests, kv_heads, q_heads / kv_heads, max_context,
+  return workspace_of(bounds_of(tokens, requests, kv_heads, q_heads / kv_heads, max_context,
                                  max_query, true), kv_heads, head_dim);
 }
 
@@ -1102,7 +1195,7 @@ extern "C" unsigned long long kvq_splitzip_prompt_attention_workspace_bytes(
     unsigned long long tokens, unsigned long long requests, unsigned long long q_heads,
     unsigned long long kv_heads, unsigned long long head_dim, unsigned long long max_query) {
   if (!sizes_ok(tokens, requests, q_heads, kv_heads, head_dim, max_query)) return 0;
-  return partial_bytes(bounds_of(tokens, requests, kv_heads, q_heads / kv_heads, max_query,
+  return workspace_of(bounds_of(tokens, requests, kv_heads, q_heads / kv_heads, max_query,
                                  max_query, false), kv_heads, head_dim);
 }
 
@@ -1126,9 +1219,9 @@ extern "C" long long kvq_splitzip_chunk_attention_paged(
     return 0;
   const unsigned long long max_context = std::min(table_width * block_tokens, kMostRows);
   const Bounds b = bounds_of(tokens, requests, kv_heads, q_heads / kv_heads, max_context, max_query, true);
-  const unsigned long long need = partial_bytes(b, kv_heads, head_dim);
+  const unsigned long long need = workspace_of(b, kv_heads, head_dim);
   if (workspace_ptr == 0 || workspace_ptr % 16 != 0 || workspace_bytes < need) return 0;
-  if (b.tile_items * kv_heads > kMostRows || b.few_items * kv_heads > kMostRows) return 0;
+  if ((b.tile_items + b.few_items) * kv_heads > kMostRows) return 0;
   const unsigned long long out_bytes = tokens * q_heads * head_dim * 2;
   if (overlap(out_ptr, out_bytes, q_ptr, extent(tokens, q_row_bytes, q_heads, q_head_bytes, 2 * head_dim)) ||
       overlap(out_ptr, out_bytes, kv_ptr, 4 * blocks * block_tokens * kv_heads * head_dim))
@@ -1145,6 +1238,7 @@ extern "C" long long kvq_splitzip_chunk_attention_paged(
   a.contexts = reinterpret_cast<const int*>(context_tokens_ptr);
   a.tables = reinterpret_cast<const int*>(tables_ptr);
   a.partial = reinterpret_cast<float*>(workspace_ptr);
+  a.jobs = reinterpret_cast<Job*>(workspace_ptr + partial_bytes(b, kv_heads, head_dim));
   a.q_row = q_row_bytes;
   a.q_head = q_head_bytes;
   a.table_stride = table_stride;
@@ -1163,9 +1257,10 @@ extern "C" long long kvq_splitzip_chunk_attention_paged(
   a.tile_target = (unsigned int)b.tile_target;
   a.max_query = (unsigned int)max_query;
   a.tile_slots = (unsigned int)tile_slots_of(b, kv_heads);
-  a.few_slots = (unsigned int)(b.few_items * kv_heads);
+  a.few_slots = a.few_groups = (unsigned int)(b.few_items * kv_heads);
+  a.tile_groups = (unsigned int)(b.tile_items * kv_heads);
   a.scale_log2 = scale * 1.4426950408889634f;
-  return launch_typed<true>(a, b, head_dim, dtype, reinterpret_cast<hipStream_t>(stream_ptr));
+  return launch_typed<true>(a, head_dim, dtype, reinterpret_cast<hipStream_t>(stream_ptr));
 }
 
 extern "C" long long kvq_splitzip_prompt_attention(
@@ -1185,7 +1280,7 @@ extern "C" long long kvq_splitzip_prompt_attention(
       !std::isfinite(scale))
     return 0;
   const Bounds b = bounds_of(tokens, requests, kv_heads, q_heads / kv_heads, max_query, max_query, false);
-  const unsigned long long need = partial_bytes(b, kv_heads, head_dim);
+  const unsigned long long need = workspace_of(b, kv_heads, head_dim);
   if (workspace_ptr == 0 || workspace_ptr % 16 != 0 || workspace_bytes < need) return 0;
   if (b.tile_items * kv_heads > kMostRows) return 0;
   const unsigned long long out_bytes = tokens * q_heads * head_dim * 2;
@@ -1205,6 +1300,7 @@ extern "C" long long kvq_splitzip_prompt_attention(
   a.v_head = v_head_bytes;
   a.starts = reinterpret_cast<const int*>(query_starts_ptr);
   a.partial = reinterpret_cast<float*>(workspace_ptr);
+  a.jobs = reinterpret_cast<Job*>(workspace_ptr + partial_bytes(b, kv_heads, head_dim));
   a.q_row = q_row_bytes;
   a.q_head = q_head_bytes;
   a.tokens = (unsigned int)tokens;
@@ -1218,7 +1314,8 @@ extern "C" long long kvq_splitzip_prompt_attention(
   a.tile_target = (unsigned int)b.tile_target;
   a.max_query = (unsigned int)max_query;
   a.tile_slots = (unsigned int)tile_slots_of(b, kv_heads);
-  a.few_slots = (unsigned int)(b.few_items * kv_heads);
+  a.few_slots = a.few_groups = (unsigned int)(b.few_items * kv_heads);
+  a.tile_groups = (unsigned int)(b.tile_items * kv_heads);
   a.scale_log2 = scale * 1.4426950408889634f;
-  return launch_typed<false>(a, b, head_dim, dtype, reinterpret_cast<hipStream_t>(stream_ptr));
+  return launch_typed<false>(a, head_dim, dtype, reinterpret_cast<hipStream_t>(stream_ptr));
 }
