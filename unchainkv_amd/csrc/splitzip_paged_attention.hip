@@ -318,6 +318,16 @@ __device__ __forceinline__ void load_to_lds(const unsigned char* src, unsigned c
       (__attribute__((address_space(3))) unsigned char*)dst, 16, 0, 0);
 }
 
+// The same from a buffer: lanes whose 16 bytes end past it get zeros.
+typedef __amdgpu_buffer_rsrc_t Buffer;
+__device__ __forceinline__ Buffer buffer_of(const unsigned char* base, unsigned int bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(base), 0, (int)bytes, 0x00020000);
+}
+__device__ __forceinline__ void load_to_lds(Buffer b, unsigned int offset, unsigned char* dst) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(b, (__attribute__((address_space(3))) unsigned char*)dst, 16,
+                                           (int)offset, 0, 0, 0);
+}
+
 // Waits until at most N of the wave's loads are in flight.
 template <int N>
 __device__ __forceinline__ void wait_loads() {
@@ -432,7 +442,7 @@ __device__ __forceinline__ void store_job(const AttendArgs& a, bool few, unsigne
 // one read spread over the banks: K's piece c of row t at c ^ (t % 16), read 16 bytes a lane by 32
 // rows; V's 64-byte quarters q at q ^ (t % 4), read transposed 8 bytes a lane, 4 tokens by 32 dims
 // per half wave.
-template <typename E, int D, bool kPaged>
+template <typename E, int D, bool kPaged, bool kRuns>
 __device__ __forceinline__ void tile_path(const AttendArgs& a, const Request& first_requests,
                                           const SplitSteps& steps, unsigned int block,
                                           unsigned char* s0, unsigned char* s1) {
@@ -493,26 +503,53 @@ __device__ __forceinline__ void tile_path(const AttendArgs& a, const Request& fi
     q[s] = *reinterpret_cast<const x8*>(q_row + 32 * s + 16 * half);
   }
 
-  // this wave's share of a tile: 16 tokens of K and V
+  // this wave's share of a tile: 16 tokens of K and V. Where they follow each other in memory
+  // (prompts; layers whose blocks are whole groups of 16 tokens) the wave forms their address once,
+  // on the scalar unit, and a lane's offsets from it never change.
   const unsigned int piece = lane % kPieces, sub = lane / kPieces;
-  int ids[kLoads];
+  unsigned int k_off[kLoads], v_off[kLoads];
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i) {
+    const unsigned int in = i * kRowsPerLoad + sub;  // the token's place among the wave's 16
+    const unsigned int k_piece = piece ^ (D == 128 ? in : (in >> 1) & 7);
+    const unsigned int v_piece = piece ^ (D == 128 ? (in & 3) << 2 : ((in >> 1) & 1) << 2);
+    k_off[i] = (kRuns ? in * (unsigned int)a.k_row : 0u) + 16 * k_piece;
+    v_off[i] = (kRuns ? in * (unsigned int)a.v_row : 0u) + 16 * v_piece;
+  }
+  constexpr int kIds = kRuns ? 1 : kLoads;
+  int ids[kIds];
   auto token_of = [&](unsigned int base, int i) {
-    return min(base + wave * 16 + i * kRowsPerLoad + sub, t_end - 1);
+    return min(base + wave * 16 + (kRuns ? 0 : i * kRowsPerLoad + sub), t_end - 1);
   };
   auto fetch_ids = [&](unsigned int base) {
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) ids[i] = block_id<kPaged>(a, table, token_of(base, i));
+    for (int i = 0; i < kIds; ++i) ids[i] = block_id<kPaged>(a, table, token_of(base, i));
   };
   auto issue = [&](unsigned int base, unsigned char* bk, unsigned char* bv) {
+    const unsigned int at = wave * 16 * kRowBytes;
+    if constexpr (kRuns) {
+      // tokens past the end are outside the buffers
+      const unsigned int first = base + wave * 16, count = min(t_end - min(first, t_end), 16u);
+      const unsigned int row = uniform(kv_row<kPaged>(a, table, p.q.start, token_of(base, 0), ids[0], bad));
+      // (sizes moved to scalars: with one in a vector register each load became a loop over lanes)
+      const Buffer kr = buffer_of(
+          kb + row * a.k_row,
+          uniform(count == 0 ? 0u : (count - 1) * (unsigned int)a.k_row + kRowBytes));
+      const Buffer vr = buffer_of(
+          vb + row * a.v_row,
+          uniform(count == 0 ? 0u : (count - 1) * (unsigned int)a.v_row + kRowBytes));
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      const unsigned int in = i * kRowsPerLoad + sub;  // the token's place among the wave's 16
-      const unsigned int row = kv_row<kPaged>(a, table, p.q.start, token_of(base, i), ids[i], bad);
-      const unsigned int k_piece = piece ^ (D == 128 ? in : (in >> 1) & 7);
-      const unsigned int v_piece = piece ^ (D == 128 ? (in & 3) << 2 : ((in >> 1) & 1) << 2);
-      const unsigned int at = (wave * 16 + i * kRowsPerLoad) * kRowBytes;
-      load_to_lds(kb + row * a.k_row + 16 * k_piece, bk + at);
-      load_to_lds(vb + row * a.v_row + 16 * v_piece, bv + at);
+      for (int i = 0; i < kLoads; ++i) {
+        load_to_lds(kr, k_off[i], bk + at + i * kRowsPerLoad * kRowBytes);
+        load_to_lds(vr, v_off[i], bv + at + i * kRowsPerLoad * kRowBytes);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const unsigned int row = kv_row<kPaged>(a, table, p.q.start, token_of(base, i), ids[i], bad);
+        load_to_lds(kb + row * a.k_row + k_off[i], bk + at + i * kRowsPerLoad * kRowBytes);
+        load_to_lds(vb + row * a.v_row + v_off[i], bv + at + i * kRowsPerLoad * kRowBytes);
+      }
     }
   };
 
@@ -918,7 +955,7 @@ __device__ __forceinline__ void few_path(const AttendArgs& a, const Request& fir
 // Workgroups take the two paths in turns of 8 (one on each XCD, so that a KV head of eight stays
 // on its XCD's L2), so that streaming and matrix work run beside each other, then what is left of
 // the longer list.
-template <typename E, int D, bool kPaged, bool kTiles, bool kFew>
+template <typename E, int D, bool kPaged, bool kTiles, bool kFew, bool kRuns>
 __global__ __launch_bounds__(kT, 2) void attention_step(AttendArgs a) {
   // (a variable for each buffer: the compiler orders a read of one behind the loads into it, and
   // not behind those into the other)
@@ -944,7 +981,7 @@ __global__ __launch_bounds__(kT, 2) void attention_step(AttendArgs a) {
   if (kFew && few) {
     if constexpr (kFew) few_path<E, D>(a, first_requests, steps, block, s0, s1);
   } else {
-    if constexpr (kTiles) tile_path<E, D, kPaged>(a, first_requests, steps, block, s0, s1);
+    if constexpr (kTiles) tile_path<E, D, kPaged, kRuns>(a, first_requests, steps, block, s0, s1);
   }
 }
 
@@ -1141,11 +1178,13 @@ template <typename E, int D, bool kPaged>
 long long launch(const AttendArgs& a, hipStream_t stream) {
   const dim3 grid(a.tile_groups + a.few_groups), threads(kT);
   if constexpr (!kPaged)
-    hipLaunchKernelGGL((attention_step<E, D, false, true, false>), grid, threads, 0, stream, a);
-  else if (a.tile_groups != 0)
-    hipLaunchKernelGGL((attention_step<E, D, true, true, true>), grid, threads, 0, stream, a);
+    hipLaunchKernelGGL((attention_step<E, D, false, true, false, true>), grid, threads, 0, stream, a);
+  else if (a.tile_groups == 0)
+    hipLaunchKernelGGL((attention_step<E, D, true, false, true, false>), grid, threads, 0, stream, a);
+  else if (a.block_tokens % 16 == 0)
+    hipLaunchKernelGGL((attention_step<E, D, true, true, true, true>), grid, threads, 0, stream, a);
   else
-    hipLaunchKernelGGL((attention_step<E, D, true, false, true>), grid, threads, 0, stream, a);
+    hipLaunchKernelGGL((attention_step<E, D, true, true, true, false>), grid, threads, 0, stream, a);
   hipError_t st = hipGetLastError();
   if (st != hipSuccess) return fail("attention_step", st);
   const unsigned int jobs = a.tile_slots * kTileParts + a.few_slots * kFewParts;
@@ -1164,6 +1203,7 @@ long long launch_typed(const AttendArgs& a, unsigned long long head_dim, unsigne
 }
 
 constexpr unsigned long long kMostRows = 0x7FFFFFFFull;
+constexpr unsigned long long kMostStride = 1ull << 27;  // 16 rows' offsets fit 32 bits
 
 // Bytes from the first to the last of rows x heads pieces of head_bytes.
 unsigned long long extent(unsigned long long rows, unsigned long long row_bytes,
@@ -1276,8 +1316,8 @@ extern "C" long long kvq_splitzip_prompt_attention(
       q_ptr == 0 || k_ptr == 0 || v_ptr == 0 ||
       (q_ptr | q_row_bytes | q_head_bytes | k_ptr | k_row_bytes | k_head_bytes | v_ptr |
        v_row_bytes | v_head_bytes) % 16 != 0 ||
-      query_starts_ptr == 0 || out_ptr == 0 || out_ptr % 16 != 0 || !(scale > 0.f) ||
-      !std::isfinite(scale))
+      k_row_bytes > kMostStride || v_row_bytes > kMostStride || query_starts_ptr == 0 ||
+      out_ptr == 0 || out_ptr % 16 != 0 || !(scale > 0.f) || !std::isfinite(scale))
     return 0;
   const Bounds b = bounds_of(tokens, requests, kv_heads, q_heads / kv_heads, max_query, max_query, false);
   const unsigned long long need = workspace_of(b, kv_heads, head_dim);
