@@ -217,8 +217,8 @@ def test_row_ranges_that_do_not_hold(sz):
     case = Case([2, 3, 40], [50, 60, 70], 4, 2, 128, 16, "bf16", seed=2)
     out, lse = case.run(sz, max_query=3)
     assert (out[5:] == MARK).all() and (lse[5:] == MARK).all()
+    case.verify(out, lse, skip=(2,))
     whole, _ = case.run(sz)
-    assert torch.equal(out[:5], whole[:5])
     case.starts = i32([0, 2, 5, 1 << 20])
     out, _ = case.run(sz)
     assert torch.equal(out[:5], whole[:5]) and (out[5:] == MARK).all()

@@ -12,11 +12,11 @@
 // group) pairs, row m = token * group + head, and a tile of rows serves them together: a single
 // token is `group` rows, and every K and V byte is read once per tile.
 //
-// Two kernels share the rows of a launch by one rule, on the GPU, where the lengths are:
-//   * attention_few: requests of at most 16 rows (a decode step, a few drafted tokens). Bound by
-//     reading K and V: a wave streams 32 tokens at a time, K straight into the matrix operand's
-//     registers, V into LDS for the transposing reads.
-//   * attention_tiles: 128 rows by 64 tokens a step. Bound by the matrix and vector units.
+// Two kernels, by the rows that a request of the call can have:
+//   * attention_few: at most 16 (decode steps). Bound by reading K and V: a wave streams 32 tokens
+//     at a time, K straight into the matrix operand's registers, V into LDS for the transposing
+//     reads.
+//   * attention_tiles: more; 256 rows by 64 tokens a step. Bound by the matrix and vector units.
 // Both give S^T = K Q^T, so that a row's scores lie in one lane (and its partners 32 or 16 lanes
 // away): the maximum and the sum need one or two lane swaps a step, rescaling is a lane's own
 // product, and the weights are the second product's operand O^T = V^T P^T as they are, with V's
@@ -36,6 +36,7 @@
 #include <cmath>
 #include <cstdint>
 #include <mutex>
+#include <type_traits>
 
 #include "splitzip_common.h"
 
@@ -46,14 +47,18 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short i16x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kT = 256;           // threads of the split kernels
-constexpr int kWaves = kT / kWave;
+constexpr int kWaves = 4;         // waves of a workgroup of attention_few, two of them on a CU
+constexpr int kTileWaves = 8;     // of one of attention_tiles, one on a CU
+constexpr int kMergeThreads = 256;
 constexpr int kFewRows = 16;      // rows of a request that attention_few takes
-constexpr int kFewStep = 32;      // tokens of a wave's step in attention_few
-constexpr int kFewRound = kWaves * kFewStep;  // tokens of a workgroup's round: unit of its splits
-constexpr int kTileRows = 128;
+constexpr int kFewStep = 32;      // tokens of a wave's step in attention_few; a workgroup's waves
+                                  // take a round of them, the unit of its splits
+constexpr int kTileRows = 32 * kTileWaves;
 constexpr int kTileTokens = 64;   // tokens of a step of attention_tiles: unit of its splits
-constexpr unsigned int kLeastTileSteps = 4;  // of a split
+// Steps of a split, at least: shorter ones cost more to join than the shorter last round saves (24
+// prompts of 3 .. 2050 tokens: 47.6 us at 24, 66 at 12; 16 requests of 6 tokens behind 300 .. 8000:
+// 41.3 and 50.2).
+constexpr unsigned int kLeastTileSteps = 24;
 // A maximum before any token: the lowest float, not -inf, so that rows whose scores are all -inf
 // have weights of zero and a sum of zero (whose quotient is NaN, as the formula's).
 constexpr float kNoMax = -3.402823466e38f;
@@ -120,7 +125,7 @@ struct AttendArgs {
   const int* starts;         // [requests + 1]
   const int* contexts;       // [requests]; null: a request's own rows (prompts)
   const int* tables;         // [requests][table_stride]; null for prompts
-  float* partial;            // slots of the tiles, then of the few
+  float* partial;            // of each slot
   struct Job* jobs;          // one for each slot
   unsigned long long q_row, q_head;  // bytes from token to token, from head to head
   unsigned long long k_row, k_head, v_row, v_head;
@@ -128,27 +133,26 @@ struct AttendArgs {
   unsigned int table_width, blocks, block_tokens;
   Divider by_block;
   unsigned int tokens, requests, q_heads, kv_heads, group;
-  unsigned int few_rows;      // most rows of a request that goes to the streaming path; 0: none
-  unsigned int tiles_too;     // whether tiles are taken (else longer requests are left out)
-  unsigned int tile_groups, few_groups;  // workgroups of the two paths
-  unsigned int few_target, tile_target;   // workgroups to split for
+  unsigned int few_target, tile_target;   // workgroups to split for, of the two paths
   unsigned int max_query;     // requests with more new tokens are left out
-  unsigned int tile_slots, few_slots;  // partial slots: of the tiles, then of the few
+  unsigned int slots;         // partial slots
   float scale_log2;
 };
 
 // One request as its lengths in device memory say, with lengths that cannot be cut down to
-// nothing: rows outside the tensor are nobody's.
+// nothing: rows outside the tensor are nobody's, and neither are those of a request that is longer
+// than the call allows.
 struct Request {
-  unsigned int start, n, ctx;
+  unsigned int r, start, n, ctx;
   bool bad;  // a context longer than the block table
 };
 
 __device__ __forceinline__ Request load_request(const AttendArgs& a, unsigned int r) {
-  Request q{0, 0, 0, false};
+  Request q{r, 0, 0, 0, false};
   if (r >= a.requests) return q;
   const int s0 = a.starts[r], s1 = a.starts[r + 1];
-  if (s0 < 0 || s1 < s0 || (unsigned int)s1 > a.tokens) return q;
+  if (s0 < 0 || s1 < s0 || (unsigned int)s1 > a.tokens || (unsigned int)(s1 - s0) > a.max_query)
+    return q;
   q.start = (unsigned int)s0;
   q.n = (unsigned int)(s1 - s0);
   q.ctx = q.n;
@@ -162,14 +166,6 @@ __device__ __forceinline__ Request load_request(const AttendArgs& a, unsigned in
     }
   }
   return q;
-}
-
-// Which kernel takes a request: 0 none, 1 attention_few, 2 attention_tiles.
-__device__ __forceinline__ int kind_of(const AttendArgs& a, const Request& q) {
-  if (q.n == 0 || q.n > a.max_query) return 0;
-  const unsigned long long rows = (unsigned long long)q.n * a.group;
-  if (rows <= a.few_rows) return 1;
-  return a.tiles_too ? 2 : 0;
 }
 
 __device__ __forceinline__ float wave_sum(float v) {
@@ -207,15 +203,7 @@ __device__ __forceinline__ unsigned int tiles_of(const AttendArgs& a, unsigned i
   return (n * a.group + kTileRows - 1) / kTileRows;
 }
 
-// Steps of a split on the streaming path and of a tile's, from the sums over all requests (each
-// lane a request, 64 at a time; `head` holds the first 64, which most launches end with). Few:
-// the even share of all rounds over few_target workgroups. Tiles: no split (0) once there are
-// tile_target tiles, else the even share of all tiles' steps, a tile of a request counted with
-// the request's mean context (a request's sum beyond kMostSteps, which the 32-bit sums do not
-// take, is not split either).
-struct SplitSteps {
-  unsigned int few, tiles;
-};
+// Sums of 64 lanes' values stay below 2^32.
 constexpr unsigned int kMostSteps = 1u << 25;
 
 // ceil(sum / parts), by a 32-bit division where it serves.
@@ -224,69 +212,96 @@ __device__ __forceinline__ unsigned int share_of(unsigned long long sum, unsigne
   return (sum >> 32) == 0 ? (unsigned int)sum / parts : (unsigned int)(sum / parts);
 }
 
-__device__ __forceinline__ SplitSteps split_steps(const AttendArgs& a, const Request& head) {
-  unsigned long long few = 0, tiles = 0, tile_steps = 0;
-  bool large = false;
-  for (unsigned int r0 = 0; r0 < a.requests; r0 += kWave) {
-    const Request q = r0 == 0 ? head : load_request(a, r0 + __lane_id());
-    const int kind = kind_of(a, q);
-    if (a.few_rows != 0)
-      few += lane_value(wave_scan(kind == 1 ? steps_of(q.ctx, kFewRound) : 0u), 63);
-    if (a.tiles_too != 0) {
-      const unsigned int t = kind == 2 ? tiles_of(a, q.n) : 0u;
-      const unsigned long long all =
-          (unsigned long long)t * steps_of(q.ctx - min(q.ctx, q.n) / 2, kTileTokens);
-      large |= __ballot(all > kMostSteps) != 0;
-      tiles += lane_value(wave_scan(t), 63);
-      tile_steps += lane_value(wave_scan((unsigned int)min(all, (unsigned long long)kMostSteps)), 63);
-    }
+// The launch's work, which every workgroup finds its own item of by itself. Requests lie one in a
+// lane, 64 at a time (`first`: the first 64, which most launches end with), each with its tiles
+// (streaming: one) of `steps` steps of kStep tokens; a request of more than `cap` steps is cut into
+// splits of at most that. cap is the even share of all tiles' steps over the workgroups to split
+// for: on the streaming path few_target, for tiles half to all of their slots, the less the more
+// tiles there are anyhow: cut requests have at least two splits, so that sum of tiles * ceil(steps
+// / cap) over them is at most (all steps / cap + tiles) and at most twice (all steps / cap), both
+// within the slots.
+template <bool kTiles>
+struct Work {
+  static constexpr unsigned int kStep = kTiles ? kTileTokens : kWaves * kFewStep;
+  const AttendArgs& a;
+  Request first;
+  unsigned int cap;  // steps of a split, at most; 0: nothing is cut
+
+  __device__ __forceinline__ unsigned int tiles(const Request& q) const {
+    return kTiles ? tiles_of(a, q.n) : q.n != 0 ? 1u : 0u;
   }
-  few *= a.kv_heads;
-  tiles *= a.kv_heads;
-  tile_steps *= a.kv_heads;
-  SplitSteps s;
-  s.few = max(1u, share_of(few, a.few_target));
-  s.tiles = tiles >= a.tile_target || large ? 0u
-                                            : max(kLeastTileSteps, share_of(tile_steps, a.tile_target));
-  return s;
-}
+  __device__ __forceinline__ unsigned int splits(unsigned int tokens) const {
+    return cap == 0 ? 1u : max(1u, steps_of(steps_of(tokens, kStep), cap));
+  }
+  __device__ __forceinline__ Request requests(unsigned int r0) const {
+    return r0 == 0 ? first : load_request(a, r0 + __lane_id());
+  }
 
-__device__ __forceinline__ unsigned int few_splits(unsigned int ctx, unsigned int steps) {
-  return max(1u, steps_of(steps_of(ctx, kFewRound), steps));
-}
-__device__ __forceinline__ unsigned int tile_splits(unsigned int ctx, unsigned int steps) {
-  return steps == 0 ? 1u : max(1u, steps_of(steps_of(ctx, kTileTokens), steps));
-}
+  __device__ __forceinline__ explicit Work(const AttendArgs& args)
+      : a(args), first(load_request(args, __lane_id())), cap(0) {
+    if (kTiles && a.requests > 1 && a.requests <= kWave) sort();
+    unsigned long long steps = 0, all = 0;
+    bool large = false;
+    for (unsigned int r0 = 0; r0 < a.requests; r0 += kWave) {
+      const Request q = requests(r0);
+      const unsigned int t = tiles(q);
+      const unsigned long long own = (unsigned long long)t * steps_of(q.ctx, kStep);
+      large |= __ballot(own > kMostSteps) != 0;
+      all += lane_value(wave_scan(t), 63);
+      steps += lane_value(wave_scan((unsigned int)min(own, (unsigned long long)kMostSteps)), 63);
+    }
+    const unsigned long long groups = all * a.kv_heads;
+    const unsigned int parts =
+        kTiles ? 4 * a.tile_target - (unsigned int)min(groups, 2ull * a.tile_target) : a.few_target;
+    if (!large) cap = max(kTiles ? kLeastTileSteps : 1u, share_of(steps * a.kv_heads, parts));
+  }
 
-// The request that item `item` belongs to, request r having count(r) of them; false past the
-// last one. All wave-uniform.
-struct Place {
-  Request q;
-  unsigned int r, index;  // index within the request
+  // The lanes' requests with the longest contexts first.
+  __device__ __forceinline__ void sort() {
+    const unsigned int lane = __lane_id();
+    const unsigned int key = min(first.n != 0 ? steps_of(first.ctx, kStep) + 1 : 0u, kMostSteps) << 6 | (63 - lane);
+    unsigned int rank = 0;
+    for (unsigned int j = 0; j < a.requests; ++j) rank += lane_value(key, (int)j) > key ? 1u : 0u;
+    const int to = 4 * (int)(lane < a.requests ? rank : lane);
+    first.r = (unsigned int)__builtin_amdgcn_ds_permute(to, (int)first.r);
+    first.start = (unsigned int)__builtin_amdgcn_ds_permute(to, (int)first.start);
+    first.n = (unsigned int)__builtin_amdgcn_ds_permute(to, (int)first.n);
+    first.ctx = (unsigned int)__builtin_amdgcn_ds_permute(to, (int)first.ctx);
+    first.bad = __builtin_amdgcn_ds_permute(to, first.bad ? 1 : 0) != 0;
+  }
+
+  // Item `item`: its request, its index among the request's items (splits of one tile beside each
+  // other) and, where the request is cut (streaming: always), among those that have a slot; past
+  // the last one, false and the slot that nobody else has. All wave-uniform.
+  __device__ __forceinline__ bool find(unsigned int item, Request& q, unsigned int& index,
+                                       unsigned int& slot) const {
+    unsigned long long before = 0, slots = 0;
+    for (unsigned int r0 = 0; r0 < a.requests; r0 += kWave) {
+      const Request l = requests(r0);
+      const unsigned int parts = splits(l.ctx), own = tiles(l) * parts, sum = wave_scan(own);
+      const unsigned int slot_own = !kTiles || parts > 1 ? own : 0u, slot_sum = wave_scan(slot_own);
+      const unsigned int all = lane_value(sum, 63);
+      if (item < before + all) {
+        const unsigned int in = item - (unsigned int)before;
+        const int at = __ffsll((long long)__ballot(sum > in)) - 1;
+        index = in - lane_value(sum - own, at);
+        q.r = lane_value(l.r, at);
+        q.start = lane_value(l.start, at);
+        q.n = lane_value(l.n, at);
+        q.ctx = lane_value(l.ctx, at);
+        q.bad = lane_value(l.bad ? 1u : 0u, at) != 0;
+        slot = lane_value(slot_own, at) == 0
+                   ? ~0u
+                   : (unsigned int)slots + lane_value(slot_sum - slot_own, at) + index;
+        return true;
+      }
+      before += all;
+      slots += lane_value(slot_sum, 63);
+    }
+    slot = (unsigned int)(slots + (item - before));
+    return false;
+  }
 };
-
-template <typename Count>
-__device__ __forceinline__ bool find_item(const AttendArgs& a, const Request& head,
-                                          unsigned int item, Count count, Place& p) {
-  unsigned long long before = 0;
-  for (unsigned int r0 = 0; r0 < a.requests; r0 += kWave) {
-    const Request q = r0 == 0 ? head : load_request(a, r0 + __lane_id());
-    const unsigned int own = count(q), sum = wave_scan(own), all = lane_value(sum, 63);
-    if (item < before + all) {
-      const unsigned int in = item - (unsigned int)before;
-      const int at = __ffsll((long long)__ballot(sum > in)) - 1;
-      p.r = r0 + (unsigned int)at;
-      p.index = in - lane_value(sum - own, at);
-      p.q.start = lane_value(q.start, at);
-      p.q.n = lane_value(q.n, at);
-      p.q.ctx = lane_value(q.ctx, at);
-      p.q.bad = lane_value(q.bad ? 1u : 0u, at) != 0;
-      return true;
-    }
-    before += all;
-  }
-  return false;
-}
 
 // Row of K and V that token t of a request has: its place in the layer through the block table
 // (bad: the table names no block of the layer there; block 0 is read instead), or its packed row.
@@ -386,29 +401,25 @@ __device__ __forceinline__ void slow_row(const AttendArgs& a, const int* table, 
 
 // Where a row's result goes: the output (of one split), or its place among the partials, a
 // slot's rows as (m, l) pairs and then their D sums.
-template <int D>
-__device__ __forceinline__ float* slot_ml(const AttendArgs& a, bool few, unsigned int slot) {
-  constexpr unsigned int kFew = kFewRows * (D + 2), kTile = kTileRows * (D + 2);
-  return few ? a.partial + (unsigned long long)a.tile_slots * kTile + (unsigned long long)slot * kFew
-             : a.partial + (unsigned long long)slot * kTile;
+template <int D, int kRows>
+__device__ __forceinline__ float* slot_ml(const AttendArgs& a, unsigned int slot) {
+  return a.partial + (unsigned long long)slot * (kRows * (D + 2));
 }
-template <int D>
-__device__ __forceinline__ float* slot_acc(const AttendArgs& a, bool few, unsigned int slot) {
-  return slot_ml<D>(a, few, slot) + 2 * (few ? kFewRows : kTileRows);
+template <int D, int kRows>
+__device__ __forceinline__ float* slot_acc(const AttendArgs& a, unsigned int slot) {
+  return slot_ml<D, kRows>(a, slot) + 2 * kRows;
 }
-
-__device__ __forceinline__ bool finite(float v) { return fabsf(v) < INFINITY; }
 
 // A row (m, l, sums) by a wave whose lanes hold D / 64 sums each, from slow_row.
-template <typename E, int D>
-__device__ __forceinline__ void store_slow(const AttendArgs& a, bool split, bool few,
+template <typename E, int D, int kRows>
+__device__ __forceinline__ void store_slow(const AttendArgs& a, bool split,
                                            unsigned int slot, unsigned int slot_row,
                                            unsigned long long out_row, bool none, float m, float l,
                                            const float (&acc)[D / 64]) {
   const unsigned int lane = __lane_id();
   if (split) {
-    float* ml = slot_ml<D>(a, few, slot) + 2 * slot_row;
-    float* dst = slot_acc<D>(a, few, slot) + slot_row * D;
+    float* ml = slot_ml<D, kRows>(a, slot) + 2 * slot_row;
+    float* dst = slot_acc<D, kRows>(a, slot) + slot_row * D;
     if (lane == 0) {
       ml[0] = m;
       ml[1] = l;
@@ -424,17 +435,18 @@ __device__ __forceinline__ void store_slow(const AttendArgs& a, bool split, bool
   }
 }
 
-// A slot's job, by one thread of its workgroup. (Row ranges that overlap each other can ask for
-// more slots than there are: their rows stay as they were.)
-__device__ __forceinline__ void store_job(const AttendArgs& a, bool few, unsigned int slot, Job j) {
-  const unsigned int slots = few ? a.few_slots : a.tile_slots;
+// A slot's job, by one thread of its workgroup; `slot` counts for one KV head. (Row ranges that
+// overlap each other can ask for more slots than there are: their rows stay as they were.)
+__device__ __forceinline__ void store_job(const AttendArgs& a, unsigned int slot, unsigned int head,
+                                          Job j) {
+  const unsigned int slots = a.slots / a.kv_heads;
   if (threadIdx.x != 0 || slot >= slots) return;
-  if (j.splits != 0 && slot + (unsigned long long)(j.splits - 1) * a.kv_heads >= slots) j.splits = 0;
-  a.jobs[(few ? a.tile_slots : 0u) + slot] = j;
+  if (slot + (unsigned long long)j.splits > slots) j.splits = 0;
+  a.jobs[slot * a.kv_heads + head] = j;
 }
 
 // ---------------------------------------------------------------------------
-// 128 rows by 64 tokens a step
+// 256 rows by 64 tokens a step
 
 // Lane l of a wave has row l % 32 of the wave's 32 and, of every 16 tokens, those with
 // (token / 4) % 2 == l / 32 (the 32x32 matrix instruction's output rows). K lies in LDS as rows
@@ -443,42 +455,43 @@ __device__ __forceinline__ void store_job(const AttendArgs& a, bool few, unsigne
 // rows; V's 64-byte quarters q at q ^ (t % 4), read transposed 8 bytes a lane, 4 tokens by 32 dims
 // per half wave.
 template <typename E, int D, bool kPaged, bool kRuns>
-__device__ __forceinline__ void tile_path(const AttendArgs& a, const Request& first_requests,
-                                          const SplitSteps& steps, unsigned int block,
-                                          unsigned char* s0, unsigned char* s1) {
+__device__ __forceinline__ void tile_path(const AttendArgs& a, unsigned int block,
+                                          unsigned char* s0, unsigned char* s1,
+                                          unsigned char* s2) {
   typedef typename Elem<E>::x8 x8;
   constexpr int kRowBytes = 2 * D, kPieces = kRowBytes / 16;  // pieces of a row
-  constexpr int kRowsPerLoad = kWave / kPieces, kLoads = 16 / kRowsPerLoad;
+  constexpr int kRowsPerLoad = kWave / kPieces, kLoads = 8 / kRowsPerLoad;
   constexpr int kTileBytes = kTileTokens * kRowBytes;
   constexpr int kSlabs = D / 16, kDimTiles = D / 32;
 
   const unsigned int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
   const unsigned int half = lane / 32, col = lane % 32;
-  const unsigned int head = block % a.kv_heads, item = block / a.kv_heads, slot = block;
-  Place p;
-  if (!find_item(a, first_requests, item, [&](const Request& q) -> unsigned int {
-        return kind_of(a, q) == 2 ? tiles_of(a, q.n) * tile_splits(q.ctx, steps.tiles) : 0u;
-      }, p)) {
-    store_job(a, false, slot, Job{});
+  const unsigned int head = block % a.kv_heads, item = block / a.kv_heads;
+  const Work<true> work(a);
+  Request request;
+  unsigned int index, slot;
+  if (!work.find(item, request, index, slot)) {
+    store_job(a, slot, head, Job{});
     return;
   }
-  const unsigned int all = tile_splits(p.q.ctx, steps.tiles);
+  slot = slot == ~0u ? slot : slot * a.kv_heads + head;
   // the tiles with the longest contexts first
-  const unsigned int tile = tiles_of(a, p.q.n) - 1 - p.index / all, split = p.index % all;
-  const unsigned int rows = p.q.n * a.group;
+  const unsigned int most = work.splits(request.ctx);
+  const unsigned int tile = tiles_of(a, request.n) - 1 - index / most, split = index % most;
+  const unsigned int rows = request.n * a.group;
   const unsigned int m0 = tile * kTileRows;
   // last visible token of a row (negative: none)
-  const int shift = (int)p.q.ctx - (int)p.q.n;
+  const int shift = (int)request.ctx - (int)request.n;
   const int last_of_tile = shift + (int)((min(rows, m0 + kTileRows) - 1) / a.group);
   const unsigned int seen = last_of_tile < 0 ? 0u : (unsigned int)last_of_tile + 1;
-  const unsigned int splits = tile_splits(seen, steps.tiles);  // of this tile
-  store_job(a, false, slot,
-            Job{p.q.start, m0, shift, (unsigned short)min(rows - m0, (unsigned int)kTileRows),
+  const unsigned int splits = most == 1 ? 1u : work.splits(seen);  // of this tile
+  if (most > 1)
+    store_job(a, slot / a.kv_heads, head,
+            Job{request.start, m0, shift, (unsigned short)min(rows - m0, (unsigned int)kTileRows),
                 (unsigned short)(split == 0 && splits > 1 ? splits : 0u)});
   if (split >= splits) return;
-  const unsigned int t_begin = split * steps.tiles * kTileTokens;
-  const unsigned int t_end =
-      splits == 1 ? seen : min(seen, t_begin + steps.tiles * kTileTokens);
+  const unsigned int t_begin = split * work.cap * kTileTokens;
+  const unsigned int t_end = splits == 1 ? seen : min(seen, t_begin + work.cap * kTileTokens);
   const unsigned int mw = m0 + wave * 32, m = mw + col;
   const bool valid = m < rows;
   const unsigned int token = valid ? m / a.group : 0u;
@@ -488,68 +501,88 @@ __device__ __forceinline__ void tile_path(const AttendArgs& a, const Request& fi
   const int first_limit = shift + (int)(mw / a.group);
   const int last_limit = mw < rows ? shift + (int)((min(rows, mw + 32) - 1) / a.group) : -1;
 
-  const int* table = kPaged ? a.tables + p.r * a.table_stride : nullptr;
+  const int* table = kPaged ? a.tables + request.r * a.table_stride : nullptr;
   const unsigned char* kb = a.k + head * a.k_head;
   const unsigned char* vb = a.v + head * a.v_head;
-  bool bad = p.q.bad;
+  bool bad = request.bad;
 
   // the row's query as the second operand: dims 16 s + 8 half .. + 7 of slab s (a lane without a
   // row has the request's first: a column of the products that nobody reads)
   x8 q[kSlabs];
-  const unsigned char* q_row = a.q + (unsigned long long)(p.q.start + token) * a.q_row +
+  const unsigned char* q_row = a.q + (unsigned long long)(request.start + token) * a.q_row +
                                (unsigned long long)q_head * a.q_head;
 #pragma unroll
   for (int s = 0; s < kSlabs; ++s) {
     q[s] = *reinterpret_cast<const x8*>(q_row + 32 * s + 16 * half);
   }
 
-  // this wave's share of a tile: 16 tokens of K and V. Where they follow each other in memory
-  // (prompts; layers whose blocks are whole groups of 16 tokens) the wave forms their address once,
+  // This wave's share of a tile's loads: 8 tokens of K and V. Where they follow each other in memory
+  // (prompts; layers whose blocks are whole groups of 8 tokens) the wave forms their address once,
   // on the scalar unit, and a lane's offsets from it never change.
   const unsigned int piece = lane % kPieces, sub = lane / kPieces;
   unsigned int k_off[kLoads], v_off[kLoads];
 #pragma unroll
   for (int i = 0; i < kLoads; ++i) {
-    const unsigned int in = i * kRowsPerLoad + sub;  // the token's place among the wave's 16
-    const unsigned int k_piece = piece ^ (D == 128 ? in : (in >> 1) & 7);
-    const unsigned int v_piece = piece ^ (D == 128 ? (in & 3) << 2 : ((in >> 1) & 1) << 2);
+    const unsigned int in = i * kRowsPerLoad + sub;  // the token's place among the wave's 8
+    const unsigned int at = 8 * (wave % 2) + in;     // and among 16
+    const unsigned int k_piece = piece ^ (D == 128 ? at : (at >> 1) & 7);
+    const unsigned int v_piece = piece ^ (D == 128 ? (at & 3) << 2 : ((at >> 1) & 1) << 2);
     k_off[i] = (kRuns ? in * (unsigned int)a.k_row : 0u) + 16 * k_piece;
     v_off[i] = (kRuns ? in * (unsigned int)a.v_row : 0u) + 16 * v_piece;
   }
   constexpr int kIds = kRuns ? 1 : kLoads;
-  int ids[kIds];
+  const unsigned int first_at = wave * 8 * kRowBytes;
   auto token_of = [&](unsigned int base, int i) {
-    return min(base + wave * 16 + (kRuns ? 0 : i * kRowsPerLoad + sub), t_end - 1);
+    return min(base + wave * 8 + (kRuns ? 0 : i * kRowsPerLoad + sub), t_end - 1);
   };
+  int ids[kIds];               // of the tile whose K is loaded next
+  unsigned int next_row[kIds], row_of[kIds];  // of that tile, and of the one whose V is
   auto fetch_ids = [&](unsigned int base) {
 #pragma unroll
     for (int i = 0; i < kIds; ++i) ids[i] = block_id<kPaged>(a, table, token_of(base, i));
   };
-  auto issue = [&](unsigned int base, unsigned char* bk, unsigned char* bv) {
-    const unsigned int at = wave * 16 * kRowBytes;
-    if constexpr (kRuns) {
-      // tokens past the end are outside the buffers
-      const unsigned int first = base + wave * 16, count = min(t_end - min(first, t_end), 16u);
-      const unsigned int row = uniform(kv_row<kPaged>(a, table, p.q.start, token_of(base, 0), ids[0], bad));
-      // (sizes moved to scalars: with one in a vector register each load became a loop over lanes)
-      const Buffer kr = buffer_of(
-          kb + row * a.k_row,
-          uniform(count == 0 ? 0u : (count - 1) * (unsigned int)a.k_row + kRowBytes));
-      const Buffer vr = buffer_of(
-          vb + row * a.v_row,
-          uniform(count == 0 ? 0u : (count - 1) * (unsigned int)a.v_row + kRowBytes));
+  auto find_rows = [&](unsigned int base) {
 #pragma unroll
-      for (int i = 0; i < kLoads; ++i) {
-        load_to_lds(kr, k_off[i], bk + at + i * kRowsPerLoad * kRowBytes);
-        load_to_lds(vr, v_off[i], bv + at + i * kRowsPerLoad * kRowBytes);
-      }
+    for (int i = 0; i < kIds; ++i) {
+      next_row[i] = kv_row<kPaged>(a, table, request.start, token_of(base, i), ids[i], bad);
+      if (kRuns) next_row[i] = uniform(next_row[i]);
+    }
+  };
+  // Sizes of the buffers of this wave's rows (kRuns): whole tiles lie inside the tensor, the last one
+  // ends with the tokens, and one behind it has none.
+  const unsigned int last_base = t_end == 0 ? 0u : (t_end - 1 - t_begin) / kTileTokens * kTileTokens + t_begin;
+  const int left = (int)t_end - (int)(last_base + wave * 8);
+  const unsigned int last_rows = uniform((unsigned int)max(min(left, 8), 0));
+  const unsigned int k_last = last_rows == 0 ? 0u : (last_rows - 1) * (unsigned int)a.k_row + kRowBytes;
+  const unsigned int v_last = last_rows == 0 ? 0u : (last_rows - 1) * (unsigned int)a.v_row + kRowBytes;
+  auto load_plane = [&](unsigned int base, const unsigned char* src, unsigned long long stride,
+                        unsigned int last_bytes, const unsigned int (&row)[kIds],
+                        const unsigned int (&off)[kLoads], unsigned char* dst) {
+    if constexpr (kRuns) {
+      const unsigned int bytes = base < last_base ? 0x7FFFFFFFu : base == last_base ? last_bytes : 0u;
+      const Buffer buffer = buffer_of(src + row[0] * stride, bytes);
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i)
+        load_to_lds(buffer, off[i], dst + first_at + i * kRowsPerLoad * kRowBytes);
     } else {
 #pragma unroll
-      for (int i = 0; i < kLoads; ++i) {
-        const unsigned int row = kv_row<kPaged>(a, table, p.q.start, token_of(base, i), ids[i], bad);
-        load_to_lds(kb + row * a.k_row + k_off[i], bk + at + i * kRowsPerLoad * kRowBytes);
-        load_to_lds(vb + row * a.v_row + v_off[i], bv + at + i * kRowsPerLoad * kRowBytes);
-      }
+      for (int i = 0; i < kLoads; ++i)
+        load_to_lds(src + row[i] * stride + off[i], dst + first_at + i * kRowsPerLoad * kRowBytes);
+    }
+  };
+  // The loads of a round in three steps: K of the tile behind `base`, V of the tile there. (Tokens
+  // past the end are outside the buffers, or the last one again.)
+  constexpr int kInFlight = 2 * kLoads + (kPaged ? kIds : 0);  // a round's
+  auto load_step = [&](int j, unsigned int base, unsigned char* to) {
+    if (j == 0) {
+      find_rows(base + kTileTokens);
+      fetch_ids(base + 2 * kTileTokens);  // (before the loads, which the next round then does not wait for)
+    } else if (j == 1) {
+      load_plane(base + kTileTokens, kb, a.k_row, k_last, next_row, k_off, to);
+    } else if (j == 2) {
+      load_plane(base, vb, a.v_row, v_last, row_of, v_off, to + kTileBytes);
+#pragma unroll
+      for (int i = 0; i < kIds; ++i) row_of[i] = next_row[i];
     }
   };
 
@@ -559,6 +592,9 @@ __device__ __forceinline__ void tile_path(const AttendArgs& a, const Request& fi
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
   float m_ref = kNoMax, l_run = 0.f;
+  f32x16 s[2];  // scores of a tile
+  x8 w[4];      // its weights,
+  f32x16 late;  // and the exponents of those that its products of O begin with computing
 
   // K operand: row col (+ 32), piece 2 s + half; V operand: tokens 4 half + i / 4 (i = lane % 16) of
   // 16, dims 16 (lane / 16 % 2) + 4 (i % 4) of 32
@@ -567,19 +603,83 @@ __device__ __forceinline__ void tile_path(const AttendArgs& a, const Request& fi
   const unsigned int v_x = D == 128 ? v_tok & 3 : (v_tok >> 1) & 1;
   const unsigned int v_at = v_tok * kRowBytes + 32 * ((lane / 16) % 2) + 8 * (lane % 4);
 
-  auto step = [&](unsigned int base, const unsigned char* bk, const unsigned char* bv) {
-    f32x16 s[2];
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) s[t][i] = 0.f;
-#pragma unroll
-      for (int c = 0; c < kSlabs; ++c) {
-        const x8 kf = *reinterpret_cast<const x8*>(bk + k_at + 32 * t * kRowBytes +
-                                                   16 * ((2 * c + half) ^ k_x));
-        s[t] = Elem<E>::mma32(kf, q[c], s[t]);
-      }
+  // The weights of the second half of a tile's tokens: value j of 16.
+  float late_sum = 0.f, pair = 0.f;
+  auto late_weight = [&](int j) {
+    const float e = __builtin_amdgcn_exp2f(late[j]);
+    late_sum += e;
+    if (j % 2 == 0) {
+      pair = e;
+    } else {
+      u32x4 x = __builtin_bit_cast(u32x4, w[2 + j / 8]);
+      x[j % 8 / 2] = pack2<E>(pair, e);
+      w[2 + j / 8] = __builtin_bit_cast(x8, x);
     }
+  };
+  // Products of a phase, each with its operand read from LDS: first those of S (16 dims, 32 tokens,
+  // the halves in turns), with the late weights of the tile before between them, then those of its
+  // O (16 tokens, 32 dims); each operand is read kAhead products before its own, in this order (left
+  // to itself the compiler waits for each read just issued).
+  constexpr int kOuts = 4 * kDimTiles, kScores = 2 * kSlabs, kAhead = 4;
+  auto operand = [&](int i, const unsigned char* bv, const unsigned char* bk) {
+    if (i < kScores)
+      return *reinterpret_cast<const x8*>(bk + k_at + 32 * (i % 2) * kRowBytes +
+                                          16 * ((2 * (i / 2) + half) ^ k_x));
+    i -= kScores;
+    const unsigned char* src =
+        bv + v_at + 16 * (i / kDimTiles) * kRowBytes + 64 * ((i % kDimTiles) ^ v_x);
+    const u32x2 lo = read_transposed(src), hi = read_transposed(src + 8 * kRowBytes);
+    return __builtin_bit_cast(x8, u32x4{lo.x, lo.y, hi.x, hi.y});
+  };
+  auto product = [&](int i, x8 f) {
+    if (i < kScores) {
+      f32x16 zero;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) zero[j] = 0.f;
+      s[i % 2] = Elem<E>::mma32(f, q[i / 2], i < 2 ? zero : s[i % 2]);
+    } else {
+      i -= kScores;
+      o[i % kDimTiles] = Elem<E>::mma32(f, w[i / kDimTiles], o[i % kDimTiles]);
+    }
+  };
+  auto products = [&](auto first, auto count, const unsigned char* from, auto between) {
+    constexpr int kFirst = decltype(first)::value, kCount = decltype(count)::value;
+    x8 f[kCount];
+    __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) f[i] = operand(kFirst + i, from + kTileBytes, from);
+#pragma unroll
+    for (int i = 0; i < kCount; ++i) {
+      __builtin_amdgcn_sched_barrier(0);
+      if (i + kAhead < kCount) f[i + kAhead] = operand(kFirst + i + kAhead, from + kTileBytes, from);
+      product(kFirst + i, f[i]);
+      between(i);
+    }
+    __builtin_amdgcn_s_setprio(0);
+  };
+  auto scores = [&](const unsigned char* from) {
+    products(std::integral_constant<int, 0>(), std::integral_constant<int, kScores>(), from, [](int) {});
+  };
+  auto both = [&](const unsigned char* from) {
+    products(std::integral_constant<int, 0>(), std::integral_constant<int, kScores + kOuts>(), from,
+             [&](int i) {
+               if (i >= kScores) return;
+#pragma unroll
+               for (int j = 0; j < 16 / kScores; ++j) late_weight(16 / kScores * i + j);
+             });
+    l_run += late_sum;
+    late_sum = 0.f;
+  };
+  auto outputs = [&](const unsigned char* from) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) late_weight(j);
+    products(std::integral_constant<int, kScores>(), std::integral_constant<int, kOuts>(), from,
+             [](int) {});
+    l_run += late_sum;
+    late_sum = 0.f;
+  };
+  // (the loads are spread over it: each takes its time to be issued)
+  auto softmax = [&](unsigned int base, auto between) {
     if ((int)base + kTileTokens - 1 > first_limit) {
       const int left = limit - (int)base - 4 * (int)half;
 #pragma unroll
@@ -588,6 +688,7 @@ __device__ __forceinline__ void tile_path(const AttendArgs& a, const Request& fi
         for (int i = 0; i < 16; ++i)
           s[t][i] = 32 * t + 8 * (i / 4) + i % 4 <= left ? s[t][i] : -INFINITY;
     }
+    between(0);
     float top = s[0][0];
 #pragma unroll
     for (int t = 0; t < 2; ++t)
@@ -595,9 +696,9 @@ __device__ __forceinline__ void tile_path(const AttendArgs& a, const Request& fi
       for (int i = 0; i < 16; ++i) top = fmaxf(top, s[t][i]);
     {
       const unsigned int u = __builtin_bit_cast(unsigned int, top);
-      const auto w = __builtin_amdgcn_permlane32_swap(u, u, false, false);
-      top = fmaxf(__builtin_bit_cast(float, (unsigned int)w[0]),
-                  __builtin_bit_cast(float, (unsigned int)w[1]));
+      const auto x = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+      top = fmaxf(__builtin_bit_cast(float, (unsigned int)x[0]),
+                  __builtin_bit_cast(float, (unsigned int)x[1]));
     }
     top *= a.scale_log2;
     if (__ballot(top > m_ref + kSlack) != 0) {
@@ -609,50 +710,123 @@ __device__ __forceinline__ void tile_path(const AttendArgs& a, const Request& fi
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[d][i] *= alpha;
     }
-    float sum = 0.f;
-    x8 w[4];
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      float e[8];
+    for (int i = 0; i < 16; ++i) late[i] = fmaf(s[1][i], a.scale_log2, -m_ref);
+    __builtin_amdgcn_sched_barrier(0);
+    between(1);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      float e[8], sum = 0.f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        e[i] = __builtin_amdgcn_exp2f(fmaf(s[c / 2][8 * (c % 2) + i], a.scale_log2, -m_ref));
+        e[i] = __builtin_amdgcn_exp2f(fmaf(s[0][8 * c + i], a.scale_log2, -m_ref));
         sum += e[i];
       }
+      l_run += sum;
       w[c] = pack8<E>(e);
-    }
-    l_run += sum;
-#pragma unroll
-    for (int c = 0; c < 4; ++c)
-#pragma unroll
-      for (int d = 0; d < kDimTiles; ++d) {
-        const unsigned char* src = bv + v_at + 16 * c * kRowBytes + 64 * (d ^ v_x);
-        const u32x2 lo = read_transposed(src), hi = read_transposed(src + 8 * kRowBytes);
-        o[d] = Elem<E>::mma32(__builtin_bit_cast(x8, u32x4{lo.x, lo.y, hi.x, hi.y}), w[c], o[d]);
+      if (c == 0) {
+        __builtin_amdgcn_sched_barrier(0);
+        between(2);
+        __builtin_amdgcn_sched_barrier(0);
       }
+    }
   };
 
-  if (t_begin < t_end) {
-    fetch_ids(t_begin);
-    issue(t_begin, s0, s0 + kTileBytes);
-    if (t_begin + kTileTokens < t_end) fetch_ids(t_begin + kTileTokens);
-    unsigned int base = t_begin;
-    auto turn = [&](unsigned char* now, unsigned char* next) {
-      // this tile's loads have landed, and every wave is done with the other buffer
-      wait_loads<0>();
-      __syncthreads();
-      if (base + kTileTokens < t_end) {
-        issue(base + kTileTokens, next, next + kTileBytes);
-        if (base + 2 * kTileTokens < t_end) fetch_ids(base + 2 * kTileTokens);
-      }
-      if ((int)base <= last_limit) step(base, now, now + kTileBytes);
-      base += kTileTokens;
+  const unsigned int count = (t_end - min(t_begin, t_end) + kTileTokens - 1) / kTileTokens;
+  if (count != 0) {
+    const unsigned int base_end = t_begin + count * kTileTokens;
+    // Round i in two phases, a barrier behind each; waves 0-3 (one on each SIMD) do their products
+    // in the first, O of tile i - 1 and S of tile i, and the softmax of tile i in the second; waves
+    // 4-7 are a phase behind, so that the matrix unit of every SIMD has one wave's products while
+    // the vector unit has the other's softmax. Tile i's K lies in buffer i % 3 and its V in buffer
+    // (i + 1) % 3, so that a round reads one buffer; K of tile i + 2 and V of tile i + 1 are loaded in
+    // round i (with the softmax) into the one that round i - 1 read, and have landed at the end of
+    // the next round.
+    auto load = [&](unsigned int base, unsigned char* to) {
+#pragma unroll
+      for (int j = 0; j < 3; ++j) load_step(j, base, to);
     };
-    while (base < t_end) {
-      turn(s0, s1);
-      if (base >= t_end) break;
-      turn(s1, s0);
+    auto phase_end = [&]() {
+      __builtin_amdgcn_sched_barrier(0);
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    // rounds 1 .. count - 1: the round's tile, the buffer it reads and the one it loads
+    auto rounds = [&](auto one) {
+      for (unsigned int base = t_begin + kTileTokens; base < base_end;) {
+        one(base, s1, s0);
+        base += kTileTokens;
+        if (base >= base_end) break;
+        one(base, s2, s1);
+        base += kTileTokens;
+        if (base >= base_end) break;
+        one(base, s0, s2);
+        base += kTileTokens;
+      }
+    };
+    const unsigned char* const last = count % 3 == 0 ? s0 : count % 3 == 1 ? s1 : s2;
+    auto with_loads = [&](unsigned int base, unsigned char* to) {
+      return [&, base, to](int j) { load_step(j, base, to); };
+    };
+    fetch_ids(t_begin);
+    find_rows(t_begin);
+    load_plane(t_begin, kb, a.k_row, k_last, next_row, k_off, s0);
+#pragma unroll
+    for (int i = 0; i < kIds; ++i) row_of[i] = next_row[i];
+    fetch_ids(t_begin + kTileTokens);
+    load(t_begin, s1);
+    wait_loads<kInFlight>();
+    phase_end();
+    if (mw >= rows) {
+      // a wave without rows
+      auto idle = [&](unsigned int base, const unsigned char*, unsigned char* to) {
+        load(base + kTileTokens, to);
+        phase_end();
+        wait_loads<kInFlight>();
+        phase_end();
+      };
+      idle(t_begin, s0, s2);
+      rounds(idle);
+      phase_end();
+      phase_end();
+    } else if (wave < 4) {
+      scores(s0);
+      phase_end();
+      softmax(t_begin, with_loads(t_begin + kTileTokens, s2));
+      wait_loads<kInFlight>();
+      phase_end();
+      rounds([&](unsigned int base, const unsigned char* from, unsigned char* to) {
+        both(from);
+        phase_end();
+        softmax(base, with_loads(base + kTileTokens, to));
+        wait_loads<kInFlight>();
+        phase_end();
+      });
+      outputs(last);
+      phase_end();
+      phase_end();
+    } else {
+      load(t_begin + kTileTokens, s2);
+      phase_end();
+      scores(s0);
+      wait_loads<kInFlight>();
+      phase_end();
+      rounds([&](unsigned int base, const unsigned char* from, unsigned char* to) {
+        softmax(base - kTileTokens, with_loads(base + kTileTokens, to));
+        phase_end();
+        both(from);
+        wait_loads<kInFlight>();
+        phase_end();
+      });
+      softmax(base_end - kTileTokens, [](int) {});
+      phase_end();
+      outputs(last);
+      phase_end();
     }
+    wait_loads<0>();
   }
 
   bad = __syncthreads_or(bad) != 0;
@@ -664,12 +838,12 @@ __device__ __forceinline__ void tile_path(const AttendArgs& a, const Request& fi
     for (int i = 0; i < 16; ++i) check = fmaf(o[d][i], 0.f, check);
   check += __shfl_xor(check, 32, 64);
   const bool again = valid && !bad && !(check == 0.f);
-  const unsigned long long out_row = (unsigned long long)(p.q.start + token) * a.q_heads + q_head;
+  const unsigned long long out_row = (unsigned long long)(request.start + token) * a.q_heads + q_head;
   if (bad) m_ref = l_run = NAN;
   if (valid && !again) {
     if (splits > 1) {
-      float* ml = slot_ml<D>(a, false, slot) + 2 * (m - m0);
-      float* dst = slot_acc<D>(a, false, slot) + (m - m0) * D;
+      float* ml = slot_ml<D, kTileRows>(a, slot) + 2 * (m - m0);
+      float* dst = slot_acc<D, kTileRows>(a, slot) + (m - m0) * D;
       if (half == 0) {
         ml[0] = m_ref;
         ml[1] = l_run;
@@ -703,12 +877,12 @@ __device__ __forceinline__ void tile_path(const AttendArgs& a, const Request& fi
     const unsigned int row_m = mw + at, tok = row_m / a.group, qh = head * a.group + row_m % a.group;
     const unsigned int own = (unsigned int)max(shift + (int)tok + 1, 0);  // tokens it sees
     float rm, rl, acc[D / 64];
-    slow_row<E, D, kPaged>(a, table, p.q.start,
-                           a.q + (unsigned long long)(p.q.start + tok) * a.q_row +
+    slow_row<E, D, kPaged>(a, table, request.start,
+                           a.q + (unsigned long long)(request.start + tok) * a.q_row +
                                (unsigned long long)qh * a.q_head,
                            head, t_begin, min(t_end, own), rm, rl, acc);
-    store_slow<E, D>(a, splits > 1, false, slot, row_m - m0,
-                     (unsigned long long)(p.q.start + tok) * a.q_heads + qh, own == 0, rm, rl, acc);
+    store_slow<E, D, kTileRows>(a, splits > 1, slot, row_m - m0,
+                     (unsigned long long)(request.start + tok) * a.q_heads + qh, own == 0, rm, rl, acc);
   }
 }
 
@@ -721,14 +895,14 @@ __device__ __forceinline__ void tile_path(const AttendArgs& a, const Request& fi
 // pieces of row t at piece ^ (t % 8), so that the 16 tokens of a transposed read spread over the
 // banks. The waves of a workgroup take turns at 32 tokens of a split and join their sums in LDS.
 template <typename E, int D>
-__device__ __forceinline__ void few_path(const AttendArgs& a, const Request& first_requests,
-                                         const SplitSteps& steps, unsigned int block,
-                                         unsigned char* s0, unsigned char* s1) {
+__device__ __forceinline__ void few_path(const AttendArgs& a, unsigned int block, unsigned char* s0,
+                                         unsigned char* s1) {
   typedef typename Elem<E>::x8 x8;
   constexpr int kRowBytes = 2 * D, kPieces = kRowBytes / 16;
   constexpr int kRowsPerLoad = kWave / kPieces, kLoads = kFewStep / kRowsPerLoad;
   constexpr int kStageBytes = kFewStep * kRowBytes;
   constexpr int kSlabs = D / 32, kDimTiles = D / 16;
+  constexpr unsigned int kRound = Work<false>::kStep;
   // the waves' sums, then their (m, l), once the stages are read
   float* const s_acc = reinterpret_cast<float*>(s0);
   float* const s_ml = reinterpret_cast<float*>(s1);
@@ -736,34 +910,36 @@ __device__ __forceinline__ void few_path(const AttendArgs& a, const Request& fir
 
   const unsigned int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
   const unsigned int col = lane % 16, grp = lane / 16;
-  const unsigned int head = block % a.kv_heads, item = block / a.kv_heads, slot = block;
-  Place p;
-  if (!find_item(a, first_requests, item, [&](const Request& q) -> unsigned int {
-        return kind_of(a, q) == 1 ? few_splits(q.ctx, steps.few) : 0u;
-      }, p)) {
-    store_job(a, true, slot, Job{});
+  const unsigned int head = block % a.kv_heads, item = block / a.kv_heads;
+  const Work<false> work(a);
+  Request request;
+  unsigned int split, slot;
+  if (!work.find(item, request, split, slot)) {
+    store_job(a, slot, head, Job{});
     return;
   }
-  const unsigned int splits = few_splits(p.q.ctx, steps.few), split = p.index;
-  store_job(a, true, slot,
-            Job{p.q.start, 0, (int)p.q.ctx - (int)p.q.n, (unsigned short)(p.q.n * a.group),
+  const unsigned int splits = work.splits(request.ctx);
+  store_job(a, slot, head,
+            Job{request.start, 0, (int)request.ctx - (int)request.n,
+                (unsigned short)(request.n * a.group),
                 (unsigned short)(split == 0 && splits > 1 ? splits : 0u)});
-  const unsigned int rows = p.q.n * a.group;
-  const unsigned int t_begin = split * steps.few * kFewRound;
-  const unsigned int t_end = min(p.q.ctx, t_begin + steps.few * kFewRound);
-  const int shift = (int)p.q.ctx - (int)p.q.n;
+  slot = slot * a.kv_heads + head;
+  const unsigned int rows = request.n * a.group;
+  const unsigned int t_begin = split * work.cap * kRound;
+  const unsigned int t_end = min(request.ctx, t_begin + work.cap * kRound);
+  const int shift = (int)request.ctx - (int)request.n;
   const bool valid = col < rows;
   const unsigned int token = valid ? col / a.group : 0u;
   const unsigned int q_head = head * a.group + (valid ? col - token * a.group : 0u);
   const int limit = valid ? shift + (int)token : -1;
 
-  const int* table = a.tables + p.r * a.table_stride;
+  const int* table = a.tables + request.r * a.table_stride;
   const unsigned char* kb = a.k + head * a.k_head;
   const unsigned char* vb = a.v + head * a.v_head;
-  bool bad = p.q.bad;
+  bool bad = request.bad;
 
   x8 q[kSlabs];
-  const unsigned char* q_row = a.q + (unsigned long long)(p.q.start + token) * a.q_row +
+  const unsigned char* q_row = a.q + (unsigned long long)(request.start + token) * a.q_row +
                                (unsigned long long)q_head * a.q_head;
 #pragma unroll
   for (int s = 0; s < kSlabs; ++s) {
@@ -855,21 +1031,21 @@ __device__ __forceinline__ void few_path(const AttendArgs& a, const Request& fir
   if (base < t_end) {
     Keys k0, k1;
     issue(base, block_id<true>(a, table, token_of(base)), k0, stage0);
-    int id = block_id<true>(a, table, token_of(base + kFewRound));
+    int id = block_id<true>(a, table, token_of(base + kRound));
     for (;;) {
       // the next step's loads go out (past the end: the last token again), then this step's
       // are waited for
-      issue(base + kFewRound, id, k1, stage1);
-      id = block_id<true>(a, table, token_of(base + 2 * kFewRound));
+      issue(base + kRound, id, k1, stage1);
+      id = block_id<true>(a, table, token_of(base + 2 * kRound));
       wait_loads<2 * kSlabs + kLoads + 1>();
       step(base, k0, stage0);
-      base += kFewRound;
+      base += kRound;
       if (base >= t_end) break;
-      issue(base + kFewRound, id, k0, stage0);
-      id = block_id<true>(a, table, token_of(base + 2 * kFewRound));
+      issue(base + kRound, id, k0, stage0);
+      id = block_id<true>(a, table, token_of(base + 2 * kRound));
       wait_loads<2 * kSlabs + kLoads + 1>();
       step(base, k1, stage1);
-      base += kFewRound;
+      base += kRound;
       if (base >= t_end) break;
     }
   }
@@ -910,12 +1086,12 @@ __device__ __forceinline__ void few_path(const AttendArgs& a, const Request& fir
   const bool again = in && !bad && !(check == 0.f);
   const unsigned int tok = in ? row_m / a.group : 0u;
   const unsigned int qh = head * a.group + (in ? row_m - tok * a.group : 0u);
-  const unsigned long long out_row = (unsigned long long)(p.q.start + tok) * a.q_heads + qh;
+  const unsigned long long out_row = (unsigned long long)(request.start + tok) * a.q_heads + qh;
   if (bad) big = l = NAN;
   if (in && !again) {
     if (splits > 1) {
-      float* ml = slot_ml<D>(a, true, slot) + 2 * row_m;
-      float* dst = slot_acc<D>(a, true, slot) + row_m * D + d0;
+      float* ml = slot_ml<D, kFewRows>(a, slot) + 2 * row_m;
+      float* dst = slot_acc<D, kFewRows>(a, slot) + row_m * D + d0;
       if (d0 == 0) {
         ml[0] = big;
         ml[1] = l;
@@ -940,49 +1116,35 @@ __device__ __forceinline__ void few_path(const AttendArgs& a, const Request& fir
     const unsigned int mm = 4 * wave + i, t = mm / a.group, h = head * a.group + mm % a.group;
     const unsigned int seen = (unsigned int)max(shift + (int)t + 1, 0);
     float rm, rl, ra[D / 64];
-    slow_row<E, D, true>(a, table, p.q.start,
-                         a.q + (unsigned long long)(p.q.start + t) * a.q_row +
+    slow_row<E, D, true>(a, table, request.start,
+                         a.q + (unsigned long long)(request.start + t) * a.q_row +
                              (unsigned long long)h * a.q_head,
                          head, t_begin, min(t_end, seen), rm, rl, ra);
-    store_slow<E, D>(a, splits > 1, true, slot, mm,
-                     (unsigned long long)(p.q.start + t) * a.q_heads + h, seen == 0, rm, rl, ra);
+    store_slow<E, D, kFewRows>(a, splits > 1, slot, mm,
+                     (unsigned long long)(request.start + t) * a.q_heads + h, seen == 0, rm, rl, ra);
   }
 }
 
 // ---------------------------------------------------------------------------
-// both paths in one launch
+// the launches
 
-// Workgroups take the two paths in turns of 8 (one on each XCD, so that a KV head of eight stays
-// on its XCD's L2), so that streaming and matrix work run beside each other, then what is left of
-// the longer list.
-template <typename E, int D, bool kPaged, bool kTiles, bool kFew, bool kRuns>
-__global__ __launch_bounds__(kT, 2) void attention_step(AttendArgs a) {
-  // (a variable for each buffer: the compiler orders a read of one behind the loads into it, and
-  // not behind those into the other)
+// (a variable for each buffer: the compiler orders a read of one behind the loads into it, and not
+// behind those into the others)
+template <typename E, int D, bool kPaged, bool kRuns>
+__global__ __launch_bounds__(kWave * kTileWaves, 2) void attention_tiles(AttendArgs a) {
   constexpr int kBuffer = 2 * kTileTokens * 2 * D;
-  static_assert(kBuffer == kWaves * kFewStep * 2 * D, "both paths' stages");
   __shared__ __align__(1024) unsigned char s0[kBuffer];
   __shared__ __align__(1024) unsigned char s1[kBuffer];
-  const Request first_requests = load_request(a, __lane_id());
-  const SplitSteps steps = split_steps(a, first_requests);
-  unsigned int block = blockIdx.x;
-  bool few = kFew;
-  if constexpr (kTiles && kFew) {
-    const unsigned int turns = min(a.tile_groups, a.few_groups) / 8;
-    if (block < 16 * turns) {
-      few = (block / 8) % 2 != 0;
-      block = block / 16 * 8 + block % 8;
-    } else {
-      block -= 8 * turns;
-      few = block >= a.tile_groups;
-      if (few) block -= a.tile_groups - 8 * turns;
-    }
-  }
-  if (kFew && few) {
-    if constexpr (kFew) few_path<E, D>(a, first_requests, steps, block, s0, s1);
-  } else {
-    if constexpr (kTiles) tile_path<E, D, kPaged, kRuns>(a, first_requests, steps, block, s0, s1);
-  }
+  __shared__ __align__(1024) unsigned char s2[kBuffer];
+  tile_path<E, D, kPaged, kRuns>(a, blockIdx.x, s0, s1, s2);
+}
+
+template <typename E, int D>
+__global__ __launch_bounds__(kWave * kWaves, 2) void attention_few(AttendArgs a) {
+  constexpr int kBuffer = kWaves * kFewStep * 2 * D;
+  __shared__ __align__(1024) unsigned char s0[kBuffer];
+  __shared__ __align__(1024) unsigned char s1[kBuffer];
+  few_path<E, D>(a, blockIdx.x, s0, s1);
 }
 
 // ---------------------------------------------------------------------------
@@ -991,57 +1153,50 @@ __global__ __launch_bounds__(kT, 2) void attention_step(AttendArgs a) {
 // A workgroup looks at its share of the slots' jobs with one load and takes those that have
 // something to join: 16 rows of a tile with a thread for 8 (D = 64: 4) sums of a row, or 4 rows of
 // the streaming path, which has more splits, with four threads that share a row's splits.
-constexpr int kTileParts = kTileRows / 16, kFewParts = kFewRows / 4;
-
-template <typename E, int D>
-__global__ __launch_bounds__(kT) void attention_merge(AttendArgs a) {
-  constexpr int kVals = D / 16;
-  constexpr int kBatch = 8;
-  __shared__ float s_part[kT][kVals + 2];
+template <typename E, int D, bool kTiles>
+__global__ __launch_bounds__(kMergeThreads) void attention_merge(AttendArgs a) {
+  constexpr int kRows = kTiles ? kTileRows : kFewRows;
+  constexpr int kVals = D / 16, kBatch = 8;
+  constexpr unsigned int kShares = kTiles ? 1 : 4;  // threads that share a row's splits
+  constexpr unsigned int kJobRows = 16 / kShares, kParts = kRows / kJobRows;
+  __shared__ float s_part[kTiles ? 1 : kMergeThreads][kVals + 2];
   const unsigned int tid = threadIdx.x, lane = tid & 63;
-  const unsigned int tile_jobs = a.tile_slots * kTileParts;
-  const unsigned int jobs = tile_jobs + a.few_slots * kFewParts;
-  auto slot_of = [&](unsigned int j) {
-    return j < tile_jobs ? j / kTileParts : a.tile_slots + (j - tile_jobs) / kFewParts;
-  };
+  const unsigned int jobs = a.slots * kParts;
   for (unsigned int j0 = blockIdx.x; j0 < jobs; j0 += kWave * gridDim.x) {
     const unsigned int mine = j0 + lane * gridDim.x;
-    unsigned long long todo = __ballot(mine < jobs && a.jobs[slot_of(min(mine, jobs - 1))].splits != 0);
+    const Job own = a.jobs[min(mine, jobs - 1) / kParts];
+    unsigned long long todo =
+        __ballot(mine < jobs && own.splits != 0 && mine % kParts * kJobRows < own.rows);
     while (todo != 0) {
       const unsigned int j = j0 + ((unsigned int)__ffsll((long long)todo) - 1) * gridDim.x;
       todo &= todo - 1;
-      const bool few = j >= tile_jobs;
-      const unsigned int job_slot = slot_of(j);
-      const Job job = a.jobs[job_slot];
-      const unsigned int slot = few ? job_slot - a.tile_slots : job_slot;
-      const unsigned int head = slot % a.kv_heads;
-      const unsigned int shares = few ? 4 : 1;  // threads that share a row's splits
-      const unsigned int share = (tid / 16) % shares, dims = (tid % 16) * kVals;
-      const unsigned int row = few ? (j - tile_jobs) % kFewParts * 4 + tid / 64
-                                   : j % kTileParts * 16 + tid / 16;
+      const unsigned int slot = j / kParts, head = slot % a.kv_heads;
+      const Job job = a.jobs[slot];
+      const unsigned int share = tid / 16 % kShares, dims = tid % 16 * kVals;
+      const unsigned int row = j % kParts * kJobRows + tid / (16 * kShares);
       const bool in = row < job.rows;
       const unsigned int use = in ? row : 0u;
       float big = kNoMax, l = 0.f, acc[kVals];
       bool bad = false;
 #pragma unroll
       for (int i = 0; i < kVals; ++i) acc[i] = 0.f;
-      for (unsigned int b = share; b < job.splits; b += shares * kBatch) {
+      for (unsigned int b = share; b < job.splits; b += kShares * kBatch) {
         f32x2 ml[kBatch];
         f32x4 v[kBatch][kVals / 4];
         // (past the last split the last one again, without weight: loads behind branches would
         // wait for each other)
 #pragma unroll
         for (int k = 0; k < kBatch; ++k) {
-          const unsigned int at = slot + min(b + k * shares, job.splits - 1u) * a.kv_heads;
-          ml[k] = *reinterpret_cast<const f32x2*>(slot_ml<D>(a, few, at) + 2 * use);
-          const float* src = slot_acc<D>(a, few, at) + use * D + dims;
+          const unsigned int at = slot + min(b + k * kShares, job.splits - 1u) * a.kv_heads;
+          ml[k] = *reinterpret_cast<const f32x2*>(slot_ml<D, kRows>(a, at) + 2 * use);
+          const float* src = slot_acc<D, kRows>(a, at) + use * D + dims;
 #pragma unroll
           for (int i = 0; i < kVals / 4; ++i) v[k][i] = *reinterpret_cast<const f32x4*>(src + 4 * i);
         }
         float top = big;
 #pragma unroll
         for (int k = 0; k < kBatch; ++k) {
-          if (b + k * shares >= job.splits) ml[k] = f32x2{kNoMax, 0.f};
+          if (b + k * kShares >= job.splits) ml[k] = f32x2{kNoMax, 0.f};
           bad |= ml[k].x != ml[k].x;
           top = fmaxf(top, ml[k].x);
         }
@@ -1052,13 +1207,13 @@ __global__ __launch_bounds__(kT) void attention_merge(AttendArgs a) {
         for (int i = 0; i < kVals; ++i) acc[i] *= alpha;
 #pragma unroll
         for (int k = 0; k < kBatch; ++k) {
-          const float f = b + k * shares < job.splits ? exp2f(ml[k].x - big) : 0.f;
+          const float f = b + k * kShares < job.splits ? exp2f(ml[k].x - big) : 0.f;
           l += ml[k].y * f;
 #pragma unroll
           for (int i = 0; i < kVals; ++i) acc[i] = f != 0.f ? fmaf(v[k][i / 4][i % 4], f, acc[i]) : acc[i];
         }
       }
-      if (few) {
+      if constexpr (!kTiles) {
         __syncthreads();  // the job before this one is done with the LDS
         float* own = s_part[tid];
         own[0] = bad ? NAN : big;
@@ -1124,82 +1279,87 @@ unsigned long long compute_units() {
   return cached[dev];
 }
 
-// Bounds of a call's grids and partial slots, from what the host knows: tokens (rows of q),
-// requests, the longest context that the tables (or the rows) can hold, and the longest request.
-struct Bounds {
-  unsigned long long few_target, tile_target;
-  unsigned long long few_items, tile_items;  // times KV heads: workgroups, and partial slots
-  bool few, tiles;
+// A call's grid and partial slots, from what the host knows: tokens (rows of q), requests, the
+// longest context that the tables (or the rows) can hold, and the longest request. Which kernel it
+// is goes by the longest request's rows alone.
+struct Plan {
+  bool tiles;
+  unsigned long long few_target, tile_target;  // workgroups resident at once
+  unsigned long long groups, slots;            // workgroups; partial slots, which have one each
 };
 
-Bounds bounds_of(unsigned long long tokens, unsigned long long requests, unsigned long long kv_heads,
-                 unsigned long long group, unsigned long long max_context,
-                 unsigned long long max_query, bool paged) {
-  Bounds b{};
-  b.few_target = b.tile_target = 2 * compute_units();  // workgroups resident at once
+Plan plan_of(unsigned long long tokens, unsigned long long requests, unsigned long long kv_heads,
+             unsigned long long group, unsigned long long max_context,
+             unsigned long long max_query, bool paged) {
+  Plan p{};
+  p.tiles = !paged || max_query * group > kFewRows;
+  p.few_target = 2 * compute_units();
+  p.tile_target = compute_units();
   const unsigned long long active = std::min(tokens, requests);
-  const unsigned long long rows = max_query * group;
-  b.few = paged && active != 0;
-  b.tiles = !paged || rows > kFewRows;
-  if (b.few) {
-    // sum over requests of ceil(rounds / steps) <= all rounds / steps + requests
-    const unsigned long long most = std::max(1ull, (max_context + kFewRound - 1) / kFewRound);
-    b.few_items = std::min(active * most, b.few_target / kv_heads + active + 1);
+  if (p.tiles) {
+    const unsigned long long tiles = tokens * group / kTileRows + active, least = kTileTokens * kLeastTileSteps;
+    const unsigned long long most = std::max(1ull, (max_context + least - 1) / least);
+    // (see Work: at most 4 * tile_target slots in all; a workgroup for each, besides those of the
+    // tiles that are not cut, writes its job)
+    const unsigned long long slots =
+        most == 1 ? 0 : std::min(tiles * most, 4 * p.tile_target / kv_heads);
+    p.groups = (tiles + slots) * kv_heads;
+    p.slots = slots * kv_heads;
+  } else {
+    const unsigned long long most = std::max(1ull, (max_context + Work<false>::kStep - 1) / Work<false>::kStep);
+    p.groups = p.slots = std::min(active * most, p.few_target / kv_heads + active + 1) * kv_heads;
   }
-  if (b.tiles) {
-    const unsigned long long tiles = tokens * group / kTileRows + active;
-    const unsigned long long most =
-        std::max(1ull, (max_context + kTileTokens * kLeastTileSteps - 1) / (kTileTokens * kLeastTileSteps));
-    // split, there are fewer than tile_target tiles, and of tiles * context / steps <= 2 *
-    // tile_target more; not split, one item a tile
-    b.tile_items = std::max(tiles, std::min(tiles * most, (3 * b.tile_target) / kv_heads + 1));
-  }
-  return b;
-}
-
-unsigned long long tile_slots_of(const Bounds& b, unsigned long long kv_heads) {
-  // (only split launches write partials)
-  return b.tiles ? std::min(b.tile_items * kv_heads, 3 * b.tile_target + kv_heads) : 0;
+  return p;
 }
 
 // The slots' partials, then their jobs.
-unsigned long long partial_bytes(const Bounds& b, unsigned long long kv_heads,
-                                 unsigned long long head_dim) {
-  return (b.few_items * kv_heads * kFewRows + tile_slots_of(b, kv_heads) * kTileRows) *
-         (head_dim + 2) * sizeof(float);
+unsigned long long partial_bytes(const Plan& p, unsigned long long head_dim) {
+  return p.slots * (p.tiles ? kTileRows : kFewRows) * (head_dim + 2) * sizeof(float);
 }
-unsigned long long workspace_of(const Bounds& b, unsigned long long kv_heads,
-                                unsigned long long head_dim) {
-  return partial_bytes(b, kv_heads, head_dim) +
-         (b.few_items * kv_heads + tile_slots_of(b, kv_heads)) * sizeof(Job);
+unsigned long long workspace_of(const Plan& p, unsigned long long head_dim) {
+  return partial_bytes(p, head_dim) + p.slots * sizeof(Job);
+}
+
+template <typename E, int D, bool kTiles>
+hipError_t launch_merge(const AttendArgs& a, hipStream_t stream) {
+  const unsigned int jobs = a.slots * (kTiles ? kTileRows / 16 : kFewRows / 4);
+  if (jobs == 0) return hipSuccess;  // (no context that is long enough to be split)
+  hipLaunchKernelGGL((attention_merge<E, D, kTiles>), dim3(std::min(jobs, 1024u)),
+                     dim3(kMergeThreads), 0, stream, a);
+  return hipGetLastError();
 }
 
 template <typename E, int D, bool kPaged>
-long long launch(const AttendArgs& a, hipStream_t stream) {
-  const dim3 grid(a.tile_groups + a.few_groups), threads(kT);
-  if constexpr (!kPaged)
-    hipLaunchKernelGGL((attention_step<E, D, false, true, false, true>), grid, threads, 0, stream, a);
-  else if (a.tile_groups == 0)
-    hipLaunchKernelGGL((attention_step<E, D, true, false, true, false>), grid, threads, 0, stream, a);
-  else if (a.block_tokens % 16 == 0)
-    hipLaunchKernelGGL((attention_step<E, D, true, true, true, true>), grid, threads, 0, stream, a);
-  else
-    hipLaunchKernelGGL((attention_step<E, D, true, true, true, false>), grid, threads, 0, stream, a);
-  hipError_t st = hipGetLastError();
-  if (st != hipSuccess) return fail("attention_step", st);
-  const unsigned int jobs = a.tile_slots * kTileParts + a.few_slots * kFewParts;
-  hipLaunchKernelGGL((attention_merge<E, D>), dim3(std::min(jobs, 1024u)), threads, 0, stream, a);
-  st = hipGetLastError();
+long long launch(const AttendArgs& a, const Plan& p, hipStream_t stream) {
+  const dim3 grid((unsigned int)p.groups);
+  hipError_t st = hipSuccess;
+  if (p.tiles) {
+    const dim3 threads(kWave * kTileWaves);
+    if constexpr (!kPaged)
+      hipLaunchKernelGGL((attention_tiles<E, D, false, true>), grid, threads, 0, stream, a);
+    else if (a.block_tokens % 8 == 0)
+      hipLaunchKernelGGL((attention_tiles<E, D, true, true>), grid, threads, 0, stream, a);
+    else
+      hipLaunchKernelGGL((attention_tiles<E, D, true, false>), grid, threads, 0, stream, a);
+    st = hipGetLastError();
+    if (st != hipSuccess) return fail("attention_tiles", st);
+    st = launch_merge<E, D, true>(a, stream);
+  } else if constexpr (kPaged) {
+    hipLaunchKernelGGL((attention_few<E, D>), grid, dim3(kWave * kWaves), 0, stream, a);
+    st = hipGetLastError();
+    if (st != hipSuccess) return fail("attention_few", st);
+    st = launch_merge<E, D, false>(a, stream);
+  }
   if (st != hipSuccess) return fail("attention_merge", st);
   return (long long)((unsigned long long)a.tokens * a.q_heads * D * 2);
 }
 
 template <bool kPaged>
-long long launch_typed(const AttendArgs& a, unsigned long long head_dim, unsigned long long dtype,
-                       hipStream_t stream) {
+long long launch_typed(const AttendArgs& a, const Plan& p, unsigned long long head_dim,
+                       unsigned long long dtype, hipStream_t stream) {
   if (head_dim == 128)
-    return dtype ? launch<_Float16, 128, kPaged>(a, stream) : launch<__bf16, 128, kPaged>(a, stream);
-  return dtype ? launch<_Float16, 64, kPaged>(a, stream) : launch<__bf16, 64, kPaged>(a, stream);
+    return dtype ? launch<_Float16, 128, kPaged>(a, p, stream) : launch<__bf16, 128, kPaged>(a, p, stream);
+  return dtype ? launch<_Float16, 64, kPaged>(a, p, stream) : launch<__bf16, 64, kPaged>(a, p, stream);
 }
 
 constexpr unsigned long long kMostRows = 0x7FFFFFFFull;
@@ -1227,16 +1387,16 @@ extern "C" unsigned long long kvq_splitzip_chunk_attention_workspace_bytes(
     unsigned long long kv_heads, unsigned long long head_dim, unsigned long long max_context,
     unsigned long long max_query) {
   if (!sizes_ok(tokens, requests, q_heads, kv_heads, head_dim, max_query)) return 0;
-  return workspace_of(bounds_of(tokens, requests, kv_heads, q_heads / kv_heads, max_context,
-                                 max_query, true), kv_heads, head_dim);
+  return workspace_of(plan_of(tokens, requests, kv_heads, q_heads / kv_heads, max_context, max_query,
+                              true), head_dim);
 }
 
 extern "C" unsigned long long kvq_splitzip_prompt_attention_workspace_bytes(
     unsigned long long tokens, unsigned long long requests, unsigned long long q_heads,
     unsigned long long kv_heads, unsigned long long head_dim, unsigned long long max_query) {
   if (!sizes_ok(tokens, requests, q_heads, kv_heads, head_dim, max_query)) return 0;
-  return workspace_of(bounds_of(tokens, requests, kv_heads, q_heads / kv_heads, max_query,
-                                 max_query, false), kv_heads, head_dim);
+  return workspace_of(plan_of(tokens, requests, kv_heads, q_heads / kv_heads, max_query, max_query,
+                              false), head_dim);
 }
 
 extern "C" long long kvq_splitzip_chunk_attention_paged(
@@ -1258,10 +1418,10 @@ extern "C" long long kvq_splitzip_chunk_attention_paged(
       !(scale > 0.f) || !std::isfinite(scale))
     return 0;
   const unsigned long long max_context = std::min(table_width * block_tokens, kMostRows);
-  const Bounds b = bounds_of(tokens, requests, kv_heads, q_heads / kv_heads, max_context, max_query, true);
-  const unsigned long long need = workspace_of(b, kv_heads, head_dim);
-  if (workspace_ptr == 0 || workspace_ptr % 16 != 0 || workspace_bytes < need) return 0;
-  if ((b.tile_items + b.few_items) * kv_heads > kMostRows) return 0;
+  const Plan plan = plan_of(tokens, requests, kv_heads, q_heads / kv_heads, max_context, max_query, true);
+  const unsigned long long need = workspace_of(plan, head_dim);
+  if (need != 0 && (workspace_ptr == 0 || workspace_ptr % 16 != 0 || workspace_bytes < need)) return 0;
+  if (plan.groups > kMostRows) return 0;
   const unsigned long long out_bytes = tokens * q_heads * head_dim * 2;
   if (overlap(out_ptr, out_bytes, q_ptr, extent(tokens, q_row_bytes, q_heads, q_head_bytes, 2 * head_dim)) ||
       overlap(out_ptr, out_bytes, kv_ptr, 4 * blocks * block_tokens * kv_heads * head_dim))
@@ -1278,7 +1438,7 @@ extern "C" long long kvq_splitzip_chunk_attention_paged(
   a.contexts = reinterpret_cast<const int*>(context_tokens_ptr);
   a.tables = reinterpret_cast<const int*>(tables_ptr);
   a.partial = reinterpret_cast<float*>(workspace_ptr);
-  a.jobs = reinterpret_cast<Job*>(workspace_ptr + partial_bytes(b, kv_heads, head_dim));
+  a.jobs = reinterpret_cast<Job*>(workspace_ptr + partial_bytes(plan, head_dim));
   a.q_row = q_row_bytes;
   a.q_head = q_head_bytes;
   a.table_stride = table_stride;
@@ -1291,16 +1451,12 @@ extern "C" long long kvq_splitzip_chunk_attention_paged(
   a.q_heads = (unsigned int)q_heads;
   a.kv_heads = (unsigned int)kv_heads;
   a.group = (unsigned int)(q_heads / kv_heads);
-  a.few_rows = kFewRows;
-  a.tiles_too = b.tiles ? 1u : 0u;
-  a.few_target = (unsigned int)b.few_target;
-  a.tile_target = (unsigned int)b.tile_target;
+  a.few_target = (unsigned int)plan.few_target;
+  a.tile_target = (unsigned int)plan.tile_target;
   a.max_query = (unsigned int)max_query;
-  a.tile_slots = (unsigned int)tile_slots_of(b, kv_heads);
-  a.few_slots = a.few_groups = (unsigned int)(b.few_items * kv_heads);
-  a.tile_groups = (unsigned int)(b.tile_items * kv_heads);
+  a.slots = (unsigned int)plan.slots;
   a.scale_log2 = scale * 1.4426950408889634f;
-  return launch_typed<true>(a, head_dim, dtype, reinterpret_cast<hipStream_t>(stream_ptr));
+  return launch_typed<true>(a, plan, head_dim, dtype, reinterpret_cast<hipStream_t>(stream_ptr));
 }
 
 extern "C" long long kvq_splitzip_prompt_attention(
@@ -1319,10 +1475,10 @@ extern "C" long long kvq_splitzip_prompt_attention(
       k_row_bytes > kMostStride || v_row_bytes > kMostStride || query_starts_ptr == 0 ||
       out_ptr == 0 || out_ptr % 16 != 0 || !(scale > 0.f) || !std::isfinite(scale))
     return 0;
-  const Bounds b = bounds_of(tokens, requests, kv_heads, q_heads / kv_heads, max_query, max_query, false);
-  const unsigned long long need = workspace_of(b, kv_heads, head_dim);
-  if (workspace_ptr == 0 || workspace_ptr % 16 != 0 || workspace_bytes < need) return 0;
-  if (b.tile_items * kv_heads > kMostRows) return 0;
+  const Plan plan = plan_of(tokens, requests, kv_heads, q_heads / kv_heads, max_query, max_query, false);
+  const unsigned long long need = workspace_of(plan, head_dim);
+  if (need != 0 && (workspace_ptr == 0 || workspace_ptr % 16 != 0 || workspace_bytes < need)) return 0;
+  if (plan.groups > kMostRows) return 0;
   const unsigned long long out_bytes = tokens * q_heads * head_dim * 2;
   if (overlap(out_ptr, out_bytes, q_ptr, extent(tokens, q_row_bytes, q_heads, q_head_bytes, 2 * head_dim)) ||
       overlap(out_ptr, out_bytes, k_ptr, extent(tokens, k_row_bytes, kv_heads, k_head_bytes, 2 * head_dim)) ||
@@ -1340,7 +1496,7 @@ extern "C" long long kvq_splitzip_prompt_attention(
   a.v_head = v_head_bytes;
   a.starts = reinterpret_cast<const int*>(query_starts_ptr);
   a.partial = reinterpret_cast<float*>(workspace_ptr);
-  a.jobs = reinterpret_cast<Job*>(workspace_ptr + partial_bytes(b, kv_heads, head_dim));
+  a.jobs = reinterpret_cast<Job*>(workspace_ptr + partial_bytes(plan, head_dim));
   a.q_row = q_row_bytes;
   a.q_head = q_head_bytes;
   a.tokens = (unsigned int)tokens;
@@ -1348,14 +1504,10 @@ extern "C" long long kvq_splitzip_prompt_attention(
   a.q_heads = (unsigned int)q_heads;
   a.kv_heads = (unsigned int)kv_heads;
   a.group = (unsigned int)(q_heads / kv_heads);
-  a.few_rows = 0;
-  a.tiles_too = 1;
-  a.few_target = (unsigned int)b.few_target;
-  a.tile_target = (unsigned int)b.tile_target;
+  a.few_target = (unsigned int)plan.few_target;
+  a.tile_target = (unsigned int)plan.tile_target;
   a.max_query = (unsigned int)max_query;
-  a.tile_slots = (unsigned int)tile_slots_of(b, kv_heads);
-  a.few_slots = a.few_groups = (unsigned int)(b.few_items * kv_heads);
-  a.tile_groups = (unsigned int)(b.tile_items * kv_heads);
+  a.slots = (unsigned int)plan.slots;
   a.scale_log2 = scale * 1.4426950408889634f;
-  return launch_typed<false>(a, head_dim, dtype, reinterpret_cast<hipStream_t>(stream_ptr));
+  return launch_typed<false>(a, plan, head_dim, dtype, reinterpret_cast<hipStream_t>(stream_ptr));
 }
