@@ -55,10 +55,9 @@ constexpr int kFewStep = 32;      // tokens of a wave's step in attention_few; a
                                   // take a round of them, the unit of its splits
 constexpr int kTileRows = 32 * kTileWaves;
 constexpr int kTileTokens = 64;   // tokens of a step of attention_tiles: unit of its splits
-// Steps of a split, at least: shorter ones cost more to join than the shorter last round saves (24
-// prompts of 3 .. 2050 tokens: 47.6 us at 24, 66 at 12; 16 requests of 6 tokens behind 300 .. 8000:
-// 41.3 and 50.2).
-constexpr unsigned int kLeastTileSteps = 24;
+// Steps of a split, at least: its start and its share of the joining take as long as some of them (4
+// requests of 64 tokens behind 4000: 39.1 us at 12, 44.8 at 16).
+constexpr unsigned int kLeastTileSteps = 12;
 // A maximum before any token: the lowest float, not -inf, so that rows whose scores are all -inf
 // have weights of zero and a sum of zero (whose quotient is NaN, as the formula's).
 constexpr float kNoMax = -3.402823466e38f;
@@ -136,6 +135,7 @@ struct AttendArgs {
   unsigned int few_target, tile_target;   // workgroups to split for, of the two paths
   unsigned int max_query;     // requests with more new tokens are left out
   unsigned int slots;         // partial slots
+  unsigned int items;         // of the tiles' grid, beside one that clears what slots they leave
   float scale_log2;
 };
 
@@ -203,6 +203,8 @@ __device__ __forceinline__ unsigned int tiles_of(const AttendArgs& a, unsigned i
   return (n * a.group + kTileRows - 1) / kTileRows;
 }
 
+constexpr unsigned int kNoSlot = ~0u;
+
 // Sums of 64 lanes' values stay below 2^32.
 constexpr unsigned int kMostSteps = 1u << 25;
 
@@ -214,12 +216,11 @@ __device__ __forceinline__ unsigned int share_of(unsigned long long sum, unsigne
 
 // The launch's work, which every workgroup finds its own item of by itself. Requests lie one in a
 // lane, 64 at a time (`first`: the first 64, which most launches end with), each with its tiles
-// (streaming: one) of `steps` steps of kStep tokens; a request of more than `cap` steps is cut into
-// splits of at most that. cap is the even share of all tiles' steps over the workgroups to split
-// for: on the streaming path few_target, for tiles half to all of their slots, the less the more
-// tiles there are anyhow: cut requests have at least two splits, so that sum of tiles * ceil(steps
-// / cap) over them is at most (all steps / cap + tiles) and at most twice (all steps / cap), both
-// within the slots.
+// (streaming: one) of `steps` steps of kStep tokens. A request of more than `cap` steps, the even
+// share of all tiles' steps over the workgroups to split for, is cut into the fewest splits of at
+// most that, all of about one length. A cut tile has at least two, so that all cut tiles together
+// have at most twice (all steps / cap) splits, in as many slots, and at most (all steps / cap) more
+// than there are tiles.
 template <bool kTiles>
 struct Work {
   static constexpr unsigned int kStep = kTiles ? kTileTokens : kWaves * kFewStep;
@@ -232,6 +233,10 @@ struct Work {
   }
   __device__ __forceinline__ unsigned int splits(unsigned int tokens) const {
     return cap == 0 ? 1u : max(1u, steps_of(steps_of(tokens, kStep), cap));
+  }
+  // tokens of a split of a request in `splits`
+  __device__ __forceinline__ unsigned int split_tokens(unsigned int tokens, unsigned int splits) const {
+    return steps_of(steps_of(tokens, kStep), splits) * kStep;
   }
   __device__ __forceinline__ Request requests(unsigned int r0) const {
     return r0 == 0 ? first : load_request(a, r0 + __lane_id());
@@ -250,9 +255,7 @@ struct Work {
       all += lane_value(wave_scan(t), 63);
       steps += lane_value(wave_scan((unsigned int)min(own, (unsigned long long)kMostSteps)), 63);
     }
-    const unsigned long long groups = all * a.kv_heads;
-    const unsigned int parts =
-        kTiles ? 4 * a.tile_target - (unsigned int)min(groups, 2ull * a.tile_target) : a.few_target;
+    const unsigned int parts = kTiles ? a.tile_target : a.few_target;
     if (!large) cap = max(kTiles ? kLeastTileSteps : 1u, share_of(steps * a.kv_heads, parts));
   }
 
@@ -271,10 +274,10 @@ struct Work {
   }
 
   // Item `item`: its request, its index among the request's items (splits of one tile beside each
-  // other) and, where the request is cut (streaming: always), among those that have a slot; past
-  // the last one, false and the slot that nobody else has. All wave-uniform.
+  // other), whether it has a slot (where the request is cut; streaming: always), and the slots that
+  // the items before it have, whose number is its own. False past the last one. All wave-uniform.
   __device__ __forceinline__ bool find(unsigned int item, Request& q, unsigned int& index,
-                                       unsigned int& slot) const {
+                                       bool& has_slot, unsigned int& slot) const {
     unsigned long long before = 0, slots = 0;
     for (unsigned int r0 = 0; r0 < a.requests; r0 += kWave) {
       const Request l = requests(r0);
@@ -290,15 +293,14 @@ struct Work {
         q.n = lane_value(l.n, at);
         q.ctx = lane_value(l.ctx, at);
         q.bad = lane_value(l.bad ? 1u : 0u, at) != 0;
-        slot = lane_value(slot_own, at) == 0
-                   ? ~0u
-                   : (unsigned int)slots + lane_value(slot_sum - slot_own, at) + index;
+        has_slot = lane_value(slot_own, at) != 0;
+        slot = (unsigned int)slots + lane_value(slot_sum - slot_own, at) + (has_slot ? index : 0u);
         return true;
       }
       before += all;
       slots += lane_value(slot_sum, 63);
     }
-    slot = (unsigned int)(slots + (item - before));
+    slot = (unsigned int)min(slots, (unsigned long long)kNoSlot);
     return false;
   }
 };
@@ -308,11 +310,11 @@ struct Work {
 template <bool kPaged>
 __device__ __forceinline__ unsigned int kv_row(const AttendArgs& a, const int* table,
                                                unsigned int start, unsigned int t, int id,
-                                               bool& bad) {
+                                               unsigned int& bad) {
   if constexpr (kPaged) {
     const unsigned int blk = div_u32(t, a.by_block.m, a.by_block.d);
     const bool ok = (unsigned int)id < a.blocks;
-    bad |= !ok;
+    bad |= ok ? 0u : 1u;
     return (ok ? (unsigned int)id : 0u) * a.block_tokens + (t - blk * a.block_tokens);
   } else {
     return start + t;
@@ -372,7 +374,7 @@ __device__ __forceinline__ void slow_row(const AttendArgs& a, const int* table, 
   for (int i = 0; i < D / 64; ++i) acc[i] = 0.f;
   for (unsigned int t = t0; t < t1; t += kWave) {
     const unsigned int own = min(t + lane, t1 - 1);
-    bool bad = false;
+    unsigned int bad = 0;
     const unsigned int row = kv_row<kPaged>(a, table, start, own, block_id<kPaged>(a, table, own), bad);
     const unsigned char* k = kb + row * a.k_row;
     float s = 0.f;
@@ -444,6 +446,11 @@ __device__ __forceinline__ void store_job(const AttendArgs& a, unsigned int slot
   if (slot + (unsigned long long)j.splits > slots) j.splits = 0;
   a.jobs[slot * a.kv_heads + head] = j;
 }
+// Nothing to join in the slots from `slot` on, by the workgroup.
+__device__ __forceinline__ void clear_jobs(const AttendArgs& a, unsigned int slot, unsigned int head) {
+  for (unsigned long long s = (unsigned long long)slot + threadIdx.x; s < a.slots / a.kv_heads; s += blockDim.x)
+    a.jobs[s * a.kv_heads + head] = Job{};
+}
 
 // ---------------------------------------------------------------------------
 // 256 rows by 64 tokens a step
@@ -470,11 +477,15 @@ __device__ __forceinline__ void tile_path(const AttendArgs& a, unsigned int bloc
   const Work<true> work(a);
   Request request;
   unsigned int index, slot;
-  if (!work.find(item, request, index, slot)) {
-    store_job(a, slot, head, Job{});
+  bool has_slot;
+  const bool found = work.find(item, request, index, has_slot, slot);
+  if (item == a.items) {  // the last one, for the slots that the others do not use
+    clear_jobs(a, slot, head);
     return;
   }
-  slot = slot == ~0u ? slot : slot * a.kv_heads + head;
+  if (!found) return;
+  const unsigned int own_slot = slot;
+  slot = slot * a.kv_heads + head;
   // the tiles with the longest contexts first
   const unsigned int most = work.splits(request.ctx);
   const unsigned int tile = tiles_of(a, request.n) - 1 - index / most, split = index % most;
@@ -484,14 +495,15 @@ __device__ __forceinline__ void tile_path(const AttendArgs& a, unsigned int bloc
   const int shift = (int)request.ctx - (int)request.n;
   const int last_of_tile = shift + (int)((min(rows, m0 + kTileRows) - 1) / a.group);
   const unsigned int seen = last_of_tile < 0 ? 0u : (unsigned int)last_of_tile + 1;
-  const unsigned int splits = most == 1 ? 1u : work.splits(seen);  // of this tile
+  const unsigned int split_tokens = work.split_tokens(request.ctx, most);
+  const unsigned int splits = most == 1 ? 1u : max(1u, steps_of(seen, split_tokens));  // of this tile
   if (most > 1)
-    store_job(a, slot / a.kv_heads, head,
+    store_job(a, own_slot, head,
             Job{request.start, m0, shift, (unsigned short)min(rows - m0, (unsigned int)kTileRows),
                 (unsigned short)(split == 0 && splits > 1 ? splits : 0u)});
   if (split >= splits) return;
-  const unsigned int t_begin = split * work.cap * kTileTokens;
-  const unsigned int t_end = splits == 1 ? seen : min(seen, t_begin + work.cap * kTileTokens);
+  const unsigned int t_begin = split * split_tokens;
+  const unsigned int t_end = splits == 1 ? seen : min(seen, t_begin + split_tokens);
   const unsigned int mw = m0 + wave * 32, m = mw + col;
   const bool valid = m < rows;
   const unsigned int token = valid ? m / a.group : 0u;
@@ -504,7 +516,7 @@ __device__ __forceinline__ void tile_path(const AttendArgs& a, unsigned int bloc
   const int* table = kPaged ? a.tables + request.r * a.table_stride : nullptr;
   const unsigned char* kb = a.k + head * a.k_head;
   const unsigned char* vb = a.v + head * a.v_head;
-  bool bad = request.bad;
+  unsigned int bad = request.bad ? 1u : 0u;
 
   // the row's query as the second operand: dims 16 s + 8 half .. + 7 of slab s (a lane without a
   // row has the request's first: a column of the products that nobody reads)
@@ -902,7 +914,7 @@ __device__ __forceinline__ void few_path(const AttendArgs& a, unsigned int block
   constexpr int kRowsPerLoad = kWave / kPieces, kLoads = kFewStep / kRowsPerLoad;
   constexpr int kStageBytes = kFewStep * kRowBytes;
   constexpr int kSlabs = D / 32, kDimTiles = D / 16;
-  constexpr unsigned int kRound = Work<false>::kStep;
+  constexpr unsigned int kRound = Work<false>::kStep;  // of all waves
   // the waves' sums, then their (m, l), once the stages are read
   float* const s_acc = reinterpret_cast<float*>(s0);
   float* const s_ml = reinterpret_cast<float*>(s1);
@@ -914,19 +926,21 @@ __device__ __forceinline__ void few_path(const AttendArgs& a, unsigned int block
   const Work<false> work(a);
   Request request;
   unsigned int split, slot;
-  if (!work.find(item, request, split, slot)) {
-    store_job(a, slot, head, Job{});
+  bool has_slot;
+  if (!work.find(item, request, split, has_slot, slot)) {
+    store_job(a, item, head, Job{});
     return;
   }
   const unsigned int splits = work.splits(request.ctx);
+  const unsigned int split_tokens = work.split_tokens(request.ctx, splits);
   store_job(a, slot, head,
             Job{request.start, 0, (int)request.ctx - (int)request.n,
                 (unsigned short)(request.n * a.group),
                 (unsigned short)(split == 0 && splits > 1 ? splits : 0u)});
   slot = slot * a.kv_heads + head;
   const unsigned int rows = request.n * a.group;
-  const unsigned int t_begin = split * work.cap * kRound;
-  const unsigned int t_end = min(request.ctx, t_begin + work.cap * kRound);
+  const unsigned int t_begin = split * split_tokens;
+  const unsigned int t_end = splits == 1 ? request.ctx : min(request.ctx, t_begin + split_tokens);
   const int shift = (int)request.ctx - (int)request.n;
   const bool valid = col < rows;
   const unsigned int token = valid ? col / a.group : 0u;
@@ -936,7 +950,7 @@ __device__ __forceinline__ void few_path(const AttendArgs& a, unsigned int block
   const int* table = a.tables + request.r * a.table_stride;
   const unsigned char* kb = a.k + head * a.k_head;
   const unsigned char* vb = a.v + head * a.v_head;
-  bool bad = request.bad;
+  unsigned int bad = request.bad ? 1u : 0u;
 
   x8 q[kSlabs];
   const unsigned char* q_row = a.q + (unsigned long long)(request.start + token) * a.q_row +
@@ -1284,8 +1298,9 @@ unsigned long long compute_units() {
 // is goes by the longest request's rows alone.
 struct Plan {
   bool tiles;
-  unsigned long long few_target, tile_target;  // workgroups resident at once
-  unsigned long long groups, slots;            // workgroups; partial slots, which have one each
+  unsigned long long few_target, tile_target;  // workgroups that splits are made for
+  unsigned long long groups, slots;            // workgroups, partial slots
+  unsigned long long items;                    // of the tiles
 };
 
 Plan plan_of(unsigned long long tokens, unsigned long long requests, unsigned long long kv_heads,
@@ -1294,17 +1309,19 @@ Plan plan_of(unsigned long long tokens, unsigned long long requests, unsigned lo
   Plan p{};
   p.tiles = !paged || max_query * group > kFewRows;
   p.few_target = 2 * compute_units();
-  p.tile_target = compute_units();
+  // (tiles: of all that run at once, three quarters. Longer splits, so fewer of them, than an even
+  // share: 16 requests of 6 tokens behind 300 .. 8000 38.0 us and 45.8, a prompt of 1443 39.3 and 52.9;
+  // with a share of a fourth to a half of it 3 chunks beside 29 decodes took 402 and not 311)
+  p.tile_target = std::max(1ull, compute_units() * 3 / 4);
   const unsigned long long active = std::min(tokens, requests);
   if (p.tiles) {
-    const unsigned long long tiles = tokens * group / kTileRows + active, least = kTileTokens * kLeastTileSteps;
-    const unsigned long long most = std::max(1ull, (max_context + least - 1) / least);
-    // (see Work: at most 4 * tile_target slots in all; a workgroup for each, besides those of the
-    // tiles that are not cut, writes its job)
-    const unsigned long long slots =
-        most == 1 ? 0 : std::min(tiles * most, 4 * p.tile_target / kv_heads);
-    p.groups = (tiles + slots) * kv_heads;
-    p.slots = slots * kv_heads;
+    const unsigned long long tiles = tokens * group / kTileRows + active;
+    const bool cut = max_context > kTileTokens * kLeastTileSteps;
+    // (see Work; the share of one KV head)
+    const unsigned long long more = cut ? p.tile_target / kv_heads + 1 : 0;
+    p.slots = 2 * more * kv_heads;
+    p.items = tiles + more;
+    p.groups = (p.items + (cut ? 1 : 0)) * kv_heads;
   } else {
     const unsigned long long most = std::max(1ull, (max_context + Work<false>::kStep - 1) / Work<false>::kStep);
     p.groups = p.slots = std::min(active * most, p.few_target / kv_heads + active + 1) * kv_heads;
@@ -1455,6 +1472,7 @@ extern "C" long long kvq_splitzip_chunk_attention_paged(
   a.tile_target = (unsigned int)plan.tile_target;
   a.max_query = (unsigned int)max_query;
   a.slots = (unsigned int)plan.slots;
+  a.items = (unsigned int)plan.items;
   a.scale_log2 = scale * 1.4426950408889634f;
   return launch_typed<true>(a, plan, head_dim, dtype, reinterpret_cast<hipStream_t>(stream_ptr));
 }
@@ -1508,6 +1526,7 @@ extern "C" long long kvq_splitzip_prompt_attention(
   a.tile_target = (unsigned int)plan.tile_target;
   a.max_query = (unsigned int)max_query;
   a.slots = (unsigned int)plan.slots;
+  a.items = (unsigned int)plan.items;
   a.scale_log2 = scale * 1.4426950408889634f;
   return launch_typed<false>(a, plan, head_dim, dtype, reinterpret_cast<hipStream_t>(stream_ptr));
 }
