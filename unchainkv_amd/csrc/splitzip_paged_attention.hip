@@ -16,7 +16,8 @@
 //   * attention_few: at most 16 (decode steps). Bound by reading K and V: a wave streams 32 tokens
 //     at a time, K straight into the matrix operand's registers, V into LDS for the transposing
 //     reads.
-//   * attention_tiles: more; 256 rows by 64 tokens a step. Bound by the matrix and vector units.
+//   * attention_tiles: more; 256 rows (64-dim heads: 128) by 64 tokens a step. Bound by the matrix and
+//     vector units.
 // Both give S^T = K Q^T, so that a row's scores lie in one lane (and its partners 32 or 16 lanes
 // away): the maximum and the sum need one or two lane swaps a step, rescaling is a lane's own
 // product, and the weights are the second product's operand O^T = V^T P^T as they are, with V's
@@ -48,12 +49,15 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short i16x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kWaves = 4;         // waves of a workgroup of attention_few, two of them on a CU
-constexpr int kTileWaves = 8;     // of one of attention_tiles, one on a CU
+// Of one of attention_tiles: 8 of 128-dim heads, whose registers and LDS leave room for one workgroup
+// on a CU, and 4 of 64-dim heads, of which a CU has three that fill each other's starts and ends (24
+// prompts of 3 .. 2050 tokens: 38.9 us, with 8 waves 49.9; 8 x 4096 640 and 709).
+constexpr int tile_waves(int D) { return D == 128 ? 8 : 4; }
+constexpr int tile_rows(int D) { return 32 * tile_waves(D); }
 constexpr int kMergeThreads = 256;
 constexpr int kFewRows = 16;      // rows of a request that attention_few takes
 constexpr int kFewStep = 32;      // tokens of a wave's step in attention_few; a workgroup's waves
                                   // take a round of them, the unit of its splits
-constexpr int kTileRows = 32 * kTileWaves;
 constexpr int kTileTokens = 64;   // tokens of a step of attention_tiles: unit of its splits
 // Steps of a split, at least: its start and its share of the joining take as long as some of them (4
 // requests of 64 tokens behind 4000: 39.1 us at 12, 44.8 at 16).
@@ -199,8 +203,9 @@ __device__ __forceinline__ unsigned int steps_of(unsigned int tokens, unsigned i
   return tokens / step + (tokens % step != 0 ? 1u : 0u);
 }
 
+template <int kRows>
 __device__ __forceinline__ unsigned int tiles_of(const AttendArgs& a, unsigned int n) {
-  return (n * a.group + kTileRows - 1) / kTileRows;
+  return (n * a.group + kRows - 1) / kRows;
 }
 
 constexpr unsigned int kNoSlot = ~0u;
@@ -221,7 +226,7 @@ __device__ __forceinline__ unsigned int share_of(unsigned long long sum, unsigne
 // most that, all of about one length. A cut tile has at least two, so that all cut tiles together
 // have at most twice (all steps / cap) splits, in as many slots, and at most (all steps / cap) more
 // than there are tiles.
-template <bool kTiles>
+template <bool kTiles, int kRows>
 struct Work {
   static constexpr unsigned int kStep = kTiles ? kTileTokens : kWaves * kFewStep;
   const AttendArgs& a;
@@ -229,7 +234,7 @@ struct Work {
   unsigned int cap;  // steps of a split, at most; 0: nothing is cut
 
   __device__ __forceinline__ unsigned int tiles(const Request& q) const {
-    return kTiles ? tiles_of(a, q.n) : q.n != 0 ? 1u : 0u;
+    return kTiles ? tiles_of<kRows>(a, q.n) : q.n != 0 ? 1u : 0u;
   }
   __device__ __forceinline__ unsigned int splits(unsigned int tokens) const {
     return cap == 0 ? 1u : max(1u, steps_of(steps_of(tokens, kStep), cap));
@@ -308,9 +313,8 @@ struct Work {
 // Row of K and V that token t of a request has: its place in the layer through the block table
 // (bad: the table names no block of the layer there; block 0 is read instead), or its packed row.
 template <bool kPaged>
-__device__ __forceinline__ unsigned int kv_row(const AttendArgs& a, const int* table,
-                                               unsigned int start, unsigned int t, int id,
-                                               unsigned int& bad) {
+__device__ __forceinline__ unsigned int kv_row(const AttendArgs& a, unsigned int start,
+                                               unsigned int t, int id, unsigned int& bad) {
   if constexpr (kPaged) {
     const unsigned int blk = div_u32(t, a.by_block.m, a.by_block.d);
     const bool ok = (unsigned int)id < a.blocks;
@@ -375,7 +379,7 @@ __device__ __forceinline__ void slow_row(const AttendArgs& a, const int* table, 
   for (unsigned int t = t0; t < t1; t += kWave) {
     const unsigned int own = min(t + lane, t1 - 1);
     unsigned int bad = 0;
-    const unsigned int row = kv_row<kPaged>(a, table, start, own, block_id<kPaged>(a, table, own), bad);
+    const unsigned int row = kv_row<kPaged>(a, start, own, block_id<kPaged>(a, table, own), bad);
     const unsigned char* k = kb + row * a.k_row;
     float s = 0.f;
     for (int c = 0; c < D / 8; ++c) {
@@ -453,7 +457,7 @@ __device__ __forceinline__ void clear_jobs(const AttendArgs& a, unsigned int slo
 }
 
 // ---------------------------------------------------------------------------
-// 256 rows by 64 tokens a step
+// 32 rows a wave by 64 tokens a step
 
 // Lane l of a wave has row l % 32 of the wave's 32 and, of every 16 tokens, those with
 // (token / 4) % 2 == l / 32 (the 32x32 matrix instruction's output rows). K lies in LDS as rows
@@ -470,11 +474,13 @@ __device__ __forceinline__ void tile_path(const AttendArgs& a, unsigned int bloc
   constexpr int kRowsPerLoad = kWave / kPieces, kLoads = 8 / kRowsPerLoad;
   constexpr int kTileBytes = kTileTokens * kRowBytes;
   constexpr int kSlabs = D / 16, kDimTiles = D / 32;
+  constexpr int kN = tile_waves(D), kTileRows = tile_rows(D);
+  constexpr int kOwn = kTileTokens / kN, kOwnRuns = kOwn / 8;  // a wave's tokens of a tile's loads
 
   const unsigned int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
   const unsigned int half = lane / 32, col = lane % 32;
   const unsigned int head = block % a.kv_heads, item = block / a.kv_heads;
-  const Work<true> work(a);
+  const Work<true, kTileRows> work(a);
   Request request;
   unsigned int index, slot;
   bool has_slot;
@@ -488,7 +494,7 @@ __device__ __forceinline__ void tile_path(const AttendArgs& a, unsigned int bloc
   slot = slot * a.kv_heads + head;
   // the tiles with the longest contexts first
   const unsigned int most = work.splits(request.ctx);
-  const unsigned int tile = tiles_of(a, request.n) - 1 - index / most, split = index % most;
+  const unsigned int tile = tiles_of<kTileRows>(a, request.n) - 1 - index / most, split = index % most;
   const unsigned int rows = request.n * a.group;
   const unsigned int m0 = tile * kTileRows;
   // last visible token of a row (negative: none)
@@ -528,24 +534,26 @@ __device__ __forceinline__ void tile_path(const AttendArgs& a, unsigned int bloc
     q[s] = *reinterpret_cast<const x8*>(q_row + 32 * s + 16 * half);
   }
 
-  // This wave's share of a tile's loads: 8 tokens of K and V. Where they follow each other in memory
-  // (prompts; layers whose blocks are whole groups of 8 tokens) the wave forms their address once,
-  // on the scalar unit, and a lane's offsets from it never change.
+  // This wave's share of a tile's loads: kOwn tokens of K and V, in runs of 8. Where a run's follow
+  // each other in memory (prompts; layers whose blocks are whole groups of 8 tokens) the wave forms
+  // their address once, on the scalar unit, and a lane's offsets from it never change.
   const unsigned int piece = lane % kPieces, sub = lane / kPieces;
-  unsigned int k_off[kLoads], v_off[kLoads];
+  unsigned int k_off[kOwnRuns][kLoads], v_off[kOwnRuns][kLoads];
 #pragma unroll
-  for (int i = 0; i < kLoads; ++i) {
-    const unsigned int in = i * kRowsPerLoad + sub;  // the token's place among the wave's 8
-    const unsigned int at = 8 * (wave % 2) + in;     // and among 16
-    const unsigned int k_piece = piece ^ (D == 128 ? at : (at >> 1) & 7);
-    const unsigned int v_piece = piece ^ (D == 128 ? (at & 3) << 2 : ((at >> 1) & 1) << 2);
-    k_off[i] = (kRuns ? in * (unsigned int)a.k_row : 0u) + 16 * k_piece;
-    v_off[i] = (kRuns ? in * (unsigned int)a.v_row : 0u) + 16 * v_piece;
-  }
-  constexpr int kIds = kRuns ? 1 : kLoads;
-  const unsigned int first_at = wave * 8 * kRowBytes;
+  for (int u = 0; u < kOwnRuns; ++u)
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const unsigned int in = i * kRowsPerLoad + sub;                // the token's place in its run
+      const unsigned int at = (kOwn * wave + 8 * u) % 16 + in;       // and among 16
+      const unsigned int k_piece = piece ^ (D == 128 ? at : (at >> 1) & 7);
+      const unsigned int v_piece = piece ^ (D == 128 ? (at & 3) << 2 : ((at >> 1) & 1) << 2);
+      k_off[u][i] = (kRuns ? in * (unsigned int)a.k_row : 0u) + 16 * k_piece;
+      v_off[u][i] = (kRuns ? in * (unsigned int)a.v_row : 0u) + 16 * v_piece;
+    }
+  constexpr int kIds = kRuns ? kOwnRuns : kOwnRuns * kLoads;
+  const unsigned int first_at = wave * kOwn * kRowBytes;
   auto token_of = [&](unsigned int base, int i) {
-    return min(base + wave * 8 + (kRuns ? 0 : i * kRowsPerLoad + sub), t_end - 1);
+    return min(base + wave * kOwn + (kRuns ? 8 * i : i * kRowsPerLoad + sub), t_end - 1);
   };
   int ids[kIds];               // of the tile whose K is loaded next
   unsigned int next_row[kIds], row_of[kIds];  // of that tile, and of the one whose V is
@@ -556,35 +564,43 @@ __device__ __forceinline__ void tile_path(const AttendArgs& a, unsigned int bloc
   auto find_rows = [&](unsigned int base) {
 #pragma unroll
     for (int i = 0; i < kIds; ++i) {
-      next_row[i] = kv_row<kPaged>(a, table, request.start, token_of(base, i), ids[i], bad);
+      next_row[i] = kv_row<kPaged>(a, request.start, token_of(base, i), ids[i], bad);
       if (kRuns) next_row[i] = uniform(next_row[i]);
     }
   };
-  // Sizes of the buffers of this wave's rows (kRuns): whole tiles lie inside the tensor, the last one
+  // Sizes of the buffers of a run's rows (kRuns): whole tiles lie inside the tensor, the last one
   // ends with the tokens, and one behind it has none.
   const unsigned int last_base = t_end == 0 ? 0u : (t_end - 1 - t_begin) / kTileTokens * kTileTokens + t_begin;
-  const int left = (int)t_end - (int)(last_base + wave * 8);
-  const unsigned int last_rows = uniform((unsigned int)max(min(left, 8), 0));
-  const unsigned int k_last = last_rows == 0 ? 0u : (last_rows - 1) * (unsigned int)a.k_row + kRowBytes;
-  const unsigned int v_last = last_rows == 0 ? 0u : (last_rows - 1) * (unsigned int)a.v_row + kRowBytes;
+  unsigned int k_last[kOwnRuns], v_last[kOwnRuns];
+#pragma unroll
+  for (int u = 0; u < kOwnRuns; ++u) {
+    const int left = (int)t_end - (int)(last_base + wave * kOwn + 8 * u);
+    const unsigned int last_rows = uniform((unsigned int)max(min(left, 8), 0));
+    k_last[u] = last_rows == 0 ? 0u : (last_rows - 1) * (unsigned int)a.k_row + kRowBytes;
+    v_last[u] = last_rows == 0 ? 0u : (last_rows - 1) * (unsigned int)a.v_row + kRowBytes;
+  }
   auto load_plane = [&](unsigned int base, const unsigned char* src, unsigned long long stride,
-                        unsigned int last_bytes, const unsigned int (&row)[kIds],
-                        const unsigned int (&off)[kLoads], unsigned char* dst) {
-    if constexpr (kRuns) {
-      const unsigned int bytes = base < last_base ? 0x7FFFFFFFu : base == last_base ? last_bytes : 0u;
-      const Buffer buffer = buffer_of(src + row[0] * stride, bytes);
+                        const unsigned int (&last_bytes)[kOwnRuns], const unsigned int (&row)[kIds],
+                        const unsigned int (&off)[kOwnRuns][kLoads], unsigned char* dst) {
 #pragma unroll
-      for (int i = 0; i < kLoads; ++i)
-        load_to_lds(buffer, off[i], dst + first_at + i * kRowsPerLoad * kRowBytes);
-    } else {
+    for (int u = 0; u < kOwnRuns; ++u)
+      if constexpr (kRuns) {
+        const unsigned int bytes =
+            base < last_base ? 0x7FFFFFFFu : base == last_base ? last_bytes[u] : 0u;
+        const Buffer buffer = buffer_of(src + row[u] * stride, bytes);
 #pragma unroll
-      for (int i = 0; i < kLoads; ++i)
-        load_to_lds(src + row[i] * stride + off[i], dst + first_at + i * kRowsPerLoad * kRowBytes);
-    }
+        for (int i = 0; i < kLoads; ++i)
+          load_to_lds(buffer, off[u][i], dst + first_at + (8 * u + i * kRowsPerLoad) * kRowBytes);
+      } else {
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i)
+          load_to_lds(src + row[u * kLoads + i] * stride + off[u][i],
+                      dst + first_at + (8 * u + i * kRowsPerLoad) * kRowBytes);
+      }
   };
   // The loads of a round in three steps: K of the tile behind `base`, V of the tile there. (Tokens
   // past the end are outside the buffers, or the last one again.)
-  constexpr int kInFlight = 2 * kLoads + (kPaged ? kIds : 0);  // a round's
+  constexpr int kInFlight = 2 * kOwnRuns * kLoads + (kPaged ? kIds : 0);  // a round's
   auto load_step = [&](int j, unsigned int base, unsigned char* to) {
     if (j == 0) {
       find_rows(base + kTileTokens);
@@ -632,7 +648,7 @@ __device__ __forceinline__ void tile_path(const AttendArgs& a, unsigned int bloc
   // the halves in turns), with the late weights of the tile before between them, then those of its
   // O (16 tokens, 32 dims); each operand is read kAhead products before its own, in this order (left
   // to itself the compiler waits for each read just issued).
-  constexpr int kOuts = 4 * kDimTiles, kScores = 2 * kSlabs, kAhead = 4;
+  constexpr int kOuts = 4 * kDimTiles, kScores = 2 * kSlabs, kAhead = D == 128 ? 4 : 2;
   auto operand = [&](int i, const unsigned char* bv, const unsigned char* bk) {
     if (i < kScores)
       return *reinterpret_cast<const x8*>(bk + k_at + 32 * (i % 2) * kRowBytes +
@@ -759,7 +775,9 @@ __device__ __forceinline__ void tile_path(const AttendArgs& a, unsigned int bloc
 #pragma unroll
       for (int j = 0; j < 3; ++j) load_step(j, base, to);
     };
-    auto phase_end = [&]() {
+    // (4 waves: each SIMD's other wave is of the workgroup beside it, and a round has one barrier)
+    auto phase_end = [&](bool always) {
+      if (!always && kN == 4) return;
       __builtin_amdgcn_sched_barrier(0);
       asm volatile("" ::: "memory");
       __builtin_amdgcn_s_barrier();
@@ -791,52 +809,52 @@ __device__ __forceinline__ void tile_path(const AttendArgs& a, unsigned int bloc
     fetch_ids(t_begin + kTileTokens);
     load(t_begin, s1);
     wait_loads<kInFlight>();
-    phase_end();
+    phase_end(true);
     if (mw >= rows) {
       // a wave without rows
       auto idle = [&](unsigned int base, const unsigned char*, unsigned char* to) {
         load(base + kTileTokens, to);
-        phase_end();
+        phase_end(false);
         wait_loads<kInFlight>();
-        phase_end();
+        phase_end(true);
       };
       idle(t_begin, s0, s2);
       rounds(idle);
-      phase_end();
-      phase_end();
-    } else if (wave < 4) {
+      phase_end(false);
+      phase_end(true);
+    } else if (kN == 4 || wave < 4) {
       scores(s0);
-      phase_end();
+      phase_end(false);
       softmax(t_begin, with_loads(t_begin + kTileTokens, s2));
       wait_loads<kInFlight>();
-      phase_end();
+      phase_end(true);
       rounds([&](unsigned int base, const unsigned char* from, unsigned char* to) {
         both(from);
-        phase_end();
+        phase_end(false);
         softmax(base, with_loads(base + kTileTokens, to));
         wait_loads<kInFlight>();
-        phase_end();
+        phase_end(true);
       });
       outputs(last);
-      phase_end();
-      phase_end();
+      phase_end(false);
+      phase_end(true);
     } else {
       load(t_begin + kTileTokens, s2);
-      phase_end();
+      phase_end(true);
       scores(s0);
       wait_loads<kInFlight>();
-      phase_end();
+      phase_end(true);
       rounds([&](unsigned int base, const unsigned char* from, unsigned char* to) {
         softmax(base - kTileTokens, with_loads(base + kTileTokens, to));
-        phase_end();
+        phase_end(true);
         both(from);
         wait_loads<kInFlight>();
-        phase_end();
+        phase_end(true);
       });
       softmax(base_end - kTileTokens, [](int) {});
-      phase_end();
+      phase_end(true);
       outputs(last);
-      phase_end();
+      phase_end(true);
     }
     wait_loads<0>();
   }
@@ -914,7 +932,7 @@ __device__ __forceinline__ void few_path(const AttendArgs& a, unsigned int block
   constexpr int kRowsPerLoad = kWave / kPieces, kLoads = kFewStep / kRowsPerLoad;
   constexpr int kStageBytes = kFewStep * kRowBytes;
   constexpr int kSlabs = D / 32, kDimTiles = D / 16;
-  constexpr unsigned int kRound = Work<false>::kStep;  // of all waves
+  constexpr unsigned int kRound = Work<false, kFewRows>::kStep;  // of all waves
   // the waves' sums, then their (m, l), once the stages are read
   float* const s_acc = reinterpret_cast<float*>(s0);
   float* const s_ml = reinterpret_cast<float*>(s1);
@@ -923,7 +941,7 @@ __device__ __forceinline__ void few_path(const AttendArgs& a, unsigned int block
   const unsigned int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
   const unsigned int col = lane % 16, grp = lane / 16;
   const unsigned int head = block % a.kv_heads, item = block / a.kv_heads;
-  const Work<false> work(a);
+  const Work<false, kFewRows> work(a);
   Request request;
   unsigned int split, slot;
   bool has_slot;
@@ -969,7 +987,7 @@ __device__ __forceinline__ void few_path(const AttendArgs& a, unsigned int block
   // lane l looks up token l % 32 of a step
   auto token_of = [&](unsigned int base) { return min(base + lane % 32, t_end - 1); };
   auto issue = [&](unsigned int base, int id, Keys& k, unsigned char* stage) {
-    const unsigned int row = kv_row<true>(a, table, 0u, token_of(base), id, bad);
+    const unsigned int row = kv_row<true>(a, 0u, token_of(base), id, bad);
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const unsigned char* src = kb + (unsigned int)__shfl(row, 16 * u + (int)col, kWave) * a.k_row;
@@ -1145,7 +1163,7 @@ __device__ __forceinline__ void few_path(const AttendArgs& a, unsigned int block
 // (a variable for each buffer: the compiler orders a read of one behind the loads into it, and not
 // behind those into the others)
 template <typename E, int D, bool kPaged, bool kRuns>
-__global__ __launch_bounds__(kWave * kTileWaves, 2) void attention_tiles(AttendArgs a) {
+__global__ __launch_bounds__(kWave * tile_waves(D), D == 128 ? 2 : 3) void attention_tiles(AttendArgs a) {
   constexpr int kBuffer = 2 * kTileTokens * 2 * D;
   __shared__ __align__(1024) unsigned char s0[kBuffer];
   __shared__ __align__(1024) unsigned char s1[kBuffer];
@@ -1169,7 +1187,7 @@ __global__ __launch_bounds__(kWave * kWaves, 2) void attention_few(AttendArgs a)
 // the streaming path, which has more splits, with four threads that share a row's splits.
 template <typename E, int D, bool kTiles>
 __global__ __launch_bounds__(kMergeThreads) void attention_merge(AttendArgs a) {
-  constexpr int kRows = kTiles ? kTileRows : kFewRows;
+  constexpr int kRows = kTiles ? tile_rows(D) : kFewRows;
   constexpr int kVals = D / 16, kBatch = 8;
   constexpr unsigned int kShares = kTiles ? 1 : 4;  // threads that share a row's splits
   constexpr unsigned int kJobRows = 16 / kShares, kParts = kRows / kJobRows;
@@ -1304,7 +1322,7 @@ struct Plan {
 };
 
 Plan plan_of(unsigned long long tokens, unsigned long long requests, unsigned long long kv_heads,
-             unsigned long long group, unsigned long long max_context,
+             unsigned long long group, unsigned long long head_dim, unsigned long long max_context,
              unsigned long long max_query, bool paged) {
   Plan p{};
   p.tiles = !paged || max_query * group > kFewRows;
@@ -1312,10 +1330,10 @@ Plan plan_of(unsigned long long tokens, unsigned long long requests, unsigned lo
   // (tiles: of all that run at once, three quarters. Longer splits, so fewer of them, than an even
   // share: 16 requests of 6 tokens behind 300 .. 8000 38.0 us and 45.8, a prompt of 1443 39.3 and 52.9;
   // with a share of a fourth to a half of it 3 chunks beside 29 decodes took 402 and not 311)
-  p.tile_target = std::max(1ull, compute_units() * 3 / 4);
+  p.tile_target = std::max(1ull, compute_units() * (head_dim == 128 ? 3 : 6) / 4);
   const unsigned long long active = std::min(tokens, requests);
   if (p.tiles) {
-    const unsigned long long tiles = tokens * group / kTileRows + active;
+    const unsigned long long tiles = tokens * group / tile_rows((int)head_dim) + active;
     const bool cut = max_context > kTileTokens * kLeastTileSteps;
     // (see Work; the share of one KV head)
     const unsigned long long more = cut ? p.tile_target / kv_heads + 1 : 0;
@@ -1323,7 +1341,7 @@ Plan plan_of(unsigned long long tokens, unsigned long long requests, unsigned lo
     p.items = tiles + more;
     p.groups = (p.items + (cut ? 1 : 0)) * kv_heads;
   } else {
-    const unsigned long long most = std::max(1ull, (max_context + Work<false>::kStep - 1) / Work<false>::kStep);
+    const unsigned long long most = std::max(1ull, (max_context + Work<false, kFewRows>::kStep - 1) / Work<false, kFewRows>::kStep);
     p.groups = p.slots = std::min(active * most, p.few_target / kv_heads + active + 1) * kv_heads;
   }
   return p;
@@ -1331,7 +1349,7 @@ Plan plan_of(unsigned long long tokens, unsigned long long requests, unsigned lo
 
 // The slots' partials, then their jobs.
 unsigned long long partial_bytes(const Plan& p, unsigned long long head_dim) {
-  return p.slots * (p.tiles ? kTileRows : kFewRows) * (head_dim + 2) * sizeof(float);
+  return p.slots * (p.tiles ? tile_rows((int)head_dim) : kFewRows) * (head_dim + 2) * sizeof(float);
 }
 unsigned long long workspace_of(const Plan& p, unsigned long long head_dim) {
   return partial_bytes(p, head_dim) + p.slots * sizeof(Job);
@@ -1339,7 +1357,7 @@ unsigned long long workspace_of(const Plan& p, unsigned long long head_dim) {
 
 template <typename E, int D, bool kTiles>
 hipError_t launch_merge(const AttendArgs& a, hipStream_t stream) {
-  const unsigned int jobs = a.slots * (kTiles ? kTileRows / 16 : kFewRows / 4);
+  const unsigned int jobs = a.slots * (kTiles ? tile_rows(D) / 16 : kFewRows / 4);
   if (jobs == 0) return hipSuccess;  // (no context that is long enough to be split)
   hipLaunchKernelGGL((attention_merge<E, D, kTiles>), dim3(std::min(jobs, 1024u)),
                      dim3(kMergeThreads), 0, stream, a);
@@ -1351,7 +1369,7 @@ long long launch(const AttendArgs& a, const Plan& p, hipStream_t stream) {
   const dim3 grid((unsigned int)p.groups);
   hipError_t st = hipSuccess;
   if (p.tiles) {
-    const dim3 threads(kWave * kTileWaves);
+    const dim3 threads(kWave * tile_waves(D));
     if constexpr (!kPaged)
       hipLaunchKernelGGL((attention_tiles<E, D, false, true>), grid, threads, 0, stream, a);
     else if (a.block_tokens % 8 == 0)
@@ -1404,7 +1422,7 @@ extern "C" unsigned long long kvq_splitzip_chunk_attention_workspace_bytes(
     unsigned long long kv_heads, unsigned long long head_dim, unsigned long long max_context,
     unsigned long long max_query) {
   if (!sizes_ok(tokens, requests, q_heads, kv_heads, head_dim, max_query)) return 0;
-  return workspace_of(plan_of(tokens, requests, kv_heads, q_heads / kv_heads, max_context, max_query,
+  return workspace_of(plan_of(tokens, requests, kv_heads, q_heads / kv_heads, head_dim, max_context, max_query,
                               true), head_dim);
 }
 
@@ -1412,7 +1430,7 @@ extern "C" unsigned long long kvq_splitzip_prompt_attention_workspace_bytes(
     unsigned long long tokens, unsigned long long requests, unsigned long long q_heads,
     unsigned long long kv_heads, unsigned long long head_dim, unsigned long long max_query) {
   if (!sizes_ok(tokens, requests, q_heads, kv_heads, head_dim, max_query)) return 0;
-  return workspace_of(plan_of(tokens, requests, kv_heads, q_heads / kv_heads, max_query, max_query,
+  return workspace_of(plan_of(tokens, requests, kv_heads, q_heads / kv_heads, head_dim, max_query, max_query,
                               false), head_dim);
 }
 
@@ -1435,7 +1453,7 @@ extern "C" long long kvq_splitzip_chunk_attention_paged(
       !(scale > 0.f) || !std::isfinite(scale))
     return 0;
   const unsigned long long max_context = std::min(table_width * block_tokens, kMostRows);
-  const Plan plan = plan_of(tokens, requests, kv_heads, q_heads / kv_heads, max_context, max_query, true);
+  const Plan plan = plan_of(tokens, requests, kv_heads, q_heads / kv_heads, head_dim, max_context, max_query, true);
   const unsigned long long need = workspace_of(plan, head_dim);
   if (need != 0 && (workspace_ptr == 0 || workspace_ptr % 16 != 0 || workspace_bytes < need)) return 0;
   if (plan.groups > kMostRows) return 0;
@@ -1493,7 +1511,7 @@ extern "C" long long kvq_splitzip_prompt_attention(
       k_row_bytes > kMostStride || v_row_bytes > kMostStride || query_starts_ptr == 0 ||
       out_ptr == 0 || out_ptr % 16 != 0 || !(scale > 0.f) || !std::isfinite(scale))
     return 0;
-  const Plan plan = plan_of(tokens, requests, kv_heads, q_heads / kv_heads, max_query, max_query, false);
+  const Plan plan = plan_of(tokens, requests, kv_heads, q_heads / kv_heads, head_dim, max_query, max_query, false);
   const unsigned long long need = workspace_of(plan, head_dim);
   if (need != 0 && (workspace_ptr == 0 || workspace_ptr % 16 != 0 || workspace_bytes < need)) return 0;
   if (plan.groups > kMostRows) return 0;
