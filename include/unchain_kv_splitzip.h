@@ -554,7 +554,8 @@ long long kvq_splitzip_write_kv_paged(
     unsigned long long v_head_bytes, unsigned long long kv_ptr, unsigned long long plane_bytes,
     unsigned long long slot_count, unsigned long long slots_ptr, unsigned long long stream_ptr);
 
-/* Workspace bytes of the two attention calls; max_context = table_width * block_tokens. */
+/* Workspace bytes of the two attention calls; max_context = table_width * block_tokens. 0: a call
+ * of these sizes needs none (its contexts are short enough to be taken whole), or declines them. */
 unsigned long long kvq_splitzip_chunk_attention_workspace_bytes(
     unsigned long long tokens, unsigned long long requests, unsigned long long q_heads,
     unsigned long long kv_heads, unsigned long long head_dim, unsigned long long max_context,
@@ -572,8 +573,8 @@ unsigned long long kvq_splitzip_prompt_attention_workspace_bytes(
  * [tokens][q_heads] for the rows' log-sum-exps. max_query (at most tokens) bounds a request's
  * rows: longer ones are left out. Rows that see nothing are 0 (lse -inf); rows of no request,
  * or of a range that is not inside q, stay; a context past its table's row, or an entry that is
- * no block, gives NaN rows. workspace: 16-byte aligned, of the size above, for one call at a
- * time. Returns the bytes of out, 0 on a failed precondition (out must not overlap an input). */
+ * no block, gives NaN rows. workspace: 16-byte aligned, of the size above (not looked at where
+ * that is 0), for one call at a time. Returns the bytes of out, 0 on a failed precondition (out must not overlap an input). */
 long long kvq_splitzip_chunk_attention_paged(
     unsigned long long q_ptr, unsigned long long q_row_bytes, unsigned long long q_head_bytes,
     unsigned long long tokens, unsigned long long q_heads, unsigned long long kv_heads,

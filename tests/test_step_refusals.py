@@ -64,14 +64,28 @@ def test_chunk_declines(lib):
     refused(lib.kvq_splitzip_chunk_attention_paged, CHUNK, [
         {name: 0} for name in ("q", "tokens", "q_heads", "kv_heads", "dim", "kv", "blocks", "block",
                                "tables", "width", "starts", "contexts", "requests", "max_query",
-                               "out", "workspace", "workspace_bytes")] + [
+                               "out")] + [
         {"dim": 96}, {"dim": 256}, {"dtype": 2}, {"q_heads": 7}, {"kv_heads": 3}, {"max_query": 5},
         {"stride": 7}, {"q": A[0] + 2}, {"q_row": 2040}, {"q_head": 250}, {"kv": A[1] + 8},
-        {"out": A[5] + 8}, {"workspace": A[6] + 8}, {"workspace_bytes": 1000},
-        {"blocks": 1 << 28}, {"tokens": 1 << 31, "max_query": 1},
+        {"out": A[5] + 8}, {"blocks": 1 << 28}, {"tokens": 1 << 31, "max_query": 1},
         {"scale": ctypes.c_float(0.0)}, {"scale": ctypes.c_float(-1.0)},
         {"scale": ctypes.c_float(float("nan"))}, {"scale": ctypes.c_float(float("inf"))},
         {"out": A[0] + 2048}, {"out": A[1] + (1 << 18)}])
+
+
+def no_workspace(size):
+    return [{"workspace": 0}, {"workspace_bytes": 0}, {"workspace_bytes": 1000}, {"workspace": A[6] + 8},
+            {"workspace_bytes": size - 1}]
+
+
+@pytest.mark.parametrize("max_query", (4, 400))  # streamed, and in tiles
+def test_chunk_declines_without_its_workspace(lib, max_query):
+    long = dict(CHUNK, tokens=400, stride=256, width=256, max_query=max_query)
+    size = lib.kvq_splitzip_chunk_attention_workspace_bytes(400, 2, 8, 2, 128, 4096, max_query)
+    assert size > 1000
+    refused(lib.kvq_splitzip_chunk_attention_paged, long, no_workspace(size))
+    # contexts that are never split need none
+    assert lib.kvq_splitzip_chunk_attention_workspace_bytes(400, 2, 8, 2, 128, 128, max_query) == 0
 
 
 PROMPT = dict(q=A[0], q_row=2048, q_head=256, k=A[1], k_row=512, k_head=256, v=A[2], v_row=512,
@@ -83,10 +97,18 @@ PROMPT = dict(q=A[0], q_row=2048, q_head=256, k=A[1], k_row=512, k_head=256, v=A
 def test_prompt_declines(lib):
     refused(lib.kvq_splitzip_prompt_attention, PROMPT, [
         {name: 0} for name in ("q", "k", "v", "tokens", "q_heads", "kv_heads", "dim", "starts",
-                               "requests", "max_query", "out", "workspace", "workspace_bytes")] + [
+                               "requests", "max_query", "out")] + [
         {"dim": 80}, {"dtype": 2}, {"q_heads": 9}, {"max_query": 5}, {"k": A[1] + 4},
-        {"k_row": 500}, {"v_head": 8}, {"out": A[4] + 4}, {"workspace_bytes": 1000},
+        {"k_row": 500}, {"v_head": 8}, {"out": A[4] + 4},
         {"scale": ctypes.c_float(-0.5)}, {"out": A[1]}, {"out": A[2] + 512}, {"out": A[0]}])
+
+
+def test_prompt_declines_without_its_workspace(lib):
+    long = dict(PROMPT, tokens=2000, max_query=2000, workspace=A[6])
+    size = lib.kvq_splitzip_prompt_attention_workspace_bytes(2000, 2, 8, 2, 128, 2000)
+    assert size > 1000
+    refused(lib.kvq_splitzip_prompt_attention, long, no_workspace(size))
+    assert lib.kvq_splitzip_prompt_attention_workspace_bytes(2000, 2, 8, 2, 128, 400) == 0
 
 
 def test_workspace_sizes(lib):

@@ -56,12 +56,17 @@ constexpr int tile_waves(int D) { return D == 128 ? 8 : 4; }
 constexpr int tile_rows(int D) { return 32 * tile_waves(D); }
 constexpr int kMergeThreads = 256;
 constexpr int kFewRows = 16;      // rows of a request that attention_few takes
-constexpr int kFewStep = 32;      // tokens of a wave's step in attention_few; a workgroup's waves
-                                  // take a round of them, the unit of its splits
+constexpr int kFewStep = 32;      // tokens of a wave's step in attention_few,
+constexpr int kFewUnit = kWaves * kFewStep;  // of a round of its workgroup's: unit of its splits
 constexpr int kTileTokens = 64;   // tokens of a step of attention_tiles: unit of its splits
 // Steps of a split, at least: its start and its share of the joining take as long as some of them (4
 // requests of 64 tokens behind 4000: 39.1 us at 12, 44.8 at 16).
 constexpr unsigned int kLeastTileSteps = 12;
+// Of a streamed split, in rounds of kFewUnit tokens (16 requests of 1024 tokens, 32 / 8 heads of 128:
+// 22.2 us at 4, 26.8 at 1; 4 of 4096: 22.4 and 24.6). A call whose block tables hold no more than
+// kWholeFewSteps is not cut at all and joins nothing: one launch (one request, 32 / 8 heads of 64, 1024
+// tokens: 14.1 us, cut 16.7; of 128, 768 tokens 13.7 and 16.0, 1024 the same, 1536 21.1 and 16.0).
+constexpr unsigned int kLeastFewSteps = 4, kWholeFewSteps = 8;
 // A maximum before any token: the lowest float, not -inf, so that rows whose scores are all -inf
 // have weights of zero and a sum of zero (whose quotient is NaN, as the formula's).
 constexpr float kNoMax = -3.402823466e38f;
@@ -228,7 +233,7 @@ __device__ __forceinline__ unsigned int share_of(unsigned long long sum, unsigne
 // than there are tiles.
 template <bool kTiles, int kRows>
 struct Work {
-  static constexpr unsigned int kStep = kTiles ? kTileTokens : kWaves * kFewStep;
+  static constexpr unsigned int kStep = kTiles ? kTileTokens : kFewUnit;
   const AttendArgs& a;
   Request first;
   unsigned int cap;  // steps of a split, at most; 0: nothing is cut
@@ -261,7 +266,8 @@ struct Work {
       steps += lane_value(wave_scan((unsigned int)min(own, (unsigned long long)kMostSteps)), 63);
     }
     const unsigned int parts = kTiles ? a.tile_target : a.few_target;
-    if (!large) cap = max(kTiles ? kLeastTileSteps : 1u, share_of(steps * a.kv_heads, parts));
+    const unsigned int least = kTiles ? kLeastTileSteps : a.slots == 0 ? kWholeFewSteps : kLeastFewSteps;
+    if (!large) cap = max(least, share_of(steps * a.kv_heads, parts));
   }
 
   // The lanes' requests with the longest contexts first.
@@ -1341,8 +1347,9 @@ Plan plan_of(unsigned long long tokens, unsigned long long requests, unsigned lo
     p.items = tiles + more;
     p.groups = (p.items + (cut ? 1 : 0)) * kv_heads;
   } else {
-    const unsigned long long most = std::max(1ull, (max_context + Work<false, kFewRows>::kStep - 1) / Work<false, kFewRows>::kStep);
-    p.groups = p.slots = std::min(active * most, p.few_target / kv_heads + active + 1) * kv_heads;
+    const bool cut = max_context > kFewUnit * kWholeFewSteps;
+    p.groups = active * kv_heads;
+    if (cut) p.groups = p.slots = (p.few_target / kv_heads + active + 1) * kv_heads;
   }
   return p;
 }

@@ -1390,7 +1390,8 @@ def chunk_attention_workspace_bytes(tokens: int, requests: int, q_heads: int, kv
                                     head_dim: int, max_context: int,
                                     max_query: int | None = None) -> int:
     """Workspace of ``chunk_attention_paged`` for ``tokens`` rows of q, with ``max_context`` the
-    tokens that a row of the block tables can hold (its width in blocks * block_tokens)."""
+    tokens that a row of the block tables can hold (its width in blocks * block_tokens). 0: none
+    is needed."""
     lib = _load()
     if lib is None or not hasattr(lib, "kvq_splitzip_chunk_attention_workspace_bytes"):
         raise RuntimeError(f"HIP codec library not loaded: {load_error()}")
@@ -1487,14 +1488,15 @@ def chunk_attention_paged(q, kv_layer, tables, query_starts, context_tokens, *,
     need = _attention_workspace(
         "kvq_splitzip_chunk_attention_workspace_bytes", device,
         (tokens, requests, q_heads, kv_heads, head_dim, width * block_tokens, max_query))
-    if not _byte_buffer_ok(workspace, device, need, torch):
-        workspace = torch.empty(max(need, 16), dtype=torch.uint8, device=device)
+    if need and not _byte_buffer_ok(workspace, device, need, torch):
+        workspace = torch.empty(need, dtype=torch.uint8, device=device)
     got = _call_on(device, torch, attend, q.data_ptr(), 2 * q.stride(0), 2 * q.stride(1), tokens,
                    q_heads, kv_heads, head_dim, dtype, kv_layer.data_ptr(), blocks, block_tokens,
                    tables.data_ptr(), tables.stride(0) if requests > 1 else width, width,
                    query_starts.data_ptr(), context_tokens.data_ptr(), requests, max_query,
-                   out.data_ptr(), 0 if lse is None else lse.data_ptr(), workspace.data_ptr(),
-                   workspace.numel(), head_dim ** -0.5 if scale is None else float(scale))
+                   out.data_ptr(), 0 if lse is None else lse.data_ptr(),
+                   workspace.data_ptr() if need else 0, need,
+                   head_dim ** -0.5 if scale is None else float(scale))
     if got < 0:
         _raise_last(lib, "splitzip chunk attention failed")
     return out if got else None
@@ -1540,13 +1542,13 @@ def prompt_attention(q, k, v, query_starts, *, max_query: int | None = None,
     need = _attention_workspace(
         "kvq_splitzip_prompt_attention_workspace_bytes", device,
         (tokens, requests, q_heads, kv_heads, head_dim, max_query))
-    if not _byte_buffer_ok(workspace, device, need, torch):
-        workspace = torch.empty(max(need, 16), dtype=torch.uint8, device=device)
+    if need and not _byte_buffer_ok(workspace, device, need, torch):
+        workspace = torch.empty(need, dtype=torch.uint8, device=device)
     got = _call_on(device, torch, attend, q.data_ptr(), 2 * q.stride(0), 2 * q.stride(1),
                    k.data_ptr(), 2 * k.stride(0), 2 * k.stride(1), v.data_ptr(),
                    2 * v.stride(0), 2 * v.stride(1), tokens, q_heads, kv_heads, head_dim, dtype,
                    query_starts.data_ptr(), requests, max_query, out.data_ptr(),
-                   0 if lse is None else lse.data_ptr(), workspace.data_ptr(), workspace.numel(),
+                   0 if lse is None else lse.data_ptr(), workspace.data_ptr() if need else 0, need,
                    head_dim ** -0.5 if scale is None else float(scale))
     if got < 0:
         _raise_last(lib, "splitzip prompt attention failed")
