@@ -55,7 +55,11 @@ constexpr int kWaves = 4;         // waves of a workgroup of attention_few, two 
 constexpr int tile_waves(int D) { return D == 128 ? 8 : 4; }
 constexpr int tile_rows(int D) { return 32 * tile_waves(D); }
 constexpr int kMergeThreads = 256;
-constexpr int kFewRows = 16;      // rows of a request that attention_few takes
+// Rows of a request that is streamed: by attention_few, and by attention_tiles where longer requests
+// are beside it (as tiles a chunk of 2048 behind 8192 and 64 single tokens, 32 / 8 heads of 64, take
+// 366 us, so 274; 3 chunks and 29 single tokens of 128-dim heads 310 and 298; 64 single tokens and 4
+// times 8, heads of 64, 202 and 218). 32 rows, as two sets of 16, gained nothing over tiles.
+constexpr int kFewRows = 16;
 constexpr int kFewStep = 32;      // tokens of a wave's step in attention_few,
 constexpr int kFewUnit = kWaves * kFewStep;  // of a round of its workgroup's: unit of its splits
 constexpr int kTileTokens = 64;   // tokens of a step of attention_tiles: unit of its splits
@@ -231,22 +235,29 @@ __device__ __forceinline__ unsigned int share_of(unsigned long long sum, unsigne
 // most that, all of about one length. A cut tile has at least two, so that all cut tiles together
 // have at most twice (all steps / cap) splits, in as many slots, and at most (all steps / cap) more
 // than there are tiles.
-template <bool kTiles, int kRows>
+template <bool kTiles, int kRows, bool kStream>
 struct Work {
   static constexpr unsigned int kStep = kTiles ? kTileTokens : kFewUnit;
   const AttendArgs& a;
   Request first;
   unsigned int cap;  // steps of a split, at most; 0: nothing is cut
 
-  __device__ __forceinline__ unsigned int tiles(const Request& q) const {
-    return kTiles ? tiles_of<kRows>(a, q.n) : q.n != 0 ? 1u : 0u;
+  // whether a request of n tokens is streamed
+  __device__ __forceinline__ bool few(unsigned int n) const {
+    return !kTiles || (kStream && n * a.group <= kFewRows);
   }
-  __device__ __forceinline__ unsigned int splits(unsigned int tokens) const {
-    return cap == 0 ? 1u : max(1u, steps_of(steps_of(tokens, kStep), cap));
+  __device__ __forceinline__ unsigned int tiles(const Request& q) const {
+    return few(q.n) ? (q.n != 0 ? 1u : 0u) : tiles_of<kRows>(a, q.n);
+  }
+  __device__ __forceinline__ unsigned int steps(const Request& q) const {
+    return steps_of(q.ctx, kStep);
+  }
+  __device__ __forceinline__ unsigned int splits(const Request& q) const {
+    return cap == 0 ? 1u : max(1u, steps_of(steps(q), cap));
   }
   // tokens of a split of a request in `splits`
-  __device__ __forceinline__ unsigned int split_tokens(unsigned int tokens, unsigned int splits) const {
-    return steps_of(steps_of(tokens, kStep), splits) * kStep;
+  __device__ __forceinline__ unsigned int split_tokens(const Request& q, unsigned int splits) const {
+    return steps_of(steps(q), splits) * kStep;
   }
   __device__ __forceinline__ Request requests(unsigned int r0) const {
     return r0 == 0 ? first : load_request(a, r0 + __lane_id());
@@ -255,25 +266,24 @@ struct Work {
   __device__ __forceinline__ explicit Work(const AttendArgs& args)
       : a(args), first(load_request(args, __lane_id())), cap(0) {
     if (kTiles && a.requests > 1 && a.requests <= kWave) sort();
-    unsigned long long steps = 0, all = 0;
+    unsigned long long sum = 0;
     bool large = false;
     for (unsigned int r0 = 0; r0 < a.requests; r0 += kWave) {
       const Request q = requests(r0);
       const unsigned int t = tiles(q);
-      const unsigned long long own = (unsigned long long)t * steps_of(q.ctx, kStep);
+      const unsigned long long own = (unsigned long long)t * steps(q);
       large |= __ballot(own > kMostSteps) != 0;
-      all += lane_value(wave_scan(t), 63);
-      steps += lane_value(wave_scan((unsigned int)min(own, (unsigned long long)kMostSteps)), 63);
+      sum += lane_value(wave_scan((unsigned int)min(own, (unsigned long long)kMostSteps)), 63);
     }
     const unsigned int parts = kTiles ? a.tile_target : a.few_target;
     const unsigned int least = kTiles ? kLeastTileSteps : a.slots == 0 ? kWholeFewSteps : kLeastFewSteps;
-    if (!large) cap = max(least, share_of(steps * a.kv_heads, parts));
+    if (!large) cap = max(least, share_of(sum * a.kv_heads, parts));
   }
 
   // The lanes' requests with the longest contexts first.
   __device__ __forceinline__ void sort() {
     const unsigned int lane = __lane_id();
-    const unsigned int key = min(first.n != 0 ? steps_of(first.ctx, kStep) + 1 : 0u, kMostSteps) << 6 | (63 - lane);
+    const unsigned int key = min(first.n != 0 ? steps(first) + 1 : 0u, kMostSteps) << 6 | (63 - lane);
     unsigned int rank = 0;
     for (unsigned int j = 0; j < a.requests; ++j) rank += lane_value(key, (int)j) > key ? 1u : 0u;
     const int to = 4 * (int)(lane < a.requests ? rank : lane);
@@ -292,7 +302,7 @@ struct Work {
     unsigned long long before = 0, slots = 0;
     for (unsigned int r0 = 0; r0 < a.requests; r0 += kWave) {
       const Request l = requests(r0);
-      const unsigned int parts = splits(l.ctx), own = tiles(l) * parts, sum = wave_scan(own);
+      const unsigned int parts = splits(l), own = tiles(l) * parts, sum = wave_scan(own);
       const unsigned int slot_own = !kTiles || parts > 1 ? own : 0u, slot_sum = wave_scan(slot_own);
       const unsigned int all = lane_value(sum, 63);
       if (item < before + all) {
@@ -411,6 +421,17 @@ __device__ __forceinline__ void slow_row(const AttendArgs& a, const int* table, 
   }
 }
 
+// Whether any lane of the workgroup has it, through `space` in LDS.
+__device__ __forceinline__ bool any_lane(unsigned int has, unsigned char* space) {
+  unsigned int* const flag = reinterpret_cast<unsigned int*>(space);
+  __syncthreads();
+  if (threadIdx.x == 0) *flag = 0;
+  __syncthreads();
+  if (has) *flag = 1;
+  __syncthreads();
+  return *flag != 0;
+}
+
 // Where a row's result goes: the output (of one split), or its place among the partials, a
 // slot's rows as (m, l) pairs and then their D sums.
 template <int D, int kRows>
@@ -472,8 +493,10 @@ __device__ __forceinline__ void clear_jobs(const AttendArgs& a, unsigned int slo
 // rows; V's 64-byte quarters q at q ^ (t % 4), read transposed 8 bytes a lane, 4 tokens by 32 dims
 // per half wave.
 template <typename E, int D, bool kPaged, bool kRuns>
-__device__ __forceinline__ void tile_path(const AttendArgs& a, unsigned int block,
-                                          unsigned char* s0, unsigned char* s1,
+__device__ __forceinline__ void tile_path(const AttendArgs& a, const Request& request,
+                                          unsigned int index, unsigned int most,
+                                          unsigned int split_tokens, unsigned int slot,
+                                          unsigned int head, unsigned char* s0, unsigned char* s1,
                                           unsigned char* s2) {
   typedef typename Elem<E>::x8 x8;
   constexpr int kRowBytes = 2 * D, kPieces = kRowBytes / 16;  // pieces of a row
@@ -485,21 +508,7 @@ __device__ __forceinline__ void tile_path(const AttendArgs& a, unsigned int bloc
 
   const unsigned int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
   const unsigned int half = lane / 32, col = lane % 32;
-  const unsigned int head = block % a.kv_heads, item = block / a.kv_heads;
-  const Work<true, kTileRows> work(a);
-  Request request;
-  unsigned int index, slot;
-  bool has_slot;
-  const bool found = work.find(item, request, index, has_slot, slot);
-  if (item == a.items) {  // the last one, for the slots that the others do not use
-    clear_jobs(a, slot, head);
-    return;
-  }
-  if (!found) return;
-  const unsigned int own_slot = slot;
-  slot = slot * a.kv_heads + head;
   // the tiles with the longest contexts first
-  const unsigned int most = work.splits(request.ctx);
   const unsigned int tile = tiles_of<kTileRows>(a, request.n) - 1 - index / most, split = index % most;
   const unsigned int rows = request.n * a.group;
   const unsigned int m0 = tile * kTileRows;
@@ -507,13 +516,13 @@ __device__ __forceinline__ void tile_path(const AttendArgs& a, unsigned int bloc
   const int shift = (int)request.ctx - (int)request.n;
   const int last_of_tile = shift + (int)((min(rows, m0 + kTileRows) - 1) / a.group);
   const unsigned int seen = last_of_tile < 0 ? 0u : (unsigned int)last_of_tile + 1;
-  const unsigned int split_tokens = work.split_tokens(request.ctx, most);
   const unsigned int splits = most == 1 ? 1u : max(1u, steps_of(seen, split_tokens));  // of this tile
   if (most > 1)
-    store_job(a, own_slot, head,
-            Job{request.start, m0, shift, (unsigned short)min(rows - m0, (unsigned int)kTileRows),
-                (unsigned short)(split == 0 && splits > 1 ? splits : 0u)});
+    store_job(a, slot, head,
+              Job{request.start, m0, shift, (unsigned short)min(rows - m0, (unsigned int)kTileRows),
+                  (unsigned short)(split == 0 && splits > 1 ? splits : 0u)});
   if (split >= splits) return;
+  slot = slot * a.kv_heads + head;
   const unsigned int t_begin = split * split_tokens;
   const unsigned int t_end = splits == 1 ? seen : min(seen, t_begin + split_tokens);
   const unsigned int mw = m0 + wave * 32, m = mw + col;
@@ -865,7 +874,7 @@ __device__ __forceinline__ void tile_path(const AttendArgs& a, unsigned int bloc
     wait_loads<0>();
   }
 
-  bad = __syncthreads_or(bad) != 0;
+  bad = any_lane(bad, s2);
   l_run += __shfl_xor(l_run, 32, 64);
   float check = l_run * 0.f;
 #pragma unroll
@@ -929,34 +938,24 @@ __device__ __forceinline__ void tile_path(const AttendArgs& a, unsigned int bloc
 // tokens: K as the first operand of S^T = K Q^T straight from memory (lane l: token l % 16, 16
 // bytes at 16 (l / 16) of every 64), V through the wave's own LDS, without a barrier, with 32-byte
 // pieces of row t at piece ^ (t % 8), so that the 16 tokens of a transposed read spread over the
-// banks. The waves of a workgroup take turns at 32 tokens of a split and join their sums in LDS.
-template <typename E, int D>
-__device__ __forceinline__ void few_path(const AttendArgs& a, unsigned int block, unsigned char* s0,
-                                         unsigned char* s1) {
+// banks. The kN waves of a workgroup take turns at 32 tokens of a split and join their sums in LDS
+// (s0, s1: the waves' stages, and then s0 their sums; s2: their (m, l)). kRows: of a slot.
+template <typename E, int D, int kN, int kRows>
+__device__ __forceinline__ void few_path(const AttendArgs& a, const Request& request, unsigned int split,
+                                         unsigned int splits, unsigned int split_tokens, unsigned int slot,
+                                         unsigned int head, unsigned char* __restrict__ s0,
+                                         unsigned char* __restrict__ s1,
+                                         unsigned char* __restrict__ s2) {
   typedef typename Elem<E>::x8 x8;
   constexpr int kRowBytes = 2 * D, kPieces = kRowBytes / 16;
   constexpr int kRowsPerLoad = kWave / kPieces, kLoads = kFewStep / kRowsPerLoad;
   constexpr int kStageBytes = kFewStep * kRowBytes;
   constexpr int kSlabs = D / 32, kDimTiles = D / 16;
-  constexpr unsigned int kRound = Work<false, kFewRows>::kStep;  // of all waves
-  // the waves' sums, then their (m, l), once the stages are read
-  float* const s_acc = reinterpret_cast<float*>(s0);
-  float* const s_ml = reinterpret_cast<float*>(s1);
+  constexpr unsigned int kRound = kN * kFewStep;
   static_assert(kStageBytes >= kFewRows * D * 4, "a wave's sums fit its stage");
 
   const unsigned int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
   const unsigned int col = lane % 16, grp = lane / 16;
-  const unsigned int head = block % a.kv_heads, item = block / a.kv_heads;
-  const Work<false, kFewRows> work(a);
-  Request request;
-  unsigned int split, slot;
-  bool has_slot;
-  if (!work.find(item, request, split, has_slot, slot)) {
-    store_job(a, item, head, Job{});
-    return;
-  }
-  const unsigned int splits = work.splits(request.ctx);
-  const unsigned int split_tokens = work.split_tokens(request.ctx, splits);
   store_job(a, slot, head,
             Job{request.start, 0, (int)request.ctx - (int)request.n,
                 (unsigned short)(request.n * a.group),
@@ -966,23 +965,21 @@ __device__ __forceinline__ void few_path(const AttendArgs& a, unsigned int block
   const unsigned int t_begin = split * split_tokens;
   const unsigned int t_end = splits == 1 ? request.ctx : min(request.ctx, t_begin + split_tokens);
   const int shift = (int)request.ctx - (int)request.n;
-  const bool valid = col < rows;
-  const unsigned int token = valid ? col / a.group : 0u;
-  const unsigned int q_head = head * a.group + (valid ? col - token * a.group : 0u);
-  const int limit = valid ? shift + (int)token : -1;
 
   const int* table = a.tables + request.r * a.table_stride;
   const unsigned char* kb = a.k + head * a.k_head;
   const unsigned char* vb = a.v + head * a.v_head;
   unsigned int bad = request.bad ? 1u : 0u;
 
+  const bool valid = col < rows;
+  const unsigned int token = valid ? col / a.group : 0u;
+  const unsigned int q_head = head * a.group + (valid ? col - token * a.group : 0u);
+  const int limit = valid ? shift + (int)token : -1;
   x8 q[kSlabs];
   const unsigned char* q_row = a.q + (unsigned long long)(request.start + token) * a.q_row +
                                (unsigned long long)q_head * a.q_head;
 #pragma unroll
-  for (int s = 0; s < kSlabs; ++s) {
-    q[s] = *reinterpret_cast<const x8*>(q_row + 64 * s + 16 * grp);
-  }
+  for (int s = 0; s < kSlabs; ++s) q[s] = *reinterpret_cast<const x8*>(q_row + 64 * s + 16 * grp);
 
   struct Keys {
     u32x4 v[2][kSlabs];
@@ -1089,10 +1086,13 @@ __device__ __forceinline__ void few_path(const AttendArgs& a, unsigned int block
   }
   wait_loads<0>();
 
-  // ---- the waves' sums meet in LDS, thread t takes row t / 16 and D / 16 dims of it ----
+  // ---- the waves' sums meet in LDS, a thread takes kVals dims of a row ----
   l_run += __shfl_xor(l_run, 16, 64);
   l_run += __shfl_xor(l_run, 32, 64);
-  bad = __syncthreads_or(bad) != 0;
+  bad = any_lane(bad, s2);
+  __syncthreads();
+  float* const s_acc = reinterpret_cast<float*>(s0);
+  float* const s_ml = reinterpret_cast<float*>(s2);
   if (grp == 0) {
     s_ml[2 * (wave * kFewRows + col)] = m_ref;
     s_ml[2 * (wave * kFewRows + col) + 1] = l_run;
@@ -1101,15 +1101,17 @@ __device__ __forceinline__ void few_path(const AttendArgs& a, unsigned int block
   for (int d = 0; d < kDimTiles; ++d)
     *reinterpret_cast<f32x4*>(s_acc + (wave * kFewRows + col) * D + 16 * d + 4 * grp) = o[d];
   __syncthreads();
-  constexpr int kVals = D / 16;
-  const unsigned int row_m = tid / 16, d0 = (tid % 16) * kVals;
+  constexpr unsigned int kShare = 4 * kN;  // threads of a row
+  constexpr int kVals = D / kShare;
+  static_assert(kVals == 4 || kVals == 8, "stored by 16 bytes");
+  const unsigned int row_m = tid / kShare, d0 = (tid % kShare) * kVals;
   float big = kNoMax, l = 0.f, acc[kVals];
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) big = fmaxf(big, s_ml[2 * (w * kFewRows + row_m)]);
+  for (int w = 0; w < kN; ++w) big = fmaxf(big, s_ml[2 * (w * kFewRows + row_m)]);
 #pragma unroll
   for (int i = 0; i < kVals; ++i) acc[i] = 0.f;
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
+  for (int w = 0; w < kN; ++w) {
     const float f = exp2f(s_ml[2 * (w * kFewRows + row_m)] - big);
     l += s_ml[2 * (w * kFewRows + row_m) + 1] * f;
 #pragma unroll
@@ -1119,7 +1121,7 @@ __device__ __forceinline__ void few_path(const AttendArgs& a, unsigned int block
 #pragma unroll
   for (int i = 0; i < kVals; ++i) check = fmaf(acc[i], 0.f, check);
 #pragma unroll
-  for (int d = 1; d < 16; d *= 2) check += __shfl_xor(check, d, 64);
+  for (unsigned int d = 1; d < kShare; d *= 2) check += __shfl_xor(check, d, 64);
   const bool in = row_m < rows;
   const bool again = in && !bad && !(check == 0.f);
   const unsigned int tok = in ? row_m / a.group : 0u;
@@ -1128,8 +1130,8 @@ __device__ __forceinline__ void few_path(const AttendArgs& a, unsigned int block
   if (bad) big = l = NAN;
   if (in && !again) {
     if (splits > 1) {
-      float* ml = slot_ml<D, kFewRows>(a, slot) + 2 * row_m;
-      float* dst = slot_acc<D, kFewRows>(a, slot) + row_m * D + d0;
+      float* ml = slot_ml<D, kRows>(a, slot) + 2 * row_m;
+      float* dst = slot_acc<D, kRows>(a, slot) + row_m * D + d0;
       if (d0 == 0) {
         ml[0] = big;
         ml[1] = l;
@@ -1149,17 +1151,17 @@ __device__ __forceinline__ void few_path(const AttendArgs& a, unsigned int block
   }
   const unsigned long long flags = __ballot(again);
 #pragma unroll 1
-  for (unsigned int i = 0; i < 4; ++i) {
-    if (((flags >> (16 * i)) & 1) == 0) continue;
-    const unsigned int mm = 4 * wave + i, t = mm / a.group, h = head * a.group + mm % a.group;
+  for (unsigned int i = 0; i < kWave / kShare; ++i) {
+    if (((flags >> (kShare * i)) & 1) == 0) continue;
+    const unsigned int mm = kWave / kShare * wave + i, t = mm / a.group, h = head * a.group + mm % a.group;
     const unsigned int seen = (unsigned int)max(shift + (int)t + 1, 0);
     float rm, rl, ra[D / 64];
     slow_row<E, D, true>(a, table, request.start,
                          a.q + (unsigned long long)(request.start + t) * a.q_row +
                              (unsigned long long)h * a.q_head,
                          head, t_begin, min(t_end, seen), rm, rl, ra);
-    store_slow<E, D, kFewRows>(a, splits > 1, slot, mm,
-                     (unsigned long long)(request.start + t) * a.q_heads + h, seen == 0, rm, rl, ra);
+    store_slow<E, D, kRows>(a, splits > 1, slot, mm,
+                            (unsigned long long)(request.start + t) * a.q_heads + h, seen == 0, rm, rl, ra);
   }
 }
 
@@ -1170,11 +1172,32 @@ __device__ __forceinline__ void few_path(const AttendArgs& a, unsigned int block
 // behind those into the others)
 template <typename E, int D, bool kPaged, bool kRuns>
 __global__ __launch_bounds__(kWave * tile_waves(D), D == 128 ? 2 : 3) void attention_tiles(AttendArgs a) {
+  constexpr int kN = tile_waves(D), kRows = tile_rows(D);
   constexpr int kBuffer = 2 * kTileTokens * 2 * D;
-  __shared__ __align__(1024) unsigned char s0[kBuffer];
-  __shared__ __align__(1024) unsigned char s1[kBuffer];
+  constexpr int kStages = kPaged ? kN * kFewStep * 2 * D : kBuffer;  // of the streaming waves
+  __shared__ __align__(1024) unsigned char s0[kStages];
+  __shared__ __align__(1024) unsigned char s1[kStages];
   __shared__ __align__(1024) unsigned char s2[kBuffer];
-  tile_path<E, D, kPaged, kRuns>(a, blockIdx.x, s0, s1, s2);
+  const unsigned int head = blockIdx.x % a.kv_heads, item = blockIdx.x / a.kv_heads;
+  const Work<true, kRows, kPaged> work(a);
+  Request request;
+  unsigned int index, slot;
+  bool has_slot;
+  const bool found = work.find(item, request, index, has_slot, slot);
+  if (item == a.items) {  // the last one, for the slots that the others do not use
+    clear_jobs(a, slot, head);
+    return;
+  }
+  if (!found) return;
+  const unsigned int most = work.splits(request), split_tokens = work.split_tokens(request, most);
+  if constexpr (kPaged) {
+    if (work.few(request.n)) {
+      if (!has_slot) slot = kNoSlot;
+      few_path<E, D, kN, kRows>(a, request, index, most, split_tokens, slot, head, s0, s1, s2);
+      return;
+    }
+  }
+  tile_path<E, D, kPaged, kRuns>(a, request, index, most, split_tokens, slot, head, s0, s1, s2);
 }
 
 template <typename E, int D>
@@ -1182,7 +1205,19 @@ __global__ __launch_bounds__(kWave * kWaves, 2) void attention_few(AttendArgs a)
   constexpr int kBuffer = kWaves * kFewStep * 2 * D;
   __shared__ __align__(1024) unsigned char s0[kBuffer];
   __shared__ __align__(1024) unsigned char s1[kBuffer];
-  few_path<E, D>(a, blockIdx.x, s0, s1);
+  __shared__ __align__(16) unsigned char s2[kWaves * 16 * 2 * sizeof(float)];
+  const unsigned int head = blockIdx.x % a.kv_heads, item = blockIdx.x / a.kv_heads;
+  const Work<false, kFewRows, true> work(a);
+  Request request;
+  unsigned int split, slot;
+  bool has_slot;
+  if (!work.find(item, request, split, has_slot, slot)) {
+    store_job(a, item, head, Job{});
+    return;
+  }
+  const unsigned int splits = work.splits(request);
+  few_path<E, D, kWaves, kFewRows>(a, request, split, splits, work.split_tokens(request, splits), slot,
+                                   head, s0, s1, s2);
 }
 
 // ---------------------------------------------------------------------------
