@@ -345,3 +345,113 @@ def test_attention_refuses(sz):
     assert sz.prompt_attention(q, k, k, starts, out=q) is None
     assert sz.prompt_attention(q.clone().requires_grad_(), k, k, starts) is None
     assert sz.prompt_attention(q, k, k, starts[:1]) is not None  # no prompts
+
+
+@pytest.mark.parametrize("q_heads,kv_heads,dim,block,dtype", [
+    (8, 2, 128, 16, "bf16"), (8, 2, 64, 8, "fp16"), (4, 4, 64, 24, "bf16"), (3, 1, 128, 7, "fp16")])
+def test_single_tokens_beside_chunks(sz, q_heads, kv_heads, dim, block, dtype):
+    """Streamed requests, short and cut into splits, in one call with tiles, cut ones too."""
+    new, contexts = [1, 70, 2, 1, 0, 33, 1, 3], [5000, 4100, 2600, 1, 900, 33, 129, 0]
+    say("beside", q_heads, kv_heads, dim, block, dtype)
+    case = Case(new, contexts, q_heads, kv_heads, dim, block, dtype, seed=dim + block)
+    case.verify(*case.run(sz))
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+def test_streamed_values_and_blocks_beside_chunks(sz, dim, value):
+    """What a streamed request's rows do not see does not reach them, nor another request; a table
+    entry that is no block makes its rows NaN, in whichever split it is read."""
+    case = Case([3, 90, 1], [2600, 300, 2500], 4, 2, dim, 16, "bf16", seed=dim)
+    t = 2598  # the second new token
+    case.kv[1, int(case.tables[0, t // 16]), t % 16, 1, 9] = value
+    case.v[0][t, 1, 9] = value
+    case.tables[2, 3] = case.kv.shape[1] + 4
+    out, lse = case.run(sz)
+    case.verify(out, lse, skip=(2,))
+    assert torch.isnan(out[93]).all() and torch.isnan(lse[93]).all()
+
+
+@pytest.mark.parametrize("longest,context", [(1, 700), (1, 3000), (40, 1500)])
+def test_more_requests_than_lanes(sz, longest, context):
+    """150 requests: three loads of lengths, in order and with empty ones between."""
+    rng = np.random.default_rng(longest + context)
+    new = [int(n) for n in rng.integers(0, 2, 150)]
+    new[77], new[149] = longest, 1
+    contexts = [int(c) for c in rng.integers(1, 90, 150)]
+    contexts[3], contexts[77], contexts[149] = context, context, 1200
+    new[3] = 1
+    say("requests", longest, context)
+    case = Case(new, contexts, 4, 2, 64, 16, "bf16", seed=longest)
+    case.verify(*case.run(sz))
+
+
+@pytest.mark.parametrize("heads,dim,dtype,new", [
+    ((4, 1), 128, "bf16", [1100, 3, 900]), ((2, 2), 64, "fp16", [1700])])
+def test_long_prompts_in_splits(sz, heads, dim, dtype, new):
+    say("long prompts", heads, dim, dtype, new)
+    q_heads, kv_heads = heads
+    rng = np.random.default_rng(dim)
+    rows = sum(new) + 1
+    packed = torch.from_numpy(rng.standard_normal((rows, q_heads + 2 * kv_heads, dim)).astype(
+        np.float32)).to(DTYPES[dtype]).cuda()
+    q, k, v = packed.split((q_heads, kv_heads, kv_heads), 1)
+    out = torch.full((rows, q_heads, dim), MARK, dtype=DTYPES[dtype], device="cuda")
+    assert sz.prompt_attention(q, k, v, starts_of(new), out=out) is out
+    torch.cuda.synchronize()
+    got, at = f64(out), 0
+    for n in new:
+        part = slice(at, at + n)
+        ref, _, mean, off = attend(f64(q[part]), f64(k[part]), f64(v[part]), 0, dim ** -0.5)
+        check(got[part], ref, mean, off, dtype, n, np.abs(f64(v[part])).max())
+        at += n
+    assert np.all(got[at:] == MARK)
+
+
+def test_one_workspace_for_steps_of_any_lengths(sz):
+    """A captured call and eager ones of other sizes take turns with one workspace: what one left in
+    it (slots of splits that the next does not have) changes nothing."""
+    long = Case([1, 40, 1], [3000, 2900, 2000], 8, 2, 128, 16, "bf16", seed=20)
+    short = Case([40, 1, 1], [50, 60, 900], 8, 2, 128, 16, "bf16", seed=21)
+    few = Case([1] * 5, [2000, 300, 4000, 1, 90], 8, 2, 128, 16, "bf16", seed=22)
+    size = max(sz.chunk_attention_workspace_bytes(c.q.shape[0], len(c.new), 8, 2, 128,
+                                                  c.tables.shape[1] * 16, most)
+               for c, most in ((long, 40), (short, 40), (few, 1)))
+    space = torch.full((size,), 255, dtype=torch.uint8, device="cuda")
+    runs = [(long, 40), (short, 40), (few, 1)]
+    for case, most in runs:
+        case.verify(*case.run(sz, workspace=space, max_query=most))
+    out = torch.full(long.q.shape, MARK, dtype=long.q.dtype, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        sz.chunk_attention_paged(long.q, long.kv, long.tables, long.starts, long.ctx, out=out,
+                                 workspace=space, max_query=40)
+    whole, _ = long.run(sz)
+    lengths = [3000, 2900, 2000]
+    for turn in range(4):
+        say("turn", turn)
+        case, most = runs[1 + turn % 2]
+        case.verify(*case.run(sz, workspace=space, max_query=most))
+        out.fill_(MARK)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, whole)
+        # the same graph with short contexts, which it does not cut
+        long.ctx.copy_(i32([50, 60, 70]))
+        short_run, _ = long.run(sz)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, short_run)
+        long.ctx.copy_(i32(lengths))
+
+
+def test_ranges_that_overlap_stay_inside_the_call(sz):
+    """Starts that run backwards name more rows than q has: more tiles than the call launches. Rows
+    may be left, every other one is right, and nothing outside is written."""
+    case = Case([40, 40, 40], [3000, 3000, 3000], 4, 1, 64, 16, "bf16", seed=30)
+    case.starts = i32([0, 120, 0, 120])
+    case.ctx = i32([3000, 3000, 3000])
+    out, _ = case.run(sz)
+    assert (out[120:] == MARK).all()
+    fresh = Case([40, 40, 40], [3000, 3000, 3000], 4, 1, 64, 16, "bf16", seed=30)
+    fresh.verify(*fresh.run(sz))
