@@ -55,6 +55,9 @@ constexpr int kWaves = 4;         // waves of a workgroup of attention_few, two 
 constexpr int tile_waves(int D) { return D == 128 ? 8 : 4; }
 constexpr int tile_rows(int D) { return 32 * tile_waves(D); }
 constexpr int kMergeThreads = 256;
+// An odd count, so that the slots of the first splits, which have the work and lie at even distances,
+// fall to all of them (32 requests of 8192 tokens: 7.2 us, 11.6 with 1024 workgroups).
+constexpr unsigned int kMergeGroups = 1021;
 // Rows of a request that is streamed: by attention_few, and by attention_tiles where longer requests
 // are beside it (as tiles a chunk of 2048 behind 8192 and 64 single tokens, 32 / 8 heads of 64, take
 // 366 us, so 274; 3 chunks and 29 single tokens of 128-dim heads 310 and 298; 64 single tokens and 4
@@ -277,7 +280,7 @@ struct Work {
     }
     const unsigned int parts = kTiles ? a.tile_target : a.few_target;
     const unsigned int least = kTiles ? kLeastTileSteps : a.slots == 0 ? kWholeFewSteps : kLeastFewSteps;
-    if (!large) cap = max(least, share_of(sum * a.kv_heads, parts));
+    if (!large && (!kTiles || a.slots != 0)) cap = max(least, share_of(sum * a.kv_heads, parts));
   }
 
   // The lanes' requests with the longest contexts first.
@@ -1229,7 +1232,7 @@ __global__ __launch_bounds__(kWave * kWaves, 2) void attention_few(AttendArgs a)
 template <typename E, int D, bool kTiles>
 __global__ __launch_bounds__(kMergeThreads) void attention_merge(AttendArgs a) {
   constexpr int kRows = kTiles ? tile_rows(D) : kFewRows;
-  constexpr int kVals = D / 16, kBatch = 8;
+  constexpr int kVals = D / 16, kBatch = 4;
   constexpr unsigned int kShares = kTiles ? 1 : 4;  // threads that share a row's splits
   constexpr unsigned int kJobRows = 16 / kShares, kParts = kRows / kJobRows;
   __shared__ float s_part[kTiles ? 1 : kMergeThreads][kVals + 2];
@@ -1241,10 +1244,13 @@ __global__ __launch_bounds__(kMergeThreads) void attention_merge(AttendArgs a) {
     unsigned long long todo =
         __ballot(mine < jobs && own.splits != 0 && mine % kParts * kJobRows < own.rows);
     while (todo != 0) {
-      const unsigned int j = j0 + ((unsigned int)__ffsll((long long)todo) - 1) * gridDim.x;
+      const int at = __ffsll((long long)todo) - 1;
+      const unsigned int j = j0 + (unsigned int)at * gridDim.x;
       todo &= todo - 1;
       const unsigned int slot = j / kParts, head = slot % a.kv_heads;
-      const Job job = a.jobs[slot];
+      const unsigned int counts = lane_value((unsigned int)own.splits << 16 | own.rows, at);
+      const Job job{lane_value(own.start, at), lane_value(own.first, at), (int)lane_value((unsigned int)own.shift, at),
+                    (unsigned short)counts, (unsigned short)(counts >> 16)};
       const unsigned int share = tid / 16 % kShares, dims = tid % 16 * kVals;
       const unsigned int row = j % kParts * kJobRows + tid / (16 * kShares);
       const bool in = row < job.rows;
@@ -1374,8 +1380,23 @@ Plan plan_of(unsigned long long tokens, unsigned long long requests, unsigned lo
   p.tile_target = std::max(1ull, compute_units() * (head_dim == 128 ? 3 : 6) / 4);
   const unsigned long long active = std::min(tokens, requests);
   if (p.tiles) {
-    const unsigned long long tiles = tokens * group / tile_rows((int)head_dim) + active;
-    const bool cut = max_context > kTileTokens * kLeastTileSteps;
+    const unsigned long long rows = (unsigned long long)tile_rows((int)head_dim);
+    const unsigned long long tiles = tokens * group / rows + active;
+    const double whole = kTileTokens * kLeastTileSteps;
+    bool cut = (double)max_context > whole;
+    if (cut && !paged) {
+      // A prompt of L of the n rows of q, of r prompts that fill them, is cut where its L / 64 steps are
+      // more than a workgroup's share of all, which is at least that of L * group / rows tiles of L
+      // tokens and of the r - 1 others at equal lengths: L > share * (L^2 + (n - L)^2 / (r - 1)).
+      // Where that holds for no length, nothing is cut, which spares the joining (7 us). Prompts that
+      // do not fill the rows are not cut then either.
+      const double n = (double)tokens, others = (double)active - 1;
+      const double share = (double)(group * kv_heads) / (double)(rows * p.tile_target);
+      double l = n;
+      if (others > 0)  // where the right side is least above the left
+        l = std::min(std::max((0.5 / share + n / others) / (1 + 1 / others), whole), (double)max_context);
+      cut = l > share * (l * l + (others > 0 ? (n - l) * (n - l) / others : 0.));
+    }
     // (see Work; the share of one KV head)
     const unsigned long long more = cut ? p.tile_target / kv_heads + 1 : 0;
     p.slots = 2 * more * kv_heads;
@@ -1401,7 +1422,7 @@ template <typename E, int D, bool kTiles>
 hipError_t launch_merge(const AttendArgs& a, hipStream_t stream) {
   const unsigned int jobs = a.slots * (kTiles ? tile_rows(D) / 16 : kFewRows / 4);
   if (jobs == 0) return hipSuccess;  // (no context that is long enough to be split)
-  hipLaunchKernelGGL((attention_merge<E, D, kTiles>), dim3(std::min(jobs, 1024u)),
+  hipLaunchKernelGGL((attention_merge<E, D, kTiles>), dim3(std::min(jobs, kMergeGroups)),
                      dim3(kMergeThreads), 0, stream, a);
   return hipGetLastError();
 }
