@@ -15,9 +15,13 @@
 // Two kernels, by the rows that a request of the call can have:
 //   * attention_few: at most 16 (decode steps). Bound by reading K and V: a wave streams 32 tokens
 //     at a time, K straight into the matrix operand's registers, V into LDS for the transposing
-//     reads.
-//   * attention_tiles: more; 256 rows (64-dim heads: 128) by 64 tokens a step. Bound by the matrix and
-//     vector units.
+//     reads. 32 requests of 8192 tokens, 32 / 8 heads of 128: 195 us for 1.07 GB, 5.5 TB/s.
+//   * attention_tiles: more; 256 rows (64-dim heads: 128) by 64 tokens a step, requests of at most 16
+//     rows streamed like the others. Bound by the matrix and vector units, and by the clock that the
+//     power limit leaves them: a prompt of 16384 tokens, 8 / 1 heads of 128: 481 us, 1.14 PFLOP/s, the
+//     matrix units busy 63 % of the cycles at 1.7 GHz (the library's product of 8192^3: 1.29, 69 %);
+//     8 of 4096, 32 / 8 heads: 1054 us, 1.04 PFLOP/s; heads of 64 reach 0.86, as they have twice the
+//     softmax for each product.
 // Both give S^T = K Q^T, so that a row's scores lie in one lane (and its partners 32 or 16 lanes
 // away): the maximum and the sum need one or two lane swaps a step, rescaling is a lane's own
 // product, and the weights are the second product's operand O^T = V^T P^T as they are, with V's
@@ -51,7 +55,7 @@ typedef short i16x4 __attribute__((ext_vector_type(4)));
 constexpr int kWaves = 4;         // waves of a workgroup of attention_few, two of them on a CU
 // Of one of attention_tiles: 8 of 128-dim heads, whose registers and LDS leave room for one workgroup
 // on a CU, and 4 of 64-dim heads, of which a CU has three that fill each other's starts and ends (24
-// prompts of 3 .. 2050 tokens: 38.9 us, with 8 waves 49.9; 8 x 4096 640 and 709).
+// prompts of up to 1247 tokens: 38.9 us, with 8 waves 49.9; 8 x 4096 640 and 709).
 constexpr int tile_waves(int D) { return D == 128 ? 8 : 4; }
 constexpr int tile_rows(int D) { return 32 * tile_waves(D); }
 constexpr int kMergeThreads = 256;

@@ -9,11 +9,13 @@
 // writes 2 KB): one launch, in which every workgroup forms the sums of all requests for itself
 // (kChunk at a time, in LDS) instead of waiting for another one's; a fresh block's id is taken
 // from the free list by the workgroups that need it for a slot, so none reads a table entry
-// that another one writes.
+// that another one writes. Measured: 5.0 us for a decode step of 64 requests, 5.9 for 256 of which
+// 16 have 1024 .. 2048 new tokens.
 //
 // Write. A copy with the destination row chosen by slot: each lane moves units of 16 bytes (or
 // the largest the tensors' strides and addresses allow), its K and V units of two tokens in
-// flight at once.
+// flight at once. Bound by HBM: 32768 tokens of 8 x 128, 268 MB read and written, 42.8 us (6.3 TB/s,
+// partly from the caches; 52.4 us, 5.1 TB/s, where its inputs are cold).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
