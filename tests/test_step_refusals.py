@@ -70,6 +70,7 @@ def test_chunk_declines(lib):
         {"out": A[5] + 8}, {"blocks": 1 << 28}, {"tokens": 1 << 31, "max_query": 1},
         {"scale": ctypes.c_float(0.0)}, {"scale": ctypes.c_float(-1.0)},
         {"scale": ctypes.c_float(float("nan"))}, {"scale": ctypes.c_float(float("inf"))},
+        {"scale": ctypes.c_float(3e38)},
         {"out": A[0] + 2048}, {"out": A[1] + (1 << 18)}])
 
 

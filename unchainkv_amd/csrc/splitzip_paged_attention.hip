@@ -579,9 +579,13 @@ __device__ __forceinline__ void tile_path(const AttendArgs& a, const Request& re
   };
   int ids[kIds];               // of the tile whose K is loaded next
   unsigned int next_row[kIds], row_of[kIds];  // of that tile, and of the one whose V is
+  // (by a lane's index of zero, which the compiler cannot see through: a scalar load would not be
+  // among the vector loads that the waits below count)
+  unsigned int zero = 0;
+  if constexpr (kPaged) asm("v_mov_b32 %0, 0" : "=v"(zero));
   auto fetch_ids = [&](unsigned int base) {
 #pragma unroll
-    for (int i = 0; i < kIds; ++i) ids[i] = block_id<kPaged>(a, table, token_of(base, i));
+    for (int i = 0; i < kIds; ++i) ids[i] = block_id<kPaged>(a, table + zero, token_of(base, i));
   };
   auto find_rows = [&](unsigned int base) {
 #pragma unroll
@@ -1465,6 +1469,8 @@ long long launch_typed(const AttendArgs& a, const Plan& p, unsigned long long he
 }
 
 constexpr unsigned long long kMostRows = 0x7FFFFFFFull;
+constexpr unsigned long long kMostGroups = 0xFFFFFFFFull / (kWave * 8);  // a grid's threads fit 32 bits
+constexpr float kLog2E = 1.4426950408889634f;
 constexpr unsigned long long kMostStride = 1ull << 27;  // 16 rows' offsets fit 32 bits
 
 // Bytes from the first to the last of rows x heads pieces of head_bytes.
@@ -1517,13 +1523,13 @@ extern "C" long long kvq_splitzip_chunk_attention_paged(
       block_tokens > kMostRows || blocks * block_tokens > kMostRows || tables_ptr == 0 ||
       table_width == 0 || table_width > kMostRows || table_stride < table_width ||
       query_starts_ptr == 0 || context_tokens_ptr == 0 || out_ptr == 0 || out_ptr % 16 != 0 ||
-      !(scale > 0.f) || !std::isfinite(scale))
+      !(scale > 0.f) || !std::isfinite(scale * kLog2E))
     return 0;
   const unsigned long long max_context = std::min(table_width * block_tokens, kMostRows);
   const Plan plan = plan_of(tokens, requests, kv_heads, q_heads / kv_heads, head_dim, max_context, max_query, true);
   const unsigned long long need = workspace_of(plan, head_dim);
   if (need != 0 && (workspace_ptr == 0 || workspace_ptr % 16 != 0 || workspace_bytes < need)) return 0;
-  if (plan.groups > kMostRows) return 0;
+  if (plan.groups > kMostGroups) return 0;
   const unsigned long long out_bytes = tokens * q_heads * head_dim * 2;
   if (overlap(out_ptr, out_bytes, q_ptr, extent(tokens, q_row_bytes, q_heads, q_head_bytes, 2 * head_dim)) ||
       overlap(out_ptr, out_bytes, kv_ptr, 4 * blocks * block_tokens * kv_heads * head_dim))
@@ -1558,7 +1564,7 @@ extern "C" long long kvq_splitzip_chunk_attention_paged(
   a.max_query = (unsigned int)max_query;
   a.slots = (unsigned int)plan.slots;
   a.items = (unsigned int)plan.items;
-  a.scale_log2 = scale * 1.4426950408889634f;
+  a.scale_log2 = scale * kLog2E;
   return launch_typed<true>(a, plan, head_dim, dtype, reinterpret_cast<hipStream_t>(stream_ptr));
 }
 
@@ -1576,12 +1582,12 @@ extern "C" long long kvq_splitzip_prompt_attention(
       (q_ptr | q_row_bytes | q_head_bytes | k_ptr | k_row_bytes | k_head_bytes | v_ptr |
        v_row_bytes | v_head_bytes) % 16 != 0 ||
       k_row_bytes > kMostStride || v_row_bytes > kMostStride || query_starts_ptr == 0 ||
-      out_ptr == 0 || out_ptr % 16 != 0 || !(scale > 0.f) || !std::isfinite(scale))
+      out_ptr == 0 || out_ptr % 16 != 0 || !(scale > 0.f) || !std::isfinite(scale * kLog2E))
     return 0;
   const Plan plan = plan_of(tokens, requests, kv_heads, q_heads / kv_heads, head_dim, max_query, max_query, false);
   const unsigned long long need = workspace_of(plan, head_dim);
   if (need != 0 && (workspace_ptr == 0 || workspace_ptr % 16 != 0 || workspace_bytes < need)) return 0;
-  if (plan.groups > kMostRows) return 0;
+  if (plan.groups > kMostGroups) return 0;
   const unsigned long long out_bytes = tokens * q_heads * head_dim * 2;
   if (overlap(out_ptr, out_bytes, q_ptr, extent(tokens, q_row_bytes, q_heads, q_head_bytes, 2 * head_dim)) ||
       overlap(out_ptr, out_bytes, k_ptr, extent(tokens, k_row_bytes, kv_heads, k_head_bytes, 2 * head_dim)) ||
@@ -1612,6 +1618,6 @@ extern "C" long long kvq_splitzip_prompt_attention(
   a.max_query = (unsigned int)max_query;
   a.slots = (unsigned int)plan.slots;
   a.items = (unsigned int)plan.items;
-  a.scale_log2 = scale * 1.4426950408889634f;
+  a.scale_log2 = scale * kLog2E;
   return launch_typed<false>(a, plan, head_dim, dtype, reinterpret_cast<hipStream_t>(stream_ptr));
 }

@@ -1509,7 +1509,7 @@ def prompt_attention(q, k, v, query_starts, *, max_query: int | None = None,
     ``query_starts[r]`` + i of ``q`` (tokens, q_heads, head_dim), ``k`` and ``v`` (tokens,
     kv_heads, head_dim), sees the prompt's rows 0 .. i. ``query_starts`` (prompts + 1) is
     int32 on the device. Types, strides (of k and v too), heads, ``max_query`` (of a prompt's
-    tokens, here a bound for the workspace alone), ``scale``, ``lse``, the rows outside any
+    tokens; longer ones' rows stay as they are), ``scale``, ``lse``, the rows outside any
     prompt and gradients as in ``chunk_attention_paged``. Returns ``out`` (tokens, q_heads, head_dim),
     or ``None`` when the kernel declines."""
     lib = _load()
