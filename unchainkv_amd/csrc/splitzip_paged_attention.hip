@@ -608,11 +608,12 @@ __device__ __forceinline__ void tile_path(const AttendArgs& a, const Request& re
   auto load_plane = [&](unsigned int base, const unsigned char* src, unsigned long long stride,
                         const unsigned int (&last_bytes)[kOwnRuns], const unsigned int (&row)[kIds],
                         const unsigned int (&off)[kOwnRuns][kLoads], unsigned char* dst) {
+    const unsigned int inside = base < last_base ? 0x7FFFFFFFu : 0u;
+    const unsigned int at_last = base == last_base ? 0x7FFFFFFFu : 0u;
 #pragma unroll
     for (int u = 0; u < kOwnRuns; ++u)
       if constexpr (kRuns) {
-        const unsigned int bytes =
-            base < last_base ? 0x7FFFFFFFu : base == last_base ? last_bytes[u] : 0u;
+        const unsigned int bytes = inside | (at_last & last_bytes[u]);
         const Buffer buffer = buffer_of(src + row[u] * stride, bytes);
 #pragma unroll
         for (int i = 0; i < kLoads; ++i)
@@ -1382,8 +1383,8 @@ Plan plan_of(unsigned long long tokens, unsigned long long requests, unsigned lo
   Plan p{};
   p.tiles = !paged || max_query * group > kFewRows;
   p.few_target = 2 * compute_units();
-  // (tiles: of all that run at once, three quarters. Longer splits, so fewer of them, than an even
-  // share: 16 requests of 6 tokens behind 300 .. 8000 38.0 us and 45.8, a prompt of 1443 39.3 and 52.9;
+  // (tiles: three quarters of the CUs, twice that with workgroups of four waves. Longer splits, so
+  // fewer of them, than an even share: 16 requests of 6 tokens behind 300 .. 8000 38.0 us and 45.8, a prompt of 1443 39.3 and 52.9;
   // with a share of a fourth to a half of it 3 chunks beside 29 decodes took 402 and not 311)
   p.tile_target = std::max(1ull, compute_units() * (head_dim == 128 ? 3 : 6) / 4);
   const unsigned long long active = std::min(tokens, requests);
@@ -1471,7 +1472,7 @@ long long launch_typed(const AttendArgs& a, const Plan& p, unsigned long long he
 constexpr unsigned long long kMostRows = 0x7FFFFFFFull;
 constexpr unsigned long long kMostGroups = 0xFFFFFFFFull / (kWave * 8);  // a grid's threads fit 32 bits
 constexpr float kLog2E = 1.4426950408889634f;
-constexpr unsigned long long kMostStride = 1ull << 27;  // 16 rows' offsets fit 32 bits
+constexpr unsigned long long kMostStride = 1ull << 27;  // 8 rows' offsets fit 31 bits
 
 // Bytes from the first to the last of rows x heads pieces of head_bytes.
 unsigned long long extent(unsigned long long rows, unsigned long long row_bytes,
