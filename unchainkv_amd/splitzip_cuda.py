@@ -1275,7 +1275,8 @@ def new_step_plan(requests: int, max_tokens: int, device, torch=None) -> StepPla
         import torch
     small = torch.empty(2 * requests + 3, dtype=torch.int32, device=device)
     starts, contexts, free_next, lacking = small.split_with_sizes((requests + 1, requests, 1, 1))
-    slots, positions = torch.empty((2, max_tokens), dtype=torch.int64, device=device).unbind(0)
+    slots = torch.empty(max_tokens, dtype=torch.int64, device=device)
+    positions = torch.empty_like(slots)
     return StepPlan(starts, contexts, slots, positions, free_next, lacking)
 
 
@@ -1418,7 +1419,7 @@ def _rows_ok(t, dtype, device) -> bool:
 def _attention_buffers(q, out, lse, torch):
     """(ok, out) of an attention call's results."""
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.dtype != q.dtype or out.shape != q.shape or out.device != q.device or \
             not out.is_contiguous():
         return False, None
