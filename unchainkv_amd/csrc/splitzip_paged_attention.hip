@@ -15,7 +15,7 @@
 // Two kernels, by the rows that a request of the call can have:
 //   * attention_few: at most 16 (decode steps). Bound by reading K and V: a wave streams 32 tokens
 //     at a time, K straight into the matrix operand's registers, V into LDS for the transposing
-//     reads. 32 requests of 8192 tokens, 32 / 8 heads of 128: 195 us for 1.07 GB, 5.5 TB/s.
+//     reads. 32 requests of 8192 tokens, 32 / 8 heads of 128: 191 us for 1.07 GB, 5.6 TB/s.
 //   * attention_tiles: more; 256 rows (64-dim heads: 128) by 64 tokens a step, requests of at most 16
 //     rows streamed like the others. Bound by the matrix and vector units, and by the clock that the
 //     power limit leaves them: a prompt of 16384 tokens, 8 / 1 heads of 128: 481 us, 1.14 PFLOP/s, the
@@ -947,11 +947,20 @@ __device__ __forceinline__ void tile_path(const AttendArgs& a, const Request& re
 // at most 16 rows, streaming
 
 // Lane l has row l % 16 and, of every 16 tokens, the four from 4 (l / 16) on. A wave's step is 32
-// tokens: K as the first operand of S^T = K Q^T straight from memory (lane l: token l % 16, 16
-// bytes at 16 (l / 16) of every 64), V through the wave's own LDS, without a barrier, with 32-byte
-// pieces of row t at piece ^ (t % 8), so that the 16 tokens of a transposed read spread over the
-// banks. The kN waves of a workgroup take turns at 32 tokens of a split and join their sums in LDS
-// (s0, s1: the waves' stages, and then s0 their sums; s2: their (m, l)). kRows: of a slot.
+// tokens: K as the first operand of S^T = K Q^T straight from memory, V through the wave's own LDS,
+// without a barrier, with 32-byte pieces of row t at piece ^ (t % 8), so that the 16 tokens of a
+// transposed read spread over the banks. The kN waves of a workgroup take turns at 32 tokens of a
+// split and join their sums in LDS (s0, s1: the waves' stages, and then s0 their sums; s2: their
+// (m, l)). kRows: of a slot.
+//
+// K's rows of 256 bytes (128 dims) are loaded whole, four of them by one load: lane l has piece l % 4
+// of the 64 bytes at 64 (l / 16), of token 4 (l % 16 / 4) + j for load j. The operand's "rows" are
+// then pieces of four tokens, of which only those that meet their own piece of Q count: four
+// products of a load, with Q's pieces c = 0 .. 3, give token 4 (l / 16) + j's score as the sum of their
+// elements c. Three of four results are thrown away, on matrix units that have nothing else to do, and
+// no load takes apart 16 rows: 32 requests of 8192 tokens 200 -> 196.6 us, 16 of 1024 19.2 -> 17.6, 64
+// single tokens of 500 .. 16000 and four times 8 354 -> 332. (64 dims: lane l has token l % 16, 16
+// bytes at 16 (l / 16) of every 64, each counting.)
 template <typename E, int D, int kN, int kRows>
 __device__ __forceinline__ void few_path(const AttendArgs& a, const Request& request, unsigned int split,
                                          unsigned int splits, unsigned int split_tokens, unsigned int slot,
@@ -964,6 +973,7 @@ __device__ __forceinline__ void few_path(const AttendArgs& a, const Request& req
   constexpr int kStageBytes = kFewStep * kRowBytes;
   constexpr int kSlabs = D / 32, kDimTiles = D / 16;
   constexpr unsigned int kRound = kN * kFewStep;
+  constexpr bool kWhole = D == 128;  // rows of K are loaded whole
   static_assert(kStageBytes >= kFewRows * D * 4, "a wave's sums fit its stage");
 
   const unsigned int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
@@ -991,7 +1001,8 @@ __device__ __forceinline__ void few_path(const AttendArgs& a, const Request& req
   const unsigned char* q_row = a.q + (unsigned long long)(request.start + token) * a.q_row +
                                (unsigned long long)q_head * a.q_head;
 #pragma unroll
-  for (int s = 0; s < kSlabs; ++s) q[s] = *reinterpret_cast<const x8*>(q_row + 64 * s + 16 * grp);
+  for (int s = 0; s < kSlabs; ++s)
+    q[s] = *reinterpret_cast<const x8*>(q_row + (kWhole ? 64 * grp + 16 * s : 64 * s + 16 * grp));
 
   struct Keys {
     u32x4 v[2][kSlabs];
@@ -1005,10 +1016,18 @@ __device__ __forceinline__ void few_path(const AttendArgs& a, const Request& req
     const unsigned int row = kv_row<true>(a, 0u, token_of(base), id, bad);
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const unsigned char* src = kb + (unsigned int)__shfl(row, 16 * u + (int)col, kWave) * a.k_row;
+      if constexpr (kWhole) {
 #pragma unroll
-      for (int s = 0; s < kSlabs; ++s)
-        k.v[u][s] = *reinterpret_cast<const u32x4*>(src + 64 * s + 16 * grp);
+        for (int j = 0; j < 4; ++j)
+          k.v[u][j] = *reinterpret_cast<const u32x4*>(
+              kb + (unsigned int)__shfl(row, 16 * u + 4 * (int)(col / 4) + j, kWave) * a.k_row + 64 * grp +
+              16 * (col % 4));
+      } else {
+        const unsigned char* src = kb + (unsigned int)__shfl(row, 16 * u + (int)col, kWave) * a.k_row;
+#pragma unroll
+        for (int s = 0; s < kSlabs; ++s)
+          k.v[u][s] = *reinterpret_cast<const u32x4*>(src + 64 * s + 16 * grp);
+      }
     }
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
@@ -1031,12 +1050,23 @@ __device__ __forceinline__ void few_path(const AttendArgs& a, const Request& req
     float s[8];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      f32x4 st = {0, 0, 0, 0};
+      if constexpr (kWhole) {
 #pragma unroll
-      for (int c = 0; c < kSlabs; ++c)
-        st = Elem<E>::mma16(__builtin_bit_cast(x8, k.v[u][c]), q[c], st);
+        for (int j = 0; j < 4; ++j) {
+          f32x4 part[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) s[4 * u + j] = st[j];
+          for (int c = 0; c < 4; ++c)
+            part[c] = Elem<E>::mma16(__builtin_bit_cast(x8, k.v[u][j]), q[c], f32x4{0, 0, 0, 0});
+          s[4 * u + j] = (part[0][0] + part[1][1]) + (part[2][2] + part[3][3]);
+        }
+      } else {
+        f32x4 st = {0, 0, 0, 0};
+#pragma unroll
+        for (int c = 0; c < kSlabs; ++c)
+          st = Elem<E>::mma16(__builtin_bit_cast(x8, k.v[u][c]), q[c], st);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[4 * u + j] = st[j];
+      }
     }
     if ((int)base + kFewStep - 1 > shift) {
       const int left = limit - (int)base - 4 * (int)grp;
