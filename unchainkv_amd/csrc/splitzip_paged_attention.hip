@@ -1325,10 +1325,13 @@ __global__ __launch_bounds__(kMergeThreads) void attention_merge(AttendArgs a) {
         for (int i = 0; i < kVals; ++i) acc[i] *= alpha;
 #pragma unroll
         for (int k = 0; k < kBatch; ++k) {
-          const float f = b + k * kShares < job.splits ? exp2f(ml[k].x - big) : 0.f;
+          // (a weight of zero joins too: a row's NaN and infinite values stay; what a row does not
+          // see is zero in its sums)
+          const bool split = b + k * kShares < job.splits;
+          const float f = split ? exp2f(ml[k].x - big) : 0.f;
           l += ml[k].y * f;
 #pragma unroll
-          for (int i = 0; i < kVals; ++i) acc[i] = f != 0.f ? fmaf(v[k][i / 4][i % 4], f, acc[i]) : acc[i];
+          for (int i = 0; i < kVals; ++i) acc[i] = split ? fmaf(v[k][i / 4][i % 4], f, acc[i]) : acc[i];
         }
       }
       if constexpr (!kTiles) {
