@@ -5,7 +5,8 @@ bound is derived in paged_attention_ref.py) unless a test says otherwise."""
 import numpy as np
 import pytest
 
-from test_gpu_paged_attention import Case, f64, say, sz  # noqa: F401 (a fixture)
+from paged_attention_ref import HALF_STEP
+from test_gpu_paged_attention import DTYPES, Case, f64, i32, say, starts_of, sz  # noqa: F401 (sz)
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
@@ -35,3 +36,36 @@ def test_values_of_a_split_without_weight(sz, dim, dtype, key, new, contexts):  
     assert torch.isfinite(rows[:, 2:]).all() and torch.isfinite(rows[:, :2, :5]).all()
     if key == 0.0:  # (a score of -inf has no bound)
         case.verify(out, lse)
+
+
+@pytest.mark.parametrize("dim,dtype", [(64, "fp16"), (128, "fp16"), (128, "bf16")])
+@pytest.mark.parametrize("new", [1, 40])
+def test_many_small_weights(sz, dim, dtype, new):  # noqa: F811
+    """32768 tokens of weight 2^-26.3 beside one of 1, which is in no value: their sum counts. Enough
+    requests (of one table) that no context is cut, so that one reference serves all tokens.
+
+    The bound is paged_attention_ref's, but for what fp16 weights lose: with 2^7 to spare a weight
+    below 2^-21 of the largest is off by 2^-32 of it at most."""
+    say("small weights", dim, dtype, new)
+    requests, heads, block, tail, score = 64, 8, 16, 32768, -18.25
+    context = 1 + tail + new - 1
+    blocks = -(-context // block)
+    kv = torch.empty((2, blocks, block, heads, dim), dtype=DTYPES[dtype], device="cuda")
+    kv[0], kv[1] = score / (dim / 8), 1.0
+    kv[:, 0, 0] = 0.0
+    q = torch.ones((requests * new, heads, dim), dtype=DTYPES[dtype], device="cuda")
+    tables = torch.arange(blocks, dtype=torch.int32, device="cuda").expand(requests, -1).contiguous()
+    lse = torch.empty(q.shape[:2], dtype=torch.float32, device="cuda")
+    out = sz.chunk_attention_paged(q, kv, tables, starts_of([new] * requests),
+                                   i32([context] * requests), scale=0.125, max_query=new, lse=lse)
+    torch.cuda.synchronize()
+    seen = tail + np.arange(new)
+    share = seen * np.exp(score) / (1 + seen * np.exp(score))
+    expect = np.tile(share, requests)[:, None, None]
+    off = 2 * (dim + 8) * 2.0 ** -24 * -score + 2.0 ** -20 + context * 2.0 ** -24
+    bound = 2 * HALF_STEP[dtype] * expect * 1.01 + 2 * off * expect
+    if dtype == "fp16":
+        bound = bound + context * 2.0 ** -32 + 2.0 ** -25
+    assert (np.abs(f64(out) - expect) <= bound).all()
+    expect = np.log1p(np.tile(seen, requests) * np.exp(score))[:, None]
+    assert (np.abs(f64(lse) - expect) <= 2 * off + 2.0 ** -22).all()

@@ -3,10 +3,14 @@
 //
 // For row i of request r (n new tokens, context c): o = sum_t p_t v_t / sum_t p_t over the tokens
 // t = 0 .. c - n + i, p_t = 2^(s_t - m), s_t = scale * log2(e) * q.k_t, m a running reference
-// that never exceeds the running maximum of s and is at most kSlack below it, so that the sums
-// stay in range and the accumulators are rescaled only when the maximum has moved by more.
+// kLift to kLift + kSlack below the running maximum of s, so that the sums stay in range and the
+// accumulators are rescaled only when the maximum has moved by kSlack.
 // Scores, weights' sums and outputs accumulate in f32; the weights are rounded to the inputs'
-// type for the second matrix product (2^-9 or 2^-12 of each, like the output's own rounding).
+// type for the second matrix product, as the matrix unit takes it (by at most 2^-8 or 2^-11 of each,
+// like the output's own rounding). fp16 has no more than that for values of 2^-14 and above, and steps
+// of 2^-24 below, so its weights are kept 2^7 larger (kLift; the largest are then 2^15): those below
+// 2^-21 of the largest are off by up to 2^-32 of it, a context of n tokens by n * 2^-32 of its
+// largest V value (n * 2^-25 without, which 32768 tokens of weight 2^-26 beside one of 1 lost whole).
 //
 // The query heads of a group read the same K and V, so a request's rows are (token, head of the
 // group) pairs, row m = token * group + head, and a tile of rows serves them together: a single
@@ -81,7 +85,7 @@ constexpr unsigned int kLeastFewSteps = 4, kWholeFewSteps = 8;
 // A maximum before any token: the lowest float, not -inf, so that rows whose scores are all -inf
 // have weights of zero and a sum of zero (whose quotient is NaN, as the formula's).
 constexpr float kNoMax = -3.402823466e38f;
-constexpr float kSlack = 8.f;     // log2: weights stay below 2^8
+constexpr float kSlack = 8.f;     // log2: weights stay below 2^(kLift + 8)
 constexpr float kLn2 = 0.6931471805599453f;
 
 template <typename E>
@@ -90,6 +94,7 @@ template <>
 struct Elem<__bf16> {
   typedef __bf16 x8 __attribute__((ext_vector_type(8)));
   typedef __bf16 x2 __attribute__((ext_vector_type(2)));
+  static constexpr float kLift = 0.f;  // log2 that the largest weights are raised by
   static __device__ __forceinline__ f32x16 mma32(x8 a, x8 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
   }
@@ -101,6 +106,7 @@ template <>
 struct Elem<_Float16> {
   typedef _Float16 x8 __attribute__((ext_vector_type(8)));
   typedef _Float16 x2 __attribute__((ext_vector_type(2)));
+  static constexpr float kLift = 7.f;
   static __device__ __forceinline__ f32x16 mma32(x8 a, x8 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
   }
@@ -756,8 +762,8 @@ __device__ __forceinline__ void tile_path(const AttendArgs& a, const Request& re
                   __builtin_bit_cast(float, (unsigned int)x[1]));
     }
     top *= a.scale_log2;
-    if (__ballot(top > m_ref + kSlack) != 0) {
-      const float now = fmaxf(m_ref, top), alpha = __builtin_amdgcn_exp2f(m_ref - now);
+    if (__ballot(top > m_ref + (Elem<E>::kLift + kSlack)) != 0) {
+      const float now = fmaxf(m_ref, top - Elem<E>::kLift), alpha = __builtin_amdgcn_exp2f(m_ref - now);
       m_ref = now;
       l_run *= alpha;
 #pragma unroll
@@ -1079,8 +1085,8 @@ __device__ __forceinline__ void few_path(const AttendArgs& a, const Request& req
     top = fmaxf(top, __shfl_xor(top, 16, 64));
     top = fmaxf(top, __shfl_xor(top, 32, 64));
     top *= a.scale_log2;
-    if (__ballot(top > m_ref + kSlack) != 0) {
-      const float now = fmaxf(m_ref, top), alpha = __builtin_amdgcn_exp2f(m_ref - now);
+    if (__ballot(top > m_ref + (Elem<E>::kLift + kSlack)) != 0) {
+      const float now = fmaxf(m_ref, top - Elem<E>::kLift), alpha = __builtin_amdgcn_exp2f(m_ref - now);
       m_ref = now;
       l_run *= alpha;
 #pragma unroll
