@@ -543,7 +543,7 @@ long long kvq_splitzip_plan_step_paged(
 /* K and V rows of `tokens` tokens into a layer by slot: head h of row t is head_bytes
  * bytes at k + t * k_row_bytes + h * k_head_bytes (v likewise) and goes to
  * kv + slots[t] * heads * head_bytes + h * head_bytes, V plane_bytes later. Rows whose slot
- * is not in [0, slot_count) are not written. The rows must not overlap the layer; of two
+ * is not in [0, slot_count) are not written. Rows and slots must not overlap the layer; of two
  * rows with one slot it is not said whose values stay. Any alignment (16-byte aligned rows,
  * heads and planes are the fast case). Returns the rows' bytes, 0 on a failed
  * precondition. */
@@ -574,7 +574,8 @@ unsigned long long kvq_splitzip_prompt_attention_workspace_bytes(
  * rows: longer ones are left out. Rows that see nothing are 0 (lse -inf); rows of no request,
  * or of a range that is not inside q, stay; a context past its table's row, or an entry that is
  * no block, gives NaN rows. workspace: 16-byte aligned, of the size above (not looked at where
- * that is 0), for one call at a time. Returns the bytes of out, 0 on a failed precondition (out must not overlap an input). */
+ * that is 0), for one call at a time. out, lse and workspace must overlap neither an input nor
+ * each other. Returns the bytes of out, 0 on a failed precondition. */
 long long kvq_splitzip_chunk_attention_paged(
     unsigned long long q_ptr, unsigned long long q_row_bytes, unsigned long long q_head_bytes,
     unsigned long long tokens, unsigned long long q_heads, unsigned long long kv_heads,

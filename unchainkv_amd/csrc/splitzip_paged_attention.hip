@@ -44,6 +44,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
+#include <initializer_list>
 #include <mutex>
 #include <type_traits>
 
@@ -1522,6 +1523,21 @@ unsigned long long extent(unsigned long long rows, unsigned long long row_bytes,
   return (rows - 1) * row_bytes + (heads - 1) * head_step + head_bytes;
 }
 
+struct Bytes {
+  unsigned long long at, count;
+};
+// Whether what a call writes lies over nothing that it reads, and over nothing else that it writes
+// (some workgroups still read when others write).
+bool results_apart(std::initializer_list<Bytes> written, std::initializer_list<Bytes> read) {
+  for (const Bytes* w = written.begin(); w != written.end(); ++w) {
+    for (const Bytes& r : read)
+      if (overlap(w->at, w->count, r.at, r.count)) return false;
+    for (const Bytes* o = written.begin(); o != w; ++o)
+      if (overlap(w->at, w->count, o->at, o->count)) return false;
+  }
+  return true;
+}
+
 bool sizes_ok(unsigned long long tokens, unsigned long long requests, unsigned long long q_heads,
               unsigned long long kv_heads, unsigned long long head_dim, unsigned long long max_query) {
   return tokens != 0 && tokens <= kMostRows && requests != 0 && requests <= kMostRows &&
@@ -1573,8 +1589,12 @@ extern "C" long long kvq_splitzip_chunk_attention_paged(
   if (need != 0 && (workspace_ptr == 0 || workspace_ptr % 16 != 0 || workspace_bytes < need)) return 0;
   if (plan.groups > kMostGroups) return 0;
   const unsigned long long out_bytes = tokens * q_heads * head_dim * 2;
-  if (overlap(out_ptr, out_bytes, q_ptr, extent(tokens, q_row_bytes, q_heads, q_head_bytes, 2 * head_dim)) ||
-      overlap(out_ptr, out_bytes, kv_ptr, 4 * blocks * block_tokens * kv_heads * head_dim))
+  if (!results_apart(
+          {{out_ptr, out_bytes}, {lse_ptr, lse_ptr ? 4 * tokens * q_heads : 0}, {workspace_ptr, need}},
+          {{q_ptr, extent(tokens, q_row_bytes, q_heads, q_head_bytes, 2 * head_dim)},
+           {kv_ptr, 4 * blocks * block_tokens * kv_heads * head_dim},
+           {tables_ptr, 4 * ((requests - 1) * table_stride + table_width)},
+           {query_starts_ptr, 4 * (requests + 1)}, {context_tokens_ptr, 4 * requests}}))
     return 0;
   AttendArgs a{};
   a.q = reinterpret_cast<const unsigned char*>(q_ptr);
@@ -1631,9 +1651,12 @@ extern "C" long long kvq_splitzip_prompt_attention(
   if (need != 0 && (workspace_ptr == 0 || workspace_ptr % 16 != 0 || workspace_bytes < need)) return 0;
   if (plan.groups > kMostGroups) return 0;
   const unsigned long long out_bytes = tokens * q_heads * head_dim * 2;
-  if (overlap(out_ptr, out_bytes, q_ptr, extent(tokens, q_row_bytes, q_heads, q_head_bytes, 2 * head_dim)) ||
-      overlap(out_ptr, out_bytes, k_ptr, extent(tokens, k_row_bytes, kv_heads, k_head_bytes, 2 * head_dim)) ||
-      overlap(out_ptr, out_bytes, v_ptr, extent(tokens, v_row_bytes, kv_heads, v_head_bytes, 2 * head_dim)))
+  if (!results_apart(
+          {{out_ptr, out_bytes}, {lse_ptr, lse_ptr ? 4 * tokens * q_heads : 0}, {workspace_ptr, need}},
+          {{q_ptr, extent(tokens, q_row_bytes, q_heads, q_head_bytes, 2 * head_dim)},
+           {k_ptr, extent(tokens, k_row_bytes, kv_heads, k_head_bytes, 2 * head_dim)},
+           {v_ptr, extent(tokens, v_row_bytes, kv_heads, v_head_bytes, 2 * head_dim)},
+           {query_starts_ptr, 4 * (requests + 1)}}))
     return 0;
   AttendArgs a{};
   a.q = reinterpret_cast<const unsigned char*>(q_ptr);

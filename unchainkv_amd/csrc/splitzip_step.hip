@@ -322,7 +322,8 @@ extern "C" long long kvq_splitzip_write_kv_paged(
   if (overlap(kv_ptr, layer_bytes, k_ptr,
               (tokens - 1) * k_row_bytes + (heads - 1) * k_head_bytes + head_bytes) ||
       overlap(kv_ptr, layer_bytes, v_ptr,
-              (tokens - 1) * v_row_bytes + (heads - 1) * v_head_bytes + head_bytes))
+              (tokens - 1) * v_row_bytes + (heads - 1) * v_head_bytes + head_bytes) ||
+      overlap(kv_ptr, layer_bytes, slots_ptr, 8 * tokens))
     return 0;
   WriteArgs a{};
   a.layer = reinterpret_cast<unsigned char*>(kv_ptr);

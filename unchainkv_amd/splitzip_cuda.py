@@ -1352,7 +1352,7 @@ def write_kv_paged(k, v, kv_layer, slots) -> int | None:
     bf16 or fp16; rows and heads may be strided (views of one projection). ``slots`` may
     be longer than the rows. Of two rows with one slot it is not said whose values stay (a
     plan's slots are distinct). Returns the rows' bytes (0 without rows), or ``None`` when the kernel
-    declines (other types or layouts, rows that overlap the layer)."""
+    declines (other types or layouts, rows or slots that overlap the layer)."""
     lib = _load()
     write = getattr(lib, "kvq_splitzip_write_kv_paged", None) if lib else None
     if write is None or not _is_cuda(k):
@@ -1452,7 +1452,8 @@ def chunk_attention_paged(q, kv_layer, tables, query_starts, context_tokens, *,
     -inf. Rows of no request, of one with more new tokens than max_query, and of one whose
     row range is not inside q stay as they are. A context longer than its table, or a table
     entry that is no block of the layer, makes the rows that read there NaN (every row of
-    the same tile, of 16 to 256 of a KV head's query rows, at least).
+    the same tile, of 16 to 256 of a KV head's query rows, at least). ``out``, ``lse`` and
+    ``workspace`` over an input or each other are declined.
     No gradient: inputs that require one are declined while gradients are recorded.
 
     Returns ``out`` (tokens, q_heads, head_dim), or ``None`` when the kernel declines."""
@@ -1511,7 +1512,7 @@ def prompt_attention(q, k, v, query_starts, *, max_query: int | None = None,
     kv_heads, head_dim), sees the prompt's rows 0 .. i. ``query_starts`` (prompts + 1) is
     int32 on the device. Types, strides (of k and v too), heads, ``max_query`` (of a prompt's
     tokens; longer ones' rows stay as they are), ``scale``, ``lse``, the rows outside any
-    prompt and gradients as in ``chunk_attention_paged``. Returns ``out`` (tokens, q_heads, head_dim),
+    prompt, results' overlaps and gradients as in ``chunk_attention_paged``. Returns ``out`` (tokens, q_heads, head_dim),
     or ``None`` when the kernel declines."""
     lib = _load()
     attend = getattr(lib, "kvq_splitzip_prompt_attention", None) if lib else None
