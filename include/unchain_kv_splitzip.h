@@ -572,7 +572,8 @@ unsigned long long kvq_splitzip_prompt_attention_workspace_bytes(
  * 128; scale positive and finite. out: [tokens][q_heads][head_dim]; lse_ptr: 0, or f32
  * [tokens][q_heads] for the rows' log-sum-exps. max_query (at most tokens) bounds a request's
  * rows: longer ones are left out. Rows that see nothing are 0 (lse -inf); rows of no request,
- * or of a range that is not inside q, stay; a context past its table's row, or an entry that is
+ * or of a range that is not inside q, stay (of ranges that overlap, as starts that run
+ * backwards give, a row is one request's or stays); a context past its table's row, or an entry that is
  * no block, gives NaN rows. workspace: 16-byte aligned, of the size above (not looked at where
  * that is 0), for one call at a time. out, lse and workspace must overlap neither an input nor
  * each other. Returns the bytes of out, 0 on a failed precondition. */

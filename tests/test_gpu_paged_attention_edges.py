@@ -6,7 +6,8 @@ import numpy as np
 import pytest
 
 from paged_attention_ref import HALF_STEP
-from test_gpu_paged_attention import DTYPES, Case, f64, i32, say, starts_of, sz  # noqa: F401 (sz)
+from test_gpu_paged_attention import (  # noqa: F401 (sz: a fixture)
+    DTYPES, MARK, Case, f64, i32, say, starts_of, sz)
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
@@ -69,3 +70,47 @@ def test_many_small_weights(sz, dim, dtype, new):  # noqa: F811
     assert (np.abs(f64(out) - expect) <= bound).all()
     expect = np.log1p(np.tile(seen, requests) * np.exp(score))[:, None]
     assert (np.abs(f64(lse) - expect) <= 2 * off + 2.0 ** -22).all()
+
+
+def test_ranges_that_overlap_leave_whole_rows_or_none(sz):  # noqa: F811
+    """Starts that run backwards ask for more items than a call launches: 1024 rows named three times
+    and 1280 more, in tiles of 256 rows (32 tokens), each cut into two splits. 3 * 32 + 40 tiles make
+    272 items; launched are 72 for the tiles of the rows, 6 for the requests and 193 for splits, so
+    that the second split of the last tile is none of them. Each row is right or as it was, and
+    nothing outside out, lse and the workspace's size is written."""
+    dim, heads, block, context = 128, 8, 16, 3000
+    gen = torch.Generator("cuda").manual_seed(31)
+    blocks = -(-context // block)
+    kv = torch.randn((2, 2 * blocks, block, 1, dim), generator=gen, device="cuda").bfloat16()
+    order = torch.randperm(2 * blocks, generator=gen, device="cuda").int().view(2, blocks)
+    tables = order[[0, 0, 0, 0, 0, 1]].contiguous()
+    starts, rows = i32([0, 1024, 0, 1024, 0, 1024, 2304]), 2304 + 3
+    q = torch.randn((rows, heads, dim), generator=gen, device="cuda").bfloat16()
+    out = torch.full(q.shape, MARK, dtype=q.dtype, device="cuda")
+    lse = torch.full(q.shape[:2], MARK, dtype=torch.float32, device="cuda")
+    need = sz.chunk_attention_workspace_bytes(rows, 6, heads, 1, dim, blocks * block)
+    space = torch.full((need + (1 << 20),), 255, dtype=torch.uint8, device="cuda")  # (NaN partials)
+    assert sz.chunk_attention_paged(q, kv, tables, starts, i32([context] * 6), out=out, lse=lse,
+                                    workspace=space[:need]) is out
+    torch.cuda.synchronize()
+    assert (space[need:] == 255).all()
+    assert (out[2304:] == MARK).all() and (lse[2304:] == MARK).all()
+    left = (out == MARK).flatten(1).all(1)
+    assert torch.equal(left, (lse == MARK).all(1))
+    say("rows left", int(left.sum()))
+    for table, first, n in ((order[0], 0, 1024), (order[1], 1024, 1280)):
+        k, v = (plane[table.long()].view(-1, dim)[:context].double() for plane in (kv[0], kv[1]))
+        keys, part = k.abs().T, slice(first, first + n)
+        x = q[part].double()
+        last = context - n + torch.arange(n, device="cuda")
+        seen = torch.arange(context, device="cuda") <= last[:, None]
+        score = torch.where(seen[:, None], x @ k.T * dim ** -0.5, -torch.inf)
+        weight = torch.softmax(score, -1)
+        expect, mean = weight @ v, weight @ v.abs()
+        off = 2 * (dim + 8) * 2.0 ** -24 * (x.abs() @ keys).amax(-1) * dim ** -0.5 + 2.0 ** -20 + \
+            context * 2.0 ** -24
+        bound = HALF_STEP["bf16"] * (mean + expect.abs()) * 1.01 + 2 * off[..., None] * mean
+        ok = ((out[part] - expect).abs() <= bound).flatten(1).all(1)
+        assert (ok | left[part]).all()
+        near = (lse[part] - torch.logsumexp(score, -1)).abs() <= 2 * off + 2.0 ** -20
+        assert (near.all(1) | left[part]).all()

@@ -483,7 +483,7 @@ __device__ __forceinline__ void store_slow(const AttendArgs& a, bool split,
 }
 
 // A slot's job, by one thread of its workgroup; `slot` counts for one KV head. (Row ranges that
-// overlap each other can ask for more slots than there are: their rows stay as they were.)
+// overlap each other can ask for more slots than there are: rows without theirs stay as they were.)
 __device__ __forceinline__ void store_job(const AttendArgs& a, unsigned int slot, unsigned int head,
                                           Job j) {
   const unsigned int slots = a.slots / a.kv_heads;
@@ -1239,6 +1239,12 @@ __global__ __launch_bounds__(kWave * tile_waves(D), D == 128 ? 2 : 3) void atten
   }
   if (!found) return;
   const unsigned int most = work.splits(request), split_tokens = work.split_tokens(request, most);
+  if (most > 1 && item - index % most + most > a.items) {
+    // (row ranges that overlap each other can ask for more items than there are: a tile without all
+    // its splits is left)
+    store_job(a, slot, head, Job{});
+    return;
+  }
   if constexpr (kPaged) {
     if (work.few(request.n)) {
       if (!has_slot) slot = kNoSlot;

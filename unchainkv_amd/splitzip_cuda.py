@@ -1452,8 +1452,9 @@ def chunk_attention_paged(q, kv_layer, tables, query_starts, context_tokens, *,
     -inf. Rows of no request, of one with more new tokens than max_query, and of one whose
     row range is not inside q stay as they are. A context longer than its table, or a table
     entry that is no block of the layer, makes the rows that read there NaN (every row of
-    the same tile, of 16 to 256 of a KV head's query rows, at least). ``out``, ``lse`` and
-    ``workspace`` over an input or each other are declined.
+    the same tile, of 16 to 256 of a KV head's query rows, at least). Where
+    query_starts run backwards, so that ranges overlap, rows are one of their requests' or stay.
+    ``out``, ``lse`` and ``workspace`` over an input or each other are declined.
     No gradient: inputs that require one are declined while gradients are recorded.
 
     Returns ``out`` (tokens, q_heads, head_dim), or ``None`` when the kernel declines."""
