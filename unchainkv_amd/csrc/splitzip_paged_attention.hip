@@ -236,11 +236,20 @@ constexpr unsigned int kNoSlot = ~0u;
 // Sums of 64 lanes' values stay below 2^32.
 constexpr unsigned int kMostSteps = 1u << 25;
 
-// ceil(sum / parts), by a 32-bit division where it serves.
-__device__ __forceinline__ unsigned int share_of(unsigned long long sum, unsigned int parts) {
-  sum += parts - 1;
-  return (sum >> 32) == 0 ? (unsigned int)sum / parts : (unsigned int)(sum / parts);
+// ceil(sum * heads / parts), by a 32-bit division where it serves, and kMostSteps where it is more
+// (no request has more steps; the sum of 2^31 requests times their heads may pass 64 bits).
+__host__ __device__ __forceinline__ constexpr unsigned int share_of(unsigned long long sum,
+                                                                    unsigned int heads, unsigned int parts) {
+  if ((sum >> 50) != 0) return kMostSteps;
+  sum = sum * heads + parts - 1;
+  if ((sum >> 32) == 0) return (unsigned int)sum / parts;
+  sum /= parts;
+  return sum < kMostSteps ? (unsigned int)sum : kMostSteps;
 }
+static_assert(share_of(0, 8, 192) == 0 && share_of(1, 1, 192) == 1 && share_of(384, 1, 192) == 2 &&
+              share_of(385, 1, 192) == 3 && share_of(1ull << 36, 1, 8192) == 1u << 23, "rounded up");
+static_assert(share_of(1ull << 37, 8, 192) == kMostSteps && share_of(1ull << 56, 4096, 512) == kMostSteps &&
+              share_of((1ull << 50) - 1, 4096, 512) == kMostSteps, "the share, or what cuts nothing");
 
 // The launch's work, which every workgroup finds its own item of by itself. Requests lie one in a
 // lane, 64 at a time (`first`: the first 64, which most launches end with), each with its tiles
@@ -291,7 +300,7 @@ struct Work {
     }
     const unsigned int parts = kTiles ? a.tile_target : a.few_target;
     const unsigned int least = kTiles ? kLeastTileSteps : a.slots == 0 ? kWholeFewSteps : kLeastFewSteps;
-    if (!large && (!kTiles || a.slots != 0)) cap = max(least, share_of(sum * a.kv_heads, parts));
+    if (!large && (!kTiles || a.slots != 0)) cap = max(least, share_of(sum, a.kv_heads, parts));
   }
 
   // The lanes' requests with the longest contexts first.
