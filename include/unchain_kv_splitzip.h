@@ -554,13 +554,19 @@ long long kvq_splitzip_write_kv_paged(
     unsigned long long v_head_bytes, unsigned long long kv_ptr, unsigned long long plane_bytes,
     unsigned long long slot_count, unsigned long long slots_ptr, unsigned long long stream_ptr);
 
-/* Workspace bytes of the two attention calls; max_context = table_width * block_tokens. 0: a call
- * of these sizes needs none (its contexts are short enough to be taken whole), or declines them. */
+/* Workspace bytes of the two attention calls, enough for every call of at most this many tokens,
+ * requests, max_context (= table_width * block_tokens) and max_query (more than tokens: as many) with
+ * these heads. 0: such calls need none (their contexts are short enough to be taken whole), or
+ * decline the sizes. */
 unsigned long long kvq_splitzip_chunk_attention_workspace_bytes(
     unsigned long long tokens, unsigned long long requests, unsigned long long q_heads,
     unsigned long long kv_heads, unsigned long long head_dim, unsigned long long max_context,
     unsigned long long max_query);
 unsigned long long kvq_splitzip_prompt_attention_workspace_bytes(
+    unsigned long long tokens, unsigned long long requests, unsigned long long q_heads,
+    unsigned long long kv_heads, unsigned long long head_dim, unsigned long long max_query);
+/* What a prompt call of exactly these sizes asks for: less than the above where it cuts nothing. */
+unsigned long long kvq_splitzip_prompt_attention_least_workspace_bytes(
     unsigned long long tokens, unsigned long long requests, unsigned long long q_heads,
     unsigned long long kv_heads, unsigned long long head_dim, unsigned long long max_query);
 

@@ -114,3 +114,19 @@ def test_ranges_that_overlap_leave_whole_rows_or_none(sz):  # noqa: F811
         assert (ok | left[part]).all()
         near = (lse[part] - torch.logsumexp(score, -1)).abs() <= 2 * off + 2.0 ** -20
         assert (near.all(1) | left[part]).all()
+
+
+def test_workspace_of_the_largest_step_serves_smaller_ones(sz):  # noqa: F811
+    """One workspace for prompts that are cut and prompts that are not: nothing else is allocated."""
+    packed = torch.randn((4096, 48, 128), device="cuda").bfloat16()
+    space = torch.empty(sz.prompt_attention_workspace_bytes(32768, 8, 32, 8, 128, 4096),
+                        dtype=torch.uint8, device="cuda")
+    for new in ([4096], [1024] * 4, [1443], [5, 900]):
+        q, k, v = packed[:sum(new)].split((32, 8, 8), 1)
+        starts, out = starts_of(new), torch.empty((sum(new), 32, 128), dtype=q.dtype, device="cuda")
+        expect = sz.prompt_attention(q, k, v, starts, max_query=max(new))
+        torch.cuda.reset_peak_memory_stats()
+        held = torch.cuda.memory_allocated()
+        assert sz.prompt_attention(q, k, v, starts, max_query=max(new), out=out, workspace=space) is out
+        assert torch.cuda.max_memory_allocated() == held
+        assert torch.equal(out, expect)

@@ -1460,7 +1460,7 @@ Plan plan_of(unsigned long long tokens, unsigned long long requests, unsigned lo
       const double share = (double)(group * kv_heads) / (double)(rows * p.tile_target);
       double l = n;
       if (others > 0)  // where the right side is least above the left
-        l = std::min(std::max((0.5 / share + n / others) / (1 + 1 / others), whole), (double)max_context);
+        l = std::min(std::max((0.5 / share + n / others) / (1 + 1 / others), whole + 1), (double)max_context);
       cut = l > share * (l * l + (others > 0 ? (n - l) * (n - l) / others : 0.));
     }
     // (see Work; the share of one KV head)
@@ -1482,6 +1482,25 @@ unsigned long long partial_bytes(const Plan& p, unsigned long long head_dim) {
 }
 unsigned long long workspace_of(const Plan& p, unsigned long long head_dim) {
   return partial_bytes(p, head_dim) + p.slots * sizeof(Job);
+}
+
+// Enough for every call of at most these sizes. (It does not grow with all of them: rows that many
+// prompts share are cut less than those of one, and streamed requests have a slot each, tiles have not.)
+unsigned long long workspace_bound(unsigned long long tokens, unsigned long long requests,
+                                   unsigned long long kv_heads, unsigned long long group,
+                                   unsigned long long head_dim, unsigned long long max_context,
+                                   unsigned long long max_query, bool paged) {
+  const unsigned long long own = workspace_of(
+      plan_of(tokens, requests, kv_heads, group, head_dim, max_context, max_query, paged), head_dim);
+  if (!paged) {
+    // (of one prompt the shortest that can be cut at all is cut the soonest; all that are cut need the same)
+    const unsigned long long n = std::min<unsigned long long>(max_query, kTileTokens * kLeastTileSteps + 1);
+    return std::max(own, workspace_of(plan_of(n, 1, kv_heads, group, head_dim, n, n, false), head_dim));
+  }
+  const unsigned long long few = std::min<unsigned long long>(max_query, kFewRows / group);
+  if (few == 0) return own;
+  return std::max(own, workspace_of(plan_of(tokens, requests, kv_heads, group, head_dim, max_context, few, true),
+                                    head_dim));
 }
 
 template <typename E, int D, bool kTiles>
@@ -1567,14 +1586,23 @@ extern "C" unsigned long long kvq_splitzip_chunk_attention_workspace_bytes(
     unsigned long long tokens, unsigned long long requests, unsigned long long q_heads,
     unsigned long long kv_heads, unsigned long long head_dim, unsigned long long max_context,
     unsigned long long max_query) {
+  max_query = std::min(max_query, tokens);
   if (!sizes_ok(tokens, requests, q_heads, kv_heads, head_dim, max_query)) return 0;
-  return workspace_of(plan_of(tokens, requests, kv_heads, q_heads / kv_heads, head_dim, max_context, max_query,
-                              true), head_dim);
+  return workspace_bound(tokens, requests, kv_heads, q_heads / kv_heads, head_dim, max_context, max_query, true);
 }
 
 extern "C" unsigned long long kvq_splitzip_prompt_attention_workspace_bytes(
     unsigned long long tokens, unsigned long long requests, unsigned long long q_heads,
     unsigned long long kv_heads, unsigned long long head_dim, unsigned long long max_query) {
+  max_query = std::min(max_query, tokens);
+  if (!sizes_ok(tokens, requests, q_heads, kv_heads, head_dim, max_query)) return 0;
+  return workspace_bound(tokens, requests, kv_heads, q_heads / kv_heads, head_dim, max_query, max_query, false);
+}
+
+extern "C" unsigned long long kvq_splitzip_prompt_attention_least_workspace_bytes(
+    unsigned long long tokens, unsigned long long requests, unsigned long long q_heads,
+    unsigned long long kv_heads, unsigned long long head_dim, unsigned long long max_query) {
+  max_query = std::min(max_query, tokens);
   if (!sizes_ok(tokens, requests, q_heads, kv_heads, head_dim, max_query)) return 0;
   return workspace_of(plan_of(tokens, requests, kv_heads, q_heads / kv_heads, head_dim, max_query, max_query,
                               false), head_dim);

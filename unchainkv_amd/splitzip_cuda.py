@@ -166,6 +166,7 @@ _SIGNATURES = (
     ("kvq_splitzip_write_kv_paged", [_U64] * 14, ctypes.c_longlong, False),
     ("kvq_splitzip_chunk_attention_workspace_bytes", [_U64] * 7, _U64, False),
     ("kvq_splitzip_prompt_attention_workspace_bytes", [_U64] * 6, _U64, False),
+    ("kvq_splitzip_prompt_attention_least_workspace_bytes", [_U64] * 6, _U64, False),
     ("kvq_splitzip_chunk_attention_paged", [_U64] * 22 + [ctypes.c_float, _U64],
      ctypes.c_longlong, False),
     ("kvq_splitzip_prompt_attention", [_U64] * 21 + [ctypes.c_float, _U64],
@@ -1387,27 +1388,46 @@ def _attention_workspace(name: str, device, sizes: tuple) -> int:
         return int(getattr(_load(), name)(*sizes))
 
 
+def _workspace_sizes(tokens: int, requests: int, q_heads: int, kv_heads: int, head_dim: int,
+                     max_query: int | None) -> tuple | None:
+    """The sizes of a workspace query; None without rows. Sizes that no attention call takes raise."""
+    if tokens < 0 or requests < 0 or not 1 <= kv_heads <= 4096 or not 1 <= q_heads <= 65536 or \
+            q_heads % kv_heads or head_dim not in (64, 128) or tokens * q_heads >= 1 << 31 or \
+            requests >= 1 << 31 or (max_query is not None and max_query < 0):
+        raise ValueError(f"no attention call takes {tokens} rows of {requests} requests, {q_heads} / "
+                         f"{kv_heads} heads of {head_dim}, max_query {max_query}")
+    if not tokens or not requests:
+        return None
+    return tokens, requests, q_heads, kv_heads, head_dim, min(max_query or tokens, tokens)
+
+
 def chunk_attention_workspace_bytes(tokens: int, requests: int, q_heads: int, kv_heads: int,
                                     head_dim: int, max_context: int,
                                     max_query: int | None = None) -> int:
     """Workspace of ``chunk_attention_paged`` for ``tokens`` rows of q, with ``max_context`` the
-    tokens that a row of the block tables can hold (its width in blocks * block_tokens). 0: none
-    is needed."""
+    tokens that a row of the block tables can hold (its width in blocks * block_tokens). It is
+    enough for every call of at most these sizes with these heads. 0: none is needed. Sizes that
+    the call declines raise ``ValueError``."""
     lib = _load()
     if lib is None or not hasattr(lib, "kvq_splitzip_chunk_attention_workspace_bytes"):
         raise RuntimeError(f"HIP codec library not loaded: {load_error()}")
-    return int(lib.kvq_splitzip_chunk_attention_workspace_bytes(
-        tokens, requests, q_heads, kv_heads, head_dim, max_context, max_query or tokens))
+    sizes = _workspace_sizes(tokens, requests, q_heads, kv_heads, head_dim, max_query)
+    if max_context < 0:
+        raise ValueError(f"a context of {max_context} tokens")
+    return 0 if sizes is None else int(lib.kvq_splitzip_chunk_attention_workspace_bytes(
+        *sizes[:5], max_context, sizes[5]))
 
 
 def prompt_attention_workspace_bytes(tokens: int, requests: int, q_heads: int, kv_heads: int,
                                      head_dim: int, max_query: int | None = None) -> int:
-    """Workspace of ``prompt_attention`` for ``tokens`` packed rows."""
+    """Workspace of ``prompt_attention`` for ``tokens`` packed rows, enough for every call of at
+    most these sizes with these heads (0: none is needed). Sizes that the call declines raise
+    ``ValueError``."""
     lib = _load()
     if lib is None or not hasattr(lib, "kvq_splitzip_prompt_attention_workspace_bytes"):
         raise RuntimeError(f"HIP codec library not loaded: {load_error()}")
-    return int(lib.kvq_splitzip_prompt_attention_workspace_bytes(
-        tokens, requests, q_heads, kv_heads, head_dim, max_query or tokens))
+    sizes = _workspace_sizes(tokens, requests, q_heads, kv_heads, head_dim, max_query)
+    return 0 if sizes is None else int(lib.kvq_splitzip_prompt_attention_workspace_bytes(*sizes))
 
 
 def _rows_ok(t, dtype, device) -> bool:
@@ -1543,7 +1563,7 @@ def prompt_attention(q, k, v, query_starts, *, max_query: int | None = None,
     if max_query <= 0:
         return None
     need = _attention_workspace(
-        "kvq_splitzip_prompt_attention_workspace_bytes", device,
+        "kvq_splitzip_prompt_attention_least_workspace_bytes", device,
         (tokens, requests, q_heads, kv_heads, head_dim, max_query))
     if need and not _byte_buffer_ok(workspace, device, need, torch):
         workspace = torch.empty(need, dtype=torch.uint8, device=device)
