@@ -1244,6 +1244,23 @@ def _call_on(device, torch, fn, *args):
         return fn(*args, _stream_handle(device, torch))
 
 
+def _tracked(torch, *tensors) -> bool:
+    """Whether autograd follows any of the tensors (None: not given): a gradient is required while
+    gradients are recorded, or there is a forward-mode tangent. The kernels give neither."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        return True
+    forward = torch.autograd.forward_ad
+    # (outside its levels no tensor has a tangent, which spares asking each)
+    return getattr(forward, "_current_level", 0) >= 0 and any(
+        t is not None and forward.unpack_dual(t).tangent is not None for t in tensors)
+
+
+def _wrote(torch, *tensors) -> None:
+    """Counts a kernel's writes into tensors that the caller holds, as torch's own in-place
+    operations do: a backward pass that has saved one of them refuses to use it."""
+    torch.autograd.graph.increment_version(tensors)
+
+
 def _index_vector_ok(t, device, count: int, dtype) -> bool:
     """A contiguous vector of at least ``count`` indexes on ``device``."""
     return t.dtype == dtype and t.dim() == 1 and t.is_contiguous() and t.device == device and \
@@ -1317,6 +1334,7 @@ def plan_step_paged(new_tokens, cached_tokens, tables, free_blocks, free_start,
             cached_tokens.numel() != requests or tables.shape[0] != requests or \
             (tables.shape[1] != 1 and tables.stride(1) != 1) or block_tokens <= 0 or max_tokens < 0:
         return None
+    given = plan or ()
     if plan is None:
         plan = new_step_plan(requests, max_tokens, device, torch)
     elif not (_index_vector_ok(plan.query_starts, device, requests + 1, i32)
@@ -1336,7 +1354,10 @@ def plan_step_paged(new_tokens, cached_tokens, tables, free_blocks, free_start,
                    plan.lacking.data_ptr())
     if got < 0:
         _raise_last(lib, "splitzip step plan failed")
-    return plan if got else None
+    if not got:
+        return None
+    _wrote(torch, tables, *given)
+    return plan
 
 
 def _kv_layer_ok(kv_layer, dtype, device) -> bool:
@@ -1353,7 +1374,8 @@ def write_kv_paged(k, v, kv_layer, slots) -> int | None:
     bf16 or fp16; rows and heads may be strided (views of one projection). ``slots`` may
     be longer than the rows. Of two rows with one slot it is not said whose values stay (a
     plan's slots are distinct). Returns the rows' bytes (0 without rows), or ``None`` when the kernel
-    declines (other types or layouts, rows or slots that overlap the layer)."""
+    declines (other types or layouts, rows or slots that overlap the layer, gradients or
+    tangents that the write would lose)."""
     lib = _load()
     write = getattr(lib, "kvq_splitzip_write_kv_paged", None) if lib else None
     if write is None or not _is_cuda(k):
@@ -1369,6 +1391,8 @@ def write_kv_paged(k, v, kv_layer, slots) -> int | None:
             (head_dim != 1 and (k.stride(2) != 1 or v.stride(2) != 1)) or \
             not _index_vector_ok(slots, device, tokens, torch.int64):
         return None
+    if _tracked(torch, k, v, kv_layer):
+        return None
     if tokens == 0:
         return 0
     got = _call_on(device, torch, write, k.data_ptr(), v.data_ptr(), tokens, heads, 2 * head_dim,
@@ -1377,7 +1401,10 @@ def write_kv_paged(k, v, kv_layer, slots) -> int | None:
                    kv_layer.shape[1] * kv_layer.shape[2], slots.data_ptr())
     if got < 0:
         _raise_last(lib, "splitzip K/V write failed")
-    return int(got) or None
+    if not got:
+        return None
+    _wrote(torch, kv_layer)
+    return int(got)
 
 
 @functools.lru_cache(maxsize=1024)
@@ -1475,7 +1502,8 @@ def chunk_attention_paged(q, kv_layer, tables, query_starts, context_tokens, *,
     the same tile, of 16 to 256 of a KV head's query rows, at least). Where
     query_starts run backwards, so that ranges overlap, rows are one of their requests' or stay.
     ``out``, ``lse`` and ``workspace`` over an input or each other are declined.
-    No gradient: inputs that require one are declined while gradients are recorded.
+    No gradient: inputs, ``out`` or ``lse`` that require one are declined while gradients are
+    recorded, and so are forward-mode tangents.
 
     Returns ``out`` (tokens, q_heads, head_dim), or ``None`` when the kernel declines."""
     lib = _load()
@@ -1489,7 +1517,7 @@ def chunk_attention_paged(q, kv_layer, tables, query_starts, context_tokens, *,
     if dtype is None or not _rows_ok(q, q.dtype, device) or \
             not _kv_layer_ok(kv_layer, q.dtype, device):
         return None
-    if (q.requires_grad or kv_layer.requires_grad) and torch.is_grad_enabled():
+    if _tracked(torch, q, kv_layer, out, lse):
         return None
     tokens, q_heads, head_dim = q.shape
     _, blocks, block_tokens, kv_heads, kv_dim = kv_layer.shape
@@ -1501,6 +1529,7 @@ def chunk_attention_paged(q, kv_layer, tables, query_starts, context_tokens, *,
             not _index_vector_ok(context_tokens, device, requests, torch.int32):
         return None
     max_query = tokens if max_query is None else min(int(max_query), tokens)
+    given = [t for t in (out, lse) if t is not None]
     ok, out = _attention_buffers(q, out, lse, torch)
     if not ok:
         return None
@@ -1522,7 +1551,11 @@ def chunk_attention_paged(q, kv_layer, tables, query_starts, context_tokens, *,
                    head_dim ** -0.5 if scale is None else float(scale))
     if got < 0:
         _raise_last(lib, "splitzip chunk attention failed")
-    return out if got else None
+    if not got:
+        return None
+    if given:
+        _wrote(torch, *given)
+    return out
 
 
 def prompt_attention(q, k, v, query_starts, *, max_query: int | None = None,
@@ -1546,7 +1579,7 @@ def prompt_attention(q, k, v, query_starts, *, max_query: int | None = None,
     if dtype is None or not _rows_ok(q, q.dtype, device) or not _rows_ok(k, q.dtype, device) or \
             not _rows_ok(v, q.dtype, device):
         return None
-    if (q.requires_grad or k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
+    if _tracked(torch, q, k, v, out, lse):
         return None
     tokens, q_heads, head_dim = q.shape
     kv_heads = k.shape[1]
@@ -1555,6 +1588,7 @@ def prompt_attention(q, k, v, query_starts, *, max_query: int | None = None,
         return None
     requests = query_starts.numel() - 1
     max_query = tokens if max_query is None else min(int(max_query), tokens)
+    given = [t for t in (out, lse) if t is not None]
     ok, out = _attention_buffers(q, out, lse, torch)
     if not ok:
         return None
@@ -1575,7 +1609,11 @@ def prompt_attention(q, k, v, query_starts, *, max_query: int | None = None,
                    head_dim ** -0.5 if scale is None else float(scale))
     if got < 0:
         _raise_last(lib, "splitzip prompt attention failed")
-    return out if got else None
+    if not got:
+        return None
+    if given:
+        _wrote(torch, *given)
+    return out
 
 
 # ---------------------------------------------------------------------------
