@@ -110,3 +110,10 @@ def test_writes_count_as_in_place_operations(entered):
     # a call that is declined has written nothing
     before = kv._version
     assert write(k=rows(2).float(), kv=kv) is None and kv._version == before
+
+
+def test_heads_without_values(entered):
+    """No default scale is formed of a head_dim of 0."""
+    q, k = rows(4)[..., :0], rows(2)[..., :0]
+    assert prompt(q, k, k) is None and prompt(q, k, k, scale=1.0) is None
+    assert chunk(q) is None and not entered

@@ -1583,7 +1583,7 @@ def prompt_attention(q, k, v, query_starts, *, max_query: int | None = None,
         return None
     tokens, q_heads, head_dim = q.shape
     kv_heads = k.shape[1]
-    if k.shape != v.shape or k.shape[0] != tokens or k.shape[2] != head_dim or \
+    if k.shape != v.shape or k.shape[0] != tokens or k.shape[2] != head_dim or head_dim == 0 or \
             not _index_vector_ok(query_starts, device, 1, torch.int32):
         return None
     requests = query_starts.numel() - 1
