@@ -117,3 +117,22 @@ def test_heads_without_values(entered):
     q, k = rows(4)[..., :0], rows(2)[..., :0]
     assert prompt(q, k, k) is None and prompt(q, k, k, scale=1.0) is None
     assert chunk(q) is None and not entered
+
+
+@pytest.mark.parametrize("width", (0, 3))
+def test_a_step_of_no_requests(entered, width):
+    """Every row is nobody's, nothing is taken from the free list, and the rows of q stay."""
+    none, tables = i32([]), torch.zeros((0, width), dtype=torch.int32)
+    for start in (4, -2):
+        for plan in (None, sz.new_step_plan(0, 5, "cpu")):
+            got = sz.plan_step_paged(none, none, tables, i32([7, 8]), i32([start]), 16, 5, plan=plan)
+            assert plan is None or got is plan
+            assert got.query_starts.tolist() == [0] and got.context_tokens.tolist() == []
+            assert got.slots.tolist() == [-1] * 5 and got.positions.tolist() == [0] * 5
+            assert got.free_next.tolist() == [max(start, 0)] and got.lacking.tolist() == [0]
+    out = torch.full((3, 4, 64), 7.0, dtype=torch.bfloat16)
+    assert sz.chunk_attention_paged(rows(4), layer(), tables, got.query_starts, got.context_tokens,
+                                    out=out) is out
+    assert (out == 7).all() and not entered
+    assert sz.plan_step_paged(none, none, tables, i32([7]), i32([0]), 0, 5) is None
+    assert sz.plan_step_paged(none, i32([1]), tables, i32([7]), i32([0]), 16, 5) is None

@@ -1311,7 +1311,7 @@ def plan_step_paged(new_tokens, cached_tokens, tables, free_blocks, free_start,
     tensors on one GPU (the rows of ``tables`` may be strided). ``max_tokens`` is the row
     count of the step's packed tensors; tokens past it get no row (query_starts still
     counts them). A block past the free list or the table's width is not given: its entry
-    and its tokens' slots are -1, and ``lacking`` counts it.
+    and its tokens' slots are -1, and ``lacking`` counts it. A step of no requests is planned, too.
 
     Returns a ``StepPlan`` (``plan``, when given: from ``new_step_plan`` or an earlier call
     of the same sizes, and overlapping none of the inputs; a step whose ``cached_tokens``
@@ -1325,7 +1325,7 @@ def plan_step_paged(new_tokens, cached_tokens, tables, free_blocks, free_start,
 
     device, i32 = new_tokens.device, torch.int32
     requests, block_tokens, max_tokens = new_tokens.numel(), int(block_tokens), int(max_tokens)
-    if not (_index_vector_ok(new_tokens, device, 1, i32)
+    if not (_index_vector_ok(new_tokens, device, 0, i32)
             and _index_vector_ok(cached_tokens, device, requests, i32)
             and _index_vector_ok(free_blocks, device, 0, i32)
             and _index_vector_ok(free_start, device, 1, i32)):
@@ -1344,6 +1344,13 @@ def plan_step_paged(new_tokens, cached_tokens, tables, free_blocks, free_start,
               and _index_vector_ok(plan.free_next, device, 1, i32)
               and _index_vector_ok(plan.lacking, device, 1, i32)):
         return None
+    if requests == 0:  # an idle step
+        plan.query_starts[:1].fill_(0)
+        plan.slots[:max_tokens].fill_(-1)
+        plan.positions[:max_tokens].fill_(0)
+        plan.free_next[:1].copy_(free_start[:1].clamp_min(0))
+        plan.lacking[:1].fill_(0)
+        return plan
     width = tables.shape[1]
     got = _call_on(device, torch, make, new_tokens.data_ptr(), cached_tokens.data_ptr(), requests,
                    tables.data_ptr(), tables.stride(0) if requests > 1 else width, width,
@@ -1533,7 +1540,7 @@ def chunk_attention_paged(q, kv_layer, tables, query_starts, context_tokens, *,
     ok, out = _attention_buffers(q, out, lse, torch)
     if not ok:
         return None
-    if tokens == 0:
+    if tokens == 0 or requests == 0:
         return out
     if max_query <= 0 or width == 0:
         return None
