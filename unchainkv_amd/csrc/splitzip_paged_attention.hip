@@ -553,9 +553,7 @@ __device__ __forceinline__ void tile_path(const AttendArgs& a, const Request& re
   const unsigned int token = valid ? m / a.group : 0u;
   const unsigned int q_head = head * a.group + (valid ? m - token * a.group : 0u);
   const int limit = valid ? shift + (int)token : -1;
-  // of the wave's rows: the last visible token of the first and of the last
-  const int first_limit = shift + (int)(mw / a.group);
-  const int last_limit = mw < rows ? shift + (int)((min(rows, mw + 32) - 1) / a.group) : -1;
+  const int first_limit = shift + (int)(mw / a.group);  // the last visible token of the wave's first row
 
   const int* table = kPaged ? a.tables + request.r * a.table_stride : nullptr;
   const unsigned char* kb = a.k + head * a.k_head;
