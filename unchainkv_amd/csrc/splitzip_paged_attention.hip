@@ -236,19 +236,22 @@ constexpr unsigned int kNoSlot = ~0u;
 // Sums of 64 lanes' values stay below 2^32.
 constexpr unsigned int kMostSteps = 1u << 25;
 
-// ceil(sum * heads / parts), by a 32-bit division where it serves, and kMostSteps where it is more
-// (no request has more steps; the sum of 2^31 requests times their heads may pass 64 bits).
+// ceil(sum * heads / parts), or a little more past 2^32 / parts (one 32-bit division serves: every
+// workgroup waits for it), but at most kMostSteps: no request that is cut has more. The sum of 2^31
+// requests times their heads may pass 64 bits.
 __host__ __device__ __forceinline__ constexpr unsigned int share_of(unsigned long long sum,
                                                                     unsigned int heads, unsigned int parts) {
-  if ((sum >> 50) != 0) return kMostSteps;
-  sum = sum * heads + parts - 1;
-  if ((sum >> 32) == 0) return (unsigned int)sum / parts;
-  sum /= parts;
-  return sum < kMostSteps ? (unsigned int)sum : kMostSteps;
+  const unsigned long long all = (sum >> 50) != 0 ? ~0ull : sum * heads + parts - 1;
+  if (all >= (unsigned long long)kMostSteps * parts) return kMostSteps;
+  const bool wide = (all >> 32) != 0;
+  const unsigned int share = (wide ? (unsigned int)(all >> 16) + parts : (unsigned int)all) / parts;
+  return wide ? share << 16 : share;
 }
 static_assert(share_of(0, 8, 192) == 0 && share_of(1, 1, 192) == 1 && share_of(384, 1, 192) == 2 &&
-              share_of(385, 1, 192) == 3 && share_of(1ull << 36, 1, 8192) == 1u << 23, "rounded up");
-static_assert(share_of(1ull << 37, 8, 192) == kMostSteps && share_of(1ull << 56, 4096, 512) == kMostSteps &&
+              share_of(385, 1, 192) == 3 && share_of(192u << 20, 8, 192) == 8u << 20, "rounded up");
+static_assert(share_of(1ull << 32, 1, 192) * 192ull >= 1ull << 32 &&
+              share_of(1ull << 32, 1, 192) < 22500000u &&  // (of 22369622)
+              share_of(1ull << 37, 8, 192) == kMostSteps && share_of(1ull << 56, 4096, 512) == kMostSteps &&
               share_of((1ull << 50) - 1, 4096, 512) == kMostSteps, "the share, or what cuts nothing");
 
 // The launch's work, which every workgroup finds its own item of by itself. Requests lie one in a
@@ -517,8 +520,8 @@ __device__ __forceinline__ void clear_jobs(const AttendArgs& a, unsigned int slo
 // per half wave.
 template <typename E, int D, bool kPaged, bool kRuns>
 __device__ __forceinline__ void tile_path(const AttendArgs& a, const Request& request,
-                                          unsigned int index, unsigned int most,
-                                          unsigned int split_tokens, unsigned int slot,
+                                          unsigned int order, unsigned int split, unsigned int most,
+                                          unsigned int split_tokens, bool whole, unsigned int slot,
                                           unsigned int head, unsigned char* s0, unsigned char* s1,
                                           unsigned char* s2) {
   typedef typename Elem<E>::x8 x8;
@@ -532,7 +535,7 @@ __device__ __forceinline__ void tile_path(const AttendArgs& a, const Request& re
   const unsigned int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
   const unsigned int half = lane / 32, col = lane % 32;
   // the tiles with the longest contexts first
-  const unsigned int tile = tiles_of<kTileRows>(a, request.n) - 1 - index / most, split = index % most;
+  const unsigned int tile = tiles_of<kTileRows>(a, request.n) - 1 - order;
   const unsigned int rows = request.n * a.group;
   const unsigned int m0 = tile * kTileRows;
   // last visible token of a row (negative: none)
@@ -543,7 +546,7 @@ __device__ __forceinline__ void tile_path(const AttendArgs& a, const Request& re
   if (most > 1)
     store_job(a, slot, head,
               Job{request.start, m0, shift, (unsigned short)min(rows - m0, (unsigned int)kTileRows),
-                  (unsigned short)(split == 0 && splits > 1 ? splits : 0u)});
+                  (unsigned short)(split == 0 && splits > 1 && whole ? splits : 0u)});
   if (split >= splits) return;
   slot = slot * a.kv_heads + head;
   const unsigned int t_begin = split * split_tokens;
@@ -977,8 +980,8 @@ __device__ __forceinline__ void tile_path(const AttendArgs& a, const Request& re
 // bytes at 16 (l / 16) of every 64, each counting.)
 template <typename E, int D, int kN, int kRows>
 __device__ __forceinline__ void few_path(const AttendArgs& a, const Request& request, unsigned int split,
-                                         unsigned int splits, unsigned int split_tokens, unsigned int slot,
-                                         unsigned int head, unsigned char* __restrict__ s0,
+                                         unsigned int splits, unsigned int split_tokens, bool whole,
+                                         unsigned int slot, unsigned int head, unsigned char* __restrict__ s0,
                                          unsigned char* __restrict__ s1,
                                          unsigned char* __restrict__ s2) {
   typedef typename Elem<E>::x8 x8;
@@ -995,7 +998,7 @@ __device__ __forceinline__ void few_path(const AttendArgs& a, const Request& req
   store_job(a, slot, head,
             Job{request.start, 0, (int)request.ctx - (int)request.n,
                 (unsigned short)(request.n * a.group),
-                (unsigned short)(split == 0 && splits > 1 ? splits : 0u)});
+                (unsigned short)(split == 0 && splits > 1 && whole ? splits : 0u)});
   slot = slot * a.kv_heads + head;
   const unsigned int rows = request.n * a.group;
   const unsigned int t_begin = split * split_tokens;
@@ -1246,20 +1249,19 @@ __global__ __launch_bounds__(kWave * tile_waves(D), D == 128 ? 2 : 3) void atten
   }
   if (!found) return;
   const unsigned int most = work.splits(request), split_tokens = work.split_tokens(request, most);
-  if (most > 1 && item - index % most + most > a.items) {
-    // (row ranges that overlap each other can ask for more items than there are: a tile without all
-    // its splits is left)
-    store_job(a, slot, head, Job{});
-    return;
-  }
+  const unsigned int order = index / most, split = index - order * most;
+  // (row ranges that overlap each other can ask for more items than there are: a tile without all its
+  // splits is left)
+  const bool whole = item - split + most <= a.items;
   if constexpr (kPaged) {
     if (work.few(request.n)) {
       if (!has_slot) slot = kNoSlot;
-      few_path<E, D, kN, kRows>(a, request, index, most, split_tokens, slot, head, s0, s1, s2);
+      few_path<E, D, kN, kRows>(a, request, split, most, split_tokens, whole, slot, head, s0, s1, s2);
       return;
     }
   }
-  tile_path<E, D, kPaged, kRuns>(a, request, index, most, split_tokens, slot, head, s0, s1, s2);
+  tile_path<E, D, kPaged, kRuns>(a, request, order, split, most, split_tokens, whole, slot, head, s0, s1,
+                                   s2);
 }
 
 template <typename E, int D>
@@ -1278,8 +1280,8 @@ __global__ __launch_bounds__(kWave * kWaves, 2) void attention_few(AttendArgs a)
     return;
   }
   const unsigned int splits = work.splits(request);
-  few_path<E, D, kWaves, kFewRows>(a, request, split, splits, work.split_tokens(request, splits), slot,
-                                   head, s0, s1, s2);
+  few_path<E, D, kWaves, kFewRows>(a, request, split, splits, work.split_tokens(request, splits), true,
+                                   slot, head, s0, s1, s2);
 }
 
 // ---------------------------------------------------------------------------

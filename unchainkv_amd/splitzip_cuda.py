@@ -1247,8 +1247,10 @@ def _call_on(device, torch, fn, *args):
 def _tracked(torch, *tensors) -> bool:
     """Whether autograd follows any of the tensors (None: not given): a gradient is required while
     gradients are recorded, or there is a forward-mode tangent. The kernels give neither."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        return True
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
     forward = torch.autograd.forward_ad
     # (outside its levels no tensor has a tangent, which spares asking each)
     return getattr(forward, "_current_level", 0) >= 0 and any(
