@@ -5,7 +5,7 @@ bound is derived in paged_attention_ref.py) unless a test says otherwise."""
 import numpy as np
 import pytest
 
-from paged_attention_ref import HALF_STEP
+from paged_attention_ref import HALF_STEP, attend
 from test_gpu_paged_attention import (  # noqa: F401 (sz: a fixture)
     DTYPES, MARK, Case, f64, i32, say, starts_of, sz)
 
@@ -130,3 +130,29 @@ def test_workspace_of_the_largest_step_serves_smaller_ones(sz):  # noqa: F811
         assert sz.prompt_attention(q, k, v, starts, max_query=max(new), out=out, workspace=space) is out
         assert torch.cuda.max_memory_allocated() == held
         assert torch.equal(out, expect)
+
+
+@pytest.mark.parametrize("dim,dtype", [(128, "bf16"), (64, "fp16")])
+def test_results_joined_by_their_log_sum_exps(sz, dim, dtype):  # noqa: F811
+    """Attention over the first tokens and over the others, joined by lse, is attention over all (each
+    part is within its bound, so the whole is, as the weights of the parts add up to 1; the parts'
+    own rounding adds another half step of the mean)."""
+    contexts, firsts = [70, 3000, 40], [32, 2000, 0]
+    case = Case([1] * 3, contexts, 4, 2, dim, 16, dtype, seed=dim, spare_rows=0)
+    parts = []
+    for first, count in ((False, firsts), (True, [c - f for c, f in zip(contexts, firsts)])):
+        tables = torch.full_like(case.tables, -1)
+        for r, f in enumerate(firsts):
+            own = case.tables[r, f // 16:] if first else case.tables[r, :f // 16]
+            tables[r, :len(own)] = own
+        lse = torch.empty(case.q.shape[:2], dtype=torch.float32, device="cuda")
+        parts.append((sz.chunk_attention_paged(case.q, case.kv, tables, case.starts, i32(count),
+                                               lse=lse).float(), lse))
+    (o1, l1), (o2, l2) = parts
+    lse = torch.logaddexp(l1, l2)
+    out = f64(o1 * (l1 - lse).exp()[..., None] + o2 * (l2 - lse).exp()[..., None])
+    for r, c in enumerate(contexts):
+        ref, ref_lse, mean, off = attend(f64(case.q[r:r + 1]), case.k[r], case.v[r], c - 1, case.scale)
+        bound = HALF_STEP[dtype] * (2 * mean + np.abs(ref)) * 1.01 + 4 * off[..., None] * mean + 2.0 ** -22
+        assert (np.abs(out[r:r + 1] - ref) <= bound + (2.0 ** -24 if dtype == "fp16" else 0)).all()
+        assert (np.abs(f64(lse[r:r + 1]) - ref_lse) <= 4 * off + 2.0 ** -20).all()

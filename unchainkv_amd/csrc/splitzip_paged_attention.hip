@@ -22,10 +22,10 @@
 //     reads. 32 requests of 8192 tokens, 32 / 8 heads of 128: 191 us for 1.07 GB, 5.6 TB/s.
 //   * attention_tiles: more; 256 rows (64-dim heads: 128) by 64 tokens a step, requests of at most 16
 //     rows streamed like the others. Bound by the matrix and vector units, and by the clock that the
-//     power limit leaves them: a prompt of 16384 tokens, 8 / 1 heads of 128: 481 us, 1.14 PFLOP/s, the
+//     power limit leaves them: a prompt of 16384 tokens, 8 / 1 heads of 128: 475 us, 1.16 PFLOP/s, the
 //     matrix units busy 63 % of the cycles at 1.7 GHz (the library's product of 8192^3: 1.29, 69 %);
-//     8 of 4096, 32 / 8 heads: 1054 us, 1.04 PFLOP/s; heads of 64 reach 0.86, as they have twice the
-//     softmax for each product.
+//     8 of 4096, 32 / 8 heads: 1063 us, 1.03 PFLOP/s; heads of 64 reach 0.86, as they have twice the
+//     softmax for each product (VALU active 0.74 of the cycles, matrix units 0.44).
 // Both give S^T = K Q^T, so that a row's scores lie in one lane (and its partners 32 or 16 lanes
 // away): the maximum and the sum need one or two lane swaps a step, rescaling is a lane's own
 // product, and the weights are the second product's operand O^T = V^T P^T as they are, with V's
@@ -65,7 +65,7 @@ constexpr int tile_waves(int D) { return D == 128 ? 8 : 4; }
 constexpr int tile_rows(int D) { return 32 * tile_waves(D); }
 constexpr int kMergeThreads = 256;
 // An odd count, so that the slots of the first splits, which have the work and lie at even distances,
-// fall to all of them (32 requests of 8192 tokens: 7.2 us, 11.6 with 1024 workgroups).
+// fall to all of them (32 requests of 8192 tokens: 6.2 us, 11.6 with 1024 workgroups).
 constexpr unsigned int kMergeGroups = 1021;
 // Rows of a request that is streamed: by attention_few, and by attention_tiles where longer requests
 // are beside it (as tiles a chunk of 2048 behind 8192 and 64 single tokens, 32 / 8 heads of 64, take
@@ -78,10 +78,11 @@ constexpr int kTileTokens = 64;   // tokens of a step of attention_tiles: unit o
 // Steps of a split, at least: its start and its share of the joining take as long as some of them (4
 // requests of 64 tokens behind 4000: 39.1 us at 12, 44.8 at 16).
 constexpr unsigned int kLeastTileSteps = 12;
-// Of a streamed split, in rounds of kFewUnit tokens (16 requests of 1024 tokens, 32 / 8 heads of 128:
-// 22.2 us at 4, 26.8 at 1; 4 of 4096: 22.4 and 24.6). A call whose block tables hold no more than
-// kWholeFewSteps is not cut at all and joins nothing: one launch (one request, 32 / 8 heads of 64, 1024
-// tokens: 14.1 us, cut 16.7; of 128, 768 tokens 13.7 and 16.0, 1024 the same, 1536 21.1 and 16.0).
+// Of a streamed split, in rounds of kFewUnit tokens (4 requests of 4096 tokens, 32 / 8 heads of 128:
+// 22.5 us at 4, 24.6 at 1). A call whose block tables hold no more than kWholeFewSteps is not cut at
+// all and joins nothing: one launch (one request, 32 / 8 heads of 64, 1024 tokens: 12.6 us, cut 16.8,
+// for the host's second submission: captured 10.8 and 11.2; of 128 dims, uncut and cut, 768 tokens 13.7
+// and 16.0, 1024 the same, 1536 21.1 and 16.0).
 constexpr unsigned int kLeastFewSteps = 4, kWholeFewSteps = 8;
 // A maximum before any token: the lowest float, not -inf, so that rows whose scores are all -inf
 // have weights of zero and a sum of zero (whose quotient is NaN, as the formula's).
