@@ -606,6 +606,102 @@ long long kvq_splitzip_prompt_attention(
     unsigned long long lse_ptr, unsigned long long workspace_ptr,
     unsigned long long workspace_bytes, float scale, unsigned long long stream_ptr);
 
+/* write_kv_paged with the position rotation: the first rotary_dim values of each head of q (tokens,
+ * q_heads; head h of row t at q + t * q_row_bytes + h * q_head_bytes) and k are rotated in pairs, (x, y) ->
+ * (x cos - y sin, y cos + x sin), values i and i + rotary_dim / 2 (adjacent 0) or 2 i and 2 i + 1 (1), with
+ * rotation (f32, rotation_rows x rotary_dim: a position's cosines, then its sines) at positions[t] (i64;
+ * outside the table: NaN); q goes to out [tokens][q_heads][head_dim], k and v to kv by slots[t] as above. dtype
+ * 0: bf16, 1: fp16; strides and addresses even (multiples of 16 bytes, and of 16 rotated values, are the fast
+ * case). kv and out must overlap neither an input nor each other. Returns the rows' bytes, 0 on a failed
+ * precondition. */
+long long kvq_splitzip_rotate_write_kv_paged(
+    unsigned long long q_ptr, unsigned long long q_row_bytes, unsigned long long q_head_bytes,
+    unsigned long long q_heads, unsigned long long k_ptr, unsigned long long k_row_bytes,
+    unsigned long long k_head_bytes, unsigned long long v_ptr, unsigned long long v_row_bytes,
+    unsigned long long v_head_bytes, unsigned long long tokens, unsigned long long kv_heads,
+    unsigned long long head_dim, unsigned long long dtype, unsigned long long kv_ptr,
+    unsigned long long plane_bytes, unsigned long long slot_count, unsigned long long slots_ptr,
+    unsigned long long positions_ptr, unsigned long long rotation_ptr, unsigned long long rotation_rows,
+    unsigned long long rotary_dim, unsigned long long adjacent, unsigned long long out_ptr,
+    unsigned long long stream_ptr);
+
+/* kvq_splitzip_chunk_attention_paged with every row of request r over all of its source_tokens[r] tokens
+ * (rows of a request without tokens are 0, lse -inf); the same arguments and workspace. */
+long long kvq_splitzip_cross_attention_paged(
+    unsigned long long q_ptr, unsigned long long q_row_bytes, unsigned long long q_head_bytes,
+    unsigned long long tokens, unsigned long long q_heads, unsigned long long kv_heads,
+    unsigned long long head_dim, unsigned long long dtype, unsigned long long kv_ptr,
+    unsigned long long blocks, unsigned long long block_tokens, unsigned long long tables_ptr,
+    unsigned long long table_stride, unsigned long long table_width,
+    unsigned long long query_starts_ptr, unsigned long long source_tokens_ptr,
+    unsigned long long requests, unsigned long long max_query, unsigned long long out_ptr,
+    unsigned long long lse_ptr, unsigned long long workspace_ptr,
+    unsigned long long workspace_bytes, float scale, unsigned long long stream_ptr);
+
+/* The same over packed sources: request r's are rows source_starts[r] .. + source_tokens[r] of k and v
+ * (source_rows rows; strides multiples of 16). max_source (at most source_rows) bounds a source's tokens:
+ * rows of requests with more stay. A source outside the rows gives NaN. Workspace: the above for max_context =
+ * max_source. */
+long long kvq_splitzip_cross_attention(
+    unsigned long long q_ptr, unsigned long long q_row_bytes, unsigned long long q_head_bytes,
+    unsigned long long k_ptr, unsigned long long k_row_bytes, unsigned long long k_head_bytes,
+    unsigned long long v_ptr, unsigned long long v_row_bytes, unsigned long long v_head_bytes,
+    unsigned long long source_rows, unsigned long long tokens, unsigned long long q_heads,
+    unsigned long long kv_heads, unsigned long long head_dim, unsigned long long dtype,
+    unsigned long long query_starts_ptr, unsigned long long source_starts_ptr,
+    unsigned long long source_tokens_ptr, unsigned long long requests, unsigned long long max_query,
+    unsigned long long max_source, unsigned long long out_ptr, unsigned long long lse_ptr,
+    unsigned long long workspace_ptr, unsigned long long workspace_bytes, float scale,
+    unsigned long long stream_ptr);
+
+/* ------------------------------------------------------------------------------
+ * Beam search over paged layers (no counterpart in the reference): the best continuations of a request's
+ * beams, and tables and layers in their order. Device arrays throughout; captured calls follow their values.
+ * ---------------------------------------------------------------------------- */
+
+/* Of each request the `candidates` best of beams x vocab by scores[b] + logit - log sum exp(logits of b), best
+ * first, equal ones by the lowest beam * vocab + token. logits: request r's beam b at element r *
+ * request_stride + b * beam_stride, vocab tokens behind each other; dtype 0: bf16, 1: fp16, 2: f32. scores
+ * f32, ended_ptr 0 or u8, both [requests][beams]. A beam of score -inf and a token of logit -inf offer -inf; an
+ * ended beam offers end_token at its score. NaN and +inf logits make their beam's offers NaN, which come
+ * first. At most 32 beams, 64 candidates, 2^20 tokens, 65535 requests * beams. Written: out_scores f32,
+ * out_parents i32, out_tokens i64 [requests][candidates]. Workspace 16-byte aligned, for one call at a time.
+ * Results and workspace must overlap neither an input nor each other. Returns requests * candidates, 0 on a
+ * failed precondition. */
+unsigned long long kvq_splitzip_beam_select_workspace_bytes(
+    unsigned long long requests, unsigned long long beams, unsigned long long vocab);
+long long kvq_splitzip_beam_select(
+    unsigned long long logits_ptr, unsigned long long dtype, unsigned long long request_stride,
+    unsigned long long beam_stride, unsigned long long scores_ptr, unsigned long long ended_ptr,
+    unsigned long long requests, unsigned long long beams, unsigned long long vocab,
+    unsigned long long candidates, unsigned long long end_token, unsigned long long out_scores_ptr,
+    unsigned long long out_parents_ptr, unsigned long long out_tokens_ptr,
+    unsigned long long workspace_ptr, unsigned long long workspace_bytes,
+    unsigned long long stream_ptr);
+
+/* Row r * beams + j of out (table_width entries, rows out_stride apart; out may be tables) lists the blocks of
+ * row r * beams + parents[r][j] of tables, as far as context_tokens[r * beams] tokens reach; entries behind
+ * them are the row's own. The last block, if partly filled, stays with the first child of its beam; the others
+ * take blocks that no parent lists, in the order of beams, and the used tokens of both planes are copied into
+ * them in each layer (layers: HOST array of layer_count addresses of (2, blocks, block_tokens, row_bytes)
+ * layers); copied_from[row]: the block copied, or -1. A child without such a block gets -1, and so does the
+ * whole context of one whose parent is outside 0 .. beams - 1; lacking[0] counts both. Blocks of the context
+ * that no row of the request lists any more are written to free_blocks (free_count entries) below entry
+ * free_start[0], in the order of requests, columns and beams; free_next[0] is the new first entry, unlisted[0]
+ * what found no room. At most 32 beams, 65535 requests. Results, layers and workspace must overlap neither an
+ * input nor each other. Returns requests * beams, 0 on a failed precondition. */
+unsigned long long kvq_splitzip_reorder_beams_workspace_bytes(
+    unsigned long long requests, unsigned long long beams, unsigned long long table_width);
+long long kvq_splitzip_reorder_beams_paged(
+    const unsigned long long* layers, unsigned long long layer_count, unsigned long long blocks,
+    unsigned long long block_tokens, unsigned long long row_bytes, unsigned long long tables_ptr,
+    unsigned long long table_stride, unsigned long long table_width, unsigned long long out_ptr,
+    unsigned long long out_stride, unsigned long long parents_ptr, unsigned long long context_tokens_ptr,
+    unsigned long long requests, unsigned long long beams, unsigned long long free_blocks_ptr,
+    unsigned long long free_count, unsigned long long free_start_ptr, unsigned long long copied_from_ptr,
+    unsigned long long free_next_ptr, unsigned long long lacking_ptr, unsigned long long unlisted_ptr,
+    unsigned long long workspace_ptr, unsigned long long workspace_bytes, unsigned long long stream_ptr);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,766 @@
+// A beam search's step over paged layers, gfx950: the best continuations of a request's beams, and
+// the block tables and layers put in the chosen order.
+//
+// Select. Beam b of a request offers every token t at score[b] + logit[b][t] - log sum_t' 2^..:
+//   value = (logit - lse) + score, lse = log sum exp(logit), the best `candidates` of all.
+// Every logit is read once, by beam_scan, which keeps of each 256 of them their maximum and of each
+// workgroup's share (max, sum of exp(logit - max)). The best n of all lie in the n segments with the largest
+// maxima (ties: the first), as each of n segments before a value's own holds one that comes before it; so
+// beam_pick, a workgroup for each request, joins the sums, takes the best n segments and reads them again,
+// and no logit is compared with more than a threshold. Values are formed and compared in 64 bits: what two
+// beams offer may differ by less than 32 hold of a sum of log probabilities.
+//
+// Reorder. Row r * beams + j of the tables follows parent p[j]: blocks that are full are shared (all
+// entries of a column are read by one thread, which then writes them), the last, partly filled block goes
+// on with the first of its children, and the others copy it into blocks that no parent left behind. Blocks
+// that no row of the request names any more go back below the free list's first entry, in an order that
+// does not depend on the launch (request, column, beam). Two launches: tables; copies of all layers, with
+// one workgroup for the list.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+
+#include "splitzip_common.h"
+
+namespace unchainkv {
+namespace {
+
+constexpr int kScanThreads = 256;
+constexpr int kLaneLogits = 8;                                // of a lane's load
+constexpr int kSegment = 32 * kLaneLogits;                    // logits whose maximum is kept
+constexpr int kRound = kScanThreads * kLaneLogits;            // logits of a workgroup's round
+constexpr int kPickThreads = 512;
+constexpr int kMostBeams = 32, kMostCandidates = 64;
+constexpr int kItems = 16;                                    // values that a lane of beam_pick holds
+constexpr unsigned int kMostVocab = 1u << 20;
+constexpr float kLowest = -3.402823466e38f;
+constexpr float kLog2E = 1.4426950408889634f;
+
+struct SelectArgs {
+  const unsigned char* logits;     // [requests][beams][vocab], strides in elements
+  const float* scores;             // [requests][beams]
+  const unsigned char* ended;      // [requests][beams] or null
+  float* maxima;                   // [requests * beams][segments]
+  float2* sums;                    // [requests * beams][chunks]: (max, sum)
+  float* out_scores;               // [requests][candidates]
+  int* out_parents;
+  long long* out_tokens;
+  unsigned long long request_stride, beam_stride;
+  unsigned int requests, beams, vocab, candidates, end_token;
+  unsigned int segments, chunks, rounds;  // of a row; rounds of a chunk
+};
+
+// Logits by their type, 8 of them from any address.
+struct Bf16 {
+  typedef struct __attribute__((packed, aligned(2))) { u32x4 v; } Raw;
+  static constexpr unsigned int kBytes = 2;
+  static __device__ __forceinline__ float one(const unsigned char* p, unsigned int i) {
+    return __uint_as_float((unsigned int)reinterpret_cast<const uint16_t*>(p)[i] << 16);
+  }
+  static __device__ __forceinline__ void eight(const unsigned char* p, float (&x)[8]) {
+    const u32x4 v = reinterpret_cast<const Raw*>(p)->v;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[2 * i] = __uint_as_float(v[i] << 16);
+      x[2 * i + 1] = __uint_as_float(v[i] & 0xFFFF0000u);
+    }
+  }
+};
+struct Fp16 {
+  typedef _Float16 x8 __attribute__((ext_vector_type(8)));
+  typedef struct __attribute__((packed, aligned(2))) { x8 v; } Raw;
+  static constexpr unsigned int kBytes = 2;
+  static __device__ __forceinline__ float one(const unsigned char* p, unsigned int i) {
+    return (float)reinterpret_cast<const _Float16*>(p)[i];
+  }
+  static __device__ __forceinline__ void eight(const unsigned char* p, float (&x)[8]) {
+    const x8 v = reinterpret_cast<const Raw*>(p)->v;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = (float)v[i];
+  }
+};
+struct Fp32 {
+  typedef float x4 __attribute__((ext_vector_type(4)));
+  typedef struct __attribute__((packed, aligned(4))) { x4 a, b; } Raw;
+  static constexpr unsigned int kBytes = 4;
+  static __device__ __forceinline__ float one(const unsigned char* p, unsigned int i) {
+    return reinterpret_cast<const float*>(p)[i];
+  }
+  static __device__ __forceinline__ void eight(const unsigned char* p, float (&x)[8]) {
+    const Raw v = *reinterpret_cast<const Raw*>(p);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[i] = v.a[i];
+      x[4 + i] = v.b[i];
+    }
+  }
+};
+
+// A beam that offers no token of its own: finished, or without a hypothesis yet.
+__device__ __forceinline__ bool is_ended(const SelectArgs& a, unsigned int row) {
+  return a.ended != nullptr && a.ended[row] != 0;
+}
+__device__ __forceinline__ bool is_open(const SelectArgs& a, unsigned int row) {
+  return !is_ended(a, row) && a.scores[row] != -INFINITY;
+}
+
+template <typename T>
+__device__ __forceinline__ const unsigned char* row_of(const SelectArgs& a, unsigned int row) {
+  const unsigned int request = row / a.beams;
+  return a.logits + (request * a.request_stride + (row - request * a.beams) * a.beam_stride) * T::kBytes;
+}
+
+// Largest of 32 lanes, in lanes 31 and 63 (row shifts by 1, 2, 4, 8, then rows 0 and 2 into the next).
+template <int kControl, int kRowMask>
+__device__ __forceinline__ float shifted(float v) {
+  const int u = __builtin_bit_cast(int, v);
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(u, u, kControl, kRowMask, 0xF, false));
+}
+__device__ __forceinline__ float max_of_32(float v) {
+  v = fmaxf(v, shifted<0x111, 0xF>(v));
+  v = fmaxf(v, shifted<0x112, 0xF>(v));
+  v = fmaxf(v, shifted<0x114, 0xF>(v));
+  v = fmaxf(v, shifted<0x118, 0xF>(v));
+  return fmaxf(v, shifted<0x142, 0xA>(v));
+}
+
+template <typename T>
+__global__ __launch_bounds__(kScanThreads) void beam_scan(SelectArgs a) {
+  __shared__ float s_max[kScanThreads / kWave], s_sum[kScanThreads / kWave];
+  const unsigned int row = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  if (!is_open(a, row)) return;
+  const unsigned char* src = row_of<T>(a, row);
+  float top = kLowest, sum = 0.f;
+  for (unsigned int n = 0; n < a.rounds; ++n) {
+    const unsigned int base = (blockIdx.x * a.rounds + n) * kRound;
+    if (base >= a.vocab) break;
+    const unsigned int at = base + tid * kLaneLogits;
+    float x[kLaneLogits];
+    if (at + kLaneLogits <= a.vocab) {
+      T::eight(src + at * T::kBytes, x);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kLaneLogits; ++i)
+        x[i] = at + i < a.vocab ? T::one(src, at + i) : -INFINITY;
+    }
+    float own = x[0];
+#pragma unroll
+    for (int i = 1; i < kLaneLogits; ++i) own = fmaxf(own, x[i]);
+    const float now = fmaxf(top, own);
+    float part = 0.f;
+#pragma unroll
+    for (int i = 0; i < kLaneLogits; ++i) part += __builtin_amdgcn_exp2f((x[i] - now) * kLog2E);
+    sum = sum * __builtin_amdgcn_exp2f((top - now) * kLog2E) + part;
+    top = now;
+    // (a NaN, or infinity, which makes the row's sum NaN: every value that is not -inf is then NaN)
+    own = part != part ? INFINITY : own;
+    own = max_of_32(own);
+    const unsigned int segment = at / kSegment;
+    if (lane % 32 == 31 && segment < a.segments)
+      a.maxima[(unsigned long long)row * a.segments + segment] = own;
+  }
+  float big = top;
+#pragma unroll
+  for (int d = 1; d < kWave; d *= 2) big = fmaxf(big, __shfl_xor(big, d, kWave));
+  sum *= __builtin_amdgcn_exp2f((top - big) * kLog2E);
+#pragma unroll
+  for (int d = 1; d < kWave; d *= 2) sum += __shfl_xor(sum, d, kWave);
+  if (lane == 0) {
+    s_max[wave] = big;
+    s_sum[wave] = sum;
+  }
+  __syncthreads();
+  if (tid == 0) {
+    float m = s_max[0], l = 0.f;
+#pragma unroll
+    for (int w = 1; w < kScanThreads / kWave; ++w) m = fmaxf(m, s_max[w]);
+#pragma unroll
+    for (int w = 0; w < kScanThreads / kWave; ++w)
+      l += s_sum[w] * __builtin_amdgcn_exp2f((s_max[w] - m) * kLog2E);
+    a.sums[(unsigned long long)row * a.chunks + blockIdx.x] = make_float2(m, l);
+  }
+}
+
+// Values as numbers that compare alike: NaN above all, -0 as 0, nothing as 0.
+__device__ __forceinline__ unsigned long long key_of(double v) {
+  if (v != v) return ~0ull;
+  const unsigned long long u = __builtin_bit_cast(unsigned long long, v + 0.0);
+  return (u >> 63) != 0 ? ~u : u | 1ull << 63;
+}
+__device__ __forceinline__ double value_of(unsigned long long key) {
+  if (key == ~0ull) return NAN;
+  return __builtin_bit_cast(double, (key >> 63) != 0 ? key & ~(1ull << 63) : ~key);
+}
+
+__device__ __forceinline__ unsigned long long wave_best(unsigned long long v) {
+#pragma unroll
+  for (int d = 1; d < kWave; d *= 2) {
+    const unsigned long long o = __shfl_xor(v, d, kWave);
+    v = o > v ? o : v;
+  }
+  return v;
+}
+__device__ __forceinline__ unsigned int wave_least(unsigned int v) {
+#pragma unroll
+  for (int d = 1; d < kWave; d *= 2) v = min(v, (unsigned int)__shfl_xor((int)v, d, kWave));
+  return v;
+}
+
+// The best of a wave's items (item t of lane l has number t * 64 + l) that are at least `least`, best
+// first and at most `most`, each given to `take(key, number)` by all lanes.
+template <typename Take>
+__device__ __forceinline__ void best_of(unsigned long long (&keys)[kItems], unsigned int most,
+                                        unsigned long long least, Take take) {
+  const unsigned int lane = __lane_id();
+  for (unsigned int n = 0; n < most; ++n) {
+    unsigned long long own = 0;
+    unsigned int at = 0;
+#pragma unroll
+    for (int t = 0; t < kItems; ++t)
+      if (keys[t] > own) {
+        own = keys[t];
+        at = t;
+      }
+    const unsigned long long best = wave_best(own);
+    if (best == 0 || best < least) break;
+    const unsigned int number = wave_least(own == best ? at * kWave + lane : ~0u);
+#pragma unroll
+    for (int t = 0; t < kItems; ++t)
+      if (t * kWave + lane == number) keys[t] = 0;
+    take(best, number, n);
+  }
+}
+
+template <typename T>
+__global__ __launch_bounds__(kPickThreads) void beam_pick(SelectArgs a) {
+  constexpr int kWaves = kPickThreads / kWave;
+  __shared__ double s_lse[kMostBeams], s_score[kMostBeams];
+  __shared__ unsigned char s_state[kMostBeams];  // 0: open, 1: ended, 2: empty
+  // the beams' best segments, and then the best values of those chosen: `most` of each
+  __shared__ unsigned long long s_key[kMostCandidates * kMostCandidates];
+  __shared__ unsigned int s_id[kMostCandidates * kMostCandidates];
+  __shared__ unsigned int s_chosen[kMostCandidates], s_count;
+  __shared__ unsigned long long s_least;
+  const unsigned int request = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
+  const unsigned int row0 = request * a.beams, most = a.candidates;
+  const unsigned long long nothing = key_of(-INFINITY);
+  // segments of an item, so that a wave holds a row's
+  const unsigned int group = (a.segments + kItems * kWave - 1) / (kItems * kWave);
+  const unsigned int items = (a.segments + group - 1) / group;
+
+  for (unsigned int i = tid; i < a.beams * most; i += kPickThreads) s_key[i] = 0;
+  if (tid == 0) {
+    s_count = 0;
+    s_least = 0;
+  }
+  if (tid < kMostCandidates) s_chosen[tid] = ~0u;
+  __syncthreads();
+  for (unsigned int b = wave; b < a.beams; b += kWaves) {
+    const unsigned int row = row0 + b;
+    const bool ended = is_ended(a, row), open = is_open(a, row);
+    const double score = a.scores[row];
+    double lse = 0.;
+    if (open) {
+      const float2* sums = a.sums + (unsigned long long)row * a.chunks;
+      float top = kLowest;
+      for (unsigned int c = lane; c < a.chunks; c += kWave) top = fmaxf(top, sums[c].x);
+#pragma unroll
+      for (int d = 1; d < kWave; d *= 2) top = fmaxf(top, __shfl_xor(top, d, kWave));
+      double sum = 0.;
+      for (unsigned int c = lane; c < a.chunks; c += kWave)
+        sum += (double)sums[c].y * exp((double)sums[c].x - (double)top);
+#pragma unroll
+      for (int d = 1; d < kWave; d *= 2) sum += __shfl_xor(sum, d, kWave);
+      lse = log(sum) + (double)top;
+    }
+    if (lane == 0) {
+      s_lse[b] = lse;
+      s_score[b] = score;
+      s_state[b] = ended ? 1 : open ? 0 : 2;
+    }
+    unsigned long long keys[kItems];
+    const float* maxima = a.maxima + (unsigned long long)row * a.segments;
+#pragma unroll
+    for (int t = 0; t < kItems; ++t) {
+      const unsigned int item = t * kWave + lane;
+      keys[t] = 0;
+      if (item >= items) continue;
+      keys[t] = nothing;
+      if (open) {
+        float m = -INFINITY;
+        for (unsigned int s = item * group; s < min(a.segments, (item + 1) * group); ++s)
+          m = fmaxf(m, maxima[s]);
+        if (m != -INFINITY) keys[t] = key_of(((double)m - lse) + score);
+      } else if (ended && a.end_token / (kSegment * group) == item) {
+        keys[t] = key_of(score);
+      }
+    }
+    best_of(keys, most, 0, [&](unsigned long long key, unsigned int number, unsigned int n) {
+      if (lane == 0) {
+        s_key[b * most + n] = key;
+        s_id[b * most + n] = b * items + number;
+      }
+    });
+  }
+  __syncthreads();
+  // the best `most` of the beams' best segments
+  for (unsigned int i = tid; i < a.beams * most; i += kPickThreads) {
+    const unsigned long long key = s_key[i];
+    if (key == 0) continue;
+    const unsigned int id = s_id[i];
+    unsigned int rank = 0;
+    for (unsigned int j = 0; j < a.beams * most; ++j)
+      rank += s_key[j] > key || (s_key[j] == key && s_id[j] < id) ? 1u : 0u;
+    if (rank < most) s_chosen[rank] = id;
+    if (rank == most - 1) s_least = key;
+  }
+  __syncthreads();
+  const unsigned long long least = s_least;
+  for (unsigned int c = wave; c < most; c += kWaves) {
+    const unsigned int id = s_chosen[c];
+    if (id == ~0u) continue;
+    const unsigned int b = id / items, first = (id - b * items) * group * kSegment;
+    const double lse = s_lse[b], score = s_score[b];
+    const unsigned int state = s_state[b];
+    const unsigned char* src = row_of<T>(a, row0 + b);
+    unsigned long long keys[kItems];
+#pragma unroll
+    for (int t = 0; t < kItems; ++t) {
+      const unsigned int in = t * kWave + lane, token = first + in;
+      keys[t] = 0;
+      if (in >= group * kSegment || token >= a.vocab) continue;
+      keys[t] = nothing;
+      if (state == 0) {
+        const float x = T::one(src, token);
+        if (x != -INFINITY) keys[t] = key_of(((double)x - lse) + score);
+      } else if (state == 1 && token == a.end_token) {
+        keys[t] = key_of(score);
+      }
+    }
+    best_of(keys, most, least, [&](unsigned long long key, unsigned int number, unsigned int) {
+      if (lane == 0) {
+        const unsigned int at = atomicAdd(&s_count, 1u);
+        s_key[at] = key;
+        s_id[at] = b * a.vocab + first + number;
+      }
+    });
+  }
+  __syncthreads();
+  const unsigned int count = s_count;
+  for (unsigned int i = tid; i < count; i += kPickThreads) {
+    const unsigned long long key = s_key[i];
+    const unsigned int id = s_id[i];
+    unsigned int rank = 0;
+    for (unsigned int j = 0; j < count; ++j)
+      rank += s_key[j] > key || (s_key[j] == key && s_id[j] < id) ? 1u : 0u;
+    if (rank >= most) continue;
+    const unsigned long long to = (unsigned long long)request * most + rank;
+    const unsigned int b = id / a.vocab;
+    a.out_scores[to] = (float)value_of(key);
+    a.out_parents[to] = (int)b;
+    a.out_tokens[to] = id - b * a.vocab;
+  }
+}
+
+// ---------------------------------------------------------------------------
+
+constexpr int kOrderThreads = 256;  // columns of a workgroup
+constexpr int kMostLayers = 64;     // of a launch
+
+struct OrderArgs {
+  const int* tables;               // [requests * beams][table_stride]
+  int* out;                        // [requests * beams][out_stride]; may be tables
+  const int* parents;              // [requests][beams]
+  const int* contexts;             // [requests * beams]
+  int* copied_from;                // [requests * beams]
+  int* free_blocks;
+  const int* free_start;
+  int* free_next;
+  int* lacking;
+  int* unlisted;
+  int2* counts;                    // [requests][chunks]: (released, lacking) of a workgroup's columns
+  int* released;                   // [requests][chunks][beams * kOrderThreads]
+  unsigned long long table_stride, out_stride;
+  unsigned int requests, beams, width, chunks, block_tokens, free_count;
+};
+
+__global__ __launch_bounds__(kOrderThreads) void order_tables(OrderArgs a) {
+  extern __shared__ int s_entry[];  // [beams][kOrderThreads]: a thread's column
+  __shared__ int s_parent[kMostBeams];
+  __shared__ unsigned int s_wave[kOrderThreads / kWave];
+  const unsigned int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const unsigned int request = blockIdx.y, beams = a.beams, row0 = request * beams;
+  const unsigned int column = blockIdx.x * kOrderThreads + tid;
+  if (tid < beams) s_parent[tid] = a.parents[row0 + tid];
+  __syncthreads();
+  unsigned long long with_child = 0;
+  unsigned int orphans = 0;
+  for (unsigned int j = 0; j < beams; ++j) {
+    const unsigned int p = (unsigned int)s_parent[j];
+    if (p < beams)
+      with_child |= 1ull << p;
+    else
+      ++orphans;
+  }
+  const unsigned int context = (unsigned int)max(a.contexts[row0], 0);
+  const unsigned int full = context / a.block_tokens;
+  const bool partly = context != full * a.block_tokens;
+  const bool in = column < a.width;
+  unsigned long long released = 0;  // the beams whose entry of this column is
+  unsigned int lacking = 0;
+  int* const own = s_entry + tid;
+  if (in)
+    for (unsigned int b = 0; b < beams; ++b)
+      own[b * kOrderThreads] = a.tables[(row0 + b) * a.table_stride + column];
+  if (in && (column < full || (partly && column == full))) {
+    const bool tail = column == full;
+    // entries that beams without children leave: those of no other beam that has one, once each
+    unsigned long long left = 0;
+    for (unsigned int b = 0; b < beams; ++b) {
+      if ((with_child >> b & 1) != 0 || own[b * kOrderThreads] < 0) continue;
+      bool again = false;
+      for (unsigned int c = 0; c < beams; ++c)
+        again |= own[c * kOrderThreads] == own[b * kOrderThreads] && (c < b || (with_child >> c & 1) != 0);
+      if (!again) left |= 1ull << b;
+    }
+    for (unsigned int j = 0; j < beams; ++j) {
+      const unsigned int p = (unsigned int)s_parent[j];
+      int id = p < beams ? own[p * kOrderThreads] : -1, from = -1;
+      if (tail && id >= 0) {
+        bool taken = false;
+        for (unsigned int i = 0; i < j; ++i) {
+          const unsigned int q = (unsigned int)s_parent[i];
+          taken |= q < beams && own[q * kOrderThreads] == id;
+        }
+        if (taken) {
+          from = id;
+          id = -1;
+          if (left != 0) {
+            const int b = __ffsll((long long)left) - 1;
+            left &= left - 1;
+            id = own[b * kOrderThreads];
+          }
+        }
+      }
+      if (tail && p < beams && id < 0) ++lacking;
+      if (tail) a.copied_from[row0 + j] = id >= 0 ? from : -1;
+      a.out[(row0 + j) * a.out_stride + column] = id;
+    }
+    released = left;
+  } else if (in) {
+    for (unsigned int b = 0; b < beams; ++b)
+      a.out[(row0 + b) * a.out_stride + column] = own[b * kOrderThreads];
+  }
+  // no block to be copied: whole blocks only, or a table that ends before the last one
+  if (blockIdx.x == 0 && tid < beams && (!partly || full >= a.width)) a.copied_from[row0 + tid] = -1;
+  if (column == 0) lacking += orphans;
+
+  // this workgroup's released blocks in the order of columns, then beams
+  const unsigned int count = (unsigned int)__popcll(released);
+  unsigned int scan = count;
+#pragma unroll
+  for (int d = 1; d < kWave; d *= 2) {
+    const unsigned int o = (unsigned int)__shfl_up((int)scan, d, kWave);
+    if (lane >= (unsigned int)d) scan += o;
+  }
+  __shared__ unsigned int s_lacking;
+  if (tid == 0) s_lacking = 0;
+  if (lane == 63) s_wave[wave] = scan;
+  __syncthreads();
+  if (lacking != 0) atomicAdd(&s_lacking, lacking);
+  unsigned int at = scan - count, all = 0;
+#pragma unroll
+  for (unsigned int w = 0; w < kOrderThreads / kWave; ++w) {
+    if (w < wave) at += s_wave[w];
+    all += s_wave[w];
+  }
+  const unsigned int group = request * a.chunks + blockIdx.x;
+  int* dst = a.released + (unsigned long long)group * (beams * kOrderThreads);
+  for (; released != 0; released &= released - 1)
+    dst[at++] = own[(__ffsll((long long)released) - 1) * kOrderThreads];
+  __syncthreads();
+  if (tid == 0) a.counts[group] = make_int2((int)all, (int)s_lacking);
+}
+
+struct CopyArgs {
+  OrderArgs o;
+  unsigned long long block_bytes, row_bytes;  // of a plane's block, of a token
+  unsigned int blocks, layers;
+  bool list;  // this launch's last workgroup writes the free list
+  unsigned char* layer[kMostLayers];
+};
+
+// The released blocks of all workgroups of order_tables, in order, below the list's first free entry.
+__device__ __forceinline__ void list_released(const OrderArgs& a) {
+  __shared__ unsigned long long s_sum[2][kOrderThreads];
+  const unsigned int tid = threadIdx.x;
+  const unsigned int groups = a.requests * a.chunks;
+  const unsigned int share = (groups + kOrderThreads - 1) / kOrderThreads;
+  const unsigned int g0 = min(groups, tid * share), g1 = min(groups, g0 + share);
+  unsigned long long own = 0, lacking = 0;
+  for (unsigned int g = g0; g < g1; ++g) {
+    own += (unsigned int)a.counts[g].x;
+    lacking += (unsigned int)a.counts[g].y;
+  }
+  s_sum[0][tid] = own;
+  s_sum[1][tid] = lacking;
+  __syncthreads();
+  unsigned long long before = 0, all = 0, all_lacking = 0;
+  for (unsigned int t = 0; t < kOrderThreads; ++t) {
+    if (t < tid) before += s_sum[0][t];
+    all += s_sum[0][t];
+    all_lacking += s_sum[1][t];
+  }
+  const long long start = min(max(a.free_start[0], 0), (int)a.free_count);
+  long long at = start - (long long)(all - before);
+  for (unsigned int g = g0; g < g1; ++g) {
+    const unsigned int count = (unsigned int)a.counts[g].x;
+    const int* src = a.released + (unsigned long long)g * (a.beams * kOrderThreads);
+    for (unsigned int i = 0; i < count; ++i, ++at)
+      if (at >= 0) a.free_blocks[at] = src[i];
+  }
+  if (tid == 0) {
+    a.free_next[0] = (int)max(start - (long long)all, 0ll);
+    a.unlisted[0] = (int)max((long long)all - start, 0ll);
+    a.lacking[0] = (int)min(all_lacking, 0x7FFFFFFFull);
+  }
+}
+
+// A workgroup copies the tokens of one row's last block, one plane of one layer.
+template <typename U>
+__global__ __launch_bounds__(kOrderThreads) void copy_tails(CopyArgs a) {
+  if (a.list && blockIdx.x + 1 == gridDim.x) {
+    list_released(a.o);
+    return;
+  }
+  const unsigned int planes = 2 * a.layers;
+  const unsigned int row = blockIdx.x / planes, plane = blockIdx.x - row * planes;
+  const int from = a.o.copied_from[row];
+  if ((unsigned int)from >= a.blocks) return;
+  const unsigned int context = (unsigned int)max(a.o.contexts[row / a.o.beams * a.o.beams], 0);
+  const unsigned int column = context / a.o.block_tokens, tokens = context - column * a.o.block_tokens;
+  const int to = a.o.out[row * a.o.out_stride + column];
+  if ((unsigned int)to >= a.blocks) return;
+  unsigned char* base = a.layer[plane / 2] + (plane % 2) * (a.blocks * a.block_bytes);
+  const U* src = reinterpret_cast<const U*>(base + (unsigned int)from * a.block_bytes);
+  U* dst = reinterpret_cast<U*>(base + (unsigned int)to * a.block_bytes);
+  const unsigned long long units = tokens * a.row_bytes / sizeof(U);
+  for (unsigned long long i = threadIdx.x; i < units; i += kOrderThreads) dst[i] = src[i];
+}
+
+}  // namespace
+}  // namespace unchainkv
+
+using namespace unchainkv;
+
+namespace {
+
+// Chunks of a row and their rounds: as many rounds as leave the chip enough workgroups.
+void scan_shape(unsigned long long rows, SelectArgs& a) {
+  const unsigned int all = (a.vocab + kRound - 1) / kRound;
+  a.rounds = 1;
+  while (a.rounds < 8 && rows * ((all + 2 * a.rounds - 1) / (2 * a.rounds)) >= 2048) a.rounds *= 2;
+  a.chunks = (all + a.rounds - 1) / a.rounds;
+  a.segments = (a.vocab + kSegment - 1) / kSegment;
+}
+
+bool select_ok(unsigned long long requests, unsigned long long beams, unsigned long long vocab,
+               unsigned long long candidates) {
+  return requests != 0 && beams != 0 && beams <= kMostBeams && vocab != 0 && vocab <= kMostVocab &&
+         candidates != 0 && candidates <= kMostCandidates && candidates <= beams * vocab &&
+         requests * beams <= 65535;
+}
+
+unsigned long long maxima_bytes(unsigned long long rows, const SelectArgs& a) {
+  return (4 * rows * a.segments + 15) / 16 * 16;
+}
+
+unsigned int chunks_of(unsigned long long width) {
+  return (unsigned int)((width + kOrderThreads - 1) / kOrderThreads);
+}
+bool order_ok(unsigned long long requests, unsigned long long beams, unsigned long long width) {
+  return requests != 0 && requests <= 65535 && beams != 0 && beams <= kMostBeams && width != 0 &&
+         width <= 1u << 24;
+}
+
+}  // namespace
+
+extern "C" unsigned long long kvq_splitzip_beam_select_workspace_bytes(unsigned long long requests,
+                                                                       unsigned long long beams,
+                                                                       unsigned long long vocab) {
+  if (!select_ok(requests, beams, vocab, 1)) return 0;
+  SelectArgs a{};
+  a.vocab = (unsigned int)vocab;
+  scan_shape(requests * beams, a);
+  return maxima_bytes(requests * beams, a) + 8 * requests * beams * a.chunks;
+}
+
+extern "C" long long kvq_splitzip_beam_select(
+    unsigned long long logits_ptr, unsigned long long dtype, unsigned long long request_stride,
+    unsigned long long beam_stride, unsigned long long scores_ptr, unsigned long long ended_ptr,
+    unsigned long long requests, unsigned long long beams, unsigned long long vocab,
+    unsigned long long candidates, unsigned long long end_token, unsigned long long out_scores_ptr,
+    unsigned long long out_parents_ptr, unsigned long long out_tokens_ptr,
+    unsigned long long workspace_ptr, unsigned long long workspace_bytes,
+    unsigned long long stream_ptr) {
+  if (!select_ok(requests, beams, vocab, candidates) || dtype > 2 || logits_ptr == 0 ||
+      logits_ptr % (dtype == 2 ? 4 : 2) != 0 || scores_ptr == 0 || (ended_ptr != 0 && end_token >= vocab) ||
+      out_scores_ptr == 0 || out_parents_ptr == 0 || out_tokens_ptr == 0 || workspace_ptr == 0 ||
+      workspace_ptr % 16 != 0)
+    return 0;
+  SelectArgs a{};
+  a.vocab = (unsigned int)vocab;
+  const unsigned long long rows = requests * beams;
+  scan_shape(rows, a);
+  const unsigned long long need = maxima_bytes(rows, a) + 8 * rows * a.chunks;
+  if (workspace_bytes < need) return 0;
+  const unsigned long long picked = requests * candidates;
+  const unsigned long long in[][2] = {
+      {logits_ptr, ((requests - 1) * request_stride + (beams - 1) * beam_stride + vocab) * (dtype == 2 ? 4 : 2)},
+      {scores_ptr, 4 * rows}, {ended_ptr, ended_ptr ? rows : 0}};
+  const unsigned long long out[][2] = {{out_scores_ptr, 4 * picked}, {out_parents_ptr, 4 * picked},
+                                       {out_tokens_ptr, 8 * picked}, {workspace_ptr, need}};
+  for (const auto& o : out) {
+    for (const auto& i : in)
+      if (overlap(o[0], o[1], i[0], i[1])) return 0;
+    for (const auto& p : out)
+      if (&o != &p && overlap(o[0], o[1], p[0], p[1])) return 0;
+  }
+  a.logits = reinterpret_cast<const unsigned char*>(logits_ptr);
+  a.scores = reinterpret_cast<const float*>(scores_ptr);
+  a.ended = reinterpret_cast<const unsigned char*>(ended_ptr);
+  a.maxima = reinterpret_cast<float*>(workspace_ptr);
+  a.sums = reinterpret_cast<float2*>(workspace_ptr + maxima_bytes(rows, a));
+  a.out_scores = reinterpret_cast<float*>(out_scores_ptr);
+  a.out_parents = reinterpret_cast<int*>(out_parents_ptr);
+  a.out_tokens = reinterpret_cast<long long*>(out_tokens_ptr);
+  a.request_stride = request_stride;
+  a.beam_stride = beam_stride;
+  a.requests = (unsigned int)requests;
+  a.beams = (unsigned int)beams;
+  a.candidates = (unsigned int)candidates;
+  a.end_token = (unsigned int)end_token;
+  hipStream_t stream = reinterpret_cast<hipStream_t>(stream_ptr);
+  const dim3 grid(a.chunks, (unsigned int)rows);
+  if (dtype == 0)
+    hipLaunchKernelGGL(beam_scan<Bf16>, grid, dim3(kScanThreads), 0, stream, a);
+  else if (dtype == 1)
+    hipLaunchKernelGGL(beam_scan<Fp16>, grid, dim3(kScanThreads), 0, stream, a);
+  else
+    hipLaunchKernelGGL(beam_scan<Fp32>, grid, dim3(kScanThreads), 0, stream, a);
+  hipError_t st = hipGetLastError();
+  if (st != hipSuccess) return fail("beam_scan", st);
+  const dim3 picks(a.requests);
+  if (dtype == 0)
+    hipLaunchKernelGGL(beam_pick<Bf16>, picks, dim3(kPickThreads), 0, stream, a);
+  else if (dtype == 1)
+    hipLaunchKernelGGL(beam_pick<Fp16>, picks, dim3(kPickThreads), 0, stream, a);
+  else
+    hipLaunchKernelGGL(beam_pick<Fp32>, picks, dim3(kPickThreads), 0, stream, a);
+  st = hipGetLastError();
+  if (st != hipSuccess) return fail("beam_pick", st);
+  return (long long)picked;
+}
+
+extern "C" unsigned long long kvq_splitzip_reorder_beams_workspace_bytes(unsigned long long requests,
+                                                                         unsigned long long beams,
+                                                                         unsigned long long width) {
+  if (!order_ok(requests, beams, width)) return 0;
+  return requests * chunks_of(width) * (8 + 4 * beams * kOrderThreads);
+}
+
+extern "C" long long kvq_splitzip_reorder_beams_paged(
+    const unsigned long long* layers, unsigned long long layer_count, unsigned long long blocks,
+    unsigned long long block_tokens, unsigned long long row_bytes, unsigned long long tables_ptr,
+    unsigned long long table_stride, unsigned long long table_width, unsigned long long out_ptr,
+    unsigned long long out_stride, unsigned long long parents_ptr, unsigned long long context_tokens_ptr,
+    unsigned long long requests, unsigned long long beams, unsigned long long free_blocks_ptr,
+    unsigned long long free_count, unsigned long long free_start_ptr, unsigned long long copied_from_ptr,
+    unsigned long long free_next_ptr, unsigned long long lacking_ptr, unsigned long long unlisted_ptr,
+    unsigned long long workspace_ptr, unsigned long long workspace_bytes, unsigned long long stream_ptr) {
+  constexpr unsigned long long kMost = 0x7FFFFFFFull;
+  if (!order_ok(requests, beams, table_width) || (layer_count != 0 && layers == nullptr) ||
+      layer_count > kMost || blocks == 0 || blocks > kMost || block_tokens == 0 || block_tokens > kMost ||
+      row_bytes == 0 || row_bytes % 2 != 0 || row_bytes > kMost || blocks * block_tokens > kMost ||
+      tables_ptr == 0 || table_stride < table_width || out_ptr == 0 || out_stride < table_width ||
+      parents_ptr == 0 || context_tokens_ptr == 0 || (free_blocks_ptr == 0 && free_count != 0) ||
+      free_count > kMost || free_start_ptr == 0 || copied_from_ptr == 0 || free_next_ptr == 0 ||
+      lacking_ptr == 0 || unlisted_ptr == 0 || workspace_ptr == 0 || workspace_ptr % 16 != 0)
+    return 0;
+  const unsigned long long need = kvq_splitzip_reorder_beams_workspace_bytes(requests, beams, table_width);
+  if (workspace_bytes < need) return 0;
+  const unsigned long long rows = requests * beams;
+  const unsigned long long table_bytes = 4 * ((rows - 1) * table_stride + table_width);
+  const unsigned long long out_bytes = 4 * ((rows - 1) * out_stride + table_width);
+  const bool in_place = out_ptr == tables_ptr && out_stride == table_stride;
+  const unsigned long long in[][2] = {{parents_ptr, 4 * rows}, {context_tokens_ptr, 4 * rows},
+                                      {free_start_ptr, 4}, {tables_ptr, in_place ? 0 : table_bytes}};
+  const unsigned long long out[][2] = {{out_ptr, out_bytes}, {free_blocks_ptr, 4 * free_count},
+                                       {copied_from_ptr, 4 * rows}, {free_next_ptr, 4},
+                                       {lacking_ptr, 4}, {unlisted_ptr, 4}, {workspace_ptr, need}};
+  const unsigned long long layer_bytes = 2 * blocks * block_tokens * row_bytes;
+  for (const auto& o : out) {
+    for (const auto& i : in)
+      if (overlap(o[0], o[1], i[0], i[1])) return 0;
+    for (const auto& p : out)
+      if (&o != &p && overlap(o[0], o[1], p[0], p[1])) return 0;
+    for (unsigned long long l = 0; l < layer_count; ++l)
+      if (overlap(o[0], o[1], layers[l], layer_bytes)) return 0;
+  }
+  bool wide = row_bytes % 16 == 0;
+  for (unsigned long long l = 0; l < layer_count; ++l) {
+    if (layers[l] == 0 || layers[l] % 2 != 0) return 0;
+    wide = wide && layers[l] % 16 == 0;
+    for (const auto& i : in)
+      if (overlap(layers[l], layer_bytes, i[0], i[1])) return 0;
+    if (overlap(layers[l], layer_bytes, tables_ptr, table_bytes)) return 0;
+  }
+  if (rows * 2 * std::min<unsigned long long>(layer_count, kMostLayers) > 0xFFFFFF) return 0;
+  CopyArgs c{};
+  OrderArgs& a = c.o;
+  a.tables = reinterpret_cast<const int*>(tables_ptr);
+  a.out = reinterpret_cast<int*>(out_ptr);
+  a.parents = reinterpret_cast<const int*>(parents_ptr);
+  a.contexts = reinterpret_cast<const int*>(context_tokens_ptr);
+  a.copied_from = reinterpret_cast<int*>(copied_from_ptr);
+  a.free_blocks = reinterpret_cast<int*>(free_blocks_ptr);
+  a.free_start = reinterpret_cast<const int*>(free_start_ptr);
+  a.free_next = reinterpret_cast<int*>(free_next_ptr);
+  a.lacking = reinterpret_cast<int*>(lacking_ptr);
+  a.unlisted = reinterpret_cast<int*>(unlisted_ptr);
+  a.table_stride = table_stride;
+  a.out_stride = out_stride;
+  a.requests = (unsigned int)requests;
+  a.beams = (unsigned int)beams;
+  a.width = (unsigned int)table_width;
+  a.chunks = chunks_of(table_width);
+  a.block_tokens = (unsigned int)block_tokens;
+  a.free_count = (unsigned int)free_count;
+  a.counts = reinterpret_cast<int2*>(workspace_ptr);
+  a.released = reinterpret_cast<int*>(workspace_ptr + 8 * requests * a.chunks);
+  hipStream_t stream = reinterpret_cast<hipStream_t>(stream_ptr);
+  hipLaunchKernelGGL(order_tables, dim3(a.chunks, a.requests), dim3(kOrderThreads),
+                     beams * kOrderThreads * sizeof(int), stream, a);
+  hipError_t st = hipGetLastError();
+  if (st != hipSuccess) return fail("order_tables", st);
+  c.block_bytes = block_tokens * row_bytes;
+  c.row_bytes = row_bytes;
+  c.blocks = (unsigned int)blocks;
+  for (unsigned long long l = 0;;) {
+    c.layers = (unsigned int)std::min<unsigned long long>(layer_count - l, kMostLayers);
+    for (unsigned int i = 0; i < c.layers; ++i) c.layer[i] = reinterpret_cast<unsigned char*>(layers[l + i]);
+    l += c.layers;
+    c.list = l == layer_count;
+    const unsigned long long groups = rows * 2 * c.layers + (c.list ? 1 : 0);
+    if (wide)
+      hipLaunchKernelGGL(copy_tails<u32x4>, dim3((unsigned int)groups), dim3(kOrderThreads), 0, stream, c);
+    else
+      hipLaunchKernelGGL(copy_tails<uint16_t>, dim3((unsigned int)groups), dim3(kOrderThreads), 0, stream, c);
+    st = hipGetLastError();
+    if (st != hipSuccess) return fail("copy_tails", st);
+    if (c.list) break;
+  }
+  return (long long)rows;
+}

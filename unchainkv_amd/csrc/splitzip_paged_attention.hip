@@ -151,7 +151,8 @@ struct AttendArgs {
   const unsigned char* v;
   const int* starts;         // [requests + 1]
   const int* contexts;       // [requests]; null: a request's own rows (prompts)
-  const int* tables;         // [requests][table_stride]; null for prompts
+  const int* tables;         // [requests][table_stride]; null: packed rows
+  const int* sources;        // [requests], the first packed row of K and V; null: the request's own
   float* partial;            // of each slot
   struct Job* jobs;          // one for each slot
   unsigned long long q_row, q_head;  // bytes from token to token, from head to head
@@ -162,6 +163,9 @@ struct AttendArgs {
   unsigned int tokens, requests, q_heads, kv_heads, group;
   unsigned int few_target, tile_target;   // workgroups to split for, of the two paths
   unsigned int max_query;     // requests with more new tokens are left out
+  unsigned int max_source;    // and, of packed sources, those with more tokens
+  unsigned int kv_rows;       // rows of packed sources
+  unsigned int causal;        // 1: row i of n sees the context without its last n - i - 1 tokens; 0: all
   unsigned int slots;         // partial slots
   unsigned int items;         // of the tiles' grid, beside one that clears what slots they leave
   float scale_log2;
@@ -172,7 +176,7 @@ struct AttendArgs {
 // than the call allows.
 struct Request {
   unsigned int r, start, n, ctx;
-  bool bad;  // a context longer than the block table
+  bool bad;  // a context longer than the block table, or rows outside the source
 };
 
 __device__ __forceinline__ Request load_request(const AttendArgs& a, unsigned int r) {
@@ -185,12 +189,22 @@ __device__ __forceinline__ Request load_request(const AttendArgs& a, unsigned in
   q.n = (unsigned int)(s1 - s0);
   q.ctx = q.n;
   if (a.contexts != nullptr) {
-    const unsigned long long most = (unsigned long long)a.table_width * a.block_tokens;
     const int c = a.contexts[r];
     q.ctx = c < 0 ? 0u : (unsigned int)c;
-    if (q.ctx > most) {
-      q.bad = true;
-      q.ctx = (unsigned int)most;
+    if (a.tables != nullptr) {
+      const unsigned long long most = (unsigned long long)a.table_width * a.block_tokens;
+      if (q.ctx > most) {
+        q.bad = true;
+        q.ctx = (unsigned int)most;
+      }
+    } else if (q.ctx > a.max_source) {
+      q.n = q.ctx = 0;
+    } else if (q.ctx != 0) {
+      const int s = a.sources[r];
+      if (s < 0 || (unsigned int)s + q.ctx > a.kv_rows) {
+        q.bad = true;
+        q.ctx = 0;
+      }
     }
   }
   return q;
@@ -352,6 +366,19 @@ struct Work {
     return false;
   }
 };
+
+// The last token of a request that its first row sees (negative: none), and how many more each row
+// behind it does.
+__device__ __forceinline__ int first_seen(const AttendArgs& a, const Request& q) {
+  return (int)q.ctx - (int)(a.causal ? q.n : 1u);
+}
+
+// The first row of K and V of a request of packed rows.
+template <bool kPaged>
+__device__ __forceinline__ unsigned int kv_start(const AttendArgs& a, const Request& q) {
+  if constexpr (kPaged) return 0;
+  return a.sources == nullptr ? q.start : q.ctx == 0 ? 0u : (unsigned int)a.sources[q.r];
+}
 
 // Row of K and V that token t of a request has: its place in the layer through the block table
 // (bad: the table names no block of the layer there; block 0 is read instead), or its packed row.
@@ -540,8 +567,8 @@ __device__ __forceinline__ void tile_path(const AttendArgs& a, const Request& re
   const unsigned int rows = request.n * a.group;
   const unsigned int m0 = tile * kTileRows;
   // last visible token of a row (negative: none)
-  const int shift = (int)request.ctx - (int)request.n;
-  const int last_of_tile = shift + (int)((min(rows, m0 + kTileRows) - 1) / a.group);
+  const int shift = first_seen(a, request);
+  const int last_of_tile = shift + (int)(a.causal * ((min(rows, m0 + kTileRows) - 1) / a.group));
   const unsigned int seen = last_of_tile < 0 ? 0u : (unsigned int)last_of_tile + 1;
   const unsigned int splits = most == 1 ? 1u : max(1u, steps_of(seen, split_tokens));  // of this tile
   if (most > 1)
@@ -556,8 +583,10 @@ __device__ __forceinline__ void tile_path(const AttendArgs& a, const Request& re
   const bool valid = m < rows;
   const unsigned int token = valid ? m / a.group : 0u;
   const unsigned int q_head = head * a.group + (valid ? m - token * a.group : 0u);
-  const int limit = valid ? shift + (int)token : -1;
-  const int first_limit = shift + (int)(mw / a.group);  // the last visible token of the wave's first row
+  const int limit = valid ? shift + (int)(a.causal * token) : -1;
+  // the last visible token of the wave's first row
+  const int first_limit = shift + (int)(a.causal * (mw / a.group));
+  const unsigned int source = kv_start<kPaged>(a, request);
 
   const int* table = kPaged ? a.tables + request.r * a.table_stride : nullptr;
   const unsigned char* kb = a.k + head * a.k_head;
@@ -608,7 +637,7 @@ __device__ __forceinline__ void tile_path(const AttendArgs& a, const Request& re
   auto find_rows = [&](unsigned int base) {
 #pragma unroll
     for (int i = 0; i < kIds; ++i) {
-      next_row[i] = kv_row<kPaged>(a, request.start, token_of(base, i), ids[i], bad);
+      next_row[i] = kv_row<kPaged>(a, source, token_of(base, i), ids[i], bad);
       if (kRuns) next_row[i] = uniform(next_row[i]);
     }
   };
@@ -950,9 +979,9 @@ __device__ __forceinline__ void tile_path(const AttendArgs& a, const Request& re
     const unsigned int at = uniform((unsigned int)__ffs((int)redo) - 1);
     redo &= redo - 1;
     const unsigned int row_m = mw + at, tok = row_m / a.group, qh = head * a.group + row_m % a.group;
-    const unsigned int own = (unsigned int)max(shift + (int)tok + 1, 0);  // tokens it sees
+    const unsigned int own = (unsigned int)max(shift + (int)(a.causal * tok) + 1, 0);  // tokens it sees
     float rm, rl, acc[D / 64];
-    slow_row<E, D, kPaged>(a, table, request.start,
+    slow_row<E, D, kPaged>(a, table, source,
                            a.q + (unsigned long long)(request.start + tok) * a.q_row +
                                (unsigned long long)qh * a.q_head,
                            head, t_begin, min(t_end, own), rm, rl, acc);
@@ -979,7 +1008,7 @@ __device__ __forceinline__ void tile_path(const AttendArgs& a, const Request& re
 // no load takes apart 16 rows: 32 requests of 8192 tokens 200 -> 196.6 us, 16 of 1024 19.2 -> 17.6, 64
 // single tokens of 500 .. 16000 and four times 8 354 -> 332. (64 dims: lane l has token l % 16, 16
 // bytes at 16 (l / 16) of every 64, each counting.)
-template <typename E, int D, int kN, int kRows>
+template <typename E, int D, int kN, int kRows, bool kPaged>
 __device__ __forceinline__ void few_path(const AttendArgs& a, const Request& request, unsigned int split,
                                          unsigned int splits, unsigned int split_tokens, bool whole,
                                          unsigned int slot, unsigned int head, unsigned char* __restrict__ s0,
@@ -997,16 +1026,17 @@ __device__ __forceinline__ void few_path(const AttendArgs& a, const Request& req
   const unsigned int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
   const unsigned int col = lane % 16, grp = lane / 16;
   store_job(a, slot, head,
-            Job{request.start, 0, (int)request.ctx - (int)request.n,
+            Job{request.start, 0, first_seen(a, request),
                 (unsigned short)(request.n * a.group),
                 (unsigned short)(split == 0 && splits > 1 && whole ? splits : 0u)});
   slot = slot * a.kv_heads + head;
   const unsigned int rows = request.n * a.group;
   const unsigned int t_begin = split * split_tokens;
   const unsigned int t_end = splits == 1 ? request.ctx : min(request.ctx, t_begin + split_tokens);
-  const int shift = (int)request.ctx - (int)request.n;
+  const int shift = first_seen(a, request);
+  const unsigned int source = kv_start<kPaged>(a, request);
 
-  const int* table = a.tables + request.r * a.table_stride;
+  const int* table = kPaged ? a.tables + request.r * a.table_stride : nullptr;
   const unsigned char* kb = a.k + head * a.k_head;
   const unsigned char* vb = a.v + head * a.v_head;
   unsigned int bad = request.bad ? 1u : 0u;
@@ -1014,7 +1044,7 @@ __device__ __forceinline__ void few_path(const AttendArgs& a, const Request& req
   const bool valid = col < rows;
   const unsigned int token = valid ? col / a.group : 0u;
   const unsigned int q_head = head * a.group + (valid ? col - token * a.group : 0u);
-  const int limit = valid ? shift + (int)token : -1;
+  const int limit = valid ? shift + (int)(a.causal * token) : -1;
   x8 q[kSlabs];
   const unsigned char* q_row = a.q + (unsigned long long)(request.start + token) * a.q_row +
                                (unsigned long long)q_head * a.q_head;
@@ -1031,7 +1061,7 @@ __device__ __forceinline__ void few_path(const AttendArgs& a, const Request& req
   // lane l looks up token l % 32 of a step
   auto token_of = [&](unsigned int base) { return min(base + lane % 32, t_end - 1); };
   auto issue = [&](unsigned int base, int id, Keys& k, unsigned char* stage) {
-    const unsigned int row = kv_row<true>(a, 0u, token_of(base), id, bad);
+    const unsigned int row = kv_row<kPaged>(a, source, token_of(base), id, bad);
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       if constexpr (kWhole) {
@@ -1125,20 +1155,20 @@ __device__ __forceinline__ void few_path(const AttendArgs& a, const Request& req
   unsigned int base = t_begin + wave * kFewStep;
   if (base < t_end) {
     Keys k0, k1;
-    issue(base, block_id<true>(a, table, token_of(base)), k0, stage0);
-    int id = block_id<true>(a, table, token_of(base + kRound));
+    issue(base, block_id<kPaged>(a, table, token_of(base)), k0, stage0);
+    int id = block_id<kPaged>(a, table, token_of(base + kRound));
     for (;;) {
       // the next step's loads go out (past the end: the last token again), then this step's
       // are waited for
       issue(base + kRound, id, k1, stage1);
-      id = block_id<true>(a, table, token_of(base + 2 * kRound));
-      wait_loads<2 * kSlabs + kLoads + 1>();
+      id = block_id<kPaged>(a, table, token_of(base + 2 * kRound));
+      wait_loads<2 * kSlabs + kLoads + (kPaged ? 1 : 0)>();
       step(base, k0, stage0);
       base += kRound;
       if (base >= t_end) break;
       issue(base + kRound, id, k0, stage0);
-      id = block_id<true>(a, table, token_of(base + 2 * kRound));
-      wait_loads<2 * kSlabs + kLoads + 1>();
+      id = block_id<kPaged>(a, table, token_of(base + 2 * kRound));
+      wait_loads<2 * kSlabs + kLoads + (kPaged ? 1 : 0)>();
       step(base, k1, stage1);
       base += kRound;
       if (base >= t_end) break;
@@ -1200,7 +1230,7 @@ __device__ __forceinline__ void few_path(const AttendArgs& a, const Request& req
       for (int i = 0; i < kVals; i += 4)
         *reinterpret_cast<f32x4*>(dst + i) = f32x4{acc[i], acc[i + 1], acc[i + 2], acc[i + 3]};
     } else {
-      const bool none = shift + (int)tok < 0 && !bad;
+      const bool none = shift + (int)(a.causal * tok) < 0 && !bad;
       const float inv = none ? 0.f : 1.f / l;
       uint32_t* dst = reinterpret_cast<uint32_t*>(a.out + out_row * kRowBytes + 2 * d0);
 #pragma unroll
@@ -1214,9 +1244,9 @@ __device__ __forceinline__ void few_path(const AttendArgs& a, const Request& req
   for (unsigned int i = 0; i < kWave / kShare; ++i) {
     if (((flags >> (kShare * i)) & 1) == 0) continue;
     const unsigned int mm = kWave / kShare * wave + i, t = mm / a.group, h = head * a.group + mm % a.group;
-    const unsigned int seen = (unsigned int)max(shift + (int)t + 1, 0);
+    const unsigned int seen = (unsigned int)max(shift + (int)(a.causal * t) + 1, 0);
     float rm, rl, ra[D / 64];
-    slow_row<E, D, true>(a, table, request.start,
+    slow_row<E, D, kPaged>(a, table, source,
                          a.q + (unsigned long long)(request.start + t) * a.q_row +
                              (unsigned long long)h * a.q_head,
                          head, t_begin, min(t_end, seen), rm, rl, ra);
@@ -1257,7 +1287,7 @@ __global__ __launch_bounds__(kWave * tile_waves(D), D == 128 ? 2 : 3) void atten
   if constexpr (kPaged) {
     if (work.few(request.n)) {
       if (!has_slot) slot = kNoSlot;
-      few_path<E, D, kN, kRows>(a, request, split, most, split_tokens, whole, slot, head, s0, s1, s2);
+      few_path<E, D, kN, kRows, kPaged>(a, request, split, most, split_tokens, whole, slot, head, s0, s1, s2);
       return;
     }
   }
@@ -1265,14 +1295,14 @@ __global__ __launch_bounds__(kWave * tile_waves(D), D == 128 ? 2 : 3) void atten
                                    s2);
 }
 
-template <typename E, int D>
+template <typename E, int D, bool kPaged>
 __global__ __launch_bounds__(kWave * kWaves, 2) void attention_few(AttendArgs a) {
   constexpr int kBuffer = kWaves * kFewStep * 2 * D;
   __shared__ __align__(1024) unsigned char s0[kBuffer];
   __shared__ __align__(1024) unsigned char s1[kBuffer];
   __shared__ __align__(16) unsigned char s2[kWaves * 16 * 2 * sizeof(float)];
   const unsigned int head = blockIdx.x % a.kv_heads, item = blockIdx.x / a.kv_heads;
-  const Work<false, kFewRows, true> work(a);
+  const Work<false, kFewRows, kPaged> work(a);
   Request request;
   unsigned int split, slot;
   bool has_slot;
@@ -1281,7 +1311,7 @@ __global__ __launch_bounds__(kWave * kWaves, 2) void attention_few(AttendArgs a)
     return;
   }
   const unsigned int splits = work.splits(request);
-  few_path<E, D, kWaves, kFewRows>(a, request, split, splits, work.split_tokens(request, splits), true,
+  few_path<E, D, kWaves, kFewRows, kPaged>(a, request, split, splits, work.split_tokens(request, splits), true,
                                    slot, head, s0, s1, s2);
 }
 
@@ -1389,7 +1419,7 @@ __global__ __launch_bounds__(kMergeThreads) void attention_merge(AttendArgs a) {
       const unsigned int m = job.first + row, tok = m / a.group;
       const unsigned long long out_row =
           (unsigned long long)(job.start + tok) * a.q_heads + head * a.group + (m - tok * a.group);
-      const bool none = job.shift + (int)tok < 0 && !bad;
+      const bool none = job.shift + (int)(a.causal * tok) < 0 && !bad;
       const float inv = bad ? NAN : none ? 0.f : 1.f / l;
       uint32_t* dst = reinterpret_cast<uint32_t*>(a.out + (out_row * D + dims) * 2);
 #pragma unroll
@@ -1528,8 +1558,8 @@ long long launch(const AttendArgs& a, const Plan& p, hipStream_t stream) {
     st = hipGetLastError();
     if (st != hipSuccess) return fail("attention_tiles", st);
     st = launch_merge<E, D, true>(a, stream);
-  } else if constexpr (kPaged) {
-    hipLaunchKernelGGL((attention_few<E, D>), grid, dim3(kWave * kWaves), 0, stream, a);
+  } else {
+    hipLaunchKernelGGL((attention_few<E, D, kPaged>), grid, dim3(kWave * kWaves), 0, stream, a);
     st = hipGetLastError();
     if (st != hipSuccess) return fail("attention_few", st);
     st = launch_merge<E, D, false>(a, stream);
@@ -1609,7 +1639,10 @@ extern "C" unsigned long long kvq_splitzip_prompt_attention_least_workspace_byte
                               false), head_dim);
 }
 
-extern "C" long long kvq_splitzip_chunk_attention_paged(
+namespace {
+
+// Over a paged layer: a step's own context (causal), or a source.
+long long attend_paged(
     unsigned long long q_ptr, unsigned long long q_row_bytes, unsigned long long q_head_bytes,
     unsigned long long tokens, unsigned long long q_heads, unsigned long long kv_heads,
     unsigned long long head_dim, unsigned long long dtype, unsigned long long kv_ptr,
@@ -1618,7 +1651,7 @@ extern "C" long long kvq_splitzip_chunk_attention_paged(
     unsigned long long query_starts_ptr, unsigned long long context_tokens_ptr,
     unsigned long long requests, unsigned long long max_query, unsigned long long out_ptr,
     unsigned long long lse_ptr, unsigned long long workspace_ptr,
-    unsigned long long workspace_bytes, float scale, unsigned long long stream_ptr) {
+    unsigned long long workspace_bytes, float scale, unsigned long long stream_ptr, bool causal) {
   if (!sizes_ok(tokens, requests, q_heads, kv_heads, head_dim, max_query) || dtype > 1 ||
       q_ptr == 0 || q_ptr % 16 != 0 || q_row_bytes % 16 != 0 || q_head_bytes % 16 != 0 ||
       kv_ptr == 0 || kv_ptr % 16 != 0 || blocks == 0 || block_tokens == 0 || blocks > kMostRows ||
@@ -1668,10 +1701,45 @@ extern "C" long long kvq_splitzip_chunk_attention_paged(
   a.few_target = (unsigned int)plan.few_target;
   a.tile_target = (unsigned int)plan.tile_target;
   a.max_query = (unsigned int)max_query;
+  a.causal = causal ? 1 : 0;
   a.slots = (unsigned int)plan.slots;
   a.items = (unsigned int)plan.items;
   a.scale_log2 = scale * kLog2E;
   return launch_typed<true>(a, plan, head_dim, dtype, reinterpret_cast<hipStream_t>(stream_ptr));
+}
+
+}  // namespace
+
+extern "C" long long kvq_splitzip_chunk_attention_paged(
+    unsigned long long q_ptr, unsigned long long q_row_bytes, unsigned long long q_head_bytes,
+    unsigned long long tokens, unsigned long long q_heads, unsigned long long kv_heads,
+    unsigned long long head_dim, unsigned long long dtype, unsigned long long kv_ptr,
+    unsigned long long blocks, unsigned long long block_tokens, unsigned long long tables_ptr,
+    unsigned long long table_stride, unsigned long long table_width,
+    unsigned long long query_starts_ptr, unsigned long long context_tokens_ptr,
+    unsigned long long requests, unsigned long long max_query, unsigned long long out_ptr,
+    unsigned long long lse_ptr, unsigned long long workspace_ptr,
+    unsigned long long workspace_bytes, float scale, unsigned long long stream_ptr) {
+  return attend_paged(q_ptr, q_row_bytes, q_head_bytes, tokens, q_heads, kv_heads, head_dim, dtype, kv_ptr,
+                      blocks, block_tokens, tables_ptr, table_stride, table_width, query_starts_ptr,
+                      context_tokens_ptr, requests, max_query, out_ptr, lse_ptr, workspace_ptr,
+                      workspace_bytes, scale, stream_ptr, true);
+}
+
+extern "C" long long kvq_splitzip_cross_attention_paged(
+    unsigned long long q_ptr, unsigned long long q_row_bytes, unsigned long long q_head_bytes,
+    unsigned long long tokens, unsigned long long q_heads, unsigned long long kv_heads,
+    unsigned long long head_dim, unsigned long long dtype, unsigned long long kv_ptr,
+    unsigned long long blocks, unsigned long long block_tokens, unsigned long long tables_ptr,
+    unsigned long long table_stride, unsigned long long table_width,
+    unsigned long long query_starts_ptr, unsigned long long context_tokens_ptr,
+    unsigned long long requests, unsigned long long max_query, unsigned long long out_ptr,
+    unsigned long long lse_ptr, unsigned long long workspace_ptr,
+    unsigned long long workspace_bytes, float scale, unsigned long long stream_ptr) {
+  return attend_paged(q_ptr, q_row_bytes, q_head_bytes, tokens, q_heads, kv_heads, head_dim, dtype, kv_ptr,
+                      blocks, block_tokens, tables_ptr, table_stride, table_width, query_starts_ptr,
+                      context_tokens_ptr, requests, max_query, out_ptr, lse_ptr, workspace_ptr,
+                      workspace_bytes, scale, stream_ptr, false);
 }
 
 extern "C" long long kvq_splitzip_prompt_attention(
@@ -1725,6 +1793,74 @@ extern "C" long long kvq_splitzip_prompt_attention(
   a.few_target = (unsigned int)plan.few_target;
   a.tile_target = (unsigned int)plan.tile_target;
   a.max_query = (unsigned int)max_query;
+  a.causal = 1;
+  a.slots = (unsigned int)plan.slots;
+  a.items = (unsigned int)plan.items;
+  a.scale_log2 = scale * kLog2E;
+  return launch_typed<false>(a, plan, head_dim, dtype, reinterpret_cast<hipStream_t>(stream_ptr));
+}
+
+extern "C" long long kvq_splitzip_cross_attention(
+    unsigned long long q_ptr, unsigned long long q_row_bytes, unsigned long long q_head_bytes,
+    unsigned long long k_ptr, unsigned long long k_row_bytes, unsigned long long k_head_bytes,
+    unsigned long long v_ptr, unsigned long long v_row_bytes, unsigned long long v_head_bytes,
+    unsigned long long source_rows, unsigned long long tokens, unsigned long long q_heads,
+    unsigned long long kv_heads, unsigned long long head_dim, unsigned long long dtype,
+    unsigned long long query_starts_ptr, unsigned long long source_starts_ptr,
+    unsigned long long source_tokens_ptr, unsigned long long requests, unsigned long long max_query,
+    unsigned long long max_source, unsigned long long out_ptr, unsigned long long lse_ptr,
+    unsigned long long workspace_ptr, unsigned long long workspace_bytes, float scale,
+    unsigned long long stream_ptr) {
+  if (!sizes_ok(tokens, requests, q_heads, kv_heads, head_dim, max_query) || dtype > 1 ||
+      q_ptr == 0 || k_ptr == 0 || v_ptr == 0 || source_rows == 0 || source_rows > kMostRows ||
+      max_source > source_rows ||
+      (q_ptr | q_row_bytes | q_head_bytes | k_ptr | k_row_bytes | k_head_bytes | v_ptr |
+       v_row_bytes | v_head_bytes) % 16 != 0 ||
+      k_row_bytes > kMostStride || v_row_bytes > kMostStride || query_starts_ptr == 0 ||
+      source_starts_ptr == 0 || source_tokens_ptr == 0 || out_ptr == 0 || out_ptr % 16 != 0 ||
+      !(scale > 0.f) || !std::isfinite(scale * kLog2E))
+    return 0;
+  // (as over a layer: sources' lengths do not follow from the rows of q)
+  const Plan plan = plan_of(tokens, requests, kv_heads, q_heads / kv_heads, head_dim, max_source, max_query, true);
+  const unsigned long long need = workspace_of(plan, head_dim);
+  if (need != 0 && (workspace_ptr == 0 || workspace_ptr % 16 != 0 || workspace_bytes < need)) return 0;
+  if (plan.groups > kMostGroups) return 0;
+  const unsigned long long out_bytes = tokens * q_heads * head_dim * 2;
+  if (!results_apart(
+          {{out_ptr, out_bytes}, {lse_ptr, lse_ptr ? 4 * tokens * q_heads : 0}, {workspace_ptr, need}},
+          {{q_ptr, extent(tokens, q_row_bytes, q_heads, q_head_bytes, 2 * head_dim)},
+           {k_ptr, extent(source_rows, k_row_bytes, kv_heads, k_head_bytes, 2 * head_dim)},
+           {v_ptr, extent(source_rows, v_row_bytes, kv_heads, v_head_bytes, 2 * head_dim)},
+           {query_starts_ptr, 4 * (requests + 1)}, {source_starts_ptr, 4 * requests},
+           {source_tokens_ptr, 4 * requests}}))
+    return 0;
+  AttendArgs a{};
+  a.q = reinterpret_cast<const unsigned char*>(q_ptr);
+  a.out = reinterpret_cast<unsigned char*>(out_ptr);
+  a.lse = reinterpret_cast<float*>(lse_ptr);
+  a.k = reinterpret_cast<const unsigned char*>(k_ptr);
+  a.v = reinterpret_cast<const unsigned char*>(v_ptr);
+  a.k_row = k_row_bytes;
+  a.k_head = k_head_bytes;
+  a.v_row = v_row_bytes;
+  a.v_head = v_head_bytes;
+  a.starts = reinterpret_cast<const int*>(query_starts_ptr);
+  a.contexts = reinterpret_cast<const int*>(source_tokens_ptr);
+  a.sources = reinterpret_cast<const int*>(source_starts_ptr);
+  a.partial = reinterpret_cast<float*>(workspace_ptr);
+  a.jobs = reinterpret_cast<Job*>(workspace_ptr + partial_bytes(plan, head_dim));
+  a.q_row = q_row_bytes;
+  a.q_head = q_head_bytes;
+  a.tokens = (unsigned int)tokens;
+  a.requests = (unsigned int)requests;
+  a.q_heads = (unsigned int)q_heads;
+  a.kv_heads = (unsigned int)kv_heads;
+  a.group = (unsigned int)(q_heads / kv_heads);
+  a.few_target = (unsigned int)plan.few_target;
+  a.tile_target = (unsigned int)plan.tile_target;
+  a.max_query = (unsigned int)max_query;
+  a.max_source = (unsigned int)max_source;
+  a.kv_rows = (unsigned int)source_rows;
   a.slots = (unsigned int)plan.slots;
   a.items = (unsigned int)plan.items;
   a.scale_log2 = scale * kLog2E;

@@ -241,6 +241,129 @@ __global__ __launch_bounds__(kStepThreads) void write_rows(WriteArgs a) {
   }
 }
 
+// Rotate and write: pairs (x, y) of a head's first `rotary` values become (x cos - y sin, y cos + x sin),
+// with the cosines and sines of the token's position from a table, in f32 and rounded once; K goes to its
+// slot with V, Q to a tensor of its own.
+struct RotateArgs {
+  const unsigned char *q, *k, *v;
+  unsigned char* out;          // [tokens][q_heads][dim]
+  unsigned char* layer;        // K plane; the V plane follows plane_bytes later
+  const float* table;          // [positions][rotary]: cosines, then sines
+  const long long* slots;
+  const long long* positions;
+  unsigned long long q_row, q_head, k_row, k_head, v_row, v_head;  // bytes
+  unsigned long long plane_bytes, slot_count, table_rows;
+  unsigned int tokens, q_heads, kv_heads, dim, rotary;
+  unsigned int first;          // token of this launch
+  unsigned int units;          // of the pairs of a head
+  unsigned int lanes_heads;    // heads that a wave's lanes take at once
+};
+
+constexpr unsigned int kMostRotated = 1u << 24;  // tokens of a launch, whose threads fit 32 bits
+
+template <typename E, int N>
+struct __attribute__((aligned(sizeof(E) * N))) Values {
+  E v[N];
+};
+
+// A wave for each token. A lane keeps the cosines and sines of N pairs and takes them to one head after
+// another: N values of its first half and N of its second, or (kAdjacent) 2 N values side by side.
+template <typename E, int N, bool kAdjacent>
+__global__ __launch_bounds__(kStepThreads) void rotate_rows(RotateArgs a) {
+  typedef Values<E, N> Unit;
+  const unsigned int lane = threadIdx.x & 63;
+  const unsigned int token = uniform(a.first + blockIdx.x * (kStepThreads / kWave) + (threadIdx.x >> 6));
+  if (token >= a.tokens) return;
+  const long long slot = a.slots[token], position = a.positions[token];
+  const bool write = slot >= 0 && (unsigned long long)slot < a.slot_count;
+  const bool known = position >= 0 && (unsigned long long)position < a.table_rows;
+  const float* const table = a.table + (known ? (unsigned long long)position * a.rotary : 0ull);
+  const unsigned char* const q = a.q + token * a.q_row;
+  const unsigned char* const k = a.k + token * a.k_row;
+  const unsigned char* const v = a.v + token * a.v_row;
+  const unsigned int head_bytes = a.dim * sizeof(E), pairs = a.rotary / 2;
+  unsigned char* const out = a.out + (unsigned long long)token * a.q_heads * head_bytes;
+  unsigned char* const layer = a.layer + (write ? (unsigned long long)slot : 0ull) * a.kv_heads * head_bytes;
+  const unsigned int heads = a.q_heads + a.kv_heads;
+  auto source = [&](unsigned int h) {
+    return h < a.q_heads ? q + h * a.q_head : k + (h - a.q_heads) * a.k_head;
+  };
+  auto target = [&](unsigned int h) {
+    return h < a.q_heads ? out + h * head_bytes : layer + (h - a.q_heads) * head_bytes;
+  };
+  const unsigned int sub = lane / min(a.units, (unsigned int)kWave);
+  for (unsigned int u = lane - sub * min(a.units, (unsigned int)kWave); u < a.units && sub < a.lanes_heads;
+       u += kWave) {
+    float c[N], s[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      c[i] = known ? table[u * N + i] : NAN;
+      s[i] = known ? table[pairs + u * N + i] : NAN;
+    }
+    const unsigned int at = (kAdjacent ? 2 * N : N) * sizeof(E) * u;
+    const unsigned int at2 = at + (kAdjacent ? N : pairs) * sizeof(E);
+    for (unsigned int h = sub; h < heads; h += a.lanes_heads) {
+      if (h >= a.q_heads && !write) break;
+      const unsigned char* src = source(h);
+      const Unit x = *reinterpret_cast<const Unit*>(src + at), y = *reinterpret_cast<const Unit*>(src + at2);
+      Unit x2, y2;
+      if constexpr (kAdjacent) {
+        E in[2 * N], res[2 * N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          in[i] = x.v[i];
+          in[N + i] = y.v[i];
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const float p = (float)in[2 * i], r = (float)in[2 * i + 1];
+          res[2 * i] = (E)(p * c[i] - r * s[i]);
+          res[2 * i + 1] = (E)(r * c[i] + p * s[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          x2.v[i] = res[i];
+          y2.v[i] = res[N + i];
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const float p = (float)x.v[i], r = (float)y.v[i];
+          x2.v[i] = (E)(p * c[i] - r * s[i]);
+          y2.v[i] = (E)(r * c[i] + p * s[i]);
+        }
+      }
+      unsigned char* dst = target(h);
+      *reinterpret_cast<Unit*>(dst + at) = x2;
+      *reinterpret_cast<Unit*>(dst + at2) = y2;
+    }
+  }
+  // what is not rotated
+  const unsigned int rest = (a.dim - a.rotary) / N;
+  for (unsigned int i = lane; i < rest * heads; i += kWave) {
+    const unsigned int h = i / rest, at = (a.rotary + (i - h * rest) * N) * sizeof(E);
+    if (h >= a.q_heads && !write) break;
+    *reinterpret_cast<Unit*>(target(h) + at) = *reinterpret_cast<const Unit*>(source(h) + at);
+  }
+  if (!write) return;
+  const unsigned int head_units = a.dim / N;
+  for (unsigned int i = lane; i < head_units * a.kv_heads; i += kWave) {
+    const unsigned int h = i / head_units, at = (i - h * head_units) * N * sizeof(E);
+    *reinterpret_cast<Unit*>(layer + a.plane_bytes + h * head_bytes + at) =
+        *reinterpret_cast<const Unit*>(v + h * a.v_head + at);
+  }
+}
+
+template <typename E, bool kAdjacent>
+void launch_rotate(const RotateArgs& a, bool wide, hipStream_t stream) {
+  const unsigned int waves = kStepThreads / kWave;
+  const dim3 grid((std::min(a.tokens - a.first, kMostRotated) + waves - 1) / waves), threads(kStepThreads);
+  if (wide)
+    hipLaunchKernelGGL((rotate_rows<E, 8, kAdjacent>), grid, threads, 0, stream, a);
+  else
+    hipLaunchKernelGGL((rotate_rows<E, 1, kAdjacent>), grid, threads, 0, stream, a);
+}
+
 }  // namespace
 }  // namespace unchainkv
 
@@ -369,4 +492,78 @@ extern "C" long long kvq_splitzip_write_kv_paged(
     if (st != hipSuccess) return fail("write_rows", st);
   }
   return (long long)(2 * tokens * a.row_bytes);
+}
+
+extern "C" long long kvq_splitzip_rotate_write_kv_paged(
+    unsigned long long q_ptr, unsigned long long q_row_bytes, unsigned long long q_head_bytes,
+    unsigned long long q_heads, unsigned long long k_ptr, unsigned long long k_row_bytes,
+    unsigned long long k_head_bytes, unsigned long long v_ptr, unsigned long long v_row_bytes,
+    unsigned long long v_head_bytes, unsigned long long tokens, unsigned long long kv_heads,
+    unsigned long long head_dim, unsigned long long dtype, unsigned long long kv_ptr,
+    unsigned long long plane_bytes, unsigned long long slot_count, unsigned long long slots_ptr,
+    unsigned long long positions_ptr, unsigned long long rotation_ptr, unsigned long long rotation_rows,
+    unsigned long long rotary_dim, unsigned long long adjacent, unsigned long long out_ptr,
+    unsigned long long stream_ptr) {
+  constexpr unsigned long long kMost = 0x7FFFFFFFull, kMostHeads = 65536, kMostDim = 4096;
+  if (q_ptr == 0 || k_ptr == 0 || v_ptr == 0 || kv_ptr == 0 || slots_ptr == 0 || positions_ptr == 0 ||
+      rotation_ptr == 0 || out_ptr == 0 || tokens == 0 || tokens > kMost || q_heads == 0 ||
+      q_heads > kMostHeads || kv_heads == 0 || kv_heads > kMostHeads || head_dim == 0 ||
+      head_dim > kMostDim || rotary_dim == 0 || rotary_dim % 2 != 0 || rotary_dim > head_dim ||
+      rotation_rows == 0 || rotation_rows > kMost || dtype > 1 || slot_count > kMost || rotation_ptr % 4 != 0 ||
+      (q_ptr | q_row_bytes | q_head_bytes | k_ptr | k_row_bytes | k_head_bytes | v_ptr | v_row_bytes |
+       v_head_bytes | kv_ptr | plane_bytes | out_ptr) % 2 != 0)
+    return 0;
+  const unsigned long long head_bytes = 2 * head_dim, row_bytes = kv_heads * head_bytes;
+  if (slot_count * row_bytes > plane_bytes) return 0;
+  const unsigned long long in[][2] = {
+      {q_ptr, (tokens - 1) * q_row_bytes + (q_heads - 1) * q_head_bytes + head_bytes},
+      {k_ptr, (tokens - 1) * k_row_bytes + (kv_heads - 1) * k_head_bytes + head_bytes},
+      {v_ptr, (tokens - 1) * v_row_bytes + (kv_heads - 1) * v_head_bytes + head_bytes},
+      {slots_ptr, 8 * tokens}, {positions_ptr, 8 * tokens}, {rotation_ptr, 4 * rotation_rows * rotary_dim}};
+  const unsigned long long out[][2] = {{kv_ptr, plane_bytes + slot_count * row_bytes},
+                                       {out_ptr, tokens * q_heads * head_bytes}};
+  for (const auto& o : out)
+    for (const auto& i : in)
+      if (overlap(o[0], o[1], i[0], i[1])) return 0;
+  if (overlap(out[0][0], out[0][1], out[1][0], out[1][1])) return 0;
+  // 8 values at a time where every row, head and address allows it, and both parts of a head are such runs
+  const bool wide = (q_ptr | q_row_bytes | k_ptr | k_row_bytes | v_ptr | v_row_bytes | kv_ptr | plane_bytes |
+                     out_ptr | (q_heads > 1 ? q_head_bytes : 0) |
+                     (kv_heads > 1 ? k_head_bytes | v_head_bytes : 0) | rotary_dim | head_bytes) % 16 == 0;
+  RotateArgs a{};
+  a.q = reinterpret_cast<const unsigned char*>(q_ptr);
+  a.k = reinterpret_cast<const unsigned char*>(k_ptr);
+  a.v = reinterpret_cast<const unsigned char*>(v_ptr);
+  a.out = reinterpret_cast<unsigned char*>(out_ptr);
+  a.layer = reinterpret_cast<unsigned char*>(kv_ptr);
+  a.table = reinterpret_cast<const float*>(rotation_ptr);
+  a.slots = reinterpret_cast<const long long*>(slots_ptr);
+  a.positions = reinterpret_cast<const long long*>(positions_ptr);
+  a.q_row = q_row_bytes;
+  a.q_head = q_head_bytes;
+  a.k_row = k_row_bytes;
+  a.k_head = k_head_bytes;
+  a.v_row = v_row_bytes;
+  a.v_head = v_head_bytes;
+  a.plane_bytes = plane_bytes;
+  a.slot_count = slot_count;
+  a.table_rows = rotation_rows;
+  a.tokens = (unsigned int)tokens;
+  a.q_heads = (unsigned int)q_heads;
+  a.kv_heads = (unsigned int)kv_heads;
+  a.dim = (unsigned int)head_dim;
+  a.rotary = (unsigned int)rotary_dim;
+  a.units = (unsigned int)(rotary_dim / 2 / (wide ? 8 : 1));
+  a.lanes_heads = std::max(1u, kWave / a.units);
+  hipStream_t stream = reinterpret_cast<hipStream_t>(stream_ptr);
+  for (unsigned long long first = 0; first < tokens; first += kMostRotated) {
+    a.first = (unsigned int)first;
+    if (dtype == 0)
+      adjacent ? launch_rotate<__bf16, true>(a, wide, stream) : launch_rotate<__bf16, false>(a, wide, stream);
+    else
+      adjacent ? launch_rotate<_Float16, true>(a, wide, stream) : launch_rotate<_Float16, false>(a, wide, stream);
+    const hipError_t st = hipGetLastError();
+    if (st != hipSuccess) return fail("rotate_rows", st);
+  }
+  return (long long)(2 * tokens * (q_heads * head_bytes + 2 * row_bytes));
 }

@@ -171,6 +171,14 @@ _SIGNATURES = (
      ctypes.c_longlong, False),
     ("kvq_splitzip_prompt_attention", [_U64] * 21 + [ctypes.c_float, _U64],
      ctypes.c_longlong, False),
+    ("kvq_splitzip_rotate_write_kv_paged", [_U64] * 25, ctypes.c_longlong, False),
+    ("kvq_splitzip_cross_attention_paged", [_U64] * 22 + [ctypes.c_float, _U64],
+     ctypes.c_longlong, False),
+    ("kvq_splitzip_cross_attention", [_U64] * 25 + [ctypes.c_float, _U64], ctypes.c_longlong, False),
+    ("kvq_splitzip_beam_select_workspace_bytes", [_U64] * 3, _U64, False),
+    ("kvq_splitzip_beam_select", [_U64] * 17, ctypes.c_longlong, False),
+    ("kvq_splitzip_reorder_beams_workspace_bytes", [_U64] * 3, _U64, False),
+    ("kvq_splitzip_reorder_beams_paged", [_U64P] + [_U64] * 23, ctypes.c_longlong, False),
     (
         "kvq_splitzip_bf16_decode_mode_paged",
         [_U64, _U64P, _U64P, _U64, _U64, _U64, _U64, _U64, _U64, _U64P, _U64, ctypes.c_int],
@@ -1416,6 +1424,92 @@ def write_kv_paged(k, v, kv_layer, slots) -> int | None:
     return int(got)
 
 
+def rotation_table(positions: int, rotary_dim: int, base: float = 10000.0, *, frequencies=None,
+                   device="cuda"):
+    """Cosines and sines of positions 0 .. positions - 1 for ``rotate_write_kv_paged``: a
+    (positions, rotary_dim) float32 tensor, in each row the rotary_dim / 2 cosines and then the
+    sines of position * frequency, with the frequencies base ** (-2 i / rotary_dim), or the
+    rotary_dim / 2 ones of ``frequencies``. Angles, cosines and sines are formed in 64 bits and
+    rounded once, so far positions lose nothing. A program makes it once."""
+    import torch
+
+    positions, rotary_dim = int(positions), int(rotary_dim)
+    if positions < 0 or rotary_dim <= 0 or rotary_dim % 2:
+        raise ValueError(f"no table of {positions} positions, {rotary_dim} values")
+    if frequencies is None:
+        exponents = torch.arange(0, rotary_dim, 2, dtype=torch.float64, device=device) / rotary_dim
+        frequencies = float(base) ** -exponents
+    else:
+        frequencies = torch.as_tensor(frequencies, dtype=torch.float64, device=device)
+        if frequencies.shape != (rotary_dim // 2,):
+            raise ValueError(f"{rotary_dim // 2} frequencies, not {tuple(frequencies.shape)}")
+    angles = torch.arange(positions, dtype=torch.float64, device=device)[:, None] * frequencies
+    return torch.cat((angles.cos(), angles.sin()), 1).float()
+
+
+def rotate_write_kv_paged(q, k, v, kv_layer, slots, positions, rotation, *,
+                          interleaved: bool = False, out=None):
+    """``write_kv_paged`` with the position rotation on the way, and the rotated queries: the first
+    rotary_dim values of every head of ``q`` (tokens, q_heads, head_dim) and ``k`` (tokens,
+    kv_heads, head_dim) are rotated in pairs, (x, y) -> (x cos - y sin, y cos + x sin), the others
+    and ``v`` are copied. Pair i of a head is its values i and i + rotary_dim / 2, or with
+    ``interleaved`` 2 i and 2 i + 1. ``rotation`` (positions, rotary_dim) float32 has the cosines and
+    then the sines of each position (``rotation_table``), ``positions`` (int64, ``StepPlan.positions``)
+    each row's. Computed in 32 bits and rounded once.
+
+    K and V go to ``kv_layer`` by ``slots`` as in ``write_kv_paged`` (types, strides, rows without a
+    slot, two rows with one slot); a row without a slot still has its rotated queries. ``slots`` and
+    ``positions`` may be longer than the rows. A position outside the table makes the rotated
+    values of its row NaN. ``out`` (contiguous, as q) takes the queries; it, like the layer, must not
+    lie over anything that is read. Nothing has a gradient.
+
+    Returns the rotated queries (tokens, q_heads, head_dim), or ``None`` when the kernel
+    declines."""
+    lib = _load()
+    rotate = getattr(lib, "kvq_splitzip_rotate_write_kv_paged", None) if lib else None
+    if rotate is None or not _is_cuda(q):
+        return None
+    import torch
+
+    device = q.device
+    dtype = _row_dtype(q.dtype, torch)
+    if dtype is None or not _rows_ok(q, q.dtype, device) or not _rows_ok(k, q.dtype, device) or \
+            not _rows_ok(v, q.dtype, device) or not _kv_layer_ok(kv_layer, q.dtype, device):
+        return None
+    tokens, q_heads, head_dim = q.shape
+    kv_heads = k.shape[1]
+    if k.shape != v.shape or k.shape[0] != tokens or k.shape[2] != head_dim or \
+            kv_layer.shape[3] != kv_heads or kv_layer.shape[4] != head_dim or \
+            not _index_vector_ok(slots, device, tokens, torch.int64) or \
+            not _index_vector_ok(positions, device, tokens, torch.int64) or \
+            rotation.dtype != torch.float32 or rotation.dim() != 2 or rotation.device != device or \
+            not rotation.is_contiguous():
+        return None
+    if _tracked(torch, q, k, v, kv_layer, rotation, out):
+        return None
+    given = out is not None
+    ok, out = _attention_buffers(q, out, None, torch)
+    if not ok:
+        return None
+    if tokens == 0:
+        return out
+    got = _call_on(device, torch, rotate, q.data_ptr(), 2 * q.stride(0), 2 * q.stride(1), q_heads,
+                   k.data_ptr(), 2 * k.stride(0), 2 * k.stride(1), v.data_ptr(), 2 * v.stride(0),
+                   2 * v.stride(1), tokens, kv_heads, head_dim, dtype, kv_layer.data_ptr(),
+                   2 * kv_layer.stride(0), kv_layer.shape[1] * kv_layer.shape[2], slots.data_ptr(),
+                   positions.data_ptr(), rotation.data_ptr(), rotation.shape[0], rotation.shape[1],
+                   1 if interleaved else 0, out.data_ptr())
+    if got < 0:
+        _raise_last(lib, "splitzip rotated K/V write failed")
+    if not got:
+        return None
+    if given:
+        _wrote(torch, kv_layer, out)
+    else:
+        _wrote(torch, kv_layer)
+    return out
+
+
 @functools.lru_cache(maxsize=1024)
 def _attention_workspace(name: str, device, sizes: tuple) -> int:
     import torch
@@ -1485,38 +1579,11 @@ def _attention_buffers(q, out, lse, torch):
     return True, out
 
 
-def chunk_attention_paged(q, kv_layer, tables, query_starts, context_tokens, *,
-                          max_query: int | None = None, scale: float | None = None, out=None,
-                          lse=None, workspace=None):
-    """Causal attention of a step's new tokens over a paged layer that holds their own K and V
-    already (``write_kv_paged``); single tokens (decode), chunks of prompts and drafted
-    tokens mixed in any way.
-
-    ``q`` (tokens, q_heads, head_dim) are the packed rows; request r's are rows
-    ``query_starts[r]`` .. ``query_starts[r + 1]``, the last of its ``context_tokens[r]``
-    tokens, so row i of its n sees tokens 0 .. context - n + i. Query head h reads KV head
-    h // (q_heads / kv_heads). ``tables`` (requests, width) int32 lists each request's blocks in
-    token order, ``query_starts`` (requests + 1) and ``context_tokens`` (requests) are int32;
-    all stay on the device (``StepPlan``), and a captured call follows their values.
-    ``max_query`` bounds the new tokens of a request (default: the rows of q); a smaller bound
-    spares a decode step the kernel for long chunks. ``scale`` (positive) defaults to head_dim
-    ** -0.5. ``lse`` (tokens, q_heads) float32 receives each row's log-sum-exp, for joining
-    with attention over other tokens. bf16 or fp16, head_dim 64 or 128; rows and heads of q
-    may be strided by multiples of 16 bytes.
-
-    A row that sees no token (context_tokens[r] less than its new tokens) is zero, its lse
-    -inf. Rows of no request, of one with more new tokens than max_query, and of one whose
-    row range is not inside q stay as they are. A context longer than its table, or a table
-    entry that is no block of the layer, makes the rows that read there NaN (every row of
-    the same tile, of 16 to 256 of a KV head's query rows, at least). Where
-    query_starts run backwards, so that ranges overlap, rows are one of their requests' or stay.
-    ``out``, ``lse`` and ``workspace`` over an input or each other are declined.
-    No gradient: inputs, ``out`` or ``lse`` that require one are declined while gradients are
-    recorded, and so are forward-mode tangents.
-
-    Returns ``out`` (tokens, q_heads, head_dim), or ``None`` when the kernel declines."""
+def _attend_paged(kind: str, q, kv_layer, tables, query_starts, context_tokens, max_query, scale,
+                  out, lse, workspace):
+    """chunk_attention_paged and cross_attention_paged."""
     lib = _load()
-    attend = getattr(lib, "kvq_splitzip_chunk_attention_paged", None) if lib else None
+    attend = getattr(lib, f"kvq_splitzip_{kind}_attention_paged", None) if lib else None
     if attend is None or not _is_cuda(q):
         return None
     import torch
@@ -1559,12 +1626,46 @@ def chunk_attention_paged(q, kv_layer, tables, query_starts, context_tokens, *,
                    workspace.data_ptr() if need else 0, need,
                    head_dim ** -0.5 if scale is None else float(scale))
     if got < 0:
-        _raise_last(lib, "splitzip chunk attention failed")
+        _raise_last(lib, f"splitzip {kind} attention failed")
     if not got:
         return None
     if given:
         _wrote(torch, *given)
     return out
+
+
+def chunk_attention_paged(q, kv_layer, tables, query_starts, context_tokens, *,
+                          max_query: int | None = None, scale: float | None = None, out=None,
+                          lse=None, workspace=None):
+    """Causal attention of a step's new tokens over a paged layer that holds their own K and V
+    already (``write_kv_paged``); single tokens (decode), chunks of prompts and drafted
+    tokens mixed in any way.
+
+    ``q`` (tokens, q_heads, head_dim) are the packed rows; request r's are rows
+    ``query_starts[r]`` .. ``query_starts[r + 1]``, the last of its ``context_tokens[r]``
+    tokens, so row i of its n sees tokens 0 .. context - n + i. Query head h reads KV head
+    h // (q_heads / kv_heads). ``tables`` (requests, width) int32 lists each request's blocks in
+    token order, ``query_starts`` (requests + 1) and ``context_tokens`` (requests) are int32;
+    all stay on the device (``StepPlan``), and a captured call follows their values.
+    ``max_query`` bounds the new tokens of a request (default: the rows of q); a smaller bound
+    spares a decode step the kernel for long chunks. ``scale`` (positive) defaults to head_dim
+    ** -0.5. ``lse`` (tokens, q_heads) float32 receives each row's log-sum-exp, for joining
+    with attention over other tokens. bf16 or fp16, head_dim 64 or 128; rows and heads of q
+    may be strided by multiples of 16 bytes.
+
+    A row that sees no token (context_tokens[r] less than its new tokens) is zero, its lse
+    -inf. Rows of no request, of one with more new tokens than max_query, and of one whose
+    row range is not inside q stay as they are. A context longer than its table, or a table
+    entry that is no block of the layer, makes the rows that read there NaN (every row of
+    the same tile, of 16 to 256 of a KV head's query rows, at least). Where
+    query_starts run backwards, so that ranges overlap, rows are one of their requests' or stay.
+    ``out``, ``lse`` and ``workspace`` over an input or each other are declined.
+    No gradient: inputs, ``out`` or ``lse`` that require one are declined while gradients are
+    recorded, and so are forward-mode tangents.
+
+    Returns ``out`` (tokens, q_heads, head_dim), or ``None`` when the kernel declines."""
+    return _attend_paged("chunk", q, kv_layer, tables, query_starts, context_tokens, max_query,
+                         scale, out, lse, workspace)
 
 
 def prompt_attention(q, k, v, query_starts, *, max_query: int | None = None,
@@ -1623,6 +1724,332 @@ def prompt_attention(q, k, v, query_starts, *, max_query: int | None = None,
     if given:
         _wrote(torch, *given)
     return out
+
+
+def cross_attention_paged(q, kv_layer, tables, query_starts, source_tokens, *,
+                          max_query: int | None = None, scale: float | None = None, out=None,
+                          lse=None, workspace=None):
+    """Attention of a request's rows over all tokens of its source, whose K and V a paged layer holds
+    (an encoder's states, written or restored once and read at every step): each of the rows
+    ``query_starts[r]`` .. ``query_starts[r + 1]`` of ``q`` sees tokens 0 .. source_tokens[r] - 1 of
+    the blocks that row r of ``tables`` lists, so the beams of a request, given as its rows, read
+    its source once. Everything else is as in ``chunk_attention_paged``: types, heads, strides,
+    ``max_query`` (of a request's rows), ``scale``, ``lse``, ``workspace`` (of
+    ``chunk_attention_workspace_bytes``), captured calls, gradients. A request without source
+    tokens has rows of zero, their lse -inf.
+
+    Returns ``out`` (tokens, q_heads, head_dim), or ``None`` when the kernel declines."""
+    return _attend_paged("cross", q, kv_layer, tables, query_starts, source_tokens, max_query, scale,
+                         out, lse, workspace)
+
+
+def cross_attention(q, k, v, query_starts, source_starts, source_tokens, *,
+                    max_query: int | None = None, max_source: int | None = None,
+                    scale: float | None = None, out=None, lse=None, workspace=None):
+    """``cross_attention_paged`` over sources that are rows of ``k`` and ``v`` (rows, kv_heads,
+    head_dim): request r's is the ``source_tokens[r]`` rows from ``source_starts[r]`` on (packed one
+    behind the other, padded to one length, or shared between requests; int32, on the device).
+    ``max_source`` bounds a source's tokens (default: all rows of k): a smaller bound, up to 1024,
+    spares a call of few rows the joining of splits. Requests whose source is longer stay as they
+    are, like those with more than ``max_query`` rows; a source that is not inside k makes its
+    request's rows NaN. Rows and heads of k and v may be strided by multiples of 16 bytes. The
+    workspace is that of ``chunk_attention_workspace_bytes`` with ``max_source`` as the context.
+
+    Returns ``out`` (tokens, q_heads, head_dim), or ``None`` when the kernel declines."""
+    lib = _load()
+    attend = getattr(lib, "kvq_splitzip_cross_attention", None) if lib else None
+    if attend is None or not _is_cuda(q):
+        return None
+    import torch
+
+    device = q.device
+    dtype = _row_dtype(q.dtype, torch)
+    if dtype is None or not _rows_ok(q, q.dtype, device) or not _rows_ok(k, q.dtype, device) or \
+            not _rows_ok(v, q.dtype, device):
+        return None
+    if _tracked(torch, q, k, v, out, lse):
+        return None
+    tokens, q_heads, head_dim = q.shape
+    rows, kv_heads = k.shape[:2]
+    requests = source_tokens.numel()
+    if k.shape != v.shape or k.shape[2] != head_dim or head_dim == 0 or \
+            not _index_vector_ok(source_tokens, device, 0, torch.int32) or \
+            not _index_vector_ok(source_starts, device, requests, torch.int32) or \
+            not _index_vector_ok(query_starts, device, requests + 1, torch.int32):
+        return None
+    max_query = tokens if max_query is None else min(int(max_query), tokens)
+    max_source = rows if max_source is None else min(int(max_source), rows)
+    given = [t for t in (out, lse) if t is not None]
+    ok, out = _attention_buffers(q, out, lse, torch)
+    if not ok:
+        return None
+    if tokens == 0 or requests == 0:
+        return out
+    if max_query <= 0 or max_source < 0 or rows == 0:
+        return None
+    need = _attention_workspace(
+        "kvq_splitzip_chunk_attention_workspace_bytes", device,
+        (tokens, requests, q_heads, kv_heads, head_dim, max_source, max_query))
+    if need and not _byte_buffer_ok(workspace, device, need, torch):
+        workspace = torch.empty(need, dtype=torch.uint8, device=device)
+    got = _call_on(device, torch, attend, q.data_ptr(), 2 * q.stride(0), 2 * q.stride(1),
+                   k.data_ptr(), 2 * k.stride(0), 2 * k.stride(1), v.data_ptr(), 2 * v.stride(0),
+                   2 * v.stride(1), rows, tokens, q_heads, kv_heads, head_dim, dtype,
+                   query_starts.data_ptr(), source_starts.data_ptr(), source_tokens.data_ptr(),
+                   requests, max_query, max_source, out.data_ptr(),
+                   0 if lse is None else lse.data_ptr(), workspace.data_ptr() if need else 0, need,
+                   head_dim ** -0.5 if scale is None else float(scale))
+    if got < 0:
+        _raise_last(lib, "splitzip cross attention failed")
+    if not got:
+        return None
+    if given:
+        _wrote(torch, *given)
+    return out
+
+
+# ---------------------------------------------------------------------------
+# beam search over a paged layer: selection, reordering
+
+class BeamChoice(NamedTuple):
+    """What ``beam_select`` gives, on the device and best first: ``scores`` (requests, candidates)
+    float32, ``parents`` int32 (the beam that each continues) and ``tokens`` int64."""
+
+    scores: object
+    parents: object
+    tokens: object
+
+
+def new_beam_choice(requests: int, candidates: int, device, torch=None) -> BeamChoice:
+    """Buffers for ``beam_select(..., choice=)``, which a captured step keeps."""
+    if torch is None:
+        import torch
+    tokens = torch.empty((requests, candidates), dtype=torch.int64, device=device)
+    scores = torch.empty((requests, candidates), dtype=torch.float32, device=device)
+    return BeamChoice(scores, torch.empty_like(scores, dtype=torch.int32), tokens)
+
+
+_LOGIT_DTYPES: dict = {}
+
+
+def beam_select_workspace_bytes(requests: int, beams: int, vocab: int) -> int:
+    """Workspace of ``beam_select``. Sizes that the call declines raise ``ValueError``."""
+    lib = _load()
+    if lib is None or not hasattr(lib, "kvq_splitzip_beam_select_workspace_bytes"):
+        raise RuntimeError(f"HIP codec library not loaded: {load_error()}")
+    need = 0
+    if requests >= 0 and beams >= 0 and vocab >= 0:
+        need = int(lib.kvq_splitzip_beam_select_workspace_bytes(max(requests, 1), beams, vocab))
+    if not need:
+        raise ValueError(f"no selection takes {requests} requests of {beams} beams, {vocab} tokens")
+    return need if requests else 0
+
+
+def _matrix_ok(t, shape, dtype, device) -> bool:
+    return t.dtype == dtype and t.shape == shape and t.device == device and t.is_contiguous()
+
+
+def beam_select(logits, scores, *, candidates: int | None = None, ended=None,
+                end_token: int | None = None, choice: BeamChoice | None = None, workspace=None):
+    """The best continuations of every request's beams. Beam b of a request offers token t at
+    ``scores[b]`` + logits[b, t] - log sum exp(logits[b]); of all beams and tokens the
+    ``candidates`` (default: as many as beams; at most 64) best are given, best first, equal ones
+    by the lowest beam and then the lowest token.
+
+    ``logits`` (requests, beams, vocab) float32, bf16 or fp16, with contiguous tokens and any strides
+    of beams and requests; ``scores`` (requests, beams) float32, the beams' sums of log
+    probabilities. At most 32 beams and 2 ** 20 tokens. A beam of score -inf (not in use: all but one
+    at a search's first step) offers nothing but -inf, and so does a token of logit -inf (not
+    allowed), whatever else the row holds. A beam whose ``ended`` (requests, beams; bool) is true goes on with
+    ``end_token`` alone, at its own score. Where too little else is offered, candidates of -inf follow.
+    A NaN or +inf logit makes all that its beam offers NaN, which comes first. Values are formed
+    and compared in 64 bits, with sums of 32-bit exponentials, and scores rounded once.
+
+    Everything stays on the device, and a captured call follows it (``choice=`` from
+    ``new_beam_choice``, ``workspace=`` of ``beam_select_workspace_bytes``); calls that overlap in
+    time need workspaces of their own. Results must not lie over inputs or each other. Nothing has a
+    gradient.
+
+    Returns a ``BeamChoice``, or ``None`` when the kernel declines."""
+    lib = _load()
+    select = getattr(lib, "kvq_splitzip_beam_select", None) if lib else None
+    if select is None or not _is_cuda(logits):
+        return None
+    import torch
+
+    if not _LOGIT_DTYPES:
+        _LOGIT_DTYPES.update({torch.bfloat16: 0, torch.float16: 1, torch.float32: 2})
+    device, dtype = logits.device, _LOGIT_DTYPES.get(logits.dtype)
+    if dtype is None or logits.dim() != 3:
+        return None
+    requests, beams, vocab = logits.shape
+    if (vocab != 1 and logits.stride(2) != 1) or logits.stride(0) < 0 or logits.stride(1) < 0 or \
+            not _matrix_ok(scores, (requests, beams), torch.float32, device):
+        return None
+    if ended is not None and (not _matrix_ok(ended, (requests, beams), torch.bool, device)
+                              or end_token is None or not 0 <= int(end_token) < vocab):
+        return None
+    if _tracked(torch, logits, scores, *(choice or ())):
+        return None
+    candidates = beams if candidates is None else int(candidates)
+    if not 0 < candidates <= 64:
+        return None
+    given = choice or ()
+    if choice is None:
+        choice = new_beam_choice(requests, candidates, device, torch)
+    elif not (_matrix_ok(choice.scores, (requests, candidates), torch.float32, device)
+              and _matrix_ok(choice.parents, (requests, candidates), torch.int32, device)
+              and _matrix_ok(choice.tokens, (requests, candidates), torch.int64, device)):
+        return None
+    if requests == 0:
+        return choice
+    need = lib.kvq_splitzip_beam_select_workspace_bytes(requests, beams, vocab)
+    if not need:
+        return None
+    if not _byte_buffer_ok(workspace, device, need, torch):
+        workspace = torch.empty(need, dtype=torch.uint8, device=device)
+    got = _call_on(device, torch, select, logits.data_ptr(), dtype, logits.stride(0),
+                   logits.stride(1), scores.data_ptr(), 0 if ended is None else ended.data_ptr(),
+                   requests, beams, vocab, candidates, 0 if ended is None else int(end_token),
+                   choice.scores.data_ptr(), choice.parents.data_ptr(), choice.tokens.data_ptr(),
+                   workspace.data_ptr(), need)
+    if got < 0:
+        _raise_last(lib, "splitzip beam selection failed")
+    if not got:
+        return None
+    if given:
+        _wrote(torch, *given)
+    return choice
+
+
+class BeamOrder(NamedTuple):
+    """What ``reorder_beams_paged`` gives, on the device (int32): ``tables`` (requests * beams,
+    width); ``copied_from`` (requests * beams), the block that each beam's last one was copied from,
+    -1 where it was not; ``free_next`` (1), the first entry of the free list that is free now;
+    ``lacking`` (1), beams without a last block of their own (their entry is -1) or without a parent;
+    ``unlisted`` (1), released blocks that the list has no room for below its first free entry."""
+
+    tables: object
+    copied_from: object
+    free_next: object
+    lacking: object
+    unlisted: object
+
+
+def new_beam_order(requests: int, beams: int, width: int, device, torch=None) -> BeamOrder:
+    """Buffers for ``reorder_beams_paged(..., order=)``, which a captured step keeps."""
+    if torch is None:
+        import torch
+    rows = requests * beams
+    small = torch.empty(rows + 3, dtype=torch.int32, device=device)
+    copied, free_next, lacking, unlisted = small.split_with_sizes((rows, 1, 1, 1))
+    return BeamOrder(torch.empty((rows, width), dtype=torch.int32, device=device), copied, free_next,
+                     lacking, unlisted)
+
+
+def reorder_beams_workspace_bytes(requests: int, beams: int, width: int) -> int:
+    """Workspace of ``reorder_beams_paged``. Sizes that the call declines raise ``ValueError``."""
+    lib = _load()
+    if lib is None or not hasattr(lib, "kvq_splitzip_reorder_beams_workspace_bytes"):
+        raise RuntimeError(f"HIP codec library not loaded: {load_error()}")
+    need = 0
+    if requests >= 0 and beams >= 0 and width >= 0:
+        need = int(lib.kvq_splitzip_reorder_beams_workspace_bytes(max(requests, 1), beams, width))
+    if not need:
+        raise ValueError(f"no reordering takes {requests} requests of {beams} beams, tables of {width}")
+    return need if requests else 0
+
+
+def reorder_beams_paged(layers, tables, parents, context_tokens, free_blocks, free_start,
+                        block_tokens: int, *, order: BeamOrder | None = None, workspace=None):
+    """The beams' block tables, and the layers, in the order of the chosen parents: beam j of
+    request r (row r * beams + j of ``tables``) goes on as beam ``parents[r, j]`` was
+    (``BeamChoice.parents``, or the beams picked of its candidates). Everything stays on the device, so
+    a captured step follows the choice.
+
+    ``tables`` (requests * beams, width) int32 lists each beam's blocks in token order, ``parents`` is
+    (requests, beams) int32, ``context_tokens`` (requests * beams) int32 are the tokens that the beams
+    hold (those of a request's beams are equal: its first one's count). Blocks that are full are
+    shared by all beams that descend from them. The last, partly filled block, in which every beam
+    writes on, has to be each beam's own: the first child of a parent keeps its parent's, the others
+    take the blocks that beams without children leave, into which their parent's tokens are copied
+    in every one of ``layers`` (contiguous (2, num_blocks, block_tokens, kv_heads, head_dim) layers
+    of one shape, bf16 or fp16; there may be none). So a request's beams need last blocks of their own
+    from the start, whatever is in them: a child for which none is left gets -1 and is counted in
+    ``lacking``. Table entries behind the context stay.
+
+    Blocks of the context that no beam of the request lists any more are released: they are written
+    into ``free_blocks`` just below entry ``free_start[0]``, in the order of requests, blocks and
+    beams, as ``plan_step_paged`` takes them from there on, and ``free_next`` is the new first entry. A
+    parent outside 0 .. beams - 1 gives a row of -1 for the context. Blocks must not be shared between
+    requests except where all beams of each list them (as a common prompt's).
+
+    ``order`` (from ``new_beam_order`` or an earlier call of the same sizes) takes the results; its
+    ``tables`` may be ``tables`` itself, to reorder in place. Other results, the layers and ``free_blocks``
+    must not lie over an input or each other. At most 32 beams.
+
+    Returns a ``BeamOrder``, or ``None`` when the kernel declines."""
+    lib = _load()
+    reorder = getattr(lib, "kvq_splitzip_reorder_beams_paged", None) if lib else None
+    if reorder is None or not _is_cuda(tables):
+        return None
+    import torch
+
+    device, i32, block_tokens = tables.device, torch.int32, int(block_tokens)
+    if tables.dtype != i32 or tables.dim() != 2 or parents.dtype != i32 or parents.dim() != 2 or \
+            parents.device != device or not parents.is_contiguous() or block_tokens <= 0:
+        return None
+    requests, beams = parents.shape
+    rows, width = tables.shape
+    if rows != requests * beams or (width != 1 and tables.stride(1) != 1) or \
+            not _index_vector_ok(context_tokens, device, rows, i32) or \
+            not _index_vector_ok(free_blocks, device, 0, i32) or \
+            not _index_vector_ok(free_start, device, 1, i32):
+        return None
+    layers = list(layers)
+    for layer in layers:
+        if _row_dtype(layer.dtype, torch) is None or \
+                not _kv_layer_ok(layer, layers[0].dtype, device) or \
+                layer.shape != layers[0].shape or layer.shape[2] != block_tokens:
+            return None
+    if _tracked(torch, *layers):
+        return None
+    given = order or ()
+    if order is None:
+        order = new_beam_order(requests, beams, width, device, torch)
+    elif order.tables.dtype != i32 or order.tables.shape != tables.shape or \
+            order.tables.device != device or (width != 1 and order.tables.stride(1) != 1) or \
+            not (_index_vector_ok(order.copied_from, device, rows, i32)
+                 and _index_vector_ok(order.free_next, device, 1, i32)
+                 and _index_vector_ok(order.lacking, device, 1, i32)
+                 and _index_vector_ok(order.unlisted, device, 1, i32)):
+        return None
+    if rows == 0:
+        order.free_next[:1].copy_(free_start[:1].clamp(0, free_blocks.numel()))
+        order.lacking[:1].fill_(0)
+        order.unlisted[:1].fill_(0)
+        return order
+    need = lib.kvq_splitzip_reorder_beams_workspace_bytes(requests, beams, width)
+    if not need:
+        return None
+    if not _byte_buffer_ok(workspace, device, need, torch):
+        workspace = torch.empty(need, dtype=torch.uint8, device=device)
+    blocks = layers[0].shape[1] if layers else 1
+    row_bytes = 2 * layers[0].stride(2) if layers else 2
+    pointers = (ctypes.c_ulonglong * max(len(layers), 1))(*[t.data_ptr() for t in layers])
+    got = _call_on(device, torch, reorder, pointers, len(layers), blocks, block_tokens, row_bytes,
+                   tables.data_ptr(), tables.stride(0) if rows > 1 else width, width,
+                   order.tables.data_ptr(), order.tables.stride(0) if rows > 1 else width,
+                   parents.data_ptr(), context_tokens.data_ptr(), requests, beams,
+                   free_blocks.data_ptr(), free_blocks.numel(), free_start.data_ptr(),
+                   order.copied_from.data_ptr(), order.free_next.data_ptr(),
+                   order.lacking.data_ptr(), order.unlisted.data_ptr(), workspace.data_ptr(), need)
+    if got < 0:
+        _raise_last(lib, "splitzip beam reordering failed")
+    if not got:
+        return None
+    _wrote(torch, free_blocks, *layers, *given)
+    return order
 
 
 # ---------------------------------------------------------------------------
