@@ -28,13 +28,14 @@ namespace unchainkv {
 namespace {
 
 constexpr int kScanThreads = 256;
-constexpr int kLaneLogits = 8;                                // of a lane's load
-constexpr int kSegment = 32 * kLaneLogits;                    // logits whose maximum is kept
-constexpr int kRound = kScanThreads * kLaneLogits;            // logits of a workgroup's round
-constexpr int kPickThreads = 512;
+constexpr int kLaneBytes = 64;                                // of a row that a lane takes at a time
+constexpr int kSegment = 256;                                 // logits whose maximum is kept
+constexpr int kPickThreads = 1024;
 constexpr int kMostBeams = 32, kMostCandidates = 64;
-constexpr int kItems = 16;                                    // values that a lane of beam_pick holds
+constexpr int kMostItems = 8;                                 // segments that a lane of beam_pick holds
+constexpr int kOwnTokens = kSegment / kWave;                  // tokens of one
 constexpr unsigned int kMostVocab = 1u << 20;
+static_assert(kMostVocab <= 8 * kMostItems * kWave * kSegment, "the largest groups hold a row");
 constexpr float kLowest = -3.402823466e38f;
 constexpr float kLog2E = 1.4426950408889634f;
 
@@ -50,53 +51,41 @@ struct SelectArgs {
   unsigned long long request_stride, beam_stride;
   unsigned int requests, beams, vocab, candidates, end_token;
   unsigned int segments, chunks, rounds;  // of a row; rounds of a chunk
+  unsigned int parts;         // waves that search a beam
+  unsigned int group, items;  // segments of an item, items of a row
 };
 
-// Logits by their type, 8 of them from any address.
+// Logits by their type, 16 bytes of them from any address.
 struct Bf16 {
   typedef struct __attribute__((packed, aligned(2))) { u32x4 v; } Raw;
-  static constexpr unsigned int kBytes = 2;
+  static constexpr int kBytes = 2, kLoad = 8;
   static __device__ __forceinline__ float one(const unsigned char* p, unsigned int i) {
     return __uint_as_float((unsigned int)reinterpret_cast<const uint16_t*>(p)[i] << 16);
   }
-  static __device__ __forceinline__ void eight(const unsigned char* p, float (&x)[8]) {
-    const u32x4 v = reinterpret_cast<const Raw*>(p)->v;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[2 * i] = __uint_as_float(v[i] << 16);
-      x[2 * i + 1] = __uint_as_float(v[i] & 0xFFFF0000u);
-    }
+  static __device__ __forceinline__ float of(const Raw& r, int i) {
+    return __uint_as_float(i % 2 == 0 ? r.v[i / 2] << 16 : r.v[i / 2] & 0xFFFF0000u);
   }
 };
 struct Fp16 {
   typedef _Float16 x8 __attribute__((ext_vector_type(8)));
   typedef struct __attribute__((packed, aligned(2))) { x8 v; } Raw;
-  static constexpr unsigned int kBytes = 2;
+  static constexpr int kBytes = 2, kLoad = 8;
   static __device__ __forceinline__ float one(const unsigned char* p, unsigned int i) {
     return (float)reinterpret_cast<const _Float16*>(p)[i];
   }
-  static __device__ __forceinline__ void eight(const unsigned char* p, float (&x)[8]) {
-    const x8 v = reinterpret_cast<const Raw*>(p)->v;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = (float)v[i];
-  }
+  static __device__ __forceinline__ float of(const Raw& r, int i) { return (float)r.v[i]; }
 };
 struct Fp32 {
   typedef float x4 __attribute__((ext_vector_type(4)));
-  typedef struct __attribute__((packed, aligned(4))) { x4 a, b; } Raw;
-  static constexpr unsigned int kBytes = 4;
+  typedef struct __attribute__((packed, aligned(4))) { x4 v; } Raw;
+  static constexpr int kBytes = 4, kLoad = 4;
   static __device__ __forceinline__ float one(const unsigned char* p, unsigned int i) {
     return reinterpret_cast<const float*>(p)[i];
   }
-  static __device__ __forceinline__ void eight(const unsigned char* p, float (&x)[8]) {
-    const Raw v = *reinterpret_cast<const Raw*>(p);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[i] = v.a[i];
-      x[4 + i] = v.b[i];
-    }
-  }
+  static __device__ __forceinline__ float of(const Raw& r, int i) { return r.v[i]; }
 };
+template <typename T>
+constexpr int kLaneLogits = kLaneBytes / T::kBytes;
 
 // A beam that offers no token of its own: finished, or without a hypothesis yet.
 __device__ __forceinline__ bool is_ended(const SelectArgs& a, unsigned int row) {
@@ -112,75 +101,92 @@ __device__ __forceinline__ const unsigned char* row_of(const SelectArgs& a, unsi
   return a.logits + (request * a.request_stride + (row - request * a.beams) * a.beam_stride) * T::kBytes;
 }
 
-// Largest of 32 lanes, in lanes 31 and 63 (row shifts by 1, 2, 4, 8, then rows 0 and 2 into the next).
 template <int kControl, int kRowMask>
 __device__ __forceinline__ float shifted(float v) {
   const int u = __builtin_bit_cast(int, v);
   return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(u, u, kControl, kRowMask, 0xF, false));
 }
-__device__ __forceinline__ float max_of_32(float v) {
+__device__ __forceinline__ float wave_max(float v) {
   v = fmaxf(v, shifted<0x111, 0xF>(v));
   v = fmaxf(v, shifted<0x112, 0xF>(v));
   v = fmaxf(v, shifted<0x114, 0xF>(v));
   v = fmaxf(v, shifted<0x118, 0xF>(v));
-  return fmaxf(v, shifted<0x142, 0xA>(v));
+  v = fmaxf(v, shifted<0x142, 0xA>(v));
+  v = fmaxf(v, shifted<0x143, 0xC>(v));
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
 }
 
+// A wave takes `rounds` times 64 lanes' 64 bytes of a row; a lane's logits follow each other, so that a
+// segment's maximum takes three or four exchanges between lanes for 32 or 16 logits of each.
 template <typename T>
 __global__ __launch_bounds__(kScanThreads) void beam_scan(SelectArgs a) {
-  __shared__ float s_max[kScanThreads / kWave], s_sum[kScanThreads / kWave];
-  const unsigned int row = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  if (!is_open(a, row)) return;
+  constexpr int kOwn = kLaneLogits<T>, kLoads = kOwn / T::kLoad, kLanes = kSegment / kOwn;
+  const unsigned int row = blockIdx.y, lane = threadIdx.x & 63;
+  const unsigned int chunk = uniform(blockIdx.x * (kScanThreads / kWave) + (threadIdx.x >> 6));
+  if (chunk >= a.chunks || !is_open(a, row)) return;
   const unsigned char* src = row_of<T>(a, row);
   float top = kLowest, sum = 0.f;
-  for (unsigned int n = 0; n < a.rounds; ++n) {
-    const unsigned int base = (blockIdx.x * a.rounds + n) * kRound;
-    if (base >= a.vocab) break;
-    const unsigned int at = base + tid * kLaneLogits;
-    float x[kLaneLogits];
-    if (at + kLaneLogits <= a.vocab) {
-      T::eight(src + at * T::kBytes, x);
+  const unsigned int first = chunk * a.rounds * (kWave * kOwn);
+  const unsigned int last = min(a.vocab, first + a.rounds * (kWave * kOwn));
+  for (unsigned int base = first; base < last; base += kWave * kOwn) {
+    const unsigned int at = base + lane * kOwn;
+    float x[kOwn];
+    if (base + kWave * kOwn <= a.vocab) {
+      typename T::Raw raw[kLoads];
+#pragma unroll
+      for (int n = 0; n < kLoads; ++n)
+        raw[n] = *reinterpret_cast<const typename T::Raw*>(src + (at + n * T::kLoad) * T::kBytes);
+#pragma unroll
+      for (int i = 0; i < kOwn; ++i) x[i] = T::of(raw[i / T::kLoad], i % T::kLoad);
     } else {
 #pragma unroll
-      for (int i = 0; i < kLaneLogits; ++i)
-        x[i] = at + i < a.vocab ? T::one(src, at + i) : -INFINITY;
+      for (int n = 0; n < kLoads; ++n) {
+        const unsigned int from = at + n * T::kLoad;
+        if (from + T::kLoad <= a.vocab) {
+          const typename T::Raw raw = *reinterpret_cast<const typename T::Raw*>(src + from * T::kBytes);
+#pragma unroll
+          for (int i = 0; i < T::kLoad; ++i) x[n * T::kLoad + i] = T::of(raw, i);
+        } else {
+#pragma unroll
+          for (int i = 0; i < T::kLoad; ++i)
+            x[n * T::kLoad + i] = from + i < a.vocab ? T::one(src, from + i) : -INFINITY;
+        }
+      }
     }
     float own = x[0];
 #pragma unroll
-    for (int i = 1; i < kLaneLogits; ++i) own = fmaxf(own, x[i]);
+    for (int i = 1; i < kOwn; ++i) own = fmaxf(own, x[i]);
     const float now = fmaxf(top, own);
-    float part = 0.f;
-#pragma unroll
-    for (int i = 0; i < kLaneLogits; ++i) part += __builtin_amdgcn_exp2f((x[i] - now) * kLog2E);
-    sum = sum * __builtin_amdgcn_exp2f((top - now) * kLog2E) + part;
+    sum *= __builtin_amdgcn_exp2f((top - now) * kLog2E);
     top = now;
+    float part = 0.f;
+    if (__all(fabsf(now) < 1e6f)) {
+      // 2^(x log2 e - r) with one rounding, r = now log2 e rounded, and that rounding put right in the sum
+      const float r = now * kLog2E;
+#pragma unroll
+      for (int i = 0; i < kOwn; ++i) part += __builtin_amdgcn_exp2f(fmaf(x[i], kLog2E, -r));
+      part *= __builtin_amdgcn_exp2f(-fmaf(now, kLog2E, -r));
+    } else {
+      // (no logit but -inf, or values whose products with log2 e leave the range or its small steps)
+#pragma unroll
+      for (int i = 0; i < kOwn; ++i) part += __builtin_amdgcn_exp2f((x[i] - now) * kLog2E);
+    }
+    sum += part;
     // (a NaN, or infinity, which makes the row's sum NaN: every value that is not -inf is then NaN)
     own = part != part ? INFINITY : own;
-    own = max_of_32(own);
+    own = fmaxf(own, shifted<0x111, 0xF>(own));
+    own = fmaxf(own, shifted<0x112, 0xF>(own));
+    own = fmaxf(own, shifted<0x114, 0xF>(own));
+    if constexpr (kLanes == 16) own = fmaxf(own, shifted<0x118, 0xF>(own));
     const unsigned int segment = at / kSegment;
-    if (lane % 32 == 31 && segment < a.segments)
+    if (lane % kLanes == kLanes - 1 && segment < a.segments)
       a.maxima[(unsigned long long)row * a.segments + segment] = own;
   }
-  float big = top;
-#pragma unroll
-  for (int d = 1; d < kWave; d *= 2) big = fmaxf(big, __shfl_xor(big, d, kWave));
+  const float big = wave_max(top);
   sum *= __builtin_amdgcn_exp2f((top - big) * kLog2E);
 #pragma unroll
   for (int d = 1; d < kWave; d *= 2) sum += __shfl_xor(sum, d, kWave);
-  if (lane == 0) {
-    s_max[wave] = big;
-    s_sum[wave] = sum;
-  }
-  __syncthreads();
-  if (tid == 0) {
-    float m = s_max[0], l = 0.f;
-#pragma unroll
-    for (int w = 1; w < kScanThreads / kWave; ++w) m = fmaxf(m, s_max[w]);
-#pragma unroll
-    for (int w = 0; w < kScanThreads / kWave; ++w)
-      l += s_sum[w] * __builtin_amdgcn_exp2f((s_max[w] - m) * kLog2E);
-    a.sums[(unsigned long long)row * a.chunks + blockIdx.x] = make_float2(m, l);
-  }
+  if (lane == 0) a.sums[(unsigned long long)row * a.chunks + chunk] = make_float2(big, sum);
 }
 
 // Values as numbers that compare alike: NaN above all, -0 as 0, nothing as 0.
@@ -194,167 +200,270 @@ __device__ __forceinline__ double value_of(unsigned long long key) {
   return __builtin_bit_cast(double, (key >> 63) != 0 ? key & ~(1ull << 63) : ~key);
 }
 
-__device__ __forceinline__ unsigned long long wave_best(unsigned long long v) {
-#pragma unroll
-  for (int d = 1; d < kWave; d *= 2) {
-    const unsigned long long o = __shfl_xor(v, d, kWave);
-    v = o > v ? o : v;
-  }
-  return v;
+// The wave's largest.
+template <int kControl, int kRowMask>
+__device__ __forceinline__ unsigned long long larger(unsigned long long v) {
+  const int lo = (int)v, hi = (int)(v >> 32);
+  const unsigned int olo = (unsigned int)__builtin_amdgcn_update_dpp(lo, lo, kControl, kRowMask, 0xF, false);
+  const unsigned int ohi = (unsigned int)__builtin_amdgcn_update_dpp(hi, hi, kControl, kRowMask, 0xF, false);
+  const unsigned long long o = (unsigned long long)ohi << 32 | olo;
+  return o > v ? o : v;
 }
-__device__ __forceinline__ unsigned int wave_least(unsigned int v) {
-#pragma unroll
-  for (int d = 1; d < kWave; d *= 2) v = min(v, (unsigned int)__shfl_xor((int)v, d, kWave));
-  return v;
+__device__ __forceinline__ unsigned long long wave_largest(unsigned long long v) {
+  v = larger<0x111, 0xF>(v);
+  v = larger<0x112, 0xF>(v);
+  v = larger<0x114, 0xF>(v);
+  v = larger<0x118, 0xF>(v);
+  v = larger<0x142, 0xA>(v);
+  v = larger<0x143, 0xC>(v);
+  const unsigned int lo = (unsigned int)__builtin_amdgcn_readlane((int)(unsigned int)v, 63);
+  const unsigned int hi = (unsigned int)__builtin_amdgcn_readlane((int)(v >> 32), 63);
+  return (unsigned long long)hi << 32 | lo;
 }
 
-// The best of a wave's items (item t of lane l has number t * 64 + l) that are at least `least`, best
-// first and at most `most`, each given to `take(key, number)` by all lanes.
-template <typename Take>
-__device__ __forceinline__ void best_of(unsigned long long (&keys)[kItems], unsigned int most,
-                                        unsigned long long least, Take take) {
+struct Beam {
+  double lse, score;
+  bool open, ended;
+  // what a token of some logit is worth (of a beam that is not open, none)
+  __device__ __forceinline__ unsigned long long key(float logit) const {
+    return logit == -INFINITY ? key_of(-INFINITY) : key_of(((double)logit - lse) + score);
+  }
+};
+
+// The best of a wave's keys (key t of lane l has number t * 64 + l, 0: none), best first, equal ones by
+// their numbers, and at most `most`; take(key, number, n) for each, by all lanes.
+template <int kCount, typename Take>
+__device__ __forceinline__ void best_of(unsigned long long (&keys)[kCount], unsigned int most, Take take) {
   const unsigned int lane = __lane_id();
   for (unsigned int n = 0; n < most; ++n) {
-    unsigned long long own = 0;
-    unsigned int at = 0;
+    unsigned long long own = keys[0];
 #pragma unroll
-    for (int t = 0; t < kItems; ++t)
-      if (keys[t] > own) {
-        own = keys[t];
-        at = t;
-      }
-    const unsigned long long best = wave_best(own);
-    if (best == 0 || best < least) break;
-    const unsigned int number = wave_least(own == best ? at * kWave + lane : ~0u);
+    for (int t = 1; t < kCount; ++t) own = keys[t] > own ? keys[t] : own;
+    const unsigned long long best = wave_largest(own);
+    if (best == 0) break;
+    unsigned int number = ~0u;
 #pragma unroll
-    for (int t = 0; t < kItems; ++t)
+    for (int t = kCount - 1; t >= 0; --t) {
+      const unsigned long long equal = __ballot(keys[t] == best);
+      if (equal != 0) number = t * kWave + (unsigned int)__ffsll((long long)equal) - 1;
+    }
+#pragma unroll
+    for (int t = 0; t < kCount; ++t)
       if (t * kWave + lane == number) keys[t] = 0;
     take(best, number, n);
   }
 }
 
-template <typename T>
+// A bound that at least `most` of the lanes' keys reach, nearly the largest one; 0 where there are not that
+// many: bits from the top, each kept while enough lanes have no less. (18 of them, with steps of 2^-6 of a
+// value: the others would take as long and spare few of the keys.)
+__device__ __forceinline__ unsigned long long reached(unsigned long long key, unsigned int most) {
+  const unsigned int high = (unsigned int)(key >> 32);
+  unsigned int bound = 0;
+  for (unsigned int bit = 1u << 31; bit >= 1u << 14; bit >>= 1) {
+    const unsigned int count = (unsigned int)__popcll(__ballot(high >= (bound | bit)));
+    if (count < most) continue;
+    bound |= bit;
+    if (count == most) break;
+  }
+  return (unsigned long long)bound << 32;
+}
+
+// How many of a list come before (key, id).
+__device__ __forceinline__ unsigned int rank_of(const unsigned long long* keys, const unsigned int* ids,
+                                                unsigned int count, unsigned long long key, unsigned int id) {
+  unsigned int rank = 0;
+#pragma unroll 8
+  for (unsigned int j = 0; j < count; ++j) {
+    const unsigned long long k = keys[j];
+    const unsigned int i = ids[j];
+    rank += (unsigned int)(k > key) | ((unsigned int)(k == key) & (unsigned int)(i < id));
+  }
+  return rank;
+}
+
+// kItems: segments, or groups of them, that a lane holds of a row; kTokens: tokens of a group that it does.
+template <typename T, int kItems, int kTokens>
 __global__ __launch_bounds__(kPickThreads) void beam_pick(SelectArgs a) {
   constexpr int kWaves = kPickThreads / kWave;
-  __shared__ double s_lse[kMostBeams], s_score[kMostBeams];
-  __shared__ unsigned char s_state[kMostBeams];  // 0: open, 1: ended, 2: empty
-  // the beams' best segments, and then the best values of those chosen: `most` of each
+  __shared__ Beam s_beam[kMostBeams];
+  // segments that may be among the best, and then values: at most 64 of each wave, `most` of each segment
   __shared__ unsigned long long s_key[kMostCandidates * kMostCandidates];
   __shared__ unsigned int s_id[kMostCandidates * kMostCandidates];
-  __shared__ unsigned int s_chosen[kMostCandidates], s_count;
+  __shared__ unsigned long long s_bound[kWaves];
+  __shared__ unsigned int s_chosen[kMostCandidates], s_segments, s_count;
   __shared__ unsigned long long s_least;
   const unsigned int request = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
   const unsigned int row0 = request * a.beams, most = a.candidates;
-  const unsigned long long nothing = key_of(-INFINITY);
-  // segments of an item, so that a wave holds a row's
-  const unsigned int group = (a.segments + kItems * kWave - 1) / (kItems * kWave);
-  const unsigned int items = (a.segments + group - 1) / group;
-
-  for (unsigned int i = tid; i < a.beams * most; i += kPickThreads) s_key[i] = 0;
+  const unsigned int group = kTokens == kOwnTokens ? 1 : a.group, items = a.items;
+  const unsigned int units = a.beams * a.parts;  // a wave's work each
   if (tid == 0) {
-    s_count = 0;
+    s_segments = s_count = 0;
     s_least = 0;
   }
   if (tid < kMostCandidates) s_chosen[tid] = ~0u;
-  __syncthreads();
-  for (unsigned int b = wave; b < a.beams; b += kWaves) {
-    const unsigned int row = row0 + b;
-    const bool ended = is_ended(a, row), open = is_open(a, row);
-    const double score = a.scores[row];
-    double lse = 0.;
-    if (open) {
-      const float2* sums = a.sums + (unsigned long long)row * a.chunks;
-      float top = kLowest;
-      for (unsigned int c = lane; c < a.chunks; c += kWave) top = fmaxf(top, sums[c].x);
-#pragma unroll
-      for (int d = 1; d < kWave; d *= 2) top = fmaxf(top, __shfl_xor(top, d, kWave));
-      double sum = 0.;
-      for (unsigned int c = lane; c < a.chunks; c += kWave)
-        sum += (double)sums[c].y * exp((double)sums[c].x - (double)top);
-#pragma unroll
-      for (int d = 1; d < kWave; d *= 2) sum += __shfl_xor(sum, d, kWave);
-      lse = log(sum) + (double)top;
-    }
-    if (lane == 0) {
-      s_lse[b] = lse;
-      s_score[b] = score;
-      s_state[b] = ended ? 1 : open ? 0 : 2;
-    }
-    unsigned long long keys[kItems];
+
+  // A part of a beam's items as keys by their maxima.
+  auto load = [&](unsigned int unit, unsigned long long (&keys)[kItems]) {
+    const unsigned int b = unit / a.parts, row = row0 + b;
+    const unsigned int from = (unit - b * a.parts) * (kItems * kWave) + lane;
+    // (all loads go out together; what a beam that is not open has there counts for nothing)
     const float* maxima = a.maxima + (unsigned long long)row * a.segments;
+    const float2* sums = a.sums + (unsigned long long)row * a.chunks;
+    float largest[kItems];
 #pragma unroll
     for (int t = 0; t < kItems; ++t) {
-      const unsigned int item = t * kWave + lane;
-      keys[t] = 0;
-      if (item >= items) continue;
-      keys[t] = nothing;
-      if (open) {
-        float m = -INFINITY;
-        for (unsigned int s = item * group; s < min(a.segments, (item + 1) * group); ++s)
-          m = fmaxf(m, maxima[s]);
-        if (m != -INFINITY) keys[t] = key_of(((double)m - lse) + score);
-      } else if (ended && a.end_token / (kSegment * group) == item) {
-        keys[t] = key_of(score);
-      }
+      const unsigned int item = min(from + t * kWave, items - 1);
+      largest[t] = maxima[item * group];
+      for (unsigned int s = item * group + 1; s < min(a.segments, (item + 1) * group); ++s)
+        largest[t] = fmaxf(largest[t], maxima[s]);
     }
-    best_of(keys, most, 0, [&](unsigned long long key, unsigned int number, unsigned int n) {
-      if (lane == 0) {
-        s_key[b * most + n] = key;
-        s_id[b * most + n] = b * items + number;
+    const float2 none = make_float2(kLowest, 0.f);
+    const float2 own = lane < a.chunks ? sums[lane] : none;
+    Beam beam{0., a.scores[row], is_open(a, row), is_ended(a, row)};
+    float top = own.x;
+    for (unsigned int c = lane + kWave; c < a.chunks; c += kWave) top = fmaxf(top, sums[c].x);
+    top = wave_max(top);
+    double sum = own.y * __builtin_amdgcn_exp2f((own.x - top) * kLog2E);
+    for (unsigned int c = lane + kWave; c < a.chunks; c += kWave)
+      sum += sums[c].y * __builtin_amdgcn_exp2f((sums[c].x - top) * kLog2E);
+#pragma unroll
+    for (int d = 1; d < kWave; d *= 2) sum += __shfl_xor(sum, d, kWave);
+    beam.lse = log(sum) + (double)top;
+#pragma unroll
+    for (int t = 0; t < kItems; ++t) largest[t] = beam.open ? largest[t] : -INFINITY;
+    if (lane == 0) s_beam[b] = beam;
+#pragma unroll
+    for (int t = 0; t < kItems; ++t) {
+      const unsigned int item = from + t * kWave;
+      keys[t] = beam.key(largest[t]);
+      if (beam.ended && a.end_token / (kSegment * group) == item) keys[t] = key_of(beam.score);
+      if (item >= items) keys[t] = 0;
+    }
+  };
+  // The items that may be among the best: those that no part has `most` above. Where one has too many, its
+  // best `most`.
+  auto offer = [&](unsigned int unit, unsigned long long (&keys)[kItems], unsigned long long least) {
+    const unsigned int b = unit / a.parts, id0 = b * items + (unit - b * a.parts) * (kItems * kWave);
+    unsigned int count = 0;
+#pragma unroll
+    for (int t = 0; t < kItems; ++t) {
+      if (keys[t] < least) keys[t] = 0;
+      count += (unsigned int)__popcll(__ballot(keys[t] != 0));
+    }
+    if (count == 0) return;
+    unsigned int at = 0;
+    if (lane == 0) at = atomicAdd(&s_segments, count > kMostCandidates ? min(count, most) : count);
+    at = uniform(at);
+    if (count <= kMostCandidates) {
+#pragma unroll
+      for (int t = 0; t < kItems; ++t) {
+        const unsigned long long mask = __ballot(keys[t] != 0);
+        if (keys[t] != 0) {
+          const unsigned int to = at + (unsigned int)__popcll(mask & ((1ull << lane) - 1));
+          s_key[to] = keys[t];
+          s_id[to] = id0 + t * kWave + lane;
+        }
+        at += (unsigned int)__popcll(mask);
       }
-    });
+    } else {
+      best_of(keys, most, [&](unsigned long long key, unsigned int number, unsigned int n) {
+        if (lane == 0) {
+          s_key[at + n] = key;
+          s_id[at + n] = id0 + number;
+        }
+      });
+    }
+  };
+  auto largest_of = [&](const unsigned long long (&keys)[kItems]) {
+    unsigned long long own = keys[0];
+#pragma unroll
+    for (int t = 1; t < kItems; ++t) own = keys[t] > own ? keys[t] : own;
+    return own;
+  };
+  // (a wave's first stays in its registers, any others are loaded again: more than 16 beams are rare)
+  unsigned long long keys0[kItems], bound = 0;
+  for (unsigned int u = wave; u < units; u += kWaves) {
+    unsigned long long keys[kItems];
+    load(u, keys);
+    bound = max(bound, reached(largest_of(keys), most));
+    if (u == wave) {
+#pragma unroll
+      for (int t = 0; t < kItems; ++t) keys0[t] = keys[t];
+    }
+  }
+  if (lane == 0) s_bound[wave] = bound;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) bound = max(bound, s_bound[w]);
+  for (unsigned int u = wave; u < units; u += kWaves) {
+    if (u == wave) {
+      offer(u, keys0, bound);
+    } else {
+      unsigned long long keys[kItems];
+      load(u, keys);
+      offer(u, keys, bound);
+    }
   }
   __syncthreads();
-  // the best `most` of the beams' best segments
-  for (unsigned int i = tid; i < a.beams * most; i += kPickThreads) {
+  // the best `most` of those
+  const unsigned int all = s_segments;
+  for (unsigned int i = tid; i < all; i += kPickThreads) {
     const unsigned long long key = s_key[i];
-    if (key == 0) continue;
-    const unsigned int id = s_id[i];
-    unsigned int rank = 0;
-    for (unsigned int j = 0; j < a.beams * most; ++j)
-      rank += s_key[j] > key || (s_key[j] == key && s_id[j] < id) ? 1u : 0u;
-    if (rank < most) s_chosen[rank] = id;
+    const unsigned int id = s_id[i], rank = rank_of(s_key, s_id, all, key, id);
+    if (rank >= most) continue;
+    s_chosen[rank] = id;
     if (rank == most - 1) s_least = key;
   }
   __syncthreads();
+  // their values that are no less than the last one's, into a list
   const unsigned long long least = s_least;
   for (unsigned int c = wave; c < most; c += kWaves) {
     const unsigned int id = s_chosen[c];
     if (id == ~0u) continue;
     const unsigned int b = id / items, first = (id - b * items) * group * kSegment;
-    const double lse = s_lse[b], score = s_score[b];
-    const unsigned int state = s_state[b];
+    const Beam beam = s_beam[b];
     const unsigned char* src = row_of<T>(a, row0 + b);
-    unsigned long long keys[kItems];
+    unsigned long long keys[kTokens], masks[kTokens];
+    unsigned int count = 0;
 #pragma unroll
-    for (int t = 0; t < kItems; ++t) {
+    for (int t = 0; t < kTokens; ++t) {
       const unsigned int in = t * kWave + lane, token = first + in;
-      keys[t] = 0;
-      if (in >= group * kSegment || token >= a.vocab) continue;
-      keys[t] = nothing;
-      if (state == 0) {
-        const float x = T::one(src, token);
-        if (x != -INFINITY) keys[t] = key_of(((double)x - lse) + score);
-      } else if (state == 1 && token == a.end_token) {
-        keys[t] = key_of(score);
-      }
+      const bool there = in < group * kSegment && token < a.vocab;
+      keys[t] = beam.key(beam.open && there ? T::one(src, token) : -INFINITY);
+      if (beam.ended && token == a.end_token) keys[t] = key_of(beam.score);
+      if (!there || keys[t] < least) keys[t] = 0;
+      masks[t] = __ballot(keys[t] != 0);
+      count += (unsigned int)__popcll(masks[t]);
     }
-    best_of(keys, most, least, [&](unsigned long long key, unsigned int number, unsigned int) {
-      if (lane == 0) {
-        const unsigned int at = atomicAdd(&s_count, 1u);
-        s_key[at] = key;
-        s_id[at] = b * a.vocab + first + number;
+    unsigned int at = 0;
+    if (lane == 0) at = atomicAdd(&s_count, min(count, most));
+    at = uniform(at);
+    if (count <= most) {
+#pragma unroll
+      for (int t = 0; t < kTokens; ++t) {
+        if (keys[t] != 0) {
+          const unsigned int to = at + (unsigned int)__popcll(masks[t] & ((1ull << lane) - 1));
+          s_key[to] = keys[t];
+          s_id[to] = b * a.vocab + first + t * kWave + lane;
+        }
+        at += (unsigned int)__popcll(masks[t]);
       }
-    });
+    } else {
+      best_of(keys, most, [&](unsigned long long key, unsigned int number, unsigned int n) {
+        if (lane == 0) {
+          s_key[at + n] = key;
+          s_id[at + n] = b * a.vocab + first + number;
+        }
+      });
+    }
   }
   __syncthreads();
   const unsigned int count = s_count;
   for (unsigned int i = tid; i < count; i += kPickThreads) {
     const unsigned long long key = s_key[i];
     const unsigned int id = s_id[i];
-    unsigned int rank = 0;
-    for (unsigned int j = 0; j < count; ++j)
-      rank += s_key[j] > key || (s_key[j] == key && s_id[j] < id) ? 1u : 0u;
+    const unsigned int rank = rank_of(s_key, s_id, count, key, id);
     if (rank >= most) continue;
     const unsigned long long to = (unsigned long long)request * most + rank;
     const unsigned int b = id / a.vocab;
@@ -557,13 +666,20 @@ using namespace unchainkv;
 
 namespace {
 
-// Chunks of a row and their rounds: as many rounds as leave the chip enough workgroups.
-void scan_shape(unsigned long long rows, SelectArgs& a) {
-  const unsigned int all = (a.vocab + kRound - 1) / kRound;
-  a.rounds = 1;
-  while (a.rounds < 8 && rows * ((all + 2 * a.rounds - 1) / (2 * a.rounds)) >= 2048) a.rounds *= 2;
+// Chunks of a row, a wave's each, of one round or, in calls that fill the chip many times over, two (64
+// requests of 8 beams, 131072 logits in bf16: 23.0 us with two, 24.6 with one, 25.8 with four). A row of more
+// segments than a wave's lanes hold is searched by several, as far as there are waves.
+void shape(unsigned long long rows, unsigned long long dtype, SelectArgs& a) {
+  const unsigned int round = kWave * kLaneBytes / (dtype == 2 ? 4 : 2);
+  const unsigned int all = (a.vocab + round - 1) / round;
+  a.rounds = rows * all >= 16384 ? 2 : 1;
   a.chunks = (all + a.rounds - 1) / a.rounds;
   a.segments = (a.vocab + kSegment - 1) / kSegment;
+  a.parts = 1;
+  while (2 * a.parts * a.beams <= kPickThreads / kWave && a.segments > kMostItems * kWave * a.parts) a.parts *= 2;
+  const unsigned int lanes = a.parts * kWave;
+  a.group = (a.segments + kMostItems * lanes - 1) / (kMostItems * lanes);
+  a.items = (a.segments + a.group - 1) / a.group;
 }
 
 bool select_ok(unsigned long long requests, unsigned long long beams, unsigned long long vocab,
@@ -573,8 +689,31 @@ bool select_ok(unsigned long long requests, unsigned long long beams, unsigned l
          requests * beams <= 65535;
 }
 
-unsigned long long maxima_bytes(unsigned long long rows, const SelectArgs& a) {
-  return (4 * rows * a.segments + 15) / 16 * 16;
+// Every row's maxima, then sums of as many chunks as it can have (f32, one round each): more for more rows or
+// tokens, whatever their type.
+unsigned long long maxima_bytes(unsigned long long rows, unsigned long long vocab) {
+  return (4 * rows * ((vocab + kSegment - 1) / kSegment) + 15) / 16 * 16;
+}
+unsigned long long select_bytes(unsigned long long rows, unsigned long long vocab) {
+  constexpr unsigned long long kLeast = kWave * kLaneLogits<Fp32>;
+  return maxima_bytes(rows, vocab) + sizeof(float2) * rows * ((vocab + kLeast - 1) / kLeast);
+}
+
+// As few registers as hold a row's items.
+template <typename T>
+void launch_pick(const SelectArgs& a, hipStream_t stream) {
+  const dim3 grid(a.requests), threads(kPickThreads);
+  const unsigned int held = (a.items + a.parts * kWave - 1) / (a.parts * kWave);
+  if (held <= 2)
+    hipLaunchKernelGGL((beam_pick<T, 2, kOwnTokens>), grid, threads, 0, stream, a);
+  else if (held <= 4)
+    hipLaunchKernelGGL((beam_pick<T, 4, kOwnTokens>), grid, threads, 0, stream, a);
+  else if (a.group == 1)
+    hipLaunchKernelGGL((beam_pick<T, kMostItems, kOwnTokens>), grid, threads, 0, stream, a);
+  else if (a.group == 2)
+    hipLaunchKernelGGL((beam_pick<T, kMostItems, 2 * kOwnTokens>), grid, threads, 0, stream, a);
+  else
+    hipLaunchKernelGGL((beam_pick<T, kMostItems, 8 * kOwnTokens>), grid, threads, 0, stream, a);
 }
 
 unsigned int chunks_of(unsigned long long width) {
@@ -591,10 +730,7 @@ extern "C" unsigned long long kvq_splitzip_beam_select_workspace_bytes(unsigned 
                                                                        unsigned long long beams,
                                                                        unsigned long long vocab) {
   if (!select_ok(requests, beams, vocab, 1)) return 0;
-  SelectArgs a{};
-  a.vocab = (unsigned int)vocab;
-  scan_shape(requests * beams, a);
-  return maxima_bytes(requests * beams, a) + 8 * requests * beams * a.chunks;
+  return select_bytes(requests * beams, vocab);
 }
 
 extern "C" long long kvq_splitzip_beam_select(
@@ -610,11 +746,7 @@ extern "C" long long kvq_splitzip_beam_select(
       out_scores_ptr == 0 || out_parents_ptr == 0 || out_tokens_ptr == 0 || workspace_ptr == 0 ||
       workspace_ptr % 16 != 0)
     return 0;
-  SelectArgs a{};
-  a.vocab = (unsigned int)vocab;
-  const unsigned long long rows = requests * beams;
-  scan_shape(rows, a);
-  const unsigned long long need = maxima_bytes(rows, a) + 8 * rows * a.chunks;
+  const unsigned long long rows = requests * beams, need = select_bytes(rows, vocab);
   if (workspace_bytes < need) return 0;
   const unsigned long long picked = requests * candidates;
   const unsigned long long in[][2] = {
@@ -628,22 +760,26 @@ extern "C" long long kvq_splitzip_beam_select(
     for (const auto& p : out)
       if (&o != &p && overlap(o[0], o[1], p[0], p[1])) return 0;
   }
+  SelectArgs a{};
+  a.vocab = (unsigned int)vocab;
+  a.beams = (unsigned int)beams;
+  shape(rows, dtype, a);
   a.logits = reinterpret_cast<const unsigned char*>(logits_ptr);
   a.scores = reinterpret_cast<const float*>(scores_ptr);
   a.ended = reinterpret_cast<const unsigned char*>(ended_ptr);
   a.maxima = reinterpret_cast<float*>(workspace_ptr);
-  a.sums = reinterpret_cast<float2*>(workspace_ptr + maxima_bytes(rows, a));
+  a.sums = reinterpret_cast<float2*>(workspace_ptr + maxima_bytes(rows, vocab));
   a.out_scores = reinterpret_cast<float*>(out_scores_ptr);
   a.out_parents = reinterpret_cast<int*>(out_parents_ptr);
   a.out_tokens = reinterpret_cast<long long*>(out_tokens_ptr);
   a.request_stride = request_stride;
   a.beam_stride = beam_stride;
   a.requests = (unsigned int)requests;
-  a.beams = (unsigned int)beams;
   a.candidates = (unsigned int)candidates;
   a.end_token = (unsigned int)end_token;
   hipStream_t stream = reinterpret_cast<hipStream_t>(stream_ptr);
-  const dim3 grid(a.chunks, (unsigned int)rows);
+  constexpr unsigned int kChunks = kScanThreads / kWave;  // of a workgroup
+  const dim3 grid((a.chunks + kChunks - 1) / kChunks, (unsigned int)rows);
   if (dtype == 0)
     hipLaunchKernelGGL(beam_scan<Bf16>, grid, dim3(kScanThreads), 0, stream, a);
   else if (dtype == 1)
@@ -652,13 +788,12 @@ extern "C" long long kvq_splitzip_beam_select(
     hipLaunchKernelGGL(beam_scan<Fp32>, grid, dim3(kScanThreads), 0, stream, a);
   hipError_t st = hipGetLastError();
   if (st != hipSuccess) return fail("beam_scan", st);
-  const dim3 picks(a.requests);
   if (dtype == 0)
-    hipLaunchKernelGGL(beam_pick<Bf16>, picks, dim3(kPickThreads), 0, stream, a);
+    launch_pick<Bf16>(a, stream);
   else if (dtype == 1)
-    hipLaunchKernelGGL(beam_pick<Fp16>, picks, dim3(kPickThreads), 0, stream, a);
+    launch_pick<Fp16>(a, stream);
   else
-    hipLaunchKernelGGL(beam_pick<Fp32>, picks, dim3(kPickThreads), 0, stream, a);
+    launch_pick<Fp32>(a, stream);
   st = hipGetLastError();
   if (st != hipSuccess) return fail("beam_pick", st);
   return (long long)picked;
