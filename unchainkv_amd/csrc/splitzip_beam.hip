@@ -476,6 +476,7 @@ __global__ __launch_bounds__(kPickThreads) void beam_pick(SelectArgs a) {
 // ---------------------------------------------------------------------------
 
 constexpr int kOrderThreads = 256;  // columns of a workgroup
+constexpr int kOrderWaves = kOrderThreads / kWave;
 constexpr int kMostLayers = 64;     // of a launch
 
 struct OrderArgs {
@@ -489,108 +490,139 @@ struct OrderArgs {
   int* free_next;
   int* lacking;
   int* unlisted;
+  int4* copies;                    // [requests * beams]: block, its copy, tokens; none: -1
   int2* counts;                    // [requests][chunks]: (released, lacking) of a workgroup's columns
-  int* released;                   // [requests][chunks][beams * kOrderThreads]
+  int* released;                   // [requests][chunks][beams * (kOrderThreads + 1)]
   unsigned long long table_stride, out_stride;
   unsigned int requests, beams, width, chunks, block_tokens, free_count;
+  Divider by_block;
 };
 
-__global__ __launch_bounds__(kOrderThreads) void order_tables(OrderArgs a) {
-  extern __shared__ int s_entry[];  // [beams][kOrderThreads]: a thread's column
-  __shared__ int s_parent[kMostBeams];
-  __shared__ unsigned int s_wave[kOrderThreads / kWave];
-  const unsigned int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const unsigned int request = blockIdx.y, beams = a.beams, row0 = request * beams;
-  const unsigned int column = blockIdx.x * kOrderThreads + tid;
-  if (tid < beams) s_parent[tid] = a.parents[row0 + tid];
-  __syncthreads();
-  unsigned long long with_child = 0;
-  unsigned int orphans = 0;
-  for (unsigned int j = 0; j < beams; ++j) {
-    const unsigned int p = (unsigned int)s_parent[j];
-    if (p < beams)
-      with_child |= 1ull << p;
-    else
-      ++orphans;
-  }
-  const unsigned int context = (unsigned int)max(a.contexts[row0], 0);
-  const unsigned int full = context / a.block_tokens;
-  const bool partly = context != full * a.block_tokens;
-  const bool in = column < a.width;
-  unsigned long long released = 0;  // the beams whose entry of this column is
-  unsigned int lacking = 0;
-  int* const own = s_entry + tid;
-  if (in)
-    for (unsigned int b = 0; b < beams; ++b)
-      own[b * kOrderThreads] = a.tables[(row0 + b) * a.table_stride + column];
-  if (in && (column < full || (partly && column == full))) {
-    const bool tail = column == full;
-    // entries that beams without children leave: those of no other beam that has one, once each
-    unsigned long long left = 0;
-    for (unsigned int b = 0; b < beams; ++b) {
-      if ((with_child >> b & 1) != 0 || own[b * kOrderThreads] < 0) continue;
-      bool again = false;
-      for (unsigned int c = 0; c < beams; ++c)
-        again |= own[c * kOrderThreads] == own[b * kOrderThreads] && (c < b || (with_child >> c & 1) != 0);
-      if (!again) left |= 1ull << b;
-    }
-    for (unsigned int j = 0; j < beams; ++j) {
-      const unsigned int p = (unsigned int)s_parent[j];
-      int id = p < beams ? own[p * kOrderThreads] : -1, from = -1;
-      if (tail && id >= 0) {
-        bool taken = false;
-        for (unsigned int i = 0; i < j; ++i) {
-          const unsigned int q = (unsigned int)s_parent[i];
-          taken |= q < beams && own[q * kOrderThreads] == id;
-        }
-        if (taken) {
-          from = id;
-          id = -1;
-          if (left != 0) {
-            const int b = __ffsll((long long)left) - 1;
-            left &= left - 1;
-            id = own[b * kOrderThreads];
-          }
-        }
-      }
-      if (tail && p < beams && id < 0) ++lacking;
-      if (tail) a.copied_from[row0 + j] = id >= 0 ? from : -1;
-      a.out[(row0 + j) * a.out_stride + column] = id;
-    }
-    released = left;
-  } else if (in) {
-    for (unsigned int b = 0; b < beams; ++b)
-      a.out[(row0 + b) * a.out_stride + column] = own[b * kOrderThreads];
-  }
-  // no block to be copied: whole blocks only, or a table that ends before the last one
-  if (blockIdx.x == 0 && tid < beams && (!partly || full >= a.width)) a.copied_from[row0 + tid] = -1;
-  if (column == 0) lacking += orphans;
-
-  // this workgroup's released blocks in the order of columns, then beams
-  const unsigned int count = (unsigned int)__popcll(released);
-  unsigned int scan = count;
+// Exclusive sum over the workgroup, and the whole.
+__device__ __forceinline__ unsigned int group_scan(unsigned int v, unsigned int* space, unsigned int& all) {
+  const unsigned int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  unsigned int scan = v;
 #pragma unroll
   for (int d = 1; d < kWave; d *= 2) {
     const unsigned int o = (unsigned int)__shfl_up((int)scan, d, kWave);
     if (lane >= (unsigned int)d) scan += o;
   }
-  __shared__ unsigned int s_lacking;
-  if (tid == 0) s_lacking = 0;
-  if (lane == 63) s_wave[wave] = scan;
+  if (lane == 63) space[wave] = scan;
   __syncthreads();
-  if (lacking != 0) atomicAdd(&s_lacking, lacking);
-  unsigned int at = scan - count, all = 0;
+  unsigned int at = scan - v;
+  all = 0;
 #pragma unroll
-  for (unsigned int w = 0; w < kOrderThreads / kWave; ++w) {
-    if (w < wave) at += s_wave[w];
-    all += s_wave[w];
+  for (unsigned int w = 0; w < kOrderWaves; ++w) {
+    if (w < wave) at += space[w];
+    all += space[w];
+  }
+  return at;
+}
+
+__global__ __launch_bounds__(kOrderThreads) void order_tables(OrderArgs a) {
+  extern __shared__ int s_entry[];  // [beams][kOrderThreads]: a thread's column
+  __shared__ int s_parent[kMostBeams], s_spare[kMostBeams];
+  __shared__ unsigned int s_wave[kOrderWaves], s_lacking, s_left;
+  const unsigned int tid = threadIdx.x, lane = tid & 63;
+  const unsigned int request = blockIdx.y, beams = a.beams, row0 = request * beams;
+  const unsigned int column = blockIdx.x * kOrderThreads + tid;
+  const unsigned int context = (unsigned int)max(a.contexts[row0], 0);
+  const unsigned int full = div_u32(context, a.by_block.m, a.by_block.d);
+  const unsigned int rest = context - full * a.block_tokens;
+  // whether this workgroup has the last, partly filled block's column
+  const bool tail = rest != 0 && full < a.width && full / kOrderThreads == blockIdx.x;
+  if (tid < beams) s_parent[tid] = a.parents[row0 + tid];
+  if (tid == 0) s_lacking = s_left = 0;
+  int* const own = s_entry + tid;
+  const bool there = column < a.width && (column < full || a.out != a.tables) && !(tail && column == full);
+  bool same = true;
+  if (there) {
+    int first = 0;
+#pragma unroll 4
+    for (unsigned int b = 0; b < beams; ++b) {
+      const int id = a.tables[(row0 + b) * a.table_stride + column];
+      own[b * kOrderThreads] = id;
+      first = b == 0 ? id : first;
+      same &= id == first;
+    }
+  }
+  __syncthreads();
+  const bool known = lane < beams && (unsigned int)s_parent[lane] < beams;
+  unsigned int with_child = 0;  // beams that have one
+  for (unsigned int j = 0; j < beams; ++j) {
+    const unsigned int p = (unsigned int)s_parent[j];
+    if (p < beams) with_child |= 1u << p;
+  }
+  const unsigned int orphans = beams - (unsigned int)__popcll(__ballot(known));
+
+  unsigned int released = 0;  // the beams whose entry of this column is
+  if (there) {
+    const bool held = column < full;
+    for (unsigned int j = 0; j < beams; ++j) {
+      const unsigned int p = held ? (unsigned int)s_parent[j] : j;
+      a.out[(row0 + j) * a.out_stride + column] = p < beams ? own[p * kOrderThreads] : -1;
+    }
+    if (held && (!same || with_child == 0)) {
+      // entries of beams without children that no other beam with one has, once each
+      for (unsigned int b = 0; b < beams; ++b) {
+        const int id = own[b * kOrderThreads];
+        if ((with_child >> b & 1) != 0 || id < 0) continue;
+        bool again = false;
+        for (unsigned int c = 0; c < beams; ++c)
+          again |= own[c * kOrderThreads] == id && (c < b || (with_child >> c & 1) != 0);
+        if (!again) released |= 1u << b;
+      }
+    }
   }
   const unsigned int group = request * a.chunks + blockIdx.x;
-  int* dst = a.released + (unsigned long long)group * (beams * kOrderThreads);
-  for (; released != 0; released &= released - 1)
-    dst[at++] = own[(__ffsll((long long)released) - 1) * kOrderThreads];
+  int* const list = a.released + (unsigned long long)group * (beams * (kOrderThreads + 1));
+  unsigned int all;
+  unsigned int at = group_scan((unsigned int)__popc(released), s_wave, all);
+  for (; released != 0; released &= released - 1) list[at++] = own[(__ffs((int)released) - 1) * kOrderThreads];
+
+  // The last blocks, by one wave, a lane for each beam: the first child of a block keeps it, the others take
+  // those that no child has, in order.
+  if (tid < kWave && tail) {
+    const int id = lane < beams ? a.tables[(row0 + lane) * a.table_stride + full] : -1;
+    const int parent = known ? s_parent[lane] : 0;
+    const int source = __shfl(id, parent, kWave);
+    bool taken = false, used = false, again = false;
+    for (unsigned int j = 0; j < beams; ++j) {
+      const bool child = __shfl(known ? 1 : 0, (int)j, kWave) != 0;
+      const int its = __shfl(source, (int)j, kWave), other = __shfl(id, (int)j, kWave);
+      taken |= child && j < lane && its == source;
+      used |= child && its == id;
+      again |= j < lane && other == id;
+    }
+    const bool moves = known && source >= 0 && taken, spare = lane < beams && id >= 0 && !used && !again;
+    const unsigned long long below = (1ull << lane) - 1, movers = __ballot(moves), spares = __ballot(spare);
+    if (spare) s_spare[__popcll(spares & below)] = id;
+    asm volatile("" ::: "memory");  // (one wave: its LDS accesses are in order)
+    const unsigned int turn = (unsigned int)__popcll(movers & below), count = (unsigned int)__popcll(spares);
+    int to = known ? source : -1;
+    if (moves) to = turn < count ? s_spare[turn] : -1;
+    const bool copied = moves && to >= 0;
+    const unsigned int without = (unsigned int)__popcll(__ballot(known && to < 0));
+    if (lane < beams) {
+      a.out[(row0 + lane) * a.out_stride + full] = to;
+      a.copied_from[row0 + lane] = copied ? source : -1;
+      a.copies[row0 + lane] = make_int4(copied ? source : -1, to, (int)rest, 0);
+    }
+    const unsigned int taking = min((unsigned int)__popcll(movers), count);
+    const unsigned int rank = (unsigned int)__popcll(spares & below);
+    if (spare && rank >= taking) list[all + rank - taking] = id;
+    if (lane == 0) {
+      s_lacking = without;
+      s_left = count - taking;
+    }
+  } else if (blockIdx.x == 0 && tid < beams && (rest == 0 || full >= a.width)) {
+    // no block to be copied: whole blocks only, or a table that ends before the last one
+    a.copied_from[row0 + tid] = -1;
+    a.copies[row0 + tid] = make_int4(-1, -1, 0, 0);
+  }
   __syncthreads();
-  if (tid == 0) a.counts[group] = make_int2((int)all, (int)s_lacking);
+  if (tid == 0)
+    a.counts[group] = make_int2((int)(all + s_left), (int)(s_lacking + (blockIdx.x == 0 ? orphans : 0u)));
 }
 
 struct CopyArgs {
@@ -603,37 +635,32 @@ struct CopyArgs {
 
 // The released blocks of all workgroups of order_tables, in order, below the list's first free entry.
 __device__ __forceinline__ void list_released(const OrderArgs& a) {
-  __shared__ unsigned long long s_sum[2][kOrderThreads];
+  __shared__ unsigned int s_wave[2][kOrderWaves];
   const unsigned int tid = threadIdx.x;
   const unsigned int groups = a.requests * a.chunks;
   const unsigned int share = (groups + kOrderThreads - 1) / kOrderThreads;
   const unsigned int g0 = min(groups, tid * share), g1 = min(groups, g0 + share);
-  unsigned long long own = 0, lacking = 0;
-  for (unsigned int g = g0; g < g1; ++g) {
-    own += (unsigned int)a.counts[g].x;
-    lacking += (unsigned int)a.counts[g].y;
-  }
-  s_sum[0][tid] = own;
-  s_sum[1][tid] = lacking;
-  __syncthreads();
-  unsigned long long before = 0, all = 0, all_lacking = 0;
-  for (unsigned int t = 0; t < kOrderThreads; ++t) {
-    if (t < tid) before += s_sum[0][t];
-    all += s_sum[0][t];
-    all_lacking += s_sum[1][t];
-  }
   const long long start = min(max(a.free_start[0], 0), (int)a.free_count);
-  long long at = start - (long long)(all - before);
+  unsigned int own = 0, lacking = 0;
   for (unsigned int g = g0; g < g1; ++g) {
+    const int2 c = a.counts[g];
+    own += (unsigned int)c.x;
+    lacking += (unsigned int)c.y;
+  }
+  unsigned int all, all_lacking;
+  const unsigned int before = group_scan(own, s_wave[0], all);
+  group_scan(lacking, s_wave[1], all_lacking);
+  long long at = start - (long long)(all - before);
+  for (unsigned int g = g0; own != 0 && g < g1; ++g) {
     const unsigned int count = (unsigned int)a.counts[g].x;
-    const int* src = a.released + (unsigned long long)g * (a.beams * kOrderThreads);
+    const int* src = a.released + (unsigned long long)g * (a.beams * (kOrderThreads + 1));
     for (unsigned int i = 0; i < count; ++i, ++at)
       if (at >= 0) a.free_blocks[at] = src[i];
   }
   if (tid == 0) {
     a.free_next[0] = (int)max(start - (long long)all, 0ll);
     a.unlisted[0] = (int)max((long long)all - start, 0ll);
-    a.lacking[0] = (int)min(all_lacking, 0x7FFFFFFFull);
+    a.lacking[0] = (int)all_lacking;
   }
 }
 
@@ -646,17 +673,21 @@ __global__ __launch_bounds__(kOrderThreads) void copy_tails(CopyArgs a) {
   }
   const unsigned int planes = 2 * a.layers;
   const unsigned int row = blockIdx.x / planes, plane = blockIdx.x - row * planes;
-  const int from = a.o.copied_from[row];
-  if ((unsigned int)from >= a.blocks) return;
-  const unsigned int context = (unsigned int)max(a.o.contexts[row / a.o.beams * a.o.beams], 0);
-  const unsigned int column = context / a.o.block_tokens, tokens = context - column * a.o.block_tokens;
-  const int to = a.o.out[row * a.o.out_stride + column];
-  if ((unsigned int)to >= a.blocks) return;
+  const int4 copy = a.o.copies[row];
+  if ((unsigned int)copy.x >= a.blocks || (unsigned int)copy.y >= a.blocks) return;
   unsigned char* base = a.layer[plane / 2] + (plane % 2) * (a.blocks * a.block_bytes);
-  const U* src = reinterpret_cast<const U*>(base + (unsigned int)from * a.block_bytes);
-  U* dst = reinterpret_cast<U*>(base + (unsigned int)to * a.block_bytes);
-  const unsigned long long units = tokens * a.row_bytes / sizeof(U);
-  for (unsigned long long i = threadIdx.x; i < units; i += kOrderThreads) dst[i] = src[i];
+  const U* src = reinterpret_cast<const U*>(base + (unsigned int)copy.x * a.block_bytes);
+  U* dst = reinterpret_cast<U*>(base + (unsigned int)copy.y * a.block_bytes);
+  const unsigned int units = (unsigned int)((unsigned int)copy.z * a.row_bytes / sizeof(U));
+  constexpr unsigned int kAtOnce = 4;
+  for (unsigned int i = threadIdx.x; i < units; i += kAtOnce * kOrderThreads) {
+    U v[kAtOnce];
+#pragma unroll
+    for (unsigned int n = 0; n < kAtOnce; ++n) v[n] = src[min(i + n * kOrderThreads, units - 1)];
+#pragma unroll
+    for (unsigned int n = 0; n < kAtOnce; ++n)
+      if (i + n * kOrderThreads < units) dst[i + n * kOrderThreads] = v[n];
+  }
 }
 
 }  // namespace
@@ -803,7 +834,7 @@ extern "C" unsigned long long kvq_splitzip_reorder_beams_workspace_bytes(unsigne
                                                                          unsigned long long beams,
                                                                          unsigned long long width) {
   if (!order_ok(requests, beams, width)) return 0;
-  return requests * chunks_of(width) * (8 + 4 * beams * kOrderThreads);
+  return 16 * requests * beams + requests * chunks_of(width) * (8 + 4 * beams * (kOrderThreads + 1));
 }
 
 extern "C" long long kvq_splitzip_reorder_beams_paged(
@@ -819,6 +850,7 @@ extern "C" long long kvq_splitzip_reorder_beams_paged(
   if (!order_ok(requests, beams, table_width) || (layer_count != 0 && layers == nullptr) ||
       layer_count > kMost || blocks == 0 || blocks > kMost || block_tokens == 0 || block_tokens > kMost ||
       row_bytes == 0 || row_bytes % 2 != 0 || row_bytes > kMost || blocks * block_tokens > kMost ||
+      block_tokens * row_bytes > kMost || requests * beams * table_width > kMost ||
       tables_ptr == 0 || table_stride < table_width || out_ptr == 0 || out_stride < table_width ||
       parents_ptr == 0 || context_tokens_ptr == 0 || (free_blocks_ptr == 0 && free_count != 0) ||
       free_count > kMost || free_start_ptr == 0 || copied_from_ptr == 0 || free_next_ptr == 0 ||
@@ -873,8 +905,10 @@ extern "C" long long kvq_splitzip_reorder_beams_paged(
   a.chunks = chunks_of(table_width);
   a.block_tokens = (unsigned int)block_tokens;
   a.free_count = (unsigned int)free_count;
-  a.counts = reinterpret_cast<int2*>(workspace_ptr);
-  a.released = reinterpret_cast<int*>(workspace_ptr + 8 * requests * a.chunks);
+  a.by_block = make_divider(a.block_tokens);
+  a.copies = reinterpret_cast<int4*>(workspace_ptr);
+  a.counts = reinterpret_cast<int2*>(workspace_ptr + 16 * rows);
+  a.released = reinterpret_cast<int*>(a.counts + requests * a.chunks);
   hipStream_t stream = reinterpret_cast<hipStream_t>(stream_ptr);
   hipLaunchKernelGGL(order_tables, dim3(a.chunks, a.requests), dim3(kOrderThreads),
                      beams * kOrderThreads * sizeof(int), stream, a);

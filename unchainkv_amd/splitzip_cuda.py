@@ -1476,10 +1476,9 @@ def rotate_write_kv_paged(q, k, v, kv_layer, slots, positions, rotation, *,
     if dtype is None or not _rows_ok(q, q.dtype, device) or not _rows_ok(k, q.dtype, device) or \
             not _rows_ok(v, q.dtype, device) or not _kv_layer_ok(kv_layer, q.dtype, device):
         return None
-    tokens, q_heads, head_dim = q.shape
-    kv_heads = k.shape[1]
-    if k.shape != v.shape or k.shape[0] != tokens or k.shape[2] != head_dim or \
-            kv_layer.shape[3] != kv_heads or kv_layer.shape[4] != head_dim or \
+    shape, (tokens, q_heads, head_dim), (_, blocks, block_tokens, kv_heads, kv_dim) = \
+        k.shape, q.shape, kv_layer.shape
+    if shape != (tokens, kv_heads, head_dim) or v.shape != shape or kv_dim != head_dim or \
             not _index_vector_ok(slots, device, tokens, torch.int64) or \
             not _index_vector_ok(positions, device, tokens, torch.int64) or \
             rotation.dtype != torch.float32 or rotation.dim() != 2 or rotation.device != device or \
@@ -1493,12 +1492,13 @@ def rotate_write_kv_paged(q, k, v, kv_layer, slots, positions, rotation, *,
         return None
     if tokens == 0:
         return out
-    got = _call_on(device, torch, rotate, q.data_ptr(), 2 * q.stride(0), 2 * q.stride(1), q_heads,
-                   k.data_ptr(), 2 * k.stride(0), 2 * k.stride(1), v.data_ptr(), 2 * v.stride(0),
-                   2 * v.stride(1), tokens, kv_heads, head_dim, dtype, kv_layer.data_ptr(),
-                   2 * kv_layer.stride(0), kv_layer.shape[1] * kv_layer.shape[2], slots.data_ptr(),
-                   positions.data_ptr(), rotation.data_ptr(), rotation.shape[0], rotation.shape[1],
-                   1 if interleaved else 0, out.data_ptr())
+    (q_row, q_head, _), (k_row, k_head, _), (v_row, v_head, _) = q.stride(), k.stride(), v.stride()
+    places, table = blocks * block_tokens, rotation.shape
+    got = _call_on(device, torch, rotate, q.data_ptr(), 2 * q_row, 2 * q_head, q_heads,
+                   k.data_ptr(), 2 * k_row, 2 * k_head, v.data_ptr(), 2 * v_row, 2 * v_head, tokens,
+                   kv_heads, head_dim, dtype, kv_layer.data_ptr(),
+                   2 * places * kv_heads * head_dim, places, slots.data_ptr(), positions.data_ptr(),
+                   rotation.data_ptr(), table[0], table[1], 1 if interleaved else 0, out.data_ptr())
     if got < 0:
         _raise_last(lib, "splitzip rotated K/V write failed")
     if not got:
@@ -1906,7 +1906,7 @@ def beam_select(logits, scores, *, candidates: int | None = None, ended=None,
     need = lib.kvq_splitzip_beam_select_workspace_bytes(requests, beams, vocab)
     if not need:
         return None
-    if not _byte_buffer_ok(workspace, device, need, torch):
+    if workspace is None or not _byte_buffer_ok(workspace, device, need, torch):
         workspace = torch.empty(need, dtype=torch.uint8, device=device)
     got = _call_on(device, torch, select, logits.data_ptr(), dtype, logits.stride(0),
                    logits.stride(1), scores.data_ptr(), 0 if ended is None else ended.data_ptr(),
@@ -1960,6 +1960,26 @@ def reorder_beams_workspace_bytes(requests: int, beams: int, width: int) -> int:
     return need if requests else 0
 
 
+def _layer_addresses(layers: tuple, device, block_tokens: int, torch):
+    """A ctypes array of the layers' addresses, or None: layers that are not alike, or that autograd
+    follows. (A call has many layers and a microsecond for each counts, so the first alone is looked at in
+    full.)"""
+    if not layers:
+        return (ctypes.c_ulonglong * 1)()
+    dtype, shape, index = layers[0].dtype, layers[0].shape, layers[0].get_device()
+    if _row_dtype(dtype, torch) is None or not _kv_layer_ok(layers[0], dtype, device) or \
+            shape[2] != block_tokens:
+        return None
+    grad = torch.is_grad_enabled()
+    for t in layers:
+        if t.dtype is not dtype or t.shape != shape or not t.is_contiguous() or \
+                t.get_device() != index or (grad and t.requires_grad):
+            return None
+    if getattr(torch.autograd.forward_ad, "_current_level", 0) >= 0 and _tracked(torch, *layers):
+        return None
+    return (ctypes.c_ulonglong * len(layers))(*[t.data_ptr() for t in layers])
+
+
 def reorder_beams_paged(layers, tables, parents, context_tokens, free_blocks, free_start,
                         block_tokens: int, *, order: BeamOrder | None = None, workspace=None):
     """The beams' block tables, and the layers, in the order of the chosen parents: beam j of
@@ -2006,13 +2026,8 @@ def reorder_beams_paged(layers, tables, parents, context_tokens, free_blocks, fr
             not _index_vector_ok(free_blocks, device, 0, i32) or \
             not _index_vector_ok(free_start, device, 1, i32):
         return None
-    layers = list(layers)
-    for layer in layers:
-        if _row_dtype(layer.dtype, torch) is None or \
-                not _kv_layer_ok(layer, layers[0].dtype, device) or \
-                layer.shape != layers[0].shape or layer.shape[2] != block_tokens:
-            return None
-    if _tracked(torch, *layers):
+    addresses = _layer_addresses(layers := tuple(layers), device, block_tokens, torch)
+    if addresses is None:
         return None
     given = order or ()
     if order is None:
@@ -2032,12 +2047,11 @@ def reorder_beams_paged(layers, tables, parents, context_tokens, free_blocks, fr
     need = lib.kvq_splitzip_reorder_beams_workspace_bytes(requests, beams, width)
     if not need:
         return None
-    if not _byte_buffer_ok(workspace, device, need, torch):
+    if workspace is None or not _byte_buffer_ok(workspace, device, need, torch):
         workspace = torch.empty(need, dtype=torch.uint8, device=device)
     blocks = layers[0].shape[1] if layers else 1
     row_bytes = 2 * layers[0].stride(2) if layers else 2
-    pointers = (ctypes.c_ulonglong * max(len(layers), 1))(*[t.data_ptr() for t in layers])
-    got = _call_on(device, torch, reorder, pointers, len(layers), blocks, block_tokens, row_bytes,
+    got = _call_on(device, torch, reorder, addresses, len(layers), blocks, block_tokens, row_bytes,
                    tables.data_ptr(), tables.stride(0) if rows > 1 else width, width,
                    order.tables.data_ptr(), order.tables.stride(0) if rows > 1 else width,
                    parents.data_ptr(), context_tokens.data_ptr(), requests, beams,
