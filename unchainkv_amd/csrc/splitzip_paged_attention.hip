@@ -84,6 +84,10 @@ constexpr unsigned int kLeastTileSteps = 12;
 // for the host's second submission: captured 10.8 and 11.2; of 128 dims, uncut and cut, 768 tokens 13.7
 // and 16.0, 1024 the same, 1536 21.1 and 16.0).
 constexpr unsigned int kLeastFewSteps = 4, kWholeFewSteps = 8;
+// Sources are taken whole up to twice that where there are as many of them as workgroups to split for: mostly
+// they are of about one length, so that nothing would be cut (32 requests of 5 rows, 1500 tokens, 20 heads of
+// 64: 52 us, 58 with the launch that then joins nothing).
+constexpr unsigned int kWholeSourceSteps = 16;
 // A maximum before any token: the lowest float, not -inf, so that rows whose scores are all -inf
 // have weights of zero and a sum of zero (whose quotient is NaN, as the formula's).
 constexpr float kNoMax = -3.402823466e38f;
@@ -317,8 +321,8 @@ struct Work {
       sum += lane_value(wave_scan((unsigned int)min(own, (unsigned long long)kMostSteps)), 63);
     }
     const unsigned int parts = kTiles ? a.tile_target : a.few_target;
-    const unsigned int least = kTiles ? kLeastTileSteps : a.slots == 0 ? kWholeFewSteps : kLeastFewSteps;
-    if (!large && (!kTiles || a.slots != 0)) cap = max(least, share_of(sum, a.kv_heads, parts));
+    const unsigned int least = kTiles ? kLeastTileSteps : kLeastFewSteps;
+    if (!large && a.slots != 0) cap = max(least, share_of(sum, a.kv_heads, parts));
   }
 
   // The lanes' requests with the longest contexts first.
@@ -1144,11 +1148,27 @@ __device__ __forceinline__ void few_path(const AttendArgs& a, const Request& req
     }
     const x8 w = pack8<E>(e);
     const unsigned char* bv = stage + v_at;
+    if (a.causal) {
 #pragma unroll
-    for (int d = 0; d < kDimTiles; ++d) {
-      const unsigned char* src = bv + 32 * (d ^ v_x);
-      const u32x2 lo = read_transposed(src), hi = read_transposed(src + 16 * kRowBytes);
-      o[d] = Elem<E>::mma16(__builtin_bit_cast(x8, u32x4{lo.x, lo.y, hi.x, hi.y}), w, o[d]);
+      for (int d = 0; d < kDimTiles; ++d) {
+        const unsigned char* src = bv + 32 * (d ^ v_x);
+        const u32x2 lo = read_transposed(src), hi = read_transposed(src + 16 * kRowBytes);
+        o[d] = Elem<E>::mma16(__builtin_bit_cast(x8, u32x4{lo.x, lo.y, hi.x, hi.y}), w, o[d]);
+      }
+    } else {
+      // (sources: what the rounding of the weights leaves has a product of its own, on matrix units that wait
+      // for memory anyway, so that the output's rounding is the only one to its type)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) e[j] -= (float)w[j];
+      const x8 rest = pack8<E>(e);
+#pragma unroll
+      for (int d = 0; d < kDimTiles; ++d) {
+        const unsigned char* src = bv + 32 * (d ^ v_x);
+        const u32x2 lo = read_transposed(src), hi = read_transposed(src + 16 * kRowBytes);
+        const x8 v = __builtin_bit_cast(x8, u32x4{lo.x, lo.y, hi.x, hi.y});
+        o[d] = Elem<E>::mma16(v, w, o[d]);
+        o[d] = Elem<E>::mma16(v, rest, o[d]);
+      }
     }
   };
 
@@ -1465,7 +1485,7 @@ struct Plan {
 
 Plan plan_of(unsigned long long tokens, unsigned long long requests, unsigned long long kv_heads,
              unsigned long long group, unsigned long long head_dim, unsigned long long max_context,
-             unsigned long long max_query, bool paged) {
+             unsigned long long max_query, bool paged, bool causal = true) {
   Plan p{};
   p.tiles = !paged || max_query * group > kFewRows;
   // (streaming: as many as run at once; 64 requests of 128 .. 32000 tokens, 8 / 1 heads of 128: 39.8 us,
@@ -1500,7 +1520,8 @@ Plan plan_of(unsigned long long tokens, unsigned long long requests, unsigned lo
     p.items = tiles + more;
     p.groups = (p.items + (cut ? 1 : 0)) * kv_heads;
   } else {
-    const bool cut = max_context > kFewUnit * kWholeFewSteps;
+    const bool many = !causal && active * kv_heads >= p.few_target;
+    const bool cut = max_context > kFewUnit * (many ? kWholeSourceSteps : kWholeFewSteps);
     p.groups = active * kv_heads;
     if (cut) p.groups = p.slots = (p.few_target / kv_heads + active + 1) * kv_heads;
   }
@@ -1661,7 +1682,8 @@ long long attend_paged(
       !(scale > 0.f) || !std::isfinite(scale * kLog2E))
     return 0;
   const unsigned long long max_context = std::min(table_width * block_tokens, kMostRows);
-  const Plan plan = plan_of(tokens, requests, kv_heads, q_heads / kv_heads, head_dim, max_context, max_query, true);
+  const Plan plan = plan_of(tokens, requests, kv_heads, q_heads / kv_heads, head_dim, max_context, max_query, true,
+                            causal);
   const unsigned long long need = workspace_of(plan, head_dim);
   if (need != 0 && (workspace_ptr == 0 || workspace_ptr % 16 != 0 || workspace_bytes < need)) return 0;
   if (plan.groups > kMostGroups) return 0;
@@ -1821,7 +1843,8 @@ extern "C" long long kvq_splitzip_cross_attention(
       !(scale > 0.f) || !std::isfinite(scale * kLog2E))
     return 0;
   // (as over a layer: sources' lengths do not follow from the rows of q)
-  const Plan plan = plan_of(tokens, requests, kv_heads, q_heads / kv_heads, head_dim, max_source, max_query, true);
+  const Plan plan = plan_of(tokens, requests, kv_heads, q_heads / kv_heads, head_dim, max_source, max_query, true,
+                            false);
   const unsigned long long need = workspace_of(plan, head_dim);
   if (need != 0 && (workspace_ptr == 0 || workspace_ptr % 16 != 0 || workspace_bytes < need)) return 0;
   if (plan.groups > kMostGroups) return 0;
