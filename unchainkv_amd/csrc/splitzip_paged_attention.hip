@@ -1012,7 +1012,11 @@ __device__ __forceinline__ void tile_path(const AttendArgs& a, const Request& re
 // no load takes apart 16 rows: 32 requests of 8192 tokens 200 -> 196.6 us, 16 of 1024 19.2 -> 17.6, 64
 // single tokens of 500 .. 16000 and four times 8 354 -> 332. (64 dims: lane l has token l % 16, 16
 // bytes at 16 (l / 16) of every 64, each counting.)
-template <typename E, int D, int kN, int kRows, bool kPaged>
+// Of 64-dim sources (kSource: every row sees all tokens) a load takes eight whole rows: lane l has piece 4 (l
+// % 2) + l / 16 of token 16 u + 4 (l % 16 / 4) + 2 s + l / 2 % 2 for load (u, s); its product with the pieces
+// 0 .. 3 of Q counts in even rows of the result and that with 4 .. 7 in odd ones: 32 requests of 5 rows, 1500
+// tokens, 20 heads 55.5 -> 53.9 us, 64 of one row, 100 .. 16000 tokens, 32 / 8 heads 118 -> 113.
+template <typename E, int D, int kN, int kRows, bool kPaged, bool kSource>
 __device__ __forceinline__ void few_path(const AttendArgs& a, const Request& request, unsigned int split,
                                          unsigned int splits, unsigned int split_tokens, bool whole,
                                          unsigned int slot, unsigned int head, unsigned char* __restrict__ s0,
@@ -1024,7 +1028,7 @@ __device__ __forceinline__ void few_path(const AttendArgs& a, const Request& req
   constexpr int kStageBytes = kFewStep * kRowBytes;
   constexpr int kSlabs = D / 32, kDimTiles = D / 16;
   constexpr unsigned int kRound = kN * kFewStep;
-  constexpr bool kWhole = D == 128;  // rows of K are loaded whole
+  constexpr bool kWhole = D == 128, kHalves = D == 64 && kSource;  // rows of K are loaded whole
   static_assert(kStageBytes >= kFewRows * D * 4, "a wave's sums fit its stage");
 
   const unsigned int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
@@ -1074,6 +1078,12 @@ __device__ __forceinline__ void few_path(const AttendArgs& a, const Request& req
           k.v[u][j] = *reinterpret_cast<const u32x4*>(
               kb + (unsigned int)__shfl(row, 16 * u + 4 * (int)(col / 4) + j, kWave) * a.k_row + 64 * grp +
               16 * (col % 4));
+      } else if constexpr (kHalves) {
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+          k.v[u][s] = *reinterpret_cast<const u32x4*>(
+              kb + (unsigned int)__shfl(row, 16 * u + 4 * (int)(col / 4) + 2 * s + (int)(col / 2 % 2), kWave) *
+                       a.k_row + 64 * (col % 2) + 16 * grp);
       } else {
         const unsigned char* src = kb + (unsigned int)__shfl(row, 16 * u + (int)col, kWave) * a.k_row;
 #pragma unroll
@@ -1110,6 +1120,15 @@ __device__ __forceinline__ void few_path(const AttendArgs& a, const Request& req
           for (int c = 0; c < 4; ++c)
             part[c] = Elem<E>::mma16(__builtin_bit_cast(x8, k.v[u][j]), q[c], f32x4{0, 0, 0, 0});
           s[4 * u + j] = (part[0][0] + part[1][1]) + (part[2][2] + part[3][3]);
+        }
+      } else if constexpr (kHalves) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const x8 rows8 = __builtin_bit_cast(x8, k.v[u][c]);
+          const f32x4 even = Elem<E>::mma16(rows8, q[0], f32x4{0, 0, 0, 0});
+          const f32x4 odd = Elem<E>::mma16(rows8, q[1], f32x4{0, 0, 0, 0});
+          s[4 * u + 2 * c] = even[0] + odd[1];
+          s[4 * u + 2 * c + 1] = even[2] + odd[3];
         }
       } else {
         f32x4 st = {0, 0, 0, 0};
@@ -1148,7 +1167,7 @@ __device__ __forceinline__ void few_path(const AttendArgs& a, const Request& req
     }
     const x8 w = pack8<E>(e);
     const unsigned char* bv = stage + v_at;
-    if (a.causal) {
+    if (!kSource && a.causal) {
 #pragma unroll
       for (int d = 0; d < kDimTiles; ++d) {
         const unsigned char* src = bv + 32 * (d ^ v_x);
@@ -1307,7 +1326,7 @@ __global__ __launch_bounds__(kWave * tile_waves(D), D == 128 ? 2 : 3) void atten
   if constexpr (kPaged) {
     if (work.few(request.n)) {
       if (!has_slot) slot = kNoSlot;
-      few_path<E, D, kN, kRows, kPaged>(a, request, split, most, split_tokens, whole, slot, head, s0, s1, s2);
+      few_path<E, D, kN, kRows, kPaged, false>(a, request, split, most, split_tokens, whole, slot, head, s0, s1, s2);
       return;
     }
   }
@@ -1315,7 +1334,7 @@ __global__ __launch_bounds__(kWave * tile_waves(D), D == 128 ? 2 : 3) void atten
                                    s2);
 }
 
-template <typename E, int D, bool kPaged>
+template <typename E, int D, bool kPaged, bool kSource>
 __global__ __launch_bounds__(kWave * kWaves, 2) void attention_few(AttendArgs a) {
   constexpr int kBuffer = kWaves * kFewStep * 2 * D;
   __shared__ __align__(1024) unsigned char s0[kBuffer];
@@ -1331,7 +1350,7 @@ __global__ __launch_bounds__(kWave * kWaves, 2) void attention_few(AttendArgs a)
     return;
   }
   const unsigned int splits = work.splits(request);
-  few_path<E, D, kWaves, kFewRows, kPaged>(a, request, split, splits, work.split_tokens(request, splits), true,
+  few_path<E, D, kWaves, kFewRows, kPaged, kSource>(a, request, split, splits, work.split_tokens(request, splits), true,
                                    slot, head, s0, s1, s2);
 }
 
@@ -1580,7 +1599,15 @@ long long launch(const AttendArgs& a, const Plan& p, hipStream_t stream) {
     if (st != hipSuccess) return fail("attention_tiles", st);
     st = launch_merge<E, D, true>(a, stream);
   } else {
-    hipLaunchKernelGGL((attention_few<E, D, kPaged>), grid, dim3(kWave * kWaves), 0, stream, a);
+    const dim3 threads(kWave * kWaves);
+    if constexpr (kPaged) {
+      if (a.causal)
+        hipLaunchKernelGGL((attention_few<E, D, true, false>), grid, threads, 0, stream, a);
+      else
+        hipLaunchKernelGGL((attention_few<E, D, true, true>), grid, threads, 0, stream, a);
+    } else {
+      hipLaunchKernelGGL((attention_few<E, D, false, true>), grid, threads, 0, stream, a);
+    }
     st = hipGetLastError();
     if (st != hipSuccess) return fail("attention_few", st);
     st = launch_merge<E, D, false>(a, stream);
