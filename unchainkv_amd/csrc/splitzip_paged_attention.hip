@@ -1509,7 +1509,9 @@ Plan plan_of(unsigned long long tokens, unsigned long long requests, unsigned lo
   p.tiles = !paged || max_query * group > kFewRows;
   // (streaming: as many as run at once; 64 requests of 128 .. 32000 tokens, 8 / 1 heads of 128: 39.8 us,
   // with three quarters of it 41.3, with half more 44.9)
-  p.few_target = 2 * compute_units();
+  // (of 64-dim sources four run on a CU: 64 requests of 128 .. 16000 tokens, 32 / 8 heads 113 us with two, 105
+  // with four; 32 of 200 .. 16000, 8 heads 73 and 66; 8 of 8000 the same)
+  p.few_target = (head_dim == 64 && !causal ? 4 : 2) * compute_units();
   // (tiles: three quarters of the CUs, twice that with workgroups of four waves. Longer splits, so
   // fewer of them, than an even share: 16 requests of 6 tokens behind 300 .. 8000 38.0 us and 45.8, a prompt of 1443 39.3 and 52.9;
   // with a share of a fourth to a half of it 3 chunks beside 29 decodes took 402 and not 311)
@@ -1539,7 +1541,7 @@ Plan plan_of(unsigned long long tokens, unsigned long long requests, unsigned lo
     p.items = tiles + more;
     p.groups = (p.items + (cut ? 1 : 0)) * kv_heads;
   } else {
-    const bool many = !causal && active * kv_heads >= p.few_target;
+    const bool many = !causal && active * kv_heads >= 2 * compute_units();
     const bool cut = max_context > kFewUnit * (many ? kWholeSourceSteps : kWholeFewSteps);
     p.groups = active * kv_heads;
     if (cut) p.groups = p.slots = (p.few_target / kv_heads + active + 1) * kv_heads;
@@ -1570,8 +1572,11 @@ unsigned long long workspace_bound(unsigned long long tokens, unsigned long long
   }
   const unsigned long long few = std::min<unsigned long long>(max_query, kFewRows / group);
   if (few == 0) return own;
-  return std::max(own, workspace_of(plan_of(tokens, requests, kv_heads, group, head_dim, max_context, few, true),
-                                    head_dim));
+  unsigned long long most = own;
+  for (const bool causal : {true, false})
+    most = std::max(most, workspace_of(plan_of(tokens, requests, kv_heads, group, head_dim, max_context, few, true,
+                                               causal), head_dim));
+  return most;
 }
 
 template <typename E, int D, bool kTiles>
