@@ -257,111 +257,136 @@ struct RotateArgs {
   unsigned int first;          // token of this launch
   unsigned int units;          // of the pairs of a head
   unsigned int lanes_heads;    // heads that a wave's lanes take at once
+  Divider by_rest, by_head;    // units of a head that are not rotated, and all
 };
 
 constexpr unsigned int kMostRotated = 1u << 24;  // tokens of a launch, whose threads fit 32 bits
 
 template <typename E, int N>
-struct __attribute__((aligned(sizeof(E) * N))) Values {
-  E v[N];
+struct Values {
+  typedef E type __attribute__((ext_vector_type(N)));
 };
 
-// A wave for each token. A lane keeps the cosines and sines of N pairs and takes them to one head after
-// another: N values of its first half and N of its second, or (kAdjacent) 2 N values side by side.
-template <typename E, int N, bool kAdjacent>
+// Two waves for each token. In the first a lane keeps the cosines and sines of N pairs and takes them to one
+// head after another: N values of its first half and N of its second, or (kAdjacent) 2 N values side by side.
+// The second copies what is not rotated, the heads' other values and V, and waits for no position or table.
+// kBatch: heads of a lane whose loads go out together.
+template <typename E, int N, bool kAdjacent, int kBatch>
 __global__ __launch_bounds__(kStepThreads) void rotate_rows(RotateArgs a) {
-  typedef Values<E, N> Unit;
+  typedef typename Values<E, N>::type Unit;
   const unsigned int lane = threadIdx.x & 63;
-  const unsigned int token = uniform(a.first + blockIdx.x * (kStepThreads / kWave) + (threadIdx.x >> 6));
+  const unsigned int job = uniform(blockIdx.x * (kStepThreads / kWave) + (threadIdx.x >> 6));
+  const unsigned int token = a.first + job / 2;
   if (token >= a.tokens) return;
-  const long long slot = a.slots[token], position = a.positions[token];
+  const long long slot = a.slots[token];
   const bool write = slot >= 0 && (unsigned long long)slot < a.slot_count;
-  const bool known = position >= 0 && (unsigned long long)position < a.table_rows;
-  const float* const table = a.table + (known ? (unsigned long long)position * a.rotary : 0ull);
   const unsigned char* const q = a.q + token * a.q_row;
   const unsigned char* const k = a.k + token * a.k_row;
-  const unsigned char* const v = a.v + token * a.v_row;
   const unsigned int head_bytes = a.dim * sizeof(E), pairs = a.rotary / 2;
   unsigned char* const out = a.out + (unsigned long long)token * a.q_heads * head_bytes;
   unsigned char* const layer = a.layer + (write ? (unsigned long long)slot : 0ull) * a.kv_heads * head_bytes;
-  const unsigned int heads = a.q_heads + a.kv_heads;
+  // heads of Q, and then of K where the token has a place
+  const unsigned int heads = a.q_heads + (write ? a.kv_heads : 0u);
   auto source = [&](unsigned int h) {
     return h < a.q_heads ? q + h * a.q_head : k + (h - a.q_heads) * a.k_head;
   };
   auto target = [&](unsigned int h) {
     return h < a.q_heads ? out + h * head_bytes : layer + (h - a.q_heads) * head_bytes;
   };
-  const unsigned int sub = lane / min(a.units, (unsigned int)kWave);
-  for (unsigned int u = lane - sub * min(a.units, (unsigned int)kWave); u < a.units && sub < a.lanes_heads;
-       u += kWave) {
-    float c[N], s[N];
+  if (job % 2 == 0) {
+    const long long position = a.positions[token];
+    const bool known = position >= 0 && (unsigned long long)position < a.table_rows;
+    const float* const table = a.table + (known ? (unsigned long long)position * a.rotary : 0ull);
+    const unsigned int width = min(a.units, (unsigned int)kWave), sub = lane / width;
+    if (sub >= a.lanes_heads) return;
+    for (unsigned int u = lane - sub * width; u < a.units; u += kWave) {
+      const unsigned int at = (kAdjacent ? 2 * N : N) * sizeof(E) * u;
+      const unsigned int at2 = at + (kAdjacent ? N : pairs) * sizeof(E);
+      float c[N], s[N];
+      for (unsigned int h0 = sub; h0 < heads; h0 += kBatch * a.lanes_heads) {
+        // (the rows' loads go out before the table's, which wait for the position)
+        Unit x[kBatch], y[kBatch];
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      c[i] = known ? table[u * N + i] : NAN;
-      s[i] = known ? table[pairs + u * N + i] : NAN;
-    }
-    const unsigned int at = (kAdjacent ? 2 * N : N) * sizeof(E) * u;
-    const unsigned int at2 = at + (kAdjacent ? N : pairs) * sizeof(E);
-    for (unsigned int h = sub; h < heads; h += a.lanes_heads) {
-      if (h >= a.q_heads && !write) break;
-      const unsigned char* src = source(h);
-      const Unit x = *reinterpret_cast<const Unit*>(src + at), y = *reinterpret_cast<const Unit*>(src + at2);
-      Unit x2, y2;
-      if constexpr (kAdjacent) {
-        E in[2 * N], res[2 * N];
+        for (int b = 0; b < kBatch; ++b) {
+          const unsigned int h = h0 + b * a.lanes_heads;
+          const unsigned char* src = source(h < heads ? h : h0);
+          x[b] = *reinterpret_cast<const Unit*>(src + at);
+          y[b] = *reinterpret_cast<const Unit*>(src + at2);
+        }
+        if (h0 == sub) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-          in[i] = x.v[i];
-          in[N + i] = y.v[i];
+          for (int i = 0; i < N; ++i) {
+            c[i] = known ? table[u * N + i] : NAN;
+            s[i] = known ? table[pairs + u * N + i] : NAN;
+          }
         }
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-          const float p = (float)in[2 * i], r = (float)in[2 * i + 1];
-          res[2 * i] = (E)(p * c[i] - r * s[i]);
-          res[2 * i + 1] = (E)(r * c[i] + p * s[i]);
-        }
+        for (int b = 0; b < kBatch; ++b) {
+          const unsigned int h = h0 + b * a.lanes_heads;
+          if (h >= heads) continue;
+          Unit x2, y2;
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-          x2.v[i] = res[i];
-          y2.v[i] = res[N + i];
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-          const float p = (float)x.v[i], r = (float)y.v[i];
-          x2.v[i] = (E)(p * c[i] - r * s[i]);
-          y2.v[i] = (E)(r * c[i] + p * s[i]);
+          for (int i = 0; i < N; ++i) {
+            // places of the pair's values among the 2 N
+            const int first = kAdjacent ? 2 * i : i, second = kAdjacent ? 2 * i + 1 : N + i;
+            const float p = (float)(first < N ? x[b][first % N] : y[b][first % N]);
+            const float r = (float)(second < N ? x[b][second % N] : y[b][second % N]);
+            const E p2 = (E)(p * c[i] - r * s[i]), r2 = (E)(r * c[i] + p * s[i]);
+            if (first < N) x2[first % N] = p2; else y2[first % N] = p2;
+            if (second < N) x2[second % N] = r2; else y2[second % N] = r2;
+          }
+          unsigned char* dst = target(h);
+          *reinterpret_cast<Unit*>(dst + at) = x2;
+          *reinterpret_cast<Unit*>(dst + at2) = y2;
         }
       }
-      unsigned char* dst = target(h);
-      *reinterpret_cast<Unit*>(dst + at) = x2;
-      *reinterpret_cast<Unit*>(dst + at2) = y2;
     }
+    return;
   }
-  // what is not rotated
-  const unsigned int rest = (a.dim - a.rotary) / N;
-  for (unsigned int i = lane; i < rest * heads; i += kWave) {
-    const unsigned int h = i / rest, at = (a.rotary + (i - h * rest) * N) * sizeof(E);
-    if (h >= a.q_heads && !write) break;
-    *reinterpret_cast<Unit*>(target(h) + at) = *reinterpret_cast<const Unit*>(source(h) + at);
+  const unsigned char* const v = a.v + token * a.v_row;
+  const unsigned int rest = (a.dim - a.rotary) / N, head_units = a.dim / N;
+  const unsigned int others = rest * heads, all = others + (write ? head_units * a.kv_heads : 0u);
+  constexpr int kCopies = 2;
+  for (unsigned int i0 = lane; i0 < all; i0 += kCopies * kWave) {
+    Unit x[kCopies];
+    unsigned char* dst[kCopies];
+#pragma unroll
+    for (int n = 0; n < kCopies; ++n) {
+      const unsigned int i = i0 + n * kWave, use = i < all ? i : i0;
+      const bool value = use >= others;
+      const unsigned int in = value ? use - others : use;
+      const unsigned int h = div_u32(in, value ? a.by_head.m : a.by_rest.m, value ? a.by_head.d : a.by_rest.d);
+      const unsigned int at = ((value ? 0u : a.rotary) + (in - h * (value ? head_units : rest)) * N) * sizeof(E);
+      x[n] = *reinterpret_cast<const Unit*>((value ? v + h * a.v_head : source(h)) + at);
+      dst[n] = (value ? layer + a.plane_bytes + h * head_bytes : target(h)) + at;
+    }
+#pragma unroll
+    for (int n = 0; n < kCopies; ++n)
+      if (i0 + n * kWave < all) *reinterpret_cast<Unit*>(dst[n]) = x[n];
   }
-  if (!write) return;
-  const unsigned int head_units = a.dim / N;
-  for (unsigned int i = lane; i < head_units * a.kv_heads; i += kWave) {
-    const unsigned int h = i / head_units, at = (i - h * head_units) * N * sizeof(E);
-    *reinterpret_cast<Unit*>(layer + a.plane_bytes + h * head_bytes + at) =
-        *reinterpret_cast<const Unit*>(v + h * a.v_head + at);
-  }
+}
+
+// As many heads at once as a lane has, up to 5: 32768 tokens of 32 + 8 heads of 128, five of them for a lane,
+// 146 us at 5, 149 at 3, 153 at 1; 4700 of 24 + 3 heads, 32 of 64 values rotated, one for a lane, 10.8 us at 1,
+// 12.0 at 3, as places past the last head load it again.
+template <typename E, int N, bool kAdjacent>
+void launch_batch(const RotateArgs& a, hipStream_t stream) {
+  const unsigned int waves = kStepThreads / kWave, own = (a.q_heads + a.kv_heads + a.lanes_heads - 1) / a.lanes_heads;
+  const dim3 grid((2 * std::min(a.tokens - a.first, kMostRotated) + waves - 1) / waves), threads(kStepThreads);
+  if (own == 1)
+    hipLaunchKernelGGL((rotate_rows<E, N, kAdjacent, 1>), grid, threads, 0, stream, a);
+  else if (own <= 3)
+    hipLaunchKernelGGL((rotate_rows<E, N, kAdjacent, 3>), grid, threads, 0, stream, a);
+  else
+    hipLaunchKernelGGL((rotate_rows<E, N, kAdjacent, 5>), grid, threads, 0, stream, a);
 }
 
 template <typename E, bool kAdjacent>
 void launch_rotate(const RotateArgs& a, bool wide, hipStream_t stream) {
-  const unsigned int waves = kStepThreads / kWave;
-  const dim3 grid((std::min(a.tokens - a.first, kMostRotated) + waves - 1) / waves), threads(kStepThreads);
   if (wide)
-    hipLaunchKernelGGL((rotate_rows<E, 8, kAdjacent>), grid, threads, 0, stream, a);
+    launch_batch<E, 8, kAdjacent>(a, stream);
   else
-    hipLaunchKernelGGL((rotate_rows<E, 1, kAdjacent>), grid, threads, 0, stream, a);
+    launch_batch<E, 1, kAdjacent>(a, stream);
 }
 
 }  // namespace
@@ -555,6 +580,8 @@ extern "C" long long kvq_splitzip_rotate_write_kv_paged(
   a.rotary = (unsigned int)rotary_dim;
   a.units = (unsigned int)(rotary_dim / 2 / (wide ? 8 : 1));
   a.lanes_heads = std::max(1u, kWave / a.units);
+  a.by_rest = make_divider((a.dim - a.rotary) / (wide ? 8 : 1));
+  a.by_head = make_divider(a.dim / (wide ? 8 : 1));
   hipStream_t stream = reinterpret_cast<hipStream_t>(stream_ptr);
   for (unsigned long long first = 0; first < tokens; first += kMostRotated) {
     a.first = (unsigned int)first;
