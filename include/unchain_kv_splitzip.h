@@ -664,7 +664,7 @@ long long kvq_splitzip_cross_attention(
  * request_stride + b * beam_stride, vocab tokens behind each other; dtype 0: bf16, 1: fp16, 2: f32. scores
  * f32, ended_ptr 0 or u8, both [requests][beams]. A beam of score -inf and a token of logit -inf offer -inf; an
  * ended beam offers end_token at its score. NaN and +inf logits make their beam's offers NaN, which come
- * first. At most 32 beams, 64 candidates, 2^20 tokens, 65535 requests * beams. Written: out_scores f32,
+ * first. At most 32 beams, 64 candidates, 2^20 tokens and requests. Written: out_scores f32,
  * out_parents i32, out_tokens i64 [requests][candidates]. Workspace 16-byte aligned, for one call at a time.
  * Results and workspace must overlap neither an input nor each other. Returns requests * candidates, 0 on a
  * failed precondition. */

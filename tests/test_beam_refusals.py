@@ -73,7 +73,7 @@ def test_select_declines(lib):  # noqa: F811
         {name: 0} for name in ("logits", "scores", "requests", "beams", "vocab", "candidates", "out_scores",
                                "parents", "tokens", "workspace", "workspace_bytes")] + [
         {"dtype": 3}, {"beams": 33}, {"candidates": 65}, {"vocab": 1, "candidates": 4}, {"end": 1000},
-        {"vocab": (1 << 20) + 1}, {"requests": 22000}, {"logits": A[0] + 2}, {"workspace": A[6] + 8},
+        {"vocab": (1 << 20) + 1}, {"requests": (1 << 20) + 1}, {"logits": A[0] + 2}, {"workspace": A[6] + 8},
         {"workspace_bytes": size - 1},
         {"out_scores": A[0]}, {"parents": A[0] + 4 * 5999}, {"tokens": A[1] + 16}, {"tokens": A[2]},
         {"parents": A[3] + 40}, {"workspace": A[1] - size + 16}, {"workspace": A[5]}])

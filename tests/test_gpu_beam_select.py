@@ -84,7 +84,8 @@ def make(requests, beams, vocab, dtype, seed=0, spread=3.0):
 @pytest.mark.parametrize("dtype", ("bf16", "fp16", "fp32"))
 @pytest.mark.parametrize("requests,beams,vocab,candidates", [
     (1, 1, 1, 1), (2, 3, 5, 15), (1, 4, 32000, 4), (3, 2, 255, 7), (2, 5, 257, 10), (5, 1, 2049, 64),
-    (1, 32, 700, 64), (2, 8, 50257, 16), (70, 2, 1000, 2), (1, 3, 300001, 6)])
+    (1, 32, 700, 64), (2, 8, 50257, 16), (70, 2, 1000, 2), (1, 3, 300001, 6), (1, 1, 1 << 20, 3),
+    (2, 20, 140000, 5)])
 def test_matches_64_bits(sz, requests, beams, vocab, candidates, dtype):
     say("select", requests, beams, vocab, candidates, dtype)
     logits, scores = make(requests, beams, vocab, dtype, seed=vocab)
@@ -184,6 +185,18 @@ def test_extreme_spreads(sz):
     for spread in (0.0, 1e-3, 60.0, 1e4, 1e30):
         logits, scores = make(2, 3, 5000, "fp32", seed=8, spread=spread)
         check(sz.beam_select(logits, scores, candidates=9), logits, scores, 9)
+
+
+def test_many_rows(sz):
+    """More rows than a grid's dimension holds."""
+    say("many rows")
+    logits, scores = make(33000, 2, 40, "bf16", seed=12)
+    got = sz.beam_select(logits, scores, candidates=3)
+    values = values_of(logits, scores)
+    want = np.argsort(-values, axis=1, kind="stable")[:, :3]
+    place = got.parents.long().cpu().numpy() * 40 + got.tokens.cpu().numpy()
+    a, b = np.take_along_axis(values, place, 1), np.take_along_axis(values, want, 1)
+    assert (np.abs(a - b) <= 2 * OFF).all() and (np.diff(np.sort(place, 1), axis=1) > 0).all()
 
 
 def test_captured_and_repeated_calls(sz):

@@ -30,6 +30,7 @@ namespace {
 constexpr int kScanThreads = 256;
 constexpr int kLaneBytes = 64;                                // of a row that a lane takes at a time
 constexpr int kSegment = 256;                                 // logits whose maximum is kept
+constexpr unsigned int kGridRows = 32768;                     // of a grid's second dimension
 constexpr int kPickThreads = 1024;
 constexpr int kMostBeams = 32, kMostCandidates = 64;
 constexpr int kMostItems = 8;                                 // segments that a lane of beam_pick holds
@@ -121,9 +122,9 @@ __device__ __forceinline__ float wave_max(float v) {
 template <typename T>
 __global__ __launch_bounds__(kScanThreads) void beam_scan(SelectArgs a) {
   constexpr int kOwn = kLaneLogits<T>, kLoads = kOwn / T::kLoad, kLanes = kSegment / kOwn;
-  const unsigned int row = blockIdx.y, lane = threadIdx.x & 63;
+  const unsigned int row = blockIdx.z * kGridRows + blockIdx.y, lane = threadIdx.x & 63;
   const unsigned int chunk = uniform(blockIdx.x * (kScanThreads / kWave) + (threadIdx.x >> 6));
-  if (chunk >= a.chunks || !is_open(a, row)) return;
+  if (chunk >= a.chunks || row >= a.requests * a.beams || !is_open(a, row)) return;
   const unsigned char* src = row_of<T>(a, row);
   float top = kLowest, sum = 0.f;
   const unsigned int first = chunk * a.rounds * (kWave * kOwn);
@@ -717,7 +718,7 @@ bool select_ok(unsigned long long requests, unsigned long long beams, unsigned l
                unsigned long long candidates) {
   return requests != 0 && beams != 0 && beams <= kMostBeams && vocab != 0 && vocab <= kMostVocab &&
          candidates != 0 && candidates <= kMostCandidates && candidates <= beams * vocab &&
-         requests * beams <= 65535;
+         requests <= 1u << 20;
 }
 
 // Every row's maxima, then sums of as many chunks as it can have (f32, one round each): more for more rows or
@@ -810,7 +811,8 @@ extern "C" long long kvq_splitzip_beam_select(
   a.end_token = (unsigned int)end_token;
   hipStream_t stream = reinterpret_cast<hipStream_t>(stream_ptr);
   constexpr unsigned int kChunks = kScanThreads / kWave;  // of a workgroup
-  const dim3 grid((a.chunks + kChunks - 1) / kChunks, (unsigned int)rows);
+  const dim3 grid((a.chunks + kChunks - 1) / kChunks, (unsigned int)std::min<unsigned long long>(rows, kGridRows),
+                  (unsigned int)((rows + kGridRows - 1) / kGridRows));
   if (dtype == 0)
     hipLaunchKernelGGL(beam_scan<Bf16>, grid, dim3(kScanThreads), 0, stream, a);
   else if (dtype == 1)
