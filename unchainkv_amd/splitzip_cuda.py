@@ -1246,7 +1246,8 @@ def _row_dtype(dtype, torch):
 
 def _call_on(device, torch, fn, *args):
     """``fn(*args, stream)`` with ``device`` current and its current stream."""
-    if device.index is None or device.index == torch.cuda.current_device():
+    index = device.index
+    if index is None or index == torch._C._cuda_getDevice():
         return fn(*args, _stream_handle(device, torch))
     with torch.cuda.device(device):
         return fn(*args, _stream_handle(device, torch))
@@ -1424,6 +1425,15 @@ def write_kv_paged(k, v, kv_layer, slots) -> int | None:
     return int(got)
 
 
+def _row_bytes(t, dtype, device) -> tuple | None:
+    """Bytes from row to row and from head to head of 16-bit (rows, heads, head_dim) with whole head
+    rows, None for anything else."""
+    if t.dtype != dtype or t.dim() != 3 or t.device != device:
+        return None
+    row, head, value = t.stride()
+    return (2 * row, 2 * head) if value == 1 or t.shape[2] == 1 else None
+
+
 def rotation_table(positions: int, rotary_dim: int, base: float = 10000.0, *, frequencies=None,
                    device="cuda"):
     """Cosines and sines of positions 0 .. positions - 1 for ``rotate_write_kv_paged``: a
@@ -1473,8 +1483,10 @@ def rotate_write_kv_paged(q, k, v, kv_layer, slots, positions, rotation, *,
 
     device = q.device
     dtype = _row_dtype(q.dtype, torch)
-    if dtype is None or not _rows_ok(q, q.dtype, device) or not _rows_ok(k, q.dtype, device) or \
-            not _rows_ok(v, q.dtype, device) or not _kv_layer_ok(kv_layer, q.dtype, device):
+    if dtype is None or not _kv_layer_ok(kv_layer, q.dtype, device):
+        return None
+    rows = _row_bytes(q, q.dtype, device), _row_bytes(k, q.dtype, device), _row_bytes(v, q.dtype, device)
+    if None in rows:
         return None
     shape, (tokens, q_heads, head_dim), (_, blocks, block_tokens, kv_heads, kv_dim) = \
         k.shape, q.shape, kv_layer.shape
@@ -1492,11 +1504,9 @@ def rotate_write_kv_paged(q, k, v, kv_layer, slots, positions, rotation, *,
         return None
     if tokens == 0:
         return out
-    (q_row, q_head, _), (k_row, k_head, _), (v_row, v_head, _) = q.stride(), k.stride(), v.stride()
     places, table = blocks * block_tokens, rotation.shape
-    got = _call_on(device, torch, rotate, q.data_ptr(), 2 * q_row, 2 * q_head, q_heads,
-                   k.data_ptr(), 2 * k_row, 2 * k_head, v.data_ptr(), 2 * v_row, 2 * v_head, tokens,
-                   kv_heads, head_dim, dtype, kv_layer.data_ptr(),
+    got = _call_on(device, torch, rotate, q.data_ptr(), *rows[0], q_heads, k.data_ptr(), *rows[1],
+                   v.data_ptr(), *rows[2], tokens, kv_heads, head_dim, dtype, kv_layer.data_ptr(),
                    2 * places * kv_heads * head_dim, places, slots.data_ptr(), positions.data_ptr(),
                    rotation.data_ptr(), table[0], table[1], 1 if interleaved else 0, out.data_ptr())
     if got < 0:
@@ -1824,9 +1834,9 @@ def new_beam_choice(requests: int, candidates: int, device, torch=None) -> BeamC
     """Buffers for ``beam_select(..., choice=)``, which a captured step keeps."""
     if torch is None:
         import torch
-    tokens = torch.empty((requests, candidates), dtype=torch.int64, device=device)
-    scores = torch.empty((requests, candidates), dtype=torch.float32, device=device)
-    return BeamChoice(scores, torch.empty_like(scores, dtype=torch.int32), tokens)
+    tokens = torch.empty(requests, candidates, dtype=torch.int64, device=device)
+    scores = torch.empty_like(tokens, dtype=torch.float32)
+    return BeamChoice(scores, torch.empty_like(tokens, dtype=torch.int32), tokens)
 
 
 _LOGIT_DTYPES: dict = {}
