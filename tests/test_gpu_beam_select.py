@@ -36,8 +36,8 @@ def values_of(logits, scores, ended=None, end_token=0):
     with np.errstate(all="ignore"):
         top = x.max(-1, keepdims=True)
         top = np.where(np.isneginf(top), 0.0, top)
-        lse = np.log(np.exp(x - top).sum(-1, keepdims=True)) + top
-        v = x - lse + s[..., None]
+        # (the largest logit first: beside one of 3e38 the logarithm would be lost)
+        v = x - top - np.log(np.exp(x - top).sum(-1, keepdims=True)) + s[..., None]
     v[np.isneginf(x)] = -np.inf
     v[np.isneginf(s)] = -np.inf
     if ended is not None:
@@ -137,6 +137,9 @@ def test_masks(sz):
     check(sz.beam_select(logits, scores, candidates=20), logits, scores, 20)
     logits[0, 0] = torch.finfo(torch.float32).min  # all at the lowest value: each has 1 / vocab
     check(sz.beam_select(logits, scores, candidates=20), logits, scores, 20)
+    alone = sz.beam_select(logits[:1, :1], scores[:1, :1].contiguous(), candidates=3)
+    assert alone.tokens.tolist() == [[0, 1, 2]]
+    assert np.allclose(alone.scores.tolist(), scores[0, 0].item() - np.log(3001), atol=1e-5)
     low, s = make(2, 2, 800, "bf16", seed=4)
     low[:, 0, 3:] = torch.finfo(torch.bfloat16).min
     check(sz.beam_select(low, s, candidates=9), low, s, 9)

@@ -1,8 +1,8 @@
 // A beam search's step over paged layers, gfx950: the best continuations of a request's beams, and the block
 // tables and layers in the order of the chosen parents.
 //
-// Select. Beam b offers token t at (x[b][t] - lse[b]) + score[b], lse = log sum_t exp(x[b][t]); of all beams and
-// tokens the best n are given, equal ones by their places.
+// Select. Beam b offers token t at x[b][t] - m - log sum_t exp(x[b][t] - m) + score[b], m = max_t x[b][t]; of all
+// beams and tokens the best n are given, equal ones by their places.
 //   * beam_scan reads every logit once, a wave 4 KB of a row at a time, and keeps the maximum of each 256 of them
 //     and, of each wave's share, (m, sum exp(x - m)): one pass, sums in f32 of at most 64 terms a lane. Bound by
 //     HBM: 64 requests of 8 beams (one of them finished), 131072 logits in bf16, 117 MB: 23.1 us, 5.1 TB/s (a
@@ -232,11 +232,12 @@ __device__ __forceinline__ unsigned long long wave_largest(unsigned long long v)
 }
 
 struct Beam {
-  double lse, score;
+  double top, rest, score;  // the largest logit, and log sum exp(x - top)
   bool open, ended;
-  // what a token of some logit is worth (of a beam that is not open, none)
+  // what a token of some logit is worth (of a beam that is not open, none); the largest logit first, beside
+  // which the logarithm would be lost where all are masked by their type's lowest value
   __device__ __forceinline__ unsigned long long key(float logit) const {
-    return logit == -INFINITY ? key_of(-INFINITY) : key_of(((double)logit - lse) + score);
+    return logit == -INFINITY ? key_of(-INFINITY) : key_of(((double)logit - top) - rest + score);
   }
 };
 
@@ -330,7 +331,7 @@ __global__ __launch_bounds__(kPickThreads) void beam_pick(SelectArgs a) {
     }
     const float2 none = make_float2(kLowest, 0.f);
     const float2 own = lane < a.chunks ? sums[lane] : none;
-    Beam beam{0., a.scores[row], is_open(a, row), is_ended(a, row)};
+    Beam beam{0., 0., a.scores[row], is_open(a, row), is_ended(a, row)};
     float top = own.x;
     for (unsigned int c = lane + kWave; c < a.chunks; c += kWave) top = fmaxf(top, sums[c].x);
     top = wave_max(top);
@@ -339,7 +340,8 @@ __global__ __launch_bounds__(kPickThreads) void beam_pick(SelectArgs a) {
       sum += sums[c].y * __builtin_amdgcn_exp2f((sums[c].x - top) * kLog2E);
 #pragma unroll
     for (int d = 1; d < kWave; d *= 2) sum += __shfl_xor(sum, d, kWave);
-    beam.lse = log(sum) + (double)top;
+    beam.top = top;
+    beam.rest = log(sum);
 #pragma unroll
     for (int t = 0; t < kItems; ++t) largest[t] = beam.open ? largest[t] : -INFINITY;
     if (lane == 0) s_beam[b] = beam;
