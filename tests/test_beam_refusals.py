@@ -132,19 +132,21 @@ def test_tensors_off_the_gpu_are_declined():
 @pytest.fixture
 def entered(monkeypatch):
     """The names of the entries that were called."""
-    names = []
+    names, u64 = [], ctypes.c_ulonglong
 
-    def entry(name, value):
+    def entry(name, count):
         def call(*args):
             names.append(name)
-            return value
-        return call
+            return 1
+        return ctypes.CFUNCTYPE(ctypes.c_longlong, *[u64] * count)(call) if count else call
 
-    calls = {n: entry(n, 1) for n in (
-        "kvq_splitzip_rotate_write_kv_paged", "kvq_splitzip_cross_attention_paged",
-        "kvq_splitzip_cross_attention", "kvq_splitzip_beam_select", "kvq_splitzip_reorder_beams_paged")}
-    sizes = {f"kvq_splitzip_{n}_workspace_bytes": lambda *a: 16 for n in ("beam_select", "reorder_beams")}
-    monkeypatch.setattr(sz, "_load", lambda: SimpleNamespace(**calls, **sizes))
+    calls = {f"kvq_splitzip_{n}": entry(n, count) for n, count in (
+        ("rotate_write_kv_paged", 25), ("cross_attention_paged", 0), ("cross_attention", 0), ("beam_select", 17),
+        ("reorder_beams_paged", 24))}
+    sizes = {f"kvq_splitzip_{n}_workspace_bytes": ctypes.CFUNCTYPE(u64, u64, u64, u64)(lambda *a: 16)
+             for n in ("beam_select", "reorder_beams")}
+    lib = SimpleNamespace(**calls, **sizes)
+    monkeypatch.setattr(sz, "_load", lambda: lib)
     monkeypatch.setattr(sz, "_is_cuda", lambda t: True)
     monkeypatch.setattr(sz, "_call_on", lambda device, torch, fn, *args: fn(*args, 0))
     monkeypatch.setattr(sz, "_attention_workspace", lambda name, device, sizes: 0)
@@ -222,6 +224,24 @@ def test_writes_count_as_in_place_operations(entered):
         assert all(t._version > b for t, b in zip(written, before))
     with torch.inference_mode():
         assert rotate(kv=layer()) is not None and order(kv=layer()) is not None
+
+
+def test_arguments_that_are_no_tensors(entered):
+    for call in (lambda: rotate(k=[1.0]), lambda: rotate(table=3), lambda: select(scores=2.0),
+                 lambda: order(kv="layer")):
+        with pytest.raises(TypeError, match="a tensor is wanted"):
+            call()
+    assert not entered
+
+
+def test_failures_of_the_entries_are_raised(entered):
+    lib = sz._load()
+    failing = ctypes.CFUNCTYPE(ctypes.c_longlong, *[ctypes.c_ulonglong] * 25)(lambda *a: -1)
+    lib.kvq_splitzip_rotate_write_kv_paged, lib.kvq_splitzip_last_error = failing, lambda: b"no such device"
+    kv = layer()
+    with pytest.raises(RuntimeError, match="no such device"):
+        rotate(kv=kv)
+    assert kv._version == 0
 
 
 def test_calls_that_do_nothing(entered):

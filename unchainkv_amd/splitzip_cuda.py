@@ -1234,6 +1234,39 @@ def decode_attention_top16(q, payloads, payload_offsets, context_tokens, kv_head
 # ---------------------------------------------------------------------------
 # a step over a paged layer: tables and slots, the K/V write, attention of chunks and prompts
 
+_BINDING = None
+
+
+def _step_binding():
+    """The native side of ``rotate_write_kv_paged``, ``beam_select`` and ``reorder_beams_paged``
+    (csrc/step_binding.cpp): their checks, allocations and arguments. It is linked to torch, so it is
+    loaded with the first such call."""
+    global _BINDING
+    if _BINDING is None:
+        import importlib.util
+
+        import torch  # noqa: F401 (whose libraries it needs)
+
+        from . import _build
+
+        try:
+            spec = importlib.util.spec_from_file_location(_build.BINDING_NAME, _build.BINDING_PATH)
+            module = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(module)
+        except (ImportError, OSError) as exc:
+            raise RuntimeError(f"step binding not loaded ({_build.BINDING_PATH}): {exc}") from exc
+        _BINDING = module
+    return _BINDING
+
+
+def _entry_address(entry) -> int:
+    """A C entry's address, which the ctypes function keeps."""
+    address = getattr(entry, "address", None)
+    if address is None:
+        address = entry.address = ctypes.cast(entry, ctypes.c_void_p).value
+    return address
+
+
 # element types of the layers and rows that these calls take, as the C entries number them
 _ROW_DTYPES: dict = {}
 
@@ -1425,15 +1458,6 @@ def write_kv_paged(k, v, kv_layer, slots) -> int | None:
     return int(got)
 
 
-def _row_bytes(t, dtype, device) -> tuple | None:
-    """Bytes from row to row and from head to head of 16-bit (rows, heads, head_dim) with whole head
-    rows, None for anything else."""
-    if t.dtype != dtype or t.dim() != 3 or t.device != device:
-        return None
-    row, head, value = t.stride()
-    return (2 * row, 2 * head) if value == 1 or t.shape[2] == 1 else None
-
-
 def rotation_table(positions: int, rotary_dim: int, base: float = 10000.0, *, frequencies=None,
                    device="cuda"):
     """Cosines and sines of positions 0 .. positions - 1 for ``rotate_write_kv_paged``: a
@@ -1481,43 +1505,11 @@ def rotate_write_kv_paged(q, k, v, kv_layer, slots, positions, rotation, *,
         return None
     import torch
 
-    device = q.device
-    dtype = _row_dtype(q.dtype, torch)
-    if dtype is None or not _kv_layer_ok(kv_layer, q.dtype, device):
-        return None
-    rows = _row_bytes(q, q.dtype, device), _row_bytes(k, q.dtype, device), _row_bytes(v, q.dtype, device)
-    if None in rows:
-        return None
-    shape, (tokens, q_heads, head_dim), (_, blocks, block_tokens, kv_heads, kv_dim) = \
-        k.shape, q.shape, kv_layer.shape
-    if shape != (tokens, kv_heads, head_dim) or v.shape != shape or kv_dim != head_dim or \
-            not _index_vector_ok(slots, device, tokens, torch.int64) or \
-            not _index_vector_ok(positions, device, tokens, torch.int64) or \
-            rotation.dtype != torch.float32 or rotation.dim() != 2 or rotation.device != device or \
-            not rotation.is_contiguous():
-        return None
-    if _tracked(torch, q, k, v, kv_layer, rotation, out):
-        return None
-    given = out is not None
-    ok, out = _attention_buffers(q, out, None, torch)
-    if not ok:
-        return None
-    if tokens == 0:
-        return out
-    places, table = blocks * block_tokens, rotation.shape
-    got = _call_on(device, torch, rotate, q.data_ptr(), *rows[0], q_heads, k.data_ptr(), *rows[1],
-                   v.data_ptr(), *rows[2], tokens, kv_heads, head_dim, dtype, kv_layer.data_ptr(),
-                   2 * places * kv_heads * head_dim, places, slots.data_ptr(), positions.data_ptr(),
-                   rotation.data_ptr(), table[0], table[1], 1 if interleaved else 0, out.data_ptr())
-    if got < 0:
+    got = _call_on(q.device, torch, _step_binding().rotate_write, _entry_address(rotate), q, k, v,
+                   kv_layer, slots, positions, rotation, interleaved, out)
+    if type(got) is int:
         _raise_last(lib, "splitzip rotated K/V write failed")
-    if not got:
-        return None
-    if given:
-        _wrote(torch, kv_layer, out)
-    else:
-        _wrote(torch, kv_layer)
-    return out
+    return got
 
 
 @functools.lru_cache(maxsize=1024)
@@ -1839,9 +1831,6 @@ def new_beam_choice(requests: int, candidates: int, device, torch=None) -> BeamC
     return BeamChoice(scores, torch.empty_like(tokens, dtype=torch.int32), tokens)
 
 
-_LOGIT_DTYPES: dict = {}
-
-
 def beam_select_workspace_bytes(requests: int, beams: int, vocab: int) -> int:
     """Workspace of ``beam_select``. Sizes that the call declines raise ``ValueError``."""
     lib = _load()
@@ -1853,10 +1842,6 @@ def beam_select_workspace_bytes(requests: int, beams: int, vocab: int) -> int:
     if not need:
         raise ValueError(f"no selection takes {requests} requests of {beams} beams, {vocab} tokens")
     return need if requests else 0
-
-
-def _matrix_ok(t, shape, dtype, device) -> bool:
-    return t.dtype == dtype and t.shape == shape and t.device == device and t.is_contiguous()
 
 
 def beam_select(logits, scores, *, candidates: int | None = None, ended=None,
@@ -1887,49 +1872,17 @@ def beam_select(logits, scores, *, candidates: int | None = None, ended=None,
         return None
     import torch
 
-    if not _LOGIT_DTYPES:
-        _LOGIT_DTYPES.update({torch.bfloat16: 0, torch.float16: 1, torch.float32: 2})
-    device, dtype = logits.device, _LOGIT_DTYPES.get(logits.dtype)
-    if dtype is None or logits.dim() != 3:
+    if candidates is None:
+        candidates = logits.shape[1] if logits.dim() == 3 else 0
+    candidates, end_token = int(candidates), -1 if end_token is None else int(end_token)
+    if not 0 < candidates <= 64 or (ended is not None and end_token < 0):
         return None
-    requests, beams, vocab = logits.shape
-    if (vocab != 1 and logits.stride(2) != 1) or logits.stride(0) < 0 or logits.stride(1) < 0 or \
-            not _matrix_ok(scores, (requests, beams), torch.float32, device):
-        return None
-    if ended is not None and (not _matrix_ok(ended, (requests, beams), torch.bool, device)
-                              or end_token is None or not 0 <= int(end_token) < vocab):
-        return None
-    if _tracked(torch, logits, scores, *(choice or ())):
-        return None
-    candidates = beams if candidates is None else int(candidates)
-    if not 0 < candidates <= 64:
-        return None
-    given = choice or ()
-    if choice is None:
-        choice = new_beam_choice(requests, candidates, device, torch)
-    elif not (_matrix_ok(choice.scores, (requests, candidates), torch.float32, device)
-              and _matrix_ok(choice.parents, (requests, candidates), torch.int32, device)
-              and _matrix_ok(choice.tokens, (requests, candidates), torch.int64, device)):
-        return None
-    if requests == 0:
-        return choice
-    need = lib.kvq_splitzip_beam_select_workspace_bytes(requests, beams, vocab)
-    if not need:
-        return None
-    if workspace is None or not _byte_buffer_ok(workspace, device, need, torch):
-        workspace = torch.empty(need, dtype=torch.uint8, device=device)
-    got = _call_on(device, torch, select, logits.data_ptr(), dtype, logits.stride(0),
-                   logits.stride(1), scores.data_ptr(), 0 if ended is None else ended.data_ptr(),
-                   requests, beams, vocab, candidates, 0 if ended is None else int(end_token),
-                   choice.scores.data_ptr(), choice.parents.data_ptr(), choice.tokens.data_ptr(),
-                   workspace.data_ptr(), need)
-    if got < 0:
+    got = _call_on(logits.device, torch, _step_binding().beam_select, _entry_address(select),
+                   _entry_address(lib.kvq_splitzip_beam_select_workspace_bytes), logits, scores,
+                   candidates, ended, max(end_token, 0), *(choice or (None,) * 3), workspace)
+    if type(got) is int:
         _raise_last(lib, "splitzip beam selection failed")
-    if not got:
-        return None
-    if given:
-        _wrote(torch, *given)
-    return choice
+    return got and (choice or BeamChoice(*got))
 
 
 class BeamOrder(NamedTuple):
@@ -1970,26 +1923,6 @@ def reorder_beams_workspace_bytes(requests: int, beams: int, width: int) -> int:
     return need if requests else 0
 
 
-def _layer_addresses(layers: tuple, device, block_tokens: int, torch):
-    """A ctypes array of the layers' addresses, or None: layers that are not alike, or that autograd
-    follows. (A call has many layers and a microsecond for each counts, so the first alone is looked at in
-    full.)"""
-    if not layers:
-        return (ctypes.c_ulonglong * 1)()
-    dtype, shape, index = layers[0].dtype, layers[0].shape, layers[0].get_device()
-    if _row_dtype(dtype, torch) is None or not _kv_layer_ok(layers[0], dtype, device) or \
-            shape[2] != block_tokens:
-        return None
-    grad = torch.is_grad_enabled()
-    for t in layers:
-        if t.dtype is not dtype or t.shape != shape or not t.is_contiguous() or \
-                t.get_device() != index or (grad and t.requires_grad):
-            return None
-    if getattr(torch.autograd.forward_ad, "_current_level", 0) >= 0 and _tracked(torch, *layers):
-        return None
-    return (ctypes.c_ulonglong * len(layers))(*[t.data_ptr() for t in layers])
-
-
 def reorder_beams_paged(layers, tables, parents, context_tokens, free_blocks, free_start,
                         block_tokens: int, *, order: BeamOrder | None = None, workspace=None):
     """The beams' block tables, and the layers, in the order of the chosen parents: beam j of
@@ -2025,55 +1958,16 @@ def reorder_beams_paged(layers, tables, parents, context_tokens, free_blocks, fr
         return None
     import torch
 
-    device, i32, block_tokens = tables.device, torch.int32, int(block_tokens)
-    if tables.dtype != i32 or tables.dim() != 2 or parents.dtype != i32 or parents.dim() != 2 or \
-            parents.device != device or not parents.is_contiguous() or block_tokens <= 0:
+    block_tokens = int(block_tokens)
+    if block_tokens <= 0:
         return None
-    requests, beams = parents.shape
-    rows, width = tables.shape
-    if rows != requests * beams or (width != 1 and tables.stride(1) != 1) or \
-            not _index_vector_ok(context_tokens, device, rows, i32) or \
-            not _index_vector_ok(free_blocks, device, 0, i32) or \
-            not _index_vector_ok(free_start, device, 1, i32):
-        return None
-    addresses = _layer_addresses(layers := tuple(layers), device, block_tokens, torch)
-    if addresses is None:
-        return None
-    given = order or ()
-    if order is None:
-        order = new_beam_order(requests, beams, width, device, torch)
-    elif order.tables.dtype != i32 or order.tables.shape != tables.shape or \
-            order.tables.device != device or (width != 1 and order.tables.stride(1) != 1) or \
-            not (_index_vector_ok(order.copied_from, device, rows, i32)
-                 and _index_vector_ok(order.free_next, device, 1, i32)
-                 and _index_vector_ok(order.lacking, device, 1, i32)
-                 and _index_vector_ok(order.unlisted, device, 1, i32)):
-        return None
-    if rows == 0:
-        order.free_next[:1].copy_(free_start[:1].clamp(0, free_blocks.numel()))
-        order.lacking[:1].fill_(0)
-        order.unlisted[:1].fill_(0)
-        return order
-    need = lib.kvq_splitzip_reorder_beams_workspace_bytes(requests, beams, width)
-    if not need:
-        return None
-    if workspace is None or not _byte_buffer_ok(workspace, device, need, torch):
-        workspace = torch.empty(need, dtype=torch.uint8, device=device)
-    blocks = layers[0].shape[1] if layers else 1
-    row_bytes = 2 * layers[0].stride(2) if layers else 2
-    got = _call_on(device, torch, reorder, addresses, len(layers), blocks, block_tokens, row_bytes,
-                   tables.data_ptr(), tables.stride(0) if rows > 1 else width, width,
-                   order.tables.data_ptr(), order.tables.stride(0) if rows > 1 else width,
-                   parents.data_ptr(), context_tokens.data_ptr(), requests, beams,
-                   free_blocks.data_ptr(), free_blocks.numel(), free_start.data_ptr(),
-                   order.copied_from.data_ptr(), order.free_next.data_ptr(),
-                   order.lacking.data_ptr(), order.unlisted.data_ptr(), workspace.data_ptr(), need)
-    if got < 0:
+    got = _call_on(tables.device, torch, _step_binding().reorder_beams, _entry_address(reorder),
+                   _entry_address(lib.kvq_splitzip_reorder_beams_workspace_bytes), tuple(layers),
+                   tables, parents, context_tokens, free_blocks, free_start, block_tokens,
+                   *(order or (None,) * 5), workspace)
+    if type(got) is int:
         _raise_last(lib, "splitzip beam reordering failed")
-    if not got:
-        return None
-    _wrote(torch, free_blocks, *layers, *given)
-    return order
+    return got and (order or BeamOrder(*got))
 
 
 # ---------------------------------------------------------------------------
