@@ -134,22 +134,22 @@ def entered(monkeypatch):
     """The names of the entries that were called."""
     names, u64 = [], ctypes.c_ulonglong
 
-    def entry(name, count):
+    def entry(name, *types):
         def call(*args):
             names.append(name)
             return 1
-        return ctypes.CFUNCTYPE(ctypes.c_longlong, *[u64] * count)(call) if count else call
+        return ctypes.CFUNCTYPE(ctypes.c_longlong, *types)(call)
 
-    calls = {f"kvq_splitzip_{n}": entry(n, count) for n, count in (
-        ("rotate_write_kv_paged", 25), ("cross_attention_paged", 0), ("cross_attention", 0), ("beam_select", 17),
-        ("reorder_beams_paged", 24))}
-    sizes = {f"kvq_splitzip_{n}_workspace_bytes": ctypes.CFUNCTYPE(u64, u64, u64, u64)(lambda *a: 16)
-             for n in ("beam_select", "reorder_beams")}
+    calls = {f"kvq_splitzip_{n}": entry(n, *[u64] * count) for n, count in (
+        ("rotate_write_kv_paged", 25), ("beam_select", 17), ("reorder_beams_paged", 24))}
+    for n, count in (("cross_attention_paged", 22), ("cross_attention", 25)):
+        calls[f"kvq_splitzip_{n}"] = entry(n, *[u64] * count, ctypes.c_float, u64)
+    sizes = {f"kvq_splitzip_{n}_workspace_bytes": ctypes.CFUNCTYPE(u64, *[u64] * count)(lambda *a: 16)
+             for n, count in (("beam_select", 3), ("reorder_beams", 3), ("chunk_attention", 7))}
     lib = SimpleNamespace(**calls, **sizes)
     monkeypatch.setattr(sz, "_load", lambda: lib)
     monkeypatch.setattr(sz, "_is_cuda", lambda t: True)
     monkeypatch.setattr(sz, "_call_on", lambda device, torch, fn, *args: fn(*args, 0))
-    monkeypatch.setattr(sz, "_attention_workspace", lambda name, device, sizes: 0)
     return names
 
 
@@ -224,11 +224,15 @@ def test_writes_count_as_in_place_operations(entered):
         assert all(t._version > b for t, b in zip(written, before))
     with torch.inference_mode():
         assert rotate(kv=layer()) is not None and order(kv=layer()) is not None
+        kv, out, choice, into = layer(), rows(4), sz.new_beam_choice(1, 2, "cpu"), sz.new_beam_order(1, 2, 1, "cpu")
+    # (such tensors count no writes, used outside that mode neither)
+    assert rotate(kv=kv, out=out) is not None and paged(kv=kv, out=out) is not None
+    assert packed(out=out) is not None and select(choice=choice) is not None and order(kv=kv, order=into) is not None
 
 
 def test_arguments_that_are_no_tensors(entered):
     for call in (lambda: rotate(k=[1.0]), lambda: rotate(table=3), lambda: select(scores=2.0),
-                 lambda: order(kv="layer")):
+                 lambda: order(kv="layer"), lambda: paged(kv=1), lambda: packed(v=(2,)), lambda: paged(out=0)):
         with pytest.raises(TypeError, match="a tensor is wanted"):
             call()
     assert not entered
@@ -242,6 +246,17 @@ def test_failures_of_the_entries_are_raised(entered):
     with pytest.raises(RuntimeError, match="no such device"):
         rotate(kv=kv)
     assert kv._version == 0
+
+
+def test_bounds_and_scales(entered):
+    """max_query and max_source count as at most the rows there are; a scale is any number."""
+    assert paged(max_query=99, scale=1) is not None and packed(max_query=2, max_source=10 ** 9, scale=0.5) is not None
+    assert paged(max_query=0) is None and paged(max_query=-3) is None and packed(max_source=-1) is None
+    with pytest.raises(TypeError):
+        paged(scale="half")
+    with pytest.raises(TypeError):
+        packed(max_query=1.5)
+    assert len(entered) == 2
 
 
 def test_calls_that_do_nothing(entered):

@@ -1,18 +1,20 @@
-// The step calls' arguments, from Python tensors to the C entries: what splitzip_cuda.rotate_write_kv_paged,
-// beam_select and reorder_beams_paged check, allocate and pass on. A small call is bound by its host time, of
-// which tensors' attributes read one by one from Python took more than the launch (rotate_write_kv_paged 13.2 us a
-// call, 5 of them the launch; a layer of reorder_beams_paged 0.35). Each function takes the
-// entries' addresses first and the stream last, and gives the results, None where the call is declined, or -1 where the entry
-// failed; an argument that is no tensor raises TypeError.
+// The step calls' arguments, from Python tensors to the C entries: what splitzip_cuda's rotate_write_kv_paged,
+// cross_attention_paged, cross_attention, beam_select and reorder_beams_paged check, allocate and pass on. A
+// small call is bound by its host time, of which tensors' attributes read one by one from Python took more than
+// the launch: us a call with them and with this, rotate_write_kv_paged 13.2 and 6, beam_select (two launches) 17.3
+// and 12, reorder_beams_paged of 16 layers (two launches) 26.5 and 14. Each function takes the entries' addresses
+// first and the stream last, and gives the results, None where the call is declined, or -1 where the entry failed;
+// an argument that is no tensor raises TypeError.
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
-#include <ATen/ops/empty_like.h>
 #include <Python.h>
 #include <c10/core/GradMode.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <array>
+#include <cmath>
 #include <cstdint>
 #include <initializer_list>
 #include <vector>
@@ -87,9 +89,10 @@ bool tracked(std::initializer_list<const at::Tensor*> tensors) {
   return false;
 }
 
-// A kernel's write into a caller's tensor, counted as torch's in-place operations are.
+// A kernel's write into a caller's tensor, counted as torch's in-place operations are. (An inference tensor, for
+// which nothing can have been saved, has no count.)
 void wrote(const at::Tensor& t) {
-  if (t.defined()) t.unsafeGetTensorImpl()->bump_version();
+  if (t.defined() && !t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
 // `given`, if it is a workspace of `need` bytes, or a new one.
@@ -161,6 +164,120 @@ PyObject* rotate_write(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return answer(got, [&] {
     wrote(kv);
     if (given) wrote(out);
+    return THPVariable_Wrap(out);
+  });
+  END_HANDLE_TH_ERRORS
+}
+
+int64_t count_of(PyObject* o, int64_t otherwise) {
+  if (o == Py_None) return otherwise;
+  const long long v = PyLong_AsLongLong(o);
+  if (v == -1 && PyErr_Occurred() != nullptr) throw python_error();
+  return std::min<int64_t>(v, otherwise);
+}
+
+// An attention call's scale, head_dim ** -0.5 where none is given.
+float scale_of(PyObject* o, int64_t dim) {
+  if (o == Py_None) return (float)(1. / std::sqrt((double)dim));
+  const double v = PyFloat_AsDouble(o);
+  if (v == -1. && PyErr_Occurred() != nullptr) throw python_error();
+  return (float)v;
+}
+
+// An attention call's results: as q, and f32 for its rows and heads.
+bool results_ok(const at::Tensor& q, const at::Tensor& out, const at::Tensor& lse) {
+  const std::array<int64_t, 2> rows = {q.size(0), q.size(1)};
+  return (!out.defined() || matrix_ok(out, q.sizes(), q.device(), q.scalar_type())) &&
+         (!lse.defined() || matrix_ok(lse, rows, q.device(), at::kFloat));
+}
+
+typedef u64 (*AttentionSize)(u64, u64, u64, u64, u64, u64, u64);
+
+// entry, its workspace's size, q, kv_layer, tables, query_starts, source_tokens, max_query, scale, out, lse,
+// workspace, stream
+PyObject* cross_paged(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!count_ok(n, 13)) return nullptr;
+  const u64 entry = number_of(args[0]), size = number_of(args[1]), stream = number_of(args[12]);
+  const at::Tensor &q = tensor_of(args[2]), &kv = tensor_of(args[3]), &tables = tensor_of(args[4]),
+                   &starts = tensor_of(args[5]), &source = tensor_of(args[6]);
+  at::Tensor out = maybe_tensor(args[9]);
+  const at::Tensor lse = maybe_tensor(args[10]), workspace = maybe_tensor(args[11]);
+  const bool given = out.defined();
+  const int dtype = row_dtype(q);
+  const at::Device device = q.device();
+  if (dtype < 0 || !rows_ok(q, q) || !layer_ok(kv, q.scalar_type(), device) || tracked({&q, &kv, &out, &lse}) ||
+      tables.scalar_type() != at::kInt || tables.dim() != 2 || tables.device() != device)
+    return none();
+  const int64_t tokens = q.size(0), heads = q.size(1), dim = q.size(2);
+  const int64_t requests = tables.size(0), width = tables.size(1);
+  if (kv.size(4) != dim || (width != 1 && tables.stride(1) != 1) ||
+      !vector_ok(starts, device, requests + 1, at::kInt) || !vector_ok(source, device, requests, at::kInt) ||
+      !results_ok(q, out, lse))
+    return none();
+  const int64_t max_query = count_of(args[7], tokens);
+  const float scale = scale_of(args[8], dim);
+  if (!given) out = at::empty(q.sizes(), q.options());
+  if (tokens == 0 || requests == 0) return THPVariable_Wrap(out);
+  if (max_query <= 0 || width == 0) return none();
+  const u64 need = reinterpret_cast<AttentionSize>(size)((u64)tokens, (u64)requests, (u64)heads, (u64)kv.size(3),
+                                                         (u64)dim, (u64)(width * kv.size(2)), (u64)max_query);
+  const at::Tensor space = need != 0 ? workspace_of(workspace, need, device) : at::Tensor();
+  typedef long long (*Entry)(u64, u64, u64, u64, u64, u64, u64, u64, u64, u64, u64, u64, u64, u64, u64, u64, u64, u64,
+                             u64, u64, u64, u64, float, u64);
+  const long long got = enter<Entry>(
+      entry, address(q), (u64)(2 * q.stride(0)), (u64)(2 * q.stride(1)), (u64)tokens, (u64)heads, (u64)kv.size(3),
+      (u64)dim, (u64)dtype, address(kv), (u64)kv.size(1), (u64)kv.size(2), address(tables),
+      (u64)(requests > 1 ? tables.stride(0) : width), (u64)width, address(starts), address(source), (u64)requests,
+      (u64)max_query, address(out), address(lse), address(space), need, scale, stream);
+  return answer(got, [&] {
+    if (given) wrote(out);
+    wrote(lse);
+    return THPVariable_Wrap(out);
+  });
+  END_HANDLE_TH_ERRORS
+}
+
+// entry, its workspace's size, q, k, v, query_starts, source_starts, source_tokens, max_query, max_source, scale,
+// out, lse, workspace, stream
+PyObject* cross_rows(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!count_ok(n, 15)) return nullptr;
+  const u64 entry = number_of(args[0]), size = number_of(args[1]), stream = number_of(args[14]);
+  const at::Tensor &q = tensor_of(args[2]), &k = tensor_of(args[3]), &v = tensor_of(args[4]),
+                   &starts = tensor_of(args[5]), &first = tensor_of(args[6]), &source = tensor_of(args[7]);
+  at::Tensor out = maybe_tensor(args[11]);
+  const at::Tensor lse = maybe_tensor(args[12]), workspace = maybe_tensor(args[13]);
+  const bool given = out.defined();
+  const int dtype = row_dtype(q);
+  const at::Device device = q.device();
+  if (dtype < 0 || !rows_ok(q, q) || !rows_ok(k, q) || !rows_ok(v, q) || tracked({&q, &k, &v, &out, &lse}))
+    return none();
+  const int64_t tokens = q.size(0), heads = q.size(1), dim = q.size(2), rows = k.size(0), kv_heads = k.size(1);
+  const int64_t requests = source.numel();
+  if (k.sizes() != v.sizes() || k.size(2) != dim || dim == 0 || !vector_ok(source, device, 0, at::kInt) ||
+      !vector_ok(first, device, requests, at::kInt) || !vector_ok(starts, device, requests + 1, at::kInt) ||
+      !results_ok(q, out, lse))
+    return none();
+  const int64_t max_query = count_of(args[8], tokens), max_source = count_of(args[9], rows);
+  const float scale = scale_of(args[10], dim);
+  if (!given) out = at::empty(q.sizes(), q.options());
+  if (tokens == 0 || requests == 0) return THPVariable_Wrap(out);
+  if (max_query <= 0 || max_source < 0 || rows == 0) return none();
+  const u64 need = reinterpret_cast<AttentionSize>(size)((u64)tokens, (u64)requests, (u64)heads, (u64)kv_heads,
+                                                         (u64)dim, (u64)max_source, (u64)max_query);
+  const at::Tensor space = need != 0 ? workspace_of(workspace, need, device) : at::Tensor();
+  typedef long long (*Entry)(u64, u64, u64, u64, u64, u64, u64, u64, u64, u64, u64, u64, u64, u64, u64, u64, u64, u64,
+                             u64, u64, u64, u64, u64, u64, u64, float, u64);
+  const long long got = enter<Entry>(
+      entry, address(q), (u64)(2 * q.stride(0)), (u64)(2 * q.stride(1)), address(k), (u64)(2 * k.stride(0)),
+      (u64)(2 * k.stride(1)), address(v), (u64)(2 * v.stride(0)), (u64)(2 * v.stride(1)), (u64)rows, (u64)tokens,
+      (u64)heads, (u64)kv_heads, (u64)dim, (u64)dtype, address(starts), address(first), address(source),
+      (u64)requests, (u64)max_query, (u64)max_source, address(out), address(lse), address(space), need, scale,
+      stream);
+  return answer(got, [&] {
+    if (given) wrote(out);
+    wrote(lse);
     return THPVariable_Wrap(out);
   });
   END_HANDLE_TH_ERRORS
@@ -271,8 +388,8 @@ PyObject* reorder_beams(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (need == kDeclined) return none();
   const at::Tensor space = workspace_of(workspace, need, device);
   const u64 stride = (u64)(rows > 1 ? tables.stride(0) : width), to = (u64)(rows > 1 ? order[0].stride(0) : width);
-  typedef long long (*Entry)(const u64*, u64, u64, u64, u64, u64, u64, u64, u64, u64, u64, u64, u64, u64, u64, u64, u64,
-                             u64, u64, u64, u64, u64, u64, u64);
+  typedef long long (*Entry)(const u64*, u64, u64, u64, u64, u64, u64, u64, u64, u64, u64, u64, u64, u64, u64, u64,
+                             u64, u64, u64, u64, u64, u64, u64, u64);
   const long long got = enter<Entry>(
       entry, (const u64*)layers.data(), (u64)count, blocks, block_tokens, row_bytes, address(tables), stride,
       (u64)width, address(order[0]), to, address(parents), address(contexts), (u64)requests, (u64)beams,
@@ -288,14 +405,18 @@ PyObject* reorder_beams(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-PyMethodDef kMethods[] = {
-    {"rotate_write", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(rotate_write)), METH_FASTCALL, nullptr},
-    {"beam_select", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(beam_select)), METH_FASTCALL, nullptr},
-    {"reorder_beams", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(reorder_beams)), METH_FASTCALL,
-     nullptr},
-    {nullptr, nullptr, 0, nullptr}};
+typedef PyObject* (*Call)(PyObject*, PyObject* const*, Py_ssize_t);
 
-PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_step_binding", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
+PyMethodDef method(const char* name, Call call) {
+  return {name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(call)), METH_FASTCALL, nullptr};
+}
+
+PyMethodDef kMethods[] = {method("rotate_write", rotate_write), method("cross_paged", cross_paged),
+                          method("cross_rows", cross_rows),     method("beam_select", beam_select),
+                          method("reorder_beams", reorder_beams), {nullptr, nullptr, 0, nullptr}};
+
+PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_step_binding", nullptr, -1, kMethods, nullptr, nullptr, nullptr,
+                       nullptr};
 
 }  // namespace
 

@@ -1238,9 +1238,9 @@ _BINDING = None
 
 
 def _step_binding():
-    """The native side of ``rotate_write_kv_paged``, ``beam_select`` and ``reorder_beams_paged``
-    (csrc/step_binding.cpp): their checks, allocations and arguments. It is linked to torch, so it is
-    loaded with the first such call."""
+    """The native side of ``rotate_write_kv_paged``, the cross attentions, ``beam_select`` and
+    ``reorder_beams_paged`` (csrc/step_binding.cpp): their checks, allocations and arguments. It is
+    linked to torch, so it is loaded with the first such call."""
     global _BINDING
     if _BINDING is None:
         import importlib.util
@@ -1581,11 +1581,38 @@ def _attention_buffers(q, out, lse, torch):
     return True, out
 
 
-def _attend_paged(kind: str, q, kv_layer, tables, query_starts, context_tokens, max_query, scale,
-                  out, lse, workspace):
-    """chunk_attention_paged and cross_attention_paged."""
+def chunk_attention_paged(q, kv_layer, tables, query_starts, context_tokens, *,
+                          max_query: int | None = None, scale: float | None = None, out=None,
+                          lse=None, workspace=None):
+    """Causal attention of a step's new tokens over a paged layer that holds their own K and V
+    already (``write_kv_paged``); single tokens (decode), chunks of prompts and drafted
+    tokens mixed in any way.
+
+    ``q`` (tokens, q_heads, head_dim) are the packed rows; request r's are rows
+    ``query_starts[r]`` .. ``query_starts[r + 1]``, the last of its ``context_tokens[r]``
+    tokens, so row i of its n sees tokens 0 .. context - n + i. Query head h reads KV head
+    h // (q_heads / kv_heads). ``tables`` (requests, width) int32 lists each request's blocks in
+    token order, ``query_starts`` (requests + 1) and ``context_tokens`` (requests) are int32;
+    all stay on the device (``StepPlan``), and a captured call follows their values.
+    ``max_query`` bounds the new tokens of a request (default: the rows of q); a smaller bound
+    spares a decode step the kernel for long chunks. ``scale`` (positive) defaults to head_dim
+    ** -0.5. ``lse`` (tokens, q_heads) float32 receives each row's log-sum-exp, for joining
+    with attention over other tokens. bf16 or fp16, head_dim 64 or 128; rows and heads of q
+    may be strided by multiples of 16 bytes.
+
+    A row that sees no token (context_tokens[r] less than its new tokens) is zero, its lse
+    -inf. Rows of no request, of one with more new tokens than max_query, and of one whose
+    row range is not inside q stay as they are. A context longer than its table, or a table
+    entry that is no block of the layer, makes the rows that read there NaN (every row of
+    the same tile, of 16 to 256 of a KV head's query rows, at least). Where
+    query_starts run backwards, so that ranges overlap, rows are one of their requests' or stay.
+    ``out``, ``lse`` and ``workspace`` over an input or each other are declined.
+    No gradient: inputs, ``out`` or ``lse`` that require one are declined while gradients are
+    recorded, and so are forward-mode tangents.
+
+    Returns ``out`` (tokens, q_heads, head_dim), or ``None`` when the kernel declines."""
     lib = _load()
-    attend = getattr(lib, f"kvq_splitzip_{kind}_attention_paged", None) if lib else None
+    attend = getattr(lib, "kvq_splitzip_chunk_attention_paged", None) if lib else None
     if attend is None or not _is_cuda(q):
         return None
     import torch
@@ -1628,46 +1655,12 @@ def _attend_paged(kind: str, q, kv_layer, tables, query_starts, context_tokens, 
                    workspace.data_ptr() if need else 0, need,
                    head_dim ** -0.5 if scale is None else float(scale))
     if got < 0:
-        _raise_last(lib, f"splitzip {kind} attention failed")
+        _raise_last(lib, "splitzip chunk attention failed")
     if not got:
         return None
     if given:
         _wrote(torch, *given)
     return out
-
-
-def chunk_attention_paged(q, kv_layer, tables, query_starts, context_tokens, *,
-                          max_query: int | None = None, scale: float | None = None, out=None,
-                          lse=None, workspace=None):
-    """Causal attention of a step's new tokens over a paged layer that holds their own K and V
-    already (``write_kv_paged``); single tokens (decode), chunks of prompts and drafted
-    tokens mixed in any way.
-
-    ``q`` (tokens, q_heads, head_dim) are the packed rows; request r's are rows
-    ``query_starts[r]`` .. ``query_starts[r + 1]``, the last of its ``context_tokens[r]``
-    tokens, so row i of its n sees tokens 0 .. context - n + i. Query head h reads KV head
-    h // (q_heads / kv_heads). ``tables`` (requests, width) int32 lists each request's blocks in
-    token order, ``query_starts`` (requests + 1) and ``context_tokens`` (requests) are int32;
-    all stay on the device (``StepPlan``), and a captured call follows their values.
-    ``max_query`` bounds the new tokens of a request (default: the rows of q); a smaller bound
-    spares a decode step the kernel for long chunks. ``scale`` (positive) defaults to head_dim
-    ** -0.5. ``lse`` (tokens, q_heads) float32 receives each row's log-sum-exp, for joining
-    with attention over other tokens. bf16 or fp16, head_dim 64 or 128; rows and heads of q
-    may be strided by multiples of 16 bytes.
-
-    A row that sees no token (context_tokens[r] less than its new tokens) is zero, its lse
-    -inf. Rows of no request, of one with more new tokens than max_query, and of one whose
-    row range is not inside q stay as they are. A context longer than its table, or a table
-    entry that is no block of the layer, makes the rows that read there NaN (every row of
-    the same tile, of 16 to 256 of a KV head's query rows, at least). Where
-    query_starts run backwards, so that ranges overlap, rows are one of their requests' or stay.
-    ``out``, ``lse`` and ``workspace`` over an input or each other are declined.
-    No gradient: inputs, ``out`` or ``lse`` that require one are declined while gradients are
-    recorded, and so are forward-mode tangents.
-
-    Returns ``out`` (tokens, q_heads, head_dim), or ``None`` when the kernel declines."""
-    return _attend_paged("chunk", q, kv_layer, tables, query_starts, context_tokens, max_query,
-                         scale, out, lse, workspace)
 
 
 def prompt_attention(q, k, v, query_starts, *, max_query: int | None = None,
@@ -1741,8 +1734,18 @@ def cross_attention_paged(q, kv_layer, tables, query_starts, source_tokens, *,
     tokens has rows of zero, their lse -inf.
 
     Returns ``out`` (tokens, q_heads, head_dim), or ``None`` when the kernel declines."""
-    return _attend_paged("cross", q, kv_layer, tables, query_starts, source_tokens, max_query, scale,
-                         out, lse, workspace)
+    lib = _load()
+    attend = getattr(lib, "kvq_splitzip_cross_attention_paged", None) if lib else None
+    if attend is None or not _is_cuda(q):
+        return None
+    import torch
+
+    got = _call_on(q.device, torch, _step_binding().cross_paged, _entry_address(attend),
+                   _entry_address(lib.kvq_splitzip_chunk_attention_workspace_bytes), q, kv_layer,
+                   tables, query_starts, source_tokens, max_query, scale, out, lse, workspace)
+    if type(got) is int:
+        _raise_last(lib, "splitzip cross attention failed")
+    return got
 
 
 def cross_attention(q, k, v, query_starts, source_starts, source_tokens, *,
@@ -1764,50 +1767,13 @@ def cross_attention(q, k, v, query_starts, source_starts, source_tokens, *,
         return None
     import torch
 
-    device = q.device
-    dtype = _row_dtype(q.dtype, torch)
-    if dtype is None or not _rows_ok(q, q.dtype, device) or not _rows_ok(k, q.dtype, device) or \
-            not _rows_ok(v, q.dtype, device):
-        return None
-    if _tracked(torch, q, k, v, out, lse):
-        return None
-    tokens, q_heads, head_dim = q.shape
-    rows, kv_heads = k.shape[:2]
-    requests = source_tokens.numel()
-    if k.shape != v.shape or k.shape[2] != head_dim or head_dim == 0 or \
-            not _index_vector_ok(source_tokens, device, 0, torch.int32) or \
-            not _index_vector_ok(source_starts, device, requests, torch.int32) or \
-            not _index_vector_ok(query_starts, device, requests + 1, torch.int32):
-        return None
-    max_query = tokens if max_query is None else min(int(max_query), tokens)
-    max_source = rows if max_source is None else min(int(max_source), rows)
-    given = [t for t in (out, lse) if t is not None]
-    ok, out = _attention_buffers(q, out, lse, torch)
-    if not ok:
-        return None
-    if tokens == 0 or requests == 0:
-        return out
-    if max_query <= 0 or max_source < 0 or rows == 0:
-        return None
-    need = _attention_workspace(
-        "kvq_splitzip_chunk_attention_workspace_bytes", device,
-        (tokens, requests, q_heads, kv_heads, head_dim, max_source, max_query))
-    if need and not _byte_buffer_ok(workspace, device, need, torch):
-        workspace = torch.empty(need, dtype=torch.uint8, device=device)
-    got = _call_on(device, torch, attend, q.data_ptr(), 2 * q.stride(0), 2 * q.stride(1),
-                   k.data_ptr(), 2 * k.stride(0), 2 * k.stride(1), v.data_ptr(), 2 * v.stride(0),
-                   2 * v.stride(1), rows, tokens, q_heads, kv_heads, head_dim, dtype,
-                   query_starts.data_ptr(), source_starts.data_ptr(), source_tokens.data_ptr(),
-                   requests, max_query, max_source, out.data_ptr(),
-                   0 if lse is None else lse.data_ptr(), workspace.data_ptr() if need else 0, need,
-                   head_dim ** -0.5 if scale is None else float(scale))
-    if got < 0:
+    got = _call_on(q.device, torch, _step_binding().cross_rows, _entry_address(attend),
+                   _entry_address(lib.kvq_splitzip_chunk_attention_workspace_bytes), q, k, v,
+                   query_starts, source_starts, source_tokens, max_query, max_source, scale, out, lse,
+                   workspace)
+    if type(got) is int:
         _raise_last(lib, "splitzip cross attention failed")
-    if not got:
-        return None
-    if given:
-        _wrote(torch, *given)
-    return out
+    return got
 
 
 # ---------------------------------------------------------------------------
