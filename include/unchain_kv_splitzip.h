@@ -625,8 +625,20 @@ long long kvq_splitzip_rotate_write_kv_paged(
     unsigned long long rotary_dim, unsigned long long adjacent, unsigned long long out_ptr,
     unsigned long long stream_ptr);
 
+/* Workspace bytes of the two calls below, as the chunk attention's for max_source = table_width *
+ * block_tokens, or the call's own: enough for every call of at most these sizes; and what a call of exactly
+ * these sizes asks for. */
+unsigned long long kvq_splitzip_cross_attention_workspace_bytes(
+    unsigned long long tokens, unsigned long long requests, unsigned long long q_heads,
+    unsigned long long kv_heads, unsigned long long head_dim, unsigned long long max_source,
+    unsigned long long max_query);
+unsigned long long kvq_splitzip_cross_attention_least_workspace_bytes(
+    unsigned long long tokens, unsigned long long requests, unsigned long long q_heads,
+    unsigned long long kv_heads, unsigned long long head_dim, unsigned long long max_source,
+    unsigned long long max_query);
+
 /* kvq_splitzip_chunk_attention_paged with every row of request r over all of its source_tokens[r] tokens
- * (rows of a request without tokens are 0, lse -inf); the same arguments and workspace. */
+ * (rows of a request without tokens are 0, lse -inf); the same arguments. */
 long long kvq_splitzip_cross_attention_paged(
     unsigned long long q_ptr, unsigned long long q_row_bytes, unsigned long long q_head_bytes,
     unsigned long long tokens, unsigned long long q_heads, unsigned long long kv_heads,
@@ -640,8 +652,7 @@ long long kvq_splitzip_cross_attention_paged(
 
 /* The same over packed sources: request r's are rows source_starts[r] .. + source_tokens[r] of k and v
  * (source_rows rows; strides multiples of 16). max_source (at most source_rows) bounds a source's tokens:
- * rows of requests with more stay. A source outside the rows gives NaN. Workspace: the above for max_context =
- * max_source. */
+ * rows of requests with more stay. A source outside the rows gives NaN. */
 long long kvq_splitzip_cross_attention(
     unsigned long long q_ptr, unsigned long long q_row_bytes, unsigned long long q_head_bytes,
     unsigned long long k_ptr, unsigned long long k_row_bytes, unsigned long long k_head_bytes,

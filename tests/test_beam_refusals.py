@@ -2,6 +2,7 @@
 calls make of gradients: no GPU needed (addresses are made up, and none is read)."""
 
 import ctypes
+import random
 from types import SimpleNamespace
 
 import pytest
@@ -38,7 +39,7 @@ def test_cross_over_a_layer_declines(lib):  # noqa: F811
         {"kv": A[1] + 8}, {"scale": ctypes.c_float(0.0)}, {"out": A[0] + 2048}, {"out": A[4]},
         {"lse": A[2]}])
     refused(lib.kvq_splitzip_cross_attention_paged, dict(CHUNK, stride=256, width=256),
-            no_workspace(lib.kvq_splitzip_chunk_attention_workspace_bytes(4, 2, 8, 2, 128, 4096, 4)))
+            no_workspace(lib.kvq_splitzip_cross_attention_least_workspace_bytes(4, 2, 8, 2, 128, 4096, 4)))
 
 
 CROSS = dict(q=A[0], q_row=2048, q_head=256, k=A[1], k_row=512, k_head=256, v=A[2], v_row=512, v_head=256,
@@ -56,9 +57,35 @@ def test_cross_over_rows_declines(lib):  # noqa: F811
         {"scale": ctypes.c_float(float("nan"))}, {"out": A[0]}, {"out": A[1] + 4999 * 512}, {"out": A[2]},
         {"out": A[4]}, {"lse": A[5] + 4}, {"lse": A[7]}])
     for max_query in (2, 4):  # streamed, and in tiles
-        size = lib.kvq_splitzip_chunk_attention_workspace_bytes(4, 2, 16, 2, 128, 5000, max_query)
+        size = lib.kvq_splitzip_cross_attention_least_workspace_bytes(4, 2, 16, 2, 128, 5000, max_query)
         refused(lib.kvq_splitzip_cross_attention, dict(CROSS, q_heads=16, max_query=max_query),
                 no_workspace(size) + [{"workspace": a - size + 16} for a in A[:6] + A[7:8]])
+
+
+def test_cross_workspace_serves_smaller_calls(lib):  # noqa: F811
+    """No call of smaller sizes asks for more; fewer sources are cut sooner, and a layer's and rows' alike."""
+    rng = random.Random(19)
+    least, bound = lib.kvq_splitzip_cross_attention_least_workspace_bytes, sz.cross_attention_workspace_bytes
+
+    def up_to(most):
+        return min(most, int(2 ** rng.uniform(0, most.bit_length())))
+
+    for q_heads, kv_heads, dim in ((8, 2, 128), (32, 8, 64), (16, 16, 64), (64, 1, 128), (1, 1, 64), (128, 8, 128)):
+        for _ in range(400):
+            most = [up_to(1 << 20), up_to(4096), up_to(1 << 14), up_to(1 << 10)]
+            tokens, requests, source, query = (up_to(n) for n in most)
+            query = min(query, tokens)
+            small = bound(tokens, requests, q_heads, kv_heads, dim, source, query)
+            assert least(tokens, requests, q_heads, kv_heads, dim, source, query) <= small
+            assert small <= bound(most[0], most[1], q_heads, kv_heads, dim, most[2], most[3])
+    # taken whole: sources of 192 workgroups; cut: of fewer
+    assert least(192, 192, 1, 1, 64, 2048, 1) == 0 < least(191, 191, 1, 1, 64, 2048, 1)
+    assert least(191, 191, 1, 1, 64, 2048, 1) <= bound(192, 192, 1, 1, 64, 2048, 1)
+    assert least(1, 1, 16, 16, 64, 768, 1) == 0 < least(1, 1, 16, 16, 64, 769, 1)
+    for sizes in ((8, 2, 8, 3, 128, 4096), (8, 2, 8, 2, 96, 4096), (-1, 2, 8, 2, 128, 4096), (8, 2, 8, 2, 128, -1)):
+        with pytest.raises(ValueError):
+            bound(*sizes)
+    assert bound(0, 2, 8, 2, 128, 4096) == 0
 
 
 SELECT = dict(logits=A[0], dtype=2, request=3000, beam=1000, scores=A[1], ended=A[2], requests=2, beams=3,
@@ -145,7 +172,7 @@ def entered(monkeypatch):
     for n, count in (("cross_attention_paged", 22), ("cross_attention", 25)):
         calls[f"kvq_splitzip_{n}"] = entry(n, *[u64] * count, ctypes.c_float, u64)
     sizes = {f"kvq_splitzip_{n}_workspace_bytes": ctypes.CFUNCTYPE(u64, *[u64] * count)(lambda *a: 16)
-             for n, count in (("beam_select", 3), ("reorder_beams", 3), ("chunk_attention", 7))}
+             for n, count in (("beam_select", 3), ("reorder_beams", 3), ("cross_attention_least", 7))}
     lib = SimpleNamespace(**calls, **sizes)
     monkeypatch.setattr(sz, "_load", lambda: lib)
     monkeypatch.setattr(sz, "_is_cuda", lambda t: True)

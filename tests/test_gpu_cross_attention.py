@@ -120,6 +120,22 @@ def test_matches_float64(sz, rows, source, q_heads, kv_heads, dim, block, dtype)
     case.verify(*case.packed(sz))
 
 
+SPLITS = [
+    # short splits of few sources, ends in each of them; as many sources as are taken whole, and one less
+    ([1], [769], 2, 2, 64, 16, "bf16"), ([3, 1], [1025, 130], 4, 2, 64, 16, "fp16"), ([5], [2049], 3, 3, 128, 16, "bf16"),
+    ([2, 1, 0, 4], [513, 9000, 700, 0], 8, 8, 128, 32, "fp16"), ([1], [16385], 4, 1, 64, 64, "bf16"),
+    ([1] * 192, [1025] + [3, 700] * 95 + [1600], 1, 1, 64, 16, "bf16"),
+    ([2] * 191, [1025] + [3, 700] * 95, 2, 1, 128, 16, "fp16")]
+
+
+@pytest.mark.parametrize("rows,source,q_heads,kv_heads,dim,block,dtype", SPLITS, ids=range(len(SPLITS)))
+def test_splits_match_float64(sz, rows, source, q_heads, kv_heads, dim, block, dtype):
+    say("splits", rows[:4], source[:4], q_heads, kv_heads, dim, block, dtype)
+    case = Case(rows, source, q_heads, kv_heads, dim, block, dtype, seed=max(source))
+    case.verify(*case.paged(sz, max_query=max(rows)))
+    case.verify(*case.packed(sz, max_query=max(rows), max_source=max(source)))
+
+
 @pytest.mark.parametrize("seed", range(6))
 def test_drawn_shapes(sz, seed):
     rng = np.random.default_rng(100 + seed)
@@ -219,7 +235,7 @@ def test_captured_calls_follow_lengths(sz):
     case = Case([4, 4, 4], [900, 1500, 1800], 4, 2, 64, 16, "bf16")
     rows, source = list(case.rows), list(case.source)
     b, b2 = case.buffers(), case.buffers()
-    ws = [torch.empty(max(sz.chunk_attention_workspace_bytes(15, 3, 4, 2, 64, n, 4), 1), dtype=torch.uint8,
+    ws = [torch.empty(max(sz.cross_attention_workspace_bytes(15, 3, 4, 2, 64, n, 4), 1), dtype=torch.uint8,
                       device="cuda") for n in (case.tables.shape[1] * 16, 1800)]
     torch.cuda.synchronize()
     graph = torch.cuda.CUDAGraph()

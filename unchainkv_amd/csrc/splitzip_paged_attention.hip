@@ -89,10 +89,15 @@ constexpr unsigned int kLeastTileSteps = 12;
 // for the host's second submission: captured 10.8 and 11.2; of 128 dims, uncut and cut, 768 tokens 13.7
 // and 16.0, 1024 the same, 1536 21.1 and 16.0).
 constexpr unsigned int kLeastFewSteps = 4, kWholeFewSteps = 8;
-// Sources are taken whole up to twice that where there are as many of them as workgroups to split for: mostly
-// they are of about one length, so that nothing would be cut (32 requests of 5 rows, 1500 tokens, 20 heads of
-// 64: 52 us, 58 with the launch that then joins nothing).
-constexpr unsigned int kWholeSourceSteps = 16;
+// Sources are mostly of about one length, so that cutting them gains no balance: up to twice that they are taken
+// whole where they fill three quarters of the CUs (12 requests of 5 rows, 1500 tokens, 20 heads of 64: 19.3 us and
+// 25.0; 30 of one row, 2000 tokens, 32 / 8 heads of 128: 41.9 and 47.1). Of those that leave most CUs idle, at most
+// an eighth of them taken, shorter ones are cut, and into more splits, up to 16 of one round (one request, captured:
+// 16 heads of 64, 1000 tokens 9.1 us and 11.2, 768 tokens 9.0 and 9.6, 640 tokens 9.0 and 8.8; 32 / 8 heads of 128,
+// 1000 tokens 11.4 and 16.4, 512 tokens 11.3 both; 8 requests of the latter, a quarter of the CUs, 2000 tokens 22.1
+// and 21.2).
+constexpr unsigned int kWholeSourceSteps = 16, kFineSplits = 16;
+constexpr unsigned int whole_fine_steps(unsigned long long head_dim) { return head_dim == 64 ? 6 : 4; }
 // A maximum before any token: the lowest float, not -inf, so that rows whose scores are all -inf
 // have weights of zero and a sum of zero (whose quotient is NaN, as the formula's).
 constexpr float kNoMax = -3.402823466e38f;
@@ -171,6 +176,7 @@ struct AttendArgs {
   Divider by_block;
   unsigned int tokens, requests, q_heads, kv_heads, group;
   unsigned int few_target, tile_target;   // workgroups to split for, of the two paths
+  unsigned int fine;          // 1: streamed splits may be shorter than kLeastFewSteps, up to kFineSplits of a request
   unsigned int max_query;     // requests with more new tokens are left out
   unsigned int max_source;    // and, of packed sources, those with more tokens
   unsigned int kv_rows;       // rows of packed sources
@@ -326,7 +332,9 @@ struct Work {
       sum += lane_value(wave_scan((unsigned int)min(own, (unsigned long long)kMostSteps)), 63);
     }
     const unsigned int parts = kTiles ? a.tile_target : a.few_target;
-    const unsigned int least = kTiles ? kLeastTileSteps : kLeastFewSteps;
+    unsigned int least = kTiles ? kLeastTileSteps : kLeastFewSteps;
+    if (!kTiles && a.fine != 0)
+      least = (unsigned int)min((unsigned long long)least, sum / (kFineSplits * a.requests) + 1);
     if (!large && a.slots != 0) cap = max(least, share_of(sum, a.kv_heads, parts));
   }
 
@@ -1501,11 +1509,16 @@ unsigned long long compute_units() {
 // longest context that the tables (or the rows) can hold, and the longest request. Which kernel it
 // is goes by the longest request's rows alone.
 struct Plan {
-  bool tiles;
+  bool tiles, fine;
   unsigned long long few_target, tile_target;  // workgroups that splits are made for
   unsigned long long groups, slots;            // workgroups, partial slots
   unsigned long long items;                    // of the tiles
 };
+
+// Splits of `active` requests at most, that are made for `target` workgroups, with one that has none.
+unsigned long long few_slots(unsigned long long target, unsigned long long kv_heads, unsigned long long active) {
+  return (target / kv_heads + active + 1) * kv_heads;
+}
 
 Plan plan_of(unsigned long long tokens, unsigned long long requests, unsigned long long kv_heads,
              unsigned long long group, unsigned long long head_dim, unsigned long long max_context,
@@ -1546,10 +1559,13 @@ Plan plan_of(unsigned long long tokens, unsigned long long requests, unsigned lo
     p.items = tiles + more;
     p.groups = (p.items + (cut ? 1 : 0)) * kv_heads;
   } else {
-    const bool many = !causal && active * kv_heads >= 2 * compute_units();
-    const bool cut = max_context > kFewUnit * (many ? kWholeSourceSteps : kWholeFewSteps);
-    p.groups = active * kv_heads;
-    if (cut) p.groups = p.slots = (p.few_target / kv_heads + active + 1) * kv_heads;
+    const unsigned long long whole = active * kv_heads, cus = compute_units();
+    p.fine = !causal && 8 * whole <= cus;
+    const unsigned int steps = causal ? kWholeFewSteps : p.fine ? whole_fine_steps(head_dim) :
+                               4 * whole >= 3 * cus ? kWholeSourceSteps : kWholeFewSteps;
+    const bool cut = max_context > kFewUnit * steps;
+    p.groups = whole;
+    if (cut) p.groups = p.slots = few_slots(p.few_target, kv_heads, active);
   }
   return p;
 }
@@ -1567,9 +1583,9 @@ unsigned long long workspace_of(const Plan& p, unsigned long long head_dim) {
 unsigned long long workspace_bound(unsigned long long tokens, unsigned long long requests,
                                    unsigned long long kv_heads, unsigned long long group,
                                    unsigned long long head_dim, unsigned long long max_context,
-                                   unsigned long long max_query, bool paged) {
+                                   unsigned long long max_query, bool paged, bool causal = true) {
   const unsigned long long own = workspace_of(
-      plan_of(tokens, requests, kv_heads, group, head_dim, max_context, max_query, paged), head_dim);
+      plan_of(tokens, requests, kv_heads, group, head_dim, max_context, max_query, paged, causal), head_dim);
   if (!paged) {
     // (of one prompt the shortest that can be cut at all is cut the soonest; all that are cut need the same)
     const unsigned long long n = std::min<unsigned long long>(max_query, kTileTokens * kLeastTileSteps + 1);
@@ -1577,11 +1593,11 @@ unsigned long long workspace_bound(unsigned long long tokens, unsigned long long
   }
   const unsigned long long few = std::min<unsigned long long>(max_query, kFewRows / group);
   if (few == 0) return own;
-  unsigned long long most = own;
-  for (const bool causal : {true, false})
-    most = std::max(most, workspace_of(plan_of(tokens, requests, kv_heads, group, head_dim, max_context, few, true,
-                                               causal), head_dim));
-  return most;
+  Plan most = plan_of(tokens, requests, kv_heads, group, head_dim, max_context, few, true, causal);
+  // (of fewer requests sources are cut that more of them leave whole)
+  if (!causal && max_context > kFewUnit * whole_fine_steps(head_dim))
+    most.slots = few_slots(most.few_target, kv_heads, std::min(tokens, requests));
+  return std::max(own, workspace_of(most, head_dim));
 }
 
 template <typename E, int D, bool kTiles>
@@ -1697,6 +1713,26 @@ extern "C" unsigned long long kvq_splitzip_prompt_attention_least_workspace_byte
                               false), head_dim);
 }
 
+extern "C" unsigned long long kvq_splitzip_cross_attention_workspace_bytes(
+    unsigned long long tokens, unsigned long long requests, unsigned long long q_heads,
+    unsigned long long kv_heads, unsigned long long head_dim, unsigned long long max_source,
+    unsigned long long max_query) {
+  max_query = std::min(max_query, tokens);
+  if (!sizes_ok(tokens, requests, q_heads, kv_heads, head_dim, max_query)) return 0;
+  return workspace_bound(tokens, requests, kv_heads, q_heads / kv_heads, head_dim, max_source, max_query, true,
+                         false);
+}
+
+extern "C" unsigned long long kvq_splitzip_cross_attention_least_workspace_bytes(
+    unsigned long long tokens, unsigned long long requests, unsigned long long q_heads,
+    unsigned long long kv_heads, unsigned long long head_dim, unsigned long long max_source,
+    unsigned long long max_query) {
+  max_query = std::min(max_query, tokens);
+  if (!sizes_ok(tokens, requests, q_heads, kv_heads, head_dim, max_query)) return 0;
+  return workspace_of(plan_of(tokens, requests, kv_heads, q_heads / kv_heads, head_dim, max_source, max_query, true,
+                              false), head_dim);
+}
+
 namespace {
 
 // Over a paged layer: a step's own context (causal), or a source.
@@ -1758,6 +1794,7 @@ long long attend_paged(
   a.kv_heads = (unsigned int)kv_heads;
   a.group = (unsigned int)(q_heads / kv_heads);
   a.few_target = (unsigned int)plan.few_target;
+  a.fine = plan.fine ? 1 : 0;
   a.tile_target = (unsigned int)plan.tile_target;
   a.max_query = (unsigned int)max_query;
   a.causal = causal ? 1 : 0;
@@ -1850,6 +1887,7 @@ extern "C" long long kvq_splitzip_prompt_attention(
   a.kv_heads = (unsigned int)kv_heads;
   a.group = (unsigned int)(q_heads / kv_heads);
   a.few_target = (unsigned int)plan.few_target;
+  a.fine = plan.fine ? 1 : 0;
   a.tile_target = (unsigned int)plan.tile_target;
   a.max_query = (unsigned int)max_query;
   a.causal = 1;
@@ -1917,6 +1955,7 @@ extern "C" long long kvq_splitzip_cross_attention(
   a.kv_heads = (unsigned int)kv_heads;
   a.group = (unsigned int)(q_heads / kv_heads);
   a.few_target = (unsigned int)plan.few_target;
+  a.fine = plan.fine ? 1 : 0;
   a.tile_target = (unsigned int)plan.tile_target;
   a.max_query = (unsigned int)max_query;
   a.max_source = (unsigned int)max_source;

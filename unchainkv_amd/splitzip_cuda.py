@@ -167,6 +167,8 @@ _SIGNATURES = (
     ("kvq_splitzip_chunk_attention_workspace_bytes", [_U64] * 7, _U64, False),
     ("kvq_splitzip_prompt_attention_workspace_bytes", [_U64] * 6, _U64, False),
     ("kvq_splitzip_prompt_attention_least_workspace_bytes", [_U64] * 6, _U64, False),
+    ("kvq_splitzip_cross_attention_workspace_bytes", [_U64] * 7, _U64, False),
+    ("kvq_splitzip_cross_attention_least_workspace_bytes", [_U64] * 7, _U64, False),
     ("kvq_splitzip_chunk_attention_paged", [_U64] * 22 + [ctypes.c_float, _U64],
      ctypes.c_longlong, False),
     ("kvq_splitzip_prompt_attention", [_U64] * 21 + [ctypes.c_float, _U64],
@@ -1721,6 +1723,23 @@ def prompt_attention(q, k, v, query_starts, *, max_query: int | None = None,
     return out
 
 
+def cross_attention_workspace_bytes(tokens: int, requests: int, q_heads: int, kv_heads: int,
+                                    head_dim: int, max_source: int,
+                                    max_query: int | None = None) -> int:
+    """Workspace of ``cross_attention_paged`` and ``cross_attention`` for ``tokens`` rows of q and
+    sources of up to ``max_source`` tokens (over a layer: what a row of the block tables can hold),
+    enough for every call of at most these sizes with these heads (0: none is needed). Sizes that
+    the calls decline raise ``ValueError``."""
+    lib = _load()
+    if lib is None or not hasattr(lib, "kvq_splitzip_cross_attention_workspace_bytes"):
+        raise RuntimeError(f"HIP codec library not loaded: {load_error()}")
+    sizes = _workspace_sizes(tokens, requests, q_heads, kv_heads, head_dim, max_query)
+    if max_source < 0:
+        raise ValueError(f"a source of {max_source} tokens")
+    return 0 if sizes is None else int(lib.kvq_splitzip_cross_attention_workspace_bytes(
+        *sizes[:5], max_source, sizes[5]))
+
+
 def cross_attention_paged(q, kv_layer, tables, query_starts, source_tokens, *,
                           max_query: int | None = None, scale: float | None = None, out=None,
                           lse=None, workspace=None):
@@ -1730,7 +1749,7 @@ def cross_attention_paged(q, kv_layer, tables, query_starts, source_tokens, *,
     the blocks that row r of ``tables`` lists, so the beams of a request, given as its rows, read
     its source once. Everything else is as in ``chunk_attention_paged``: types, heads, strides,
     ``max_query`` (of a request's rows), ``scale``, ``lse``, ``workspace`` (of
-    ``chunk_attention_workspace_bytes``), captured calls, gradients. A request without source
+    ``cross_attention_workspace_bytes``), captured calls, gradients. A request without source
     tokens has rows of zero, their lse -inf.
 
     Returns ``out`` (tokens, q_heads, head_dim), or ``None`` when the kernel declines."""
@@ -1741,7 +1760,7 @@ def cross_attention_paged(q, kv_layer, tables, query_starts, source_tokens, *,
     import torch
 
     got = _call_on(q.device, torch, _step_binding().cross_paged, _entry_address(attend),
-                   _entry_address(lib.kvq_splitzip_chunk_attention_workspace_bytes), q, kv_layer,
+                   _entry_address(lib.kvq_splitzip_cross_attention_least_workspace_bytes), q, kv_layer,
                    tables, query_starts, source_tokens, max_query, scale, out, lse, workspace)
     if type(got) is int:
         _raise_last(lib, "splitzip cross attention failed")
@@ -1755,10 +1774,11 @@ def cross_attention(q, k, v, query_starts, source_starts, source_tokens, *,
     head_dim): request r's is the ``source_tokens[r]`` rows from ``source_starts[r]`` on (packed one
     behind the other, padded to one length, or shared between requests; int32, on the device).
     ``max_source`` bounds a source's tokens (default: all rows of k): a smaller bound, up to 1024,
-    spares a call of few rows the joining of splits. Requests whose source is longer stay as they
+    spares a call of few rows the joining of splits (up to 512 where requests * kv_heads is 32 or
+    less). Requests whose source is longer stay as they
     are, like those with more than ``max_query`` rows; a source that is not inside k makes its
     request's rows NaN. Rows and heads of k and v may be strided by multiples of 16 bytes. The
-    workspace is that of ``chunk_attention_workspace_bytes`` with ``max_source`` as the context.
+    workspace is that of ``cross_attention_workspace_bytes``.
 
     Returns ``out`` (tokens, q_heads, head_dim), or ``None`` when the kernel declines."""
     lib = _load()
@@ -1768,7 +1788,7 @@ def cross_attention(q, k, v, query_starts, source_starts, source_tokens, *,
     import torch
 
     got = _call_on(q.device, torch, _step_binding().cross_rows, _entry_address(attend),
-                   _entry_address(lib.kvq_splitzip_chunk_attention_workspace_bytes), q, k, v,
+                   _entry_address(lib.kvq_splitzip_cross_attention_least_workspace_bytes), q, k, v,
                    query_starts, source_starts, source_tokens, max_query, max_source, scale, out, lse,
                    workspace)
     if type(got) is int:
