@@ -5,8 +5,8 @@
 // and 12, reorder_beams_paged of 16 layers (two launches) 26.5 and 14. Each function takes the entries' addresses
 // first and the stream last, and gives the results, None where the call is declined, or -1 where the entry failed;
 // an argument that is no tensor raises TypeError.
-#include <ATen/EmptyTensor.h>
 #include <ATen/core/Tensor.h>
+#include <ATen/ops/empty.h>
 #include <Python.h>
 #include <c10/core/GradMode.h>
 #include <torch/csrc/Exceptions.h>
@@ -95,19 +95,12 @@ void wrote(const at::Tensor& t) {
   if (t.defined() && !t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
-// A new tensor on the current device of that type (at::empty's own work without its dispatch: 0.3 us of 0.9).
-at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType dtype, at::Device device) {
-  const c10::DispatchKey key = c10::computeDispatchKey(dtype, at::kStrided, device);
-  return at::detail::empty_generic(sizes, c10::GetAllocator(device.type()), c10::DispatchKeySet(key), dtype,
-                                   std::nullopt);
-}
-
 // `given`, if it is a workspace of `need` bytes, or a new one.
 at::Tensor workspace_of(const at::Tensor& given, u64 need, at::Device device) {
   if (given.defined() && given.scalar_type() == at::kByte && given.is_contiguous() && given.device() == device &&
       (u64)given.numel() >= need)
     return given;
-  return fresh({(int64_t)need}, at::kByte, device);
+  return at::empty({(int64_t)need}, at::TensorOptions().dtype(at::kByte).device(device));
 }
 
 PyObject* none() { Py_RETURN_NONE; }
@@ -157,7 +150,7 @@ PyObject* rotate_write(PyObject*, PyObject* const* args, Py_ssize_t n) {
       !rotation.is_contiguous() || tracked({&q, &k, &v, &kv, &rotation, &out}) ||
       (given && !matrix_ok(out, q.sizes(), device, q.scalar_type())))
     return none();
-  if (!given) out = fresh(q.sizes(), q.scalar_type(), device);
+  if (!given) out = at::empty(q.sizes(), q.options());
   if (tokens == 0) return THPVariable_Wrap(out);
   const u64 places = (u64)(kv.size(1) * kv.size(2));
   typedef long long (*Entry)(u64, u64, u64, u64, u64, u64, u64, u64, u64, u64, u64, u64, u64, u64, u64, u64, u64, u64,
@@ -224,7 +217,7 @@ PyObject* cross_paged(PyObject*, PyObject* const* args, Py_ssize_t n) {
     return none();
   const int64_t max_query = count_of(args[7], tokens);
   const float scale = scale_of(args[8], dim);
-  if (!given) out = fresh(q.sizes(), q.scalar_type(), device);
+  if (!given) out = at::empty(q.sizes(), q.options());
   if (tokens == 0 || requests == 0) return THPVariable_Wrap(out);
   if (max_query <= 0 || width == 0) return none();
   const u64 need = reinterpret_cast<AttentionSize>(size)((u64)tokens, (u64)requests, (u64)heads, (u64)kv.size(3),
@@ -268,7 +261,7 @@ PyObject* cross_rows(PyObject*, PyObject* const* args, Py_ssize_t n) {
     return none();
   const int64_t max_query = count_of(args[8], tokens), max_source = count_of(args[9], rows);
   const float scale = scale_of(args[10], dim);
-  if (!given) out = fresh(q.sizes(), q.scalar_type(), device);
+  if (!given) out = at::empty(q.sizes(), q.options());
   if (tokens == 0 || requests == 0) return THPVariable_Wrap(out);
   if (max_query <= 0 || max_source < 0 || rows == 0) return none();
   const u64 need = reinterpret_cast<AttentionSize>(size)((u64)tokens, (u64)requests, (u64)heads, (u64)kv_heads,
@@ -315,9 +308,10 @@ PyObject* beam_select(PyObject*, PyObject* const* args, Py_ssize_t n) {
                   matrix_ok(tokens, picked, device, at::kLong))))
     return none();
   if (!given) {
-    best = fresh(picked, at::kFloat, device);
-    parents = fresh(picked, at::kInt, device);
-    tokens = fresh(picked, at::kLong, device);
+    const at::TensorOptions on = at::TensorOptions().device(device);
+    best = at::empty(picked, on.dtype(at::kFloat));
+    parents = at::empty(picked, on.dtype(at::kInt));
+    tokens = at::empty(picked, on.dtype(at::kLong));
   }
   if (requests == 0) return tuple_of({best, parents, tokens});
   const u64 need = reinterpret_cast<u64 (*)(u64, u64, u64)>(size)((u64)requests, (u64)beams, (u64)vocab);
@@ -372,10 +366,11 @@ PyObject* reorder_beams(PyObject*, PyObject* const* args, Py_ssize_t n) {
     row_bytes = 2 * (u64)(layer.size(3) * layer.size(4));
   }
   const bool given = order[0].defined();
+  const at::TensorOptions ints = at::TensorOptions().dtype(at::kInt).device(device);
   if (!given) {
-    order[0] = fresh({rows, width}, at::kInt, device);
-    order[1] = fresh({rows}, at::kInt, device);
-    for (int i = 2; i < 5; ++i) order[i] = fresh({1}, at::kInt, device);
+    order[0] = at::empty({rows, width}, ints);
+    order[1] = at::empty({rows}, ints);
+    for (int i = 2; i < 5; ++i) order[i] = at::empty({1}, ints);
   } else if (order[0].scalar_type() != at::kInt || order[0].sizes() != tables.sizes() ||
              order[0].device() != device || (width != 1 && order[0].stride(1) != 1) ||
              !vector_ok(order[1], device, rows, at::kInt) || !vector_ok(order[2], device, 1, at::kInt) ||
