@@ -195,3 +195,33 @@ def test_a_captured_search(sz):
         graph.replay()
         torch.cuda.synchronize()
         dense.follow()
+
+
+def test_results_are_ordinary_tensors(sz):
+    """What the calls allocate for themselves can be used as any other tensor, in either mode."""
+    q = torch.randn((3, 4, 64), device="cuda").bfloat16()
+    k, v = q[:, :2], q[:, 2:]
+    kv = torch.zeros((2, 4, 16, 2, 64), dtype=torch.bfloat16, device="cuda")
+    at = torch.arange(3, device="cuda")
+    tables, starts, count = i32([[0, 1]]), i32([0, 3]), i32([3])
+
+    def calls():
+        choice = sz.beam_select(torch.randn((2, 3, 50), device="cuda"), torch.zeros((2, 3), device="cuda"))
+        order = sz.reorder_beams_paged([kv], i32([[0], [1]]), i32([[0, 0]]), i32([3, 3]), i32([3, 2]), i32([0]), 16)
+        return [sz.rotate_write_kv_paged(q, k, v, kv, at, at, sz.rotation_table(9, 64)),
+                sz.cross_attention_paged(q, kv, tables, starts, count),
+                sz.cross_attention(q, k, v, starts, i32([0]), count), *choice, *order]
+
+    for got in calls():
+        assert type(got) is torch.Tensor and got.device == q.device and got.is_contiguous()
+        assert not got.is_inference() and not got.requires_grad and got._version == 0
+        assert torch.equal(got.clone(), got.cpu().cuda()) and torch.empty_like(got).shape == got.shape
+        leaf = got.float().clone().requires_grad_()
+        (leaf * leaf).sum().backward()
+        assert torch.equal(leaf.grad, 2 * leaf)
+        got.add_(1)
+        assert got._version == 1
+    with torch.inference_mode():
+        results = calls()
+        assert all(got.is_inference() for got in results)
+    assert all(torch.isfinite(got.float()).all() for got in results)

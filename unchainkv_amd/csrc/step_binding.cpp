@@ -2,7 +2,7 @@
 // cross_attention_paged, cross_attention, beam_select and reorder_beams_paged check, allocate and pass on. A
 // small call is bound by its host time, of which tensors' attributes read one by one from Python took more than
 // the launch: us a call with them and with this, rotate_write_kv_paged 13.2 and 6, beam_select (two launches) 17.3
-// and 12, reorder_beams_paged of 16 layers (two launches) 26.5 and 14. Each function takes the entries' addresses
+// and 12, reorder_beams_paged of 16 layers (two launches) 26.5 and 14.5. Each function takes the entries' addresses
 // first and the stream last, and gives the results, None where the call is declined, or -1 where the entry failed;
 // an argument that is no tensor raises TypeError.
 #include <ATen/core/Tensor.h>
