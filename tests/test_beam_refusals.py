@@ -9,6 +9,7 @@ import pytest
 
 from beam_order_ref import reorder
 from test_step_refusals import A, CHUNK, SCALE, lib, no_workspace, refused  # noqa: F401 (lib: a fixture)
+from unchainkv_amd import _build
 from unchainkv_amd import splitzip_cuda as sz
 
 MiB = 1 << 20
@@ -159,6 +160,8 @@ def test_tensors_off_the_gpu_are_declined():
 @pytest.fixture
 def entered(monkeypatch):
     """The names of the entries that were called."""
+    if not _build.BINDING_PATH.exists():
+        _build.build_binding()
     names, u64 = [], ctypes.c_ulonglong
 
     def entry(name, *types):

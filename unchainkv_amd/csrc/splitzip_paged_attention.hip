@@ -1887,7 +1887,6 @@ extern "C" long long kvq_splitzip_prompt_attention(
   a.kv_heads = (unsigned int)kv_heads;
   a.group = (unsigned int)(q_heads / kv_heads);
   a.few_target = (unsigned int)plan.few_target;
-  a.fine = plan.fine ? 1 : 0;
   a.tile_target = (unsigned int)plan.tile_target;
   a.max_query = (unsigned int)max_query;
   a.causal = 1;

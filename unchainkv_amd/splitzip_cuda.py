@@ -1935,7 +1935,8 @@ def reorder_beams_paged(layers, tables, parents, context_tokens, free_blocks, fr
 
     ``order`` (from ``new_beam_order`` or an earlier call of the same sizes) takes the results; its
     ``tables`` may be ``tables`` itself, to reorder in place. Other results, the layers and ``free_blocks``
-    must not lie over an input or each other. At most 32 beams.
+    must not lie over an input or each other. ``workspace`` (of ``reorder_beams_workspace_bytes``) as
+    in ``beam_select``. At most 32 beams.
 
     Returns a ``BeamOrder``, or ``None`` when the kernel declines."""
     lib = _load()
