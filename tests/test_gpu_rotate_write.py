@@ -98,6 +98,34 @@ def test_matches_the_rotation(sz, tokens, q_heads, kv_heads, dim, rotary, dtype,
     check(sz, tokens, q_heads, kv_heads, dim, rotary, adjacent, dtype, seed=tokens)
 
 
+@pytest.mark.parametrize("adjacent", (False, True))
+@pytest.mark.parametrize("tokens,q_heads,kv_heads,dim,rotary,spread,shift", [
+    (5, 64, 20, 128, 20, 0, 0), (3, 64, 20, 128, 128, 0, 0), (4, 71, 9, 64, 64, 0, 1), (6, 200, 4, 64, 48, 4, 0),
+    (3, 128, 128, 68, 20, 0, 4), (2, 300, 1, 128, 126, 0, 0), (1, 1, 400, 64, 4, 0, 0)])
+def test_many_heads(sz, tokens, q_heads, kv_heads, dim, rotary, spread, shift, adjacent):
+    """Heads shared by several waves, in units of 16, 8 and 2 bytes; one token without a slot."""
+    say("heads", tokens, q_heads, kv_heads, dim, rotary, spread, shift, adjacent)
+    check(sz, tokens, q_heads, kv_heads, dim, rotary, adjacent, "bf16", spread, shift, seed=q_heads,
+          drop=[(tokens - 1, -1)] if tokens > 2 else ())
+
+
+def test_more_tokens_than_a_launch_takes(sz):
+    say("many tokens")
+    tokens = (1 << 24) + 5
+    at = torch.arange(tokens, device="cuda")
+    q = (at % 251).to(torch.bfloat16).view(-1, 1, 1).expand(-1, 1, 2).contiguous()
+    k, v = q + 1, q + 2
+    kv = torch.full((2, tokens + 3, 1, 1, 2), MARK, dtype=torch.bfloat16, device="cuda")
+    # quarters of a turn: (x, y) -> (x, y), (-y, x), (-x, -y), (y, -x)
+    table = torch.tensor([[1.0, 0.0], [0.0, 1.0], [-1.0, 0.0], [0.0, -1.0]], device="cuda")
+    got = sz.rotate_write_kv_paged(q, k, v, kv, at.flip(0), at % 4, table)
+    for turned, x in ((got, q), (kv[0, :tokens].flip(0)[:, 0], k)):
+        x, y = x[..., 0], x[..., 1]
+        for turn, pair in enumerate(((x, y), (-y, x), (-x, -y), (y, -x))):
+            assert torch.equal(turned[turn::4], torch.stack(pair, -1)[turn::4])
+    assert torch.equal(kv[1, :tokens].flip(0)[:, 0], v) and (kv[:, tokens:] == MARK).all()
+
+
 @pytest.mark.parametrize("spread,shift", [(8, 0), (0, 1), (3, 5), (16, 8)])
 def test_strides_and_addresses(sz, spread, shift):
     say("strides", spread, shift)

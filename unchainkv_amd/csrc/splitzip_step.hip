@@ -260,26 +260,32 @@ struct RotateArgs {
   unsigned int first;          // token of this launch
   unsigned int units;          // of the pairs of a head
   unsigned int lanes_heads;    // heads that a wave's lanes take at once
+  unsigned int rotating, waves_log;  // waves of a token that rotate, and the logarithm of all
   Divider by_rest, by_head;    // units of a head that are not rotated, and all
 };
 
-constexpr unsigned int kMostRotated = 1u << 24;  // tokens of a launch, whose threads fit 32 bits
+// Of a lane, before another wave of the token takes its share: 8192 tokens of 64 + 2 x 20 heads of 128, all rotated
+// 82.6 us (one wave for each sort 86.8; one batch a lane 112), 20 of 128 values rotated 142 (307); 125 tokens of the
+// latter's kind 4.5 (39).
+constexpr unsigned int kRotatedBatches = 2, kCopiedUnits = 4;
+constexpr unsigned int kMostRotated = 1u << 25;  // waves of a launch, whose threads fit 32 bits
 
 template <typename E, int N>
 struct Values {
   typedef E type __attribute__((ext_vector_type(N)));
 };
 
-// Two waves for each token. In the first a lane keeps the cosines and sines of N pairs and takes them to one
-// head after another: N values of its first half and N of its second, or (kAdjacent) 2 N values side by side.
-// The second copies what is not rotated, the heads' other values and V, and waits for no position or table.
-// kBatch: heads of a lane whose loads go out together.
-template <typename E, int N, bool kAdjacent, int kBatch>
+// Two sorts of waves for each token. In the first a lane keeps the cosines and sines of N pairs and takes them to
+// one head after another: N values of its first half and N of its second, or (kAdjacent) 2 N values side by side.
+// The second copies what is not rotated, the heads' other values and V, kUnit at a time, and waits for no position
+// or table. kBatch: heads of a lane whose loads go out together.
+template <typename E, int N, int kUnit, bool kAdjacent, int kBatch>
 __global__ __launch_bounds__(kStepThreads) void rotate_rows(RotateArgs a) {
   typedef typename Values<E, N>::type Unit;
+  typedef typename Values<uint16_t, kUnit>::type Copy;
   const unsigned int lane = threadIdx.x & 63;
   const unsigned int job = uniform(blockIdx.x * (kStepThreads / kWave) + (threadIdx.x >> 6));
-  const unsigned int token = a.first + job / 2;
+  const unsigned int waves = 1u << a.waves_log, wave = job & (waves - 1), token = a.first + (job >> a.waves_log);
   if (token >= a.tokens) return;
   const long long slot = a.slots[token];
   const bool write = slot >= 0 && (unsigned long long)slot < a.slot_count;
@@ -296,7 +302,7 @@ __global__ __launch_bounds__(kStepThreads) void rotate_rows(RotateArgs a) {
   auto target = [&](unsigned int h) {
     return h < a.q_heads ? out + h * head_bytes : layer + (h - a.q_heads) * head_bytes;
   };
-  if (job % 2 == 0) {
+  if (wave < a.rotating) {
     const long long position = a.positions[token];
     const bool known = position >= 0 && (unsigned long long)position < a.table_rows;
     const float* const table = a.table + (known ? (unsigned long long)position * a.rotary : 0ull);
@@ -306,7 +312,8 @@ __global__ __launch_bounds__(kStepThreads) void rotate_rows(RotateArgs a) {
       const unsigned int at = (kAdjacent ? 2 * N : N) * sizeof(E) * u;
       const unsigned int at2 = at + (kAdjacent ? N : pairs) * sizeof(E);
       float c[N], s[N];
-      for (unsigned int h0 = sub; h0 < heads; h0 += kBatch * a.lanes_heads) {
+      const unsigned int start = wave * kBatch * a.lanes_heads + sub, step = a.rotating * kBatch * a.lanes_heads;
+      for (unsigned int h0 = start; h0 < heads; h0 += step) {
         // (the rows' loads go out before the table's, which wait for the position)
         Unit x[kBatch], y[kBatch];
 #pragma unroll
@@ -316,7 +323,7 @@ __global__ __launch_bounds__(kStepThreads) void rotate_rows(RotateArgs a) {
           x[b] = *reinterpret_cast<const Unit*>(src + at);
           y[b] = *reinterpret_cast<const Unit*>(src + at2);
         }
-        if (h0 == sub) {
+        if (h0 == start) {
 #pragma unroll
           for (int i = 0; i < N; ++i) {
             c[i] = known ? table[u * N + i] : NAN;
@@ -347,11 +354,12 @@ __global__ __launch_bounds__(kStepThreads) void rotate_rows(RotateArgs a) {
     return;
   }
   const unsigned char* const v = a.v + token * a.v_row;
-  const unsigned int rest = (a.dim - a.rotary) / N, head_units = a.dim / N;
+  const unsigned int rest = (a.dim - a.rotary) / kUnit, head_units = a.dim / kUnit;
   const unsigned int others = rest * heads, all = others + (write ? head_units * a.kv_heads : 0u);
-  constexpr int kCopies = 2;
-  for (unsigned int i0 = lane; i0 < all; i0 += kCopies * kWave) {
-    Unit x[kCopies];
+  constexpr int kCopies = kUnit == 8 ? 2 : 4;
+  const unsigned int copying = waves - a.rotating;
+  for (unsigned int i0 = (wave - a.rotating) * kCopies * kWave + lane; i0 < all; i0 += copying * kCopies * kWave) {
+    Copy x[kCopies];
     unsigned char* dst[kCopies];
 #pragma unroll
     for (int n = 0; n < kCopies; ++n) {
@@ -359,37 +367,56 @@ __global__ __launch_bounds__(kStepThreads) void rotate_rows(RotateArgs a) {
       const bool value = use >= others;
       const unsigned int in = value ? use - others : use;
       const unsigned int h = div_u32(in, value ? a.by_head.m : a.by_rest.m, value ? a.by_head.d : a.by_rest.d);
-      const unsigned int at = ((value ? 0u : a.rotary) + (in - h * (value ? head_units : rest)) * N) * sizeof(E);
-      x[n] = *reinterpret_cast<const Unit*>((value ? v + h * a.v_head : source(h)) + at);
+      const unsigned int at = ((value ? 0u : a.rotary) + (in - h * (value ? head_units : rest)) * kUnit) * sizeof(E);
+      x[n] = *reinterpret_cast<const Copy*>((value ? v + h * a.v_head : source(h)) + at);
       dst[n] = (value ? layer + a.plane_bytes + h * head_bytes : target(h)) + at;
     }
 #pragma unroll
     for (int n = 0; n < kCopies; ++n)
-      if (i0 + n * kWave < all) *reinterpret_cast<Unit*>(dst[n]) = x[n];
+      if (i0 + n * kWave < all) *reinterpret_cast<Copy*>(dst[n]) = x[n];
   }
 }
 
 // As many heads at once as a lane has, up to 5: 32768 tokens of 32 + 8 heads of 128, five of them for a lane,
 // 146 us at 5, 149 at 3, 153 at 1; 4700 of 24 + 3 heads, 32 of 64 values rotated, one for a lane, 10.8 us at 1,
 // 12.0 at 3, as places past the last head load it again.
-template <typename E, int N, bool kAdjacent>
-void launch_batch(const RotateArgs& a, hipStream_t stream) {
-  const unsigned int waves = kStepThreads / kWave, own = (a.q_heads + a.kv_heads + a.lanes_heads - 1) / a.lanes_heads;
-  const dim3 grid((2 * std::min(a.tokens - a.first, kMostRotated) + waves - 1) / waves), threads(kStepThreads);
-  if (own == 1)
-    hipLaunchKernelGGL((rotate_rows<E, N, kAdjacent, 1>), grid, threads, 0, stream, a);
-  else if (own <= 3)
-    hipLaunchKernelGGL((rotate_rows<E, N, kAdjacent, 3>), grid, threads, 0, stream, a);
-  else
-    hipLaunchKernelGGL((rotate_rows<E, N, kAdjacent, 5>), grid, threads, 0, stream, a);
+template <typename E, int N, int kUnit, bool kAdjacent>
+void launch_batch(RotateArgs a, hipStream_t stream) {
+  const unsigned int own = (a.q_heads + a.kv_heads + a.lanes_heads - 1) / a.lanes_heads;
+  const unsigned int batch = own == 1 ? 1 : own <= 3 ? 3 : 5;
+  const unsigned int copies = ((a.dim - a.rotary) * (a.q_heads + a.kv_heads) + a.dim * a.kv_heads) / kUnit;
+  // (one of each sort, or up to 8 in all, at most half of them rotating)
+  auto waves = [](unsigned int work, unsigned int each) { return std::max((work + each - 1) / each, 1u); };
+  a.rotating = std::min(waves(own, kRotatedBatches * batch), 4u);
+  a.waves_log = 1;
+  while (a.waves_log < 3 && 1u << a.waves_log < a.rotating + waves(copies, kCopiedUnits * kWave)) ++a.waves_log;
+  a.by_rest = make_divider((a.dim - a.rotary) / kUnit);
+  a.by_head = make_divider(a.dim / kUnit);
+  constexpr unsigned int kWaves = kStepThreads / kWave;
+  const unsigned int most = kMostRotated >> a.waves_log;
+  for (unsigned int left = a.tokens; left != 0;) {
+    const unsigned int now = std::min(left, most);
+    a.first = a.tokens - left;
+    const dim3 grid(((now << a.waves_log) + kWaves - 1) / kWaves), threads(kStepThreads);
+    if (batch == 1)
+      hipLaunchKernelGGL((rotate_rows<E, N, kUnit, kAdjacent, 1>), grid, threads, 0, stream, a);
+    else if (batch == 3)
+      hipLaunchKernelGGL((rotate_rows<E, N, kUnit, kAdjacent, 3>), grid, threads, 0, stream, a);
+    else
+      hipLaunchKernelGGL((rotate_rows<E, N, kUnit, kAdjacent, 5>), grid, threads, 0, stream, a);
+    left -= now;
+  }
 }
 
+// unit: values of a copy
 template <typename E, bool kAdjacent>
-void launch_rotate(const RotateArgs& a, bool wide, hipStream_t stream) {
-  if (wide)
-    launch_batch<E, 8, kAdjacent>(a, stream);
+void launch_rotate(const RotateArgs& a, unsigned int unit, hipStream_t stream) {
+  if (unit == 8)
+    launch_batch<E, 8, 8, kAdjacent>(a, stream);
+  else if (unit == 4)
+    launch_batch<E, 2, 4, kAdjacent>(a, stream);
   else
-    launch_batch<E, 1, kAdjacent>(a, stream);
+    launch_batch<E, 1, 1, kAdjacent>(a, stream);
 }
 
 }  // namespace
@@ -554,10 +581,12 @@ extern "C" long long kvq_splitzip_rotate_write_kv_paged(
     for (const auto& i : in)
       if (overlap(o[0], o[1], i[0], i[1])) return 0;
   if (overlap(out[0][0], out[0][1], out[1][0], out[1][1])) return 0;
-  // 8 values at a time where every row, head and address allows it, and both parts of a head are such runs
-  const bool wide = (q_ptr | q_row_bytes | k_ptr | k_row_bytes | v_ptr | v_row_bytes | kv_ptr | plane_bytes |
-                     out_ptr | (q_heads > 1 ? q_head_bytes : 0) |
-                     (kv_heads > 1 ? k_head_bytes | v_head_bytes : 0) | rotary_dim | head_bytes) % 16 == 0;
+  // 8 values at a time where every row, head and address allows it, and both parts of a head are such runs;
+  // else two pairs and copies of 4 values, or one by one
+  const unsigned long long all = q_ptr | q_row_bytes | k_ptr | k_row_bytes | v_ptr | v_row_bytes | kv_ptr |
+                                 plane_bytes | out_ptr | (q_heads > 1 ? q_head_bytes : 0) |
+                                 (kv_heads > 1 ? k_head_bytes | v_head_bytes : 0) | head_bytes;
+  const unsigned int unit = (all | rotary_dim) % 16 == 0 ? 8 : (all | 2 * rotary_dim) % 8 == 0 ? 4 : 1;
   RotateArgs a{};
   a.q = reinterpret_cast<const unsigned char*>(q_ptr);
   a.k = reinterpret_cast<const unsigned char*>(k_ptr);
@@ -581,19 +610,14 @@ extern "C" long long kvq_splitzip_rotate_write_kv_paged(
   a.kv_heads = (unsigned int)kv_heads;
   a.dim = (unsigned int)head_dim;
   a.rotary = (unsigned int)rotary_dim;
-  a.units = (unsigned int)(rotary_dim / 2 / (wide ? 8 : 1));
+  a.units = (unsigned int)(rotary_dim / 2 / (unit == 8 ? 8 : unit == 4 ? 2 : 1));
   a.lanes_heads = std::max(1u, kWave / a.units);
-  a.by_rest = make_divider((a.dim - a.rotary) / (wide ? 8 : 1));
-  a.by_head = make_divider(a.dim / (wide ? 8 : 1));
   hipStream_t stream = reinterpret_cast<hipStream_t>(stream_ptr);
-  for (unsigned long long first = 0; first < tokens; first += kMostRotated) {
-    a.first = (unsigned int)first;
-    if (dtype == 0)
-      adjacent ? launch_rotate<__bf16, true>(a, wide, stream) : launch_rotate<__bf16, false>(a, wide, stream);
-    else
-      adjacent ? launch_rotate<_Float16, true>(a, wide, stream) : launch_rotate<_Float16, false>(a, wide, stream);
-    const hipError_t st = hipGetLastError();
-    if (st != hipSuccess) return fail("rotate_rows", st);
-  }
+  if (dtype == 0)
+    adjacent ? launch_rotate<__bf16, true>(a, unit, stream) : launch_rotate<__bf16, false>(a, unit, stream);
+  else
+    adjacent ? launch_rotate<_Float16, true>(a, unit, stream) : launch_rotate<_Float16, false>(a, unit, stream);
+  const hipError_t st = hipGetLastError();
+  if (st != hipSuccess) return fail("rotate_rows", st);
   return (long long)(2 * tokens * (q_heads * head_bytes + 2 * row_bytes));
 }
