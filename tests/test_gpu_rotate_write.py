@@ -109,6 +109,17 @@ def test_many_heads(sz, tokens, q_heads, kv_heads, dim, rotary, spread, shift, a
           drop=[(tokens - 1, -1)] if tokens > 2 else ())
 
 
+@pytest.mark.parametrize("tokens,q_heads,kv_heads,dim,rotary,shift", [
+    (257, 32, 8, 128, 128, 0), (256, 32, 8, 128, 128, 0), (700, 2, 1, 64, 32, 0), (85, 1, 1, 2, 2, 0),
+    (33, 16, 2, 128, 64, 0), (9, 2, 2, 128, 128, 1), (300, 3, 1, 64, 20, 4), (31, 8, 8, 64, 64, 0)])
+def test_tokens_that_share_a_workgroup(sz, tokens, q_heads, kv_heads, dim, rotary, shift):
+    """As many tokens as a workgroup's threads hold units of, ends of them, and one more unit than threads."""
+    say("shared", tokens, q_heads, kv_heads, dim, rotary, shift)
+    for adjacent in (False, True):
+        check(sz, tokens, q_heads, kv_heads, dim, rotary, adjacent, "fp16", shift=shift, seed=tokens,
+              drop=[(0, -1), (tokens // 2, -1), (tokens - 1, 1 << 40)])
+
+
 def test_more_tokens_than_a_launch_takes(sz):
     say("many tokens")
     tokens = (1 << 24) + 5

@@ -246,7 +246,7 @@ __global__ __launch_bounds__(kStepThreads) void write_rows(WriteArgs a) {
 // the cosines and sines of the token's position from a table, in f32 and rounded once; K goes to its slot with V,
 // Q to a tensor of its own. Bound by HBM: 32768 tokens of 32 + 2 x 8 heads of 128, 808 MB read and written, 145
 // us, 5.6 TB/s (a large copy: 5.1; one wave a token with a head at a time: 156). A decode step of 64 tokens by
-// latency, 4.4 us (one wave a token: 6.2): the position's load, then the table's row.
+// latency, 3.9 us: the position's load, then the table's row.
 struct RotateArgs {
   const unsigned char *q, *k, *v;
   unsigned char* out;          // [tokens][q_heads][dim]
@@ -263,11 +263,17 @@ struct RotateArgs {
   unsigned int rotating, waves_log;  // waves of a token that rotate, and the logarithm of all
   Divider by_rest, by_head;    // units of a head that are not rotated, and all
 };
+struct SmallArgs : RotateArgs {
+  unsigned int together;       // tokens of a workgroup
+  Divider by_units, by_turned, by_copied;  // rotated units of a head, of a token, and others of a token
+};
 
 // Of a lane, before another wave of the token takes its share: 8192 tokens of 64 + 2 x 20 heads of 128, all rotated
 // 82.6 us (one wave for each sort 86.8; one batch a lane 112), 20 of 128 values rotated 142 (307); 125 tokens of the
 // latter's kind 4.5 (39).
 constexpr unsigned int kRotatedBatches = 2, kCopiedUnits = 4;
+constexpr unsigned int kFewTokens = 256;
+constexpr unsigned int kMostSmall = 1u << 22;    // workgroups of a launch,
 constexpr unsigned int kMostRotated = 1u << 25;  // waves of a launch, whose threads fit 32 bits
 
 template <typename E, int N>
@@ -275,10 +281,30 @@ struct Values {
   typedef E type __attribute__((ext_vector_type(N)));
 };
 
+// N pairs turned by their cosines and sines: N values of a head's first half and N of its second, or (kAdjacent) 2 N
+// values side by side.
+template <typename E, int N, bool kAdjacent>
+__device__ __forceinline__ void turn(typename Values<E, N>::type x, typename Values<E, N>::type y,
+                                     const float (&c)[N], const float (&s)[N], unsigned char* dst,
+                                     unsigned char* dst2) {
+  typename Values<E, N>::type x2, y2;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    // places of the pair's values among the 2 N
+    const int first = kAdjacent ? 2 * i : i, second = kAdjacent ? 2 * i + 1 : N + i;
+    const float p = (float)(first < N ? x[first % N] : y[first % N]);
+    const float r = (float)(second < N ? x[second % N] : y[second % N]);
+    const E p2 = (E)(p * c[i] - r * s[i]), r2 = (E)(r * c[i] + p * s[i]);
+    if (first < N) x2[first % N] = p2; else y2[first % N] = p2;
+    if (second < N) x2[second % N] = r2; else y2[second % N] = r2;
+  }
+  *reinterpret_cast<typename Values<E, N>::type*>(dst) = x2;
+  *reinterpret_cast<typename Values<E, N>::type*>(dst2) = y2;
+}
+
 // Two sorts of waves for each token. In the first a lane keeps the cosines and sines of N pairs and takes them to
-// one head after another: N values of its first half and N of its second, or (kAdjacent) 2 N values side by side.
-// The second copies what is not rotated, the heads' other values and V, kUnit at a time, and waits for no position
-// or table. kBatch: heads of a lane whose loads go out together.
+// one head after another. The second copies what is not rotated, the heads' other values and V, kUnit at a time,
+// and waits for no position or table. kBatch: heads of a lane whose loads go out together.
 template <typename E, int N, int kUnit, bool kAdjacent, int kBatch>
 __global__ __launch_bounds__(kStepThreads) void rotate_rows(RotateArgs a) {
   typedef typename Values<E, N>::type Unit;
@@ -334,20 +360,8 @@ __global__ __launch_bounds__(kStepThreads) void rotate_rows(RotateArgs a) {
         for (int b = 0; b < kBatch; ++b) {
           const unsigned int h = h0 + b * a.lanes_heads;
           if (h >= heads) continue;
-          Unit x2, y2;
-#pragma unroll
-          for (int i = 0; i < N; ++i) {
-            // places of the pair's values among the 2 N
-            const int first = kAdjacent ? 2 * i : i, second = kAdjacent ? 2 * i + 1 : N + i;
-            const float p = (float)(first < N ? x[b][first % N] : y[b][first % N]);
-            const float r = (float)(second < N ? x[b][second % N] : y[b][second % N]);
-            const E p2 = (E)(p * c[i] - r * s[i]), r2 = (E)(r * c[i] + p * s[i]);
-            if (first < N) x2[first % N] = p2; else y2[first % N] = p2;
-            if (second < N) x2[second % N] = r2; else y2[second % N] = r2;
-          }
           unsigned char* dst = target(h);
-          *reinterpret_cast<Unit*>(dst + at) = x2;
-          *reinterpret_cast<Unit*>(dst + at2) = y2;
+          turn<E, N, kAdjacent>(x[b], y[b], c, s, dst + at, dst + at2);
         }
       }
     }
@@ -377,21 +391,88 @@ __global__ __launch_bounds__(kStepThreads) void rotate_rows(RotateArgs a) {
   }
 }
 
+// A thread for each unit of a token, first those that are rotated, and several tokens to a workgroup: where a
+// token has no more units than a workgroup threads (32768 tokens of 2 + 2 x 1 heads of 64 11.1 us, by rotate_rows
+// 24.4; 4 + 2 x 1 of 128 31.6 and 34.9; 16 + 2 x 2 of 128, half of them rotated, 75.0 and 82.3), and twice that
+// where there are a few hundred tokens (64 of 32 + 2 x 8 heads of 128 3.6 us and 3.9, 256 of them 4.0 and 4.3, 512
+// 5.7 and 4.7, 32768 209 and 148, as each unit loads its own cosines).
+template <typename E, int N, int kUnit, bool kAdjacent>
+__global__ __launch_bounds__(2 * kStepThreads) void rotate_small(SmallArgs a) {
+  typedef typename Values<E, N>::type Unit;
+  typedef typename Values<uint16_t, kUnit>::type Copy;
+  const unsigned int head_bytes = a.dim * sizeof(E), pairs = a.rotary / 2, turned = a.together * a.by_turned.d;
+  const bool turns = threadIdx.x < turned;
+  const Divider by = turns ? a.by_turned : a.by_copied;
+  const unsigned int i = turns ? threadIdx.x : threadIdx.x - turned, among = div_u32(i, by.m, by.d);
+  const unsigned int unit = i - among * by.d, token = a.first + blockIdx.x * a.together + among;
+  if (among >= a.together || token >= a.tokens) return;
+  const long long slot = a.slots[token];
+  const bool write = slot >= 0 && (unsigned long long)slot < a.slot_count;
+  unsigned char* const out = a.out + (unsigned long long)token * a.q_heads * head_bytes;
+  unsigned char* const layer = a.layer + (write ? (unsigned long long)slot : 0ull) * a.kv_heads * head_bytes;
+  const unsigned int others = (a.dim - a.rotary) / kUnit * (a.q_heads + a.kv_heads);
+  const bool value = !turns && unit >= others;
+  const unsigned int in = value ? unit - others : unit;
+  const Divider by_head = turns ? a.by_units : value ? a.by_head : a.by_rest;
+  const unsigned int h = div_u32(in, by_head.m, by_head.d), u = in - h * by_head.d;
+  const bool query = !value && h < a.q_heads;
+  if (!query && !write) return;
+  const unsigned int own = query || value ? h : h - a.q_heads;  // its head of Q, K or V
+  const unsigned char* const src = query   ? a.q + token * a.q_row + own * a.q_head
+                                   : value ? a.v + token * a.v_row + own * a.v_head
+                                           : a.k + token * a.k_row + own * a.k_head;
+  unsigned char* const dst = (query ? out : layer + (value ? a.plane_bytes : 0ull)) + own * head_bytes;
+  if (turns) {
+    const unsigned int at = (kAdjacent ? 2 * N : N) * sizeof(E) * u;
+    const unsigned int at2 = at + (kAdjacent ? N : pairs) * sizeof(E);
+    const Unit x = *reinterpret_cast<const Unit*>(src + at), y = *reinterpret_cast<const Unit*>(src + at2);
+    const long long position = a.positions[token];
+    const bool known = position >= 0 && (unsigned long long)position < a.table_rows;
+    const float* const table = a.table + (known ? (unsigned long long)position * a.rotary : 0ull) + u * N;
+    float c[N], s[N];
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      c[n] = known ? table[n] : NAN;
+      s[n] = known ? table[pairs + n] : NAN;
+    }
+    turn<E, N, kAdjacent>(x, y, c, s, dst + at, dst + at2);
+  } else {
+    const unsigned int at = ((value ? 0u : a.rotary) + u * kUnit) * sizeof(E);
+    *reinterpret_cast<Copy*>(dst + at) = *reinterpret_cast<const Copy*>(src + at);
+  }
+}
+
 // As many heads at once as a lane has, up to 5: 32768 tokens of 32 + 8 heads of 128, five of them for a lane,
-// 146 us at 5, 149 at 3, 153 at 1; 4700 of 24 + 3 heads, 32 of 64 values rotated, one for a lane, 10.8 us at 1,
-// 12.0 at 3, as places past the last head load it again.
+// 146 us at 5, 149 at 3, 153 at 1; of 24 + 3 heads of 128, 32 of them rotated, one for a lane, 100.7 us at 1, 107 at
+// 3, 141 at 5, as places past the last head load it again.
 template <typename E, int N, int kUnit, bool kAdjacent>
 void launch_batch(RotateArgs a, hipStream_t stream) {
   const unsigned int own = (a.q_heads + a.kv_heads + a.lanes_heads - 1) / a.lanes_heads;
   const unsigned int batch = own == 1 ? 1 : own <= 3 ? 3 : 5;
   const unsigned int copies = ((a.dim - a.rotary) * (a.q_heads + a.kv_heads) + a.dim * a.kv_heads) / kUnit;
+  a.by_rest = make_divider((a.dim - a.rotary) / kUnit);
+  a.by_head = make_divider(a.dim / kUnit);
+  const unsigned int turned = a.units * (a.q_heads + a.kv_heads);
+  const unsigned int units = turned + copies;
+  if (units <= kStepThreads || (units <= 2 * kStepThreads && a.tokens <= kFewTokens)) {
+    SmallArgs m{a};
+    const dim3 threads(units <= kStepThreads ? kStepThreads : 2 * kStepThreads);
+    m.together = threads.x / units;
+    m.by_units = make_divider(a.units);
+    m.by_turned = make_divider(turned);
+    m.by_copied = make_divider(copies);
+    const unsigned int most = kMostSmall * m.together;
+    for (m.first = 0; m.first < a.tokens; m.first += std::min(most, a.tokens - m.first))
+      hipLaunchKernelGGL((rotate_small<E, N, kUnit, kAdjacent>),
+                         dim3((std::min(most, a.tokens - m.first) + m.together - 1) / m.together), threads, 0, stream,
+                         m);
+    return;
+  }
   // (one of each sort, or up to 8 in all, at most half of them rotating)
   auto waves = [](unsigned int work, unsigned int each) { return std::max((work + each - 1) / each, 1u); };
   a.rotating = std::min(waves(own, kRotatedBatches * batch), 4u);
   a.waves_log = 1;
   while (a.waves_log < 3 && 1u << a.waves_log < a.rotating + waves(copies, kCopiedUnits * kWave)) ++a.waves_log;
-  a.by_rest = make_divider((a.dim - a.rotary) / kUnit);
-  a.by_head = make_divider(a.dim / kUnit);
   constexpr unsigned int kWaves = kStepThreads / kWave;
   const unsigned int most = kMostRotated >> a.waves_log;
   for (unsigned int left = a.tokens; left != 0;) {
