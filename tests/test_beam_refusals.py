@@ -82,6 +82,8 @@ def test_cross_workspace_serves_smaller_calls(lib):  # noqa: F811
     # taken whole: sources of 192 workgroups; cut: of fewer
     assert least(192, 192, 1, 1, 64, 2048, 1) == 0 < least(191, 191, 1, 1, 64, 2048, 1)
     assert least(191, 191, 1, 1, 64, 2048, 1) <= bound(192, 192, 1, 1, 64, 2048, 1)
+    assert least(64, 4, 1, 1, 64, 600, 60) > 0 == least(1000, 999, 1, 1, 64, 600, 60)
+    assert least(64, 4, 1, 1, 64, 600, 60) <= bound(1000, 999, 1, 1, 64, 600, 60)
     assert least(1, 1, 16, 16, 64, 768, 1) == 0 < least(1, 1, 16, 16, 64, 769, 1)
     for sizes in ((8, 2, 8, 3, 128, 4096), (8, 2, 8, 2, 96, 4096), (-1, 2, 8, 2, 128, 4096), (8, 2, 8, 2, 128, -1)):
         with pytest.raises(ValueError):

@@ -83,6 +83,11 @@ constexpr int kTileTokens = 64;   // tokens of a step of attention_tiles: unit o
 // Steps of a split, at least: its start and its share of the joining take as long as some of them (4
 // requests of 64 tokens behind 4000: 39.1 us at 12, 44.8 at 16).
 constexpr unsigned int kLeastTileSteps = 12;
+// Over sources a tile has no steps that its first rows spare, and shorter splits gain where there are few tiles (one
+// request of 64 rows, 1500 tokens, 16 heads of 64: 14.3 us at 4, 20.7 at 12; 4 of 3 rows, 5000 tokens, 7 / 1 heads of
+// 128 17.7 and 22.5; 4 of 300, 1500, 32 / 8 heads the same). Of tiles for at most half the CUs sources
+// of fewer than kLeastTileSteps are cut too (one of 64 rows, 600 tokens 13.1 and 15.4, 400 tokens 12.8 and 12.4).
+constexpr unsigned int kLeastSourceTileSteps = 4, kWholeSourceTileSteps = 8;
 // Of a streamed split, in rounds of kFewUnit tokens (4 requests of 4096 tokens, 32 / 8 heads of 128:
 // 22.5 us at 4, 24.6 at 1). A call whose block tables hold no more than kWholeFewSteps is not cut at
 // all and joins nothing: one launch (one request, 32 / 8 heads of 64, 1024 tokens: 12.6 us, cut 16.8,
@@ -332,7 +337,7 @@ struct Work {
       sum += lane_value(wave_scan((unsigned int)min(own, (unsigned long long)kMostSteps)), 63);
     }
     const unsigned int parts = kTiles ? a.tile_target : a.few_target;
-    unsigned int least = kTiles ? kLeastTileSteps : kLeastFewSteps;
+    unsigned int least = kTiles ? (a.causal ? kLeastTileSteps : kLeastSourceTileSteps) : kLeastFewSteps;
     if (!kTiles && a.fine != 0)
       least = (unsigned int)min((unsigned long long)least, sum / (kFineSplits * a.requests) + 1);
     if (!large && a.slots != 0) cap = max(least, share_of(sum, a.kv_heads, parts));
@@ -1538,7 +1543,8 @@ Plan plan_of(unsigned long long tokens, unsigned long long requests, unsigned lo
   if (p.tiles) {
     const unsigned long long rows = (unsigned long long)tile_rows((int)head_dim);
     const unsigned long long tiles = tokens * group / rows + active;
-    const double whole = kTileTokens * kLeastTileSteps;
+    const bool half = !causal && 2 * tiles * kv_heads <= compute_units();
+    const double whole = kTileTokens * (half ? kWholeSourceTileSteps : kLeastTileSteps);
     bool cut = (double)max_context > whole;
     if (cut && !paged) {
       // A prompt of L of the n rows of q, of r prompts that fill them, is cut where its L / 64 steps are
@@ -1584,8 +1590,11 @@ unsigned long long workspace_bound(unsigned long long tokens, unsigned long long
                                    unsigned long long kv_heads, unsigned long long group,
                                    unsigned long long head_dim, unsigned long long max_context,
                                    unsigned long long max_query, bool paged, bool causal = true) {
-  const unsigned long long own = workspace_of(
-      plan_of(tokens, requests, kv_heads, group, head_dim, max_context, max_query, paged, causal), head_dim);
+  Plan plan = plan_of(tokens, requests, kv_heads, group, head_dim, max_context, max_query, paged, causal);
+  // (of fewer tiles sources are cut that more of them leave whole)
+  if (!causal && plan.tiles && max_context > kTileTokens * kWholeSourceTileSteps)
+    plan.slots = 2 * (plan.tile_target / kv_heads + 1) * kv_heads;
+  const unsigned long long own = workspace_of(plan, head_dim);
   if (!paged) {
     // (of one prompt the shortest that can be cut at all is cut the soonest; all that are cut need the same)
     const unsigned long long n = std::min<unsigned long long>(max_query, kTileTokens * kLeastTileSteps + 1);
@@ -1594,7 +1603,7 @@ unsigned long long workspace_bound(unsigned long long tokens, unsigned long long
   const unsigned long long few = std::min<unsigned long long>(max_query, kFewRows / group);
   if (few == 0) return own;
   Plan most = plan_of(tokens, requests, kv_heads, group, head_dim, max_context, few, true, causal);
-  // (of fewer requests sources are cut that more of them leave whole)
+  // (and of fewer requests)
   if (!causal && max_context > kFewUnit * whole_fine_steps(head_dim))
     most.slots = few_slots(most.few_target, kv_heads, std::min(tokens, requests));
   return std::max(own, workspace_of(most, head_dim));
