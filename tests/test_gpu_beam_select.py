@@ -123,6 +123,29 @@ def test_sorted_and_crowded_rows(sz):
             check(sz.beam_select(logits, scores, candidates=candidates), logits, scores, candidates)
 
 
+@pytest.mark.parametrize("dtype", ("bf16", "fp32"))
+@pytest.mark.parametrize("requests,beams,vocab,candidates", [
+    (2, 1, 300, 64), (1, 16, 2989, 32), (3, 8, 689, 16), (20, 10, 1572, 20), (1, 1, 7, 5), (2, 3, 8, 20),
+    (1, 2, 1029, 64), (3, 4, 3, 12)])
+def test_more_candidates_than_segments(sz, requests, beams, vocab, candidates, dtype):
+    """Rows that are short for what is asked of them, whole and with one beam or one value in use; rows that end
+    inside a load, or are shorter than one."""
+    say("short", requests, beams, vocab, candidates, dtype)
+    logits, scores = make(requests, beams, vocab, dtype, seed=candidates)
+    check(sz.beam_select(logits, scores, candidates=candidates), logits, scores, candidates)
+    one = scores.clone()
+    one[:, 1:] = -float("inf")
+    check(sz.beam_select(logits, one, candidates=candidates), logits, one, candidates)
+    ended = torch.zeros((requests, beams), dtype=torch.bool, device="cuda")
+    ended[:, 0] = True
+    choice = sz.beam_select(logits, scores, candidates=candidates, ended=ended, end_token=vocab - 1)
+    check(choice, logits, scores, candidates, ended, vocab - 1)
+    logits[:] = 1.5
+    check(sz.beam_select(logits, one, candidates=candidates), logits, one, candidates, exact=True)
+    logits[..., 1:] = -float("inf")
+    check(sz.beam_select(logits, one, candidates=candidates), logits, one, candidates, exact=True)
+
+
 def test_masks(sz):
     """Tokens that are not allowed, by -inf and by the lowest value; rows that allow none; beams not in
     use; too little to offer."""

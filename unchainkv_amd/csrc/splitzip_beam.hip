@@ -148,20 +148,21 @@ __global__ __launch_bounds__(kScanThreads) void beam_scan(SelectArgs a) {
         raw[n] = *reinterpret_cast<const typename T::Raw*>(src + (at + n * T::kLoad) * T::kBytes);
 #pragma unroll
       for (int i = 0; i < kOwn; ++i) x[i] = T::of(raw[i / T::kLoad], i % T::kLoad);
+    } else if (a.vocab >= T::kLoad) {
+      // The row's end: loads that would pass it are of its last logits, of which those count that no load before
+      // has (all go out together; behind a branch for each the call took 1.5 us more).
+      typename T::Raw raw[kLoads];
+#pragma unroll
+      for (int n = 0; n < kLoads; ++n)
+        raw[n] = *reinterpret_cast<const typename T::Raw*>(src + min(at + n * T::kLoad, a.vocab - T::kLoad) * T::kBytes);
+#pragma unroll
+      for (int i = 0; i < kOwn; ++i) {
+        const unsigned int from = at + i / T::kLoad * T::kLoad;
+        x[i] = from + T::kLoad <= a.vocab + i % T::kLoad ? T::of(raw[i / T::kLoad], i % T::kLoad) : -INFINITY;
+      }
     } else {
 #pragma unroll
-      for (int n = 0; n < kLoads; ++n) {
-        const unsigned int from = at + n * T::kLoad;
-        if (from + T::kLoad <= a.vocab) {
-          const typename T::Raw raw = *reinterpret_cast<const typename T::Raw*>(src + from * T::kBytes);
-#pragma unroll
-          for (int i = 0; i < T::kLoad; ++i) x[n * T::kLoad + i] = T::of(raw, i);
-        } else {
-#pragma unroll
-          for (int i = 0; i < T::kLoad; ++i)
-            x[n * T::kLoad + i] = from + i < a.vocab ? T::one(src, from + i) : -INFINITY;
-        }
-      }
+      for (int i = 0; i < kOwn; ++i) x[i] = at + i < a.vocab ? T::one(src, at + i) : -INFINITY;
     }
     float own = x[0];
 #pragma unroll
@@ -298,7 +299,7 @@ template <typename T, int kItems, int kTokens>
 __global__ __launch_bounds__(kPickThreads) void beam_pick(SelectArgs a) {
   constexpr int kWaves = kPickThreads / kWave;
   __shared__ Beam s_beam[kMostBeams];
-  // segments that may be among the best, and then values: at most 64 of each wave, `most` of each segment
+  // segments that may be among the best, and then values: at most 64 of each wave, and of each segment
   __shared__ unsigned long long s_key[kMostCandidates * kMostCandidates];
   __shared__ unsigned int s_id[kMostCandidates * kMostCandidates];
   __shared__ unsigned long long s_bound[kWaves];
@@ -437,21 +438,53 @@ __global__ __launch_bounds__(kPickThreads) void beam_pick(SelectArgs a) {
     const Beam beam = s_beam[b];
     const unsigned char* src = row_of<T>(a, row0 + b);
     unsigned long long keys[kTokens], masks[kTokens];
-    unsigned int count = 0;
+    auto keep = [&](unsigned long long bound) {
+      unsigned int count = 0;
+#pragma unroll
+      for (int t = 0; t < kTokens; ++t) {
+        if (keys[t] < bound) keys[t] = 0;
+        masks[t] = __ballot(keys[t] != 0);
+        count += (unsigned int)__popcll(masks[t]);
+      }
+      return count;
+    };
 #pragma unroll
     for (int t = 0; t < kTokens; ++t) {
       const unsigned int in = t * kWave + lane, token = first + in;
       const bool there = in < group * kSegment && token < a.vocab;
       keys[t] = beam.key(beam.open && there ? T::one(src, token) : -INFINITY);
       if (beam.ended && token == a.end_token) keys[t] = key_of(beam.score);
-      if (!there || keys[t] < least) keys[t] = 0;
-      masks[t] = __ballot(keys[t] != 0);
-      count += (unsigned int)__popcll(masks[t]);
+      if (!there) keys[t] = 0;
+    }
+    unsigned int count = keep(least);
+    if (count > most) {
+      // (few segments, whose maxima bound too little)
+      unsigned long long own = keys[0];
+#pragma unroll
+      for (int t = 1; t < kTokens; ++t) own = keys[t] > own ? keys[t] : own;
+      count = keep(max(1ull, reached(own, most)));
+      if (count > kMostCandidates) {
+        // Equal ones, as of a beam that is not in use: the first of them, where the largest are enough.
+        const unsigned long long top = wave_largest(own);
+        unsigned int equal = 0;
+#pragma unroll
+        for (int t = 0; t < kTokens; ++t) equal += (unsigned int)__popcll(__ballot(keys[t] == top));
+        if (equal >= most) {
+          unsigned int before = 0;
+#pragma unroll
+          for (int t = 0; t < kTokens; ++t) {
+            const unsigned long long mask = __ballot(keys[t] == top);
+            if (keys[t] != top || before + (unsigned int)__popcll(mask & ((1ull << lane) - 1)) >= most) keys[t] = 0;
+            before += (unsigned int)__popcll(mask);
+          }
+          count = keep(1);
+        }
+      }
     }
     unsigned int at = 0;
-    if (lane == 0) at = atomicAdd(&s_count, min(count, most));
+    if (lane == 0) at = atomicAdd(&s_count, count > kMostCandidates ? most : count);
     at = uniform(at);
-    if (count <= most) {
+    if (count <= kMostCandidates) {
 #pragma unroll
       for (int t = 0; t < kTokens; ++t) {
         if (keys[t] != 0) {
