@@ -522,6 +522,7 @@ __global__ __launch_bounds__(kPickThreads) void beam_pick(SelectArgs a) {
 
 constexpr int kOrderThreads = 256;  // columns of a workgroup
 constexpr int kOrderWaves = kOrderThreads / kWave;
+constexpr unsigned int kAtOnce = 8;  // of a column's entries
 constexpr int kMostLayers = 64;     // of a launch
 
 struct OrderArgs {
@@ -578,17 +579,24 @@ __global__ __launch_bounds__(kOrderThreads) void order_tables(OrderArgs a) {
   const bool tail = rest != 0 && full < a.width && full / kOrderThreads == blockIdx.x;
   if (tid < beams) s_parent[tid] = a.parents[row0 + tid];
   if (tid == 0) s_lacking = s_left = 0;
+  // the last blocks of a lane's beam (read with the rest: nobody else has that column)
+  const int last = tail && tid < beams ? a.tables[(row0 + tid) * a.table_stride + full] : -1;
   int* const own = s_entry + tid;
   const bool there = column < a.width && (column < full || a.out != a.tables) && !(tail && column == full);
   bool same = true;
   if (there) {
     int first = 0;
-#pragma unroll 4
-    for (unsigned int b = 0; b < beams; ++b) {
-      const int id = a.tables[(row0 + b) * a.table_stride + column];
-      own[b * kOrderThreads] = id;
-      first = b == 0 ? id : first;
-      same &= id == first;
+    for (unsigned int b0 = 0; b0 < beams; b0 += kAtOnce) {
+      int id[kAtOnce];  // (past the last beam its entry again: the loads wait for none before)
+#pragma unroll
+      for (unsigned int n = 0; n < kAtOnce; ++n)
+        id[n] = a.tables[(row0 + min(b0 + n, beams - 1)) * a.table_stride + column];
+      first = b0 == 0 ? id[0] : first;
+#pragma unroll
+      for (unsigned int n = 0; n < kAtOnce; ++n) {
+        if (b0 + n < beams) own[(b0 + n) * kOrderThreads] = id[n];
+        same &= id[n] == first;
+      }
     }
   }
   __syncthreads();
@@ -603,19 +611,21 @@ __global__ __launch_bounds__(kOrderThreads) void order_tables(OrderArgs a) {
   unsigned int released = 0;  // the beams whose entry of this column is
   if (there) {
     const bool held = column < full;
+#pragma unroll 4
     for (unsigned int j = 0; j < beams; ++j) {
       const unsigned int p = held ? (unsigned int)s_parent[j] : j;
-      a.out[(row0 + j) * a.out_stride + column] = p < beams ? own[p * kOrderThreads] : -1;
+      const int id = own[min(p, beams - 1) * kOrderThreads];
+      a.out[(row0 + j) * a.out_stride + column] = p < beams ? id : -1;
     }
     if (held && (!same || with_child == 0)) {
       // entries of beams without children that no other beam with one has, once each
       for (unsigned int b = 0; b < beams; ++b) {
         const int id = own[b * kOrderThreads];
         if ((with_child >> b & 1) != 0 || id < 0) continue;
-        bool again = false;
-        for (unsigned int c = 0; c < beams; ++c)
-          again |= own[c * kOrderThreads] == id && (c < b || (with_child >> c & 1) != 0);
-        if (!again) released |= 1u << b;
+        unsigned int equal = 0;  // the beams that list it
+#pragma unroll 8
+        for (unsigned int c = 0; c < beams; ++c) equal |= own[c * kOrderThreads] == id ? 1u << c : 0u;
+        if ((equal & (with_child | ((1u << b) - 1))) == 0) released |= 1u << b;
       }
     }
   }
@@ -628,13 +638,13 @@ __global__ __launch_bounds__(kOrderThreads) void order_tables(OrderArgs a) {
   // The last blocks, by one wave, a lane for each beam: the first child of a block keeps it, the others take
   // those that no child has, in order.
   if (tid < kWave && tail) {
-    const int id = lane < beams ? a.tables[(row0 + lane) * a.table_stride + full] : -1;
-    const int parent = known ? s_parent[lane] : 0;
+    const int id = last, parent = known ? s_parent[lane] : 0;
     const int source = __shfl(id, parent, kWave);
     bool taken = false, used = false, again = false;
+    const unsigned long long children = __ballot(known);
     for (unsigned int j = 0; j < beams; ++j) {
-      const bool child = __shfl(known ? 1 : 0, (int)j, kWave) != 0;
-      const int its = __shfl(source, (int)j, kWave), other = __shfl(id, (int)j, kWave);
+      const bool child = (children >> j & 1) != 0;
+      const int its = __builtin_amdgcn_readlane(source, (int)j), other = __builtin_amdgcn_readlane(id, (int)j);
       taken |= child && j < lane && its == source;
       used |= child && its == id;
       again |= j < lane && other == id;
