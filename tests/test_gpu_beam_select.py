@@ -268,3 +268,21 @@ def test_refuses(sz):
     assert sz.beam_select(logits[:0], scores[:0], candidates=2).tokens.shape == (0, 2)
     with pytest.raises(ValueError):
         sz.beam_select_workspace_bytes(1, 33, 100)
+
+
+@pytest.mark.parametrize("dtype", ("bf16", "fp32"))
+@pytest.mark.parametrize("beams", (1, 4, 16, 17, 32))
+def test_rows_that_one_workgroup_scans(sz, beams, dtype):
+    """As many logits as a request's one workgroup reads by itself, and one more."""
+    chunk = 2048 if dtype == "bf16" else 1024
+    for vocab in (max(16 // beams, 1) * chunk, max(16 // beams, 1) * chunk + 1):
+        say("one launch", beams, vocab, dtype)
+        logits, scores = make(3, beams, vocab, dtype, seed=beams)
+        logits[1, 0, : vocab // 2] = -float("inf")
+        scores[2, beams // 2:] = -float("inf")
+        if beams > 1:
+            scores[2, 0] = -3.0
+        ended = torch.zeros((3, beams), dtype=torch.bool, device="cuda")
+        ended[0, beams - 1] = beams > 1
+        choice = sz.beam_select(logits, scores, candidates=min(2 * beams, 64), ended=ended, end_token=vocab - 1)
+        check(choice, logits, scores, min(2 * beams, 64), ended, vocab - 1)

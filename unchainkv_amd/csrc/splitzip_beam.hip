@@ -44,6 +44,11 @@ constexpr int kPickThreads = 1024;
 constexpr int kMostBeams = 32, kMostCandidates = 64;
 constexpr int kMostItems = 8;                                 // segments that a lane of beam_pick holds
 constexpr int kOwnTokens = kSegment / kWave;                  // tokens of one
+// Chunks of a request's rows, 4 KB each, up to which beam_pick scans them by itself, a wave each: one launch (4 beams,
+// 8000 logits in bf16, captured: 9.7 us and 9.9, 300 logits 9.5 and 10.8, and 3.5 us less of the host's time; twice as
+// many chunks 12.2 and 10.0, as a CU reads no faster).
+constexpr unsigned int kWholeChunks = 16;
+constexpr unsigned int kChunkSegments = kWave * kLaneBytes / 2 / kSegment;  // of one, at most
 constexpr unsigned int kMostVocab = 1u << 20;
 static_assert(kMostVocab <= 8 * kMostItems * kWave * kSegment, "the largest groups hold a row");
 constexpr float kLowest = -3.402823466e38f;
@@ -126,14 +131,13 @@ __device__ __forceinline__ float wave_max(float v) {
   return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
 }
 
-// A wave takes `rounds` times 64 lanes' 64 bytes of a row; a lane's logits follow each other, so that a
-// segment's maximum takes three or four exchanges between lanes for 32 or 16 logits of each.
+// A row's chunk by a wave: `rounds` times 64 lanes' 64 bytes; a lane's logits follow each other, so that a
+// segment's maximum takes three or four exchanges between lanes for 32 or 16 logits of each. maxima, sums: the row's.
 template <typename T>
-__global__ __launch_bounds__(kScanThreads) void beam_scan(SelectArgs a) {
+__device__ __forceinline__ void scan_chunk(const SelectArgs& a, unsigned int row, unsigned int chunk, float* maxima,
+                                           float2* sums) {
   constexpr int kOwn = kLaneLogits<T>, kLoads = kOwn / T::kLoad, kLanes = kSegment / kOwn;
-  const unsigned int row = blockIdx.z * kGridRows + blockIdx.y, lane = threadIdx.x & 63;
-  const unsigned int chunk = uniform(blockIdx.x * (kScanThreads / kWave) + (threadIdx.x >> 6));
-  if (chunk >= a.chunks || row >= a.requests * a.beams || !is_open(a, row)) return;
+  const unsigned int lane = __lane_id();
   const unsigned char* src = row_of<T>(a, row);
   float top = kLowest, sum = 0.f;
   const unsigned int first = chunk * a.rounds * (kWave * kOwn);
@@ -191,13 +195,22 @@ __global__ __launch_bounds__(kScanThreads) void beam_scan(SelectArgs a) {
     if constexpr (kLanes == 16) own = fmaxf(own, shifted<0x118, 0xF>(own));
     const unsigned int segment = at / kSegment;
     if (lane % kLanes == kLanes - 1 && segment < a.segments)
-      a.maxima[(unsigned long long)row * a.segments + segment] = own;
+      maxima[segment] = own;
   }
   const float big = wave_max(top);
   sum *= __builtin_amdgcn_exp2f((top - big) * kLog2E);
 #pragma unroll
   for (int d = 1; d < kWave; d *= 2) sum += __shfl_xor(sum, d, kWave);
-  if (lane == 0) a.sums[(unsigned long long)row * a.chunks + chunk] = make_float2(big, sum);
+  if (lane == 0) sums[chunk] = make_float2(big, sum);
+}
+
+template <typename T>
+__global__ __launch_bounds__(kScanThreads) void beam_scan(SelectArgs a) {
+  const unsigned int row = blockIdx.z * kGridRows + blockIdx.y;
+  const unsigned int chunk = uniform(blockIdx.x * (kScanThreads / kWave) + (threadIdx.x >> 6));
+  if (chunk >= a.chunks || row >= a.requests * a.beams || !is_open(a, row)) return;
+  scan_chunk<T>(a, row, chunk, a.maxima + (unsigned long long)row * a.segments,
+                a.sums + (unsigned long long)row * a.chunks);
 }
 
 // Values as numbers that compare alike: NaN above all, -0 as 0, nothing as 0.
@@ -294,8 +307,9 @@ __device__ __forceinline__ unsigned int rank_of(const unsigned long long* keys, 
   return rank;
 }
 
-// kItems: segments, or groups of them, that a lane holds of a row; kTokens: tokens of a group that it does.
-template <typename T, int kItems, int kTokens>
+// kItems: segments, or groups of them, that a lane holds of a row; kTokens: tokens of a group that it does. kWhole: it
+// scans the rows itself before.
+template <typename T, int kItems, int kTokens, bool kWhole>
 __global__ __launch_bounds__(kPickThreads) void beam_pick(SelectArgs a) {
   constexpr int kWaves = kPickThreads / kWave;
   __shared__ Beam s_beam[kMostBeams];
@@ -305,6 +319,8 @@ __global__ __launch_bounds__(kPickThreads) void beam_pick(SelectArgs a) {
   __shared__ unsigned long long s_bound[kWaves];
   __shared__ unsigned int s_chosen[kMostCandidates], s_segments, s_count;
   __shared__ unsigned long long s_least;
+  __shared__ float s_maxima[kWhole ? kWholeChunks * kChunkSegments : 1];
+  __shared__ float2 s_sums[kWhole ? kWholeChunks : 1];
   const unsigned int request = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
   const unsigned int row0 = request * a.beams, most = a.candidates;
   const unsigned int group = kTokens == kOwnTokens ? 1 : a.group, items = a.items;
@@ -314,14 +330,21 @@ __global__ __launch_bounds__(kPickThreads) void beam_pick(SelectArgs a) {
     s_least = 0;
   }
   if (tid < kMostCandidates) s_chosen[tid] = ~0u;
+  if constexpr (kWhole) {
+    static_assert(kWholeChunks <= kWaves);
+    const unsigned int b = wave / a.chunks;
+    if (b < a.beams && is_open(a, row0 + b))
+      scan_chunk<T>(a, row0 + b, wave - b * a.chunks, s_maxima + b * a.segments, s_sums + b * a.chunks);
+    __syncthreads();
+  }
 
   // A part of a beam's items as keys by their maxima.
   auto load = [&](unsigned int unit, unsigned long long (&keys)[kItems]) {
     const unsigned int b = unit / a.parts, row = row0 + b;
     const unsigned int from = (unit - b * a.parts) * (kItems * kWave) + lane;
     // (all loads go out together; what a beam that is not open has there counts for nothing)
-    const float* maxima = a.maxima + (unsigned long long)row * a.segments;
-    const float2* sums = a.sums + (unsigned long long)row * a.chunks;
+    const float* maxima = kWhole ? s_maxima + b * a.segments : a.maxima + (unsigned long long)row * a.segments;
+    const float2* sums = kWhole ? s_sums + b * a.chunks : a.sums + (unsigned long long)row * a.chunks;
     float largest[kItems];
 #pragma unroll
     for (int t = 0; t < kItems; ++t) {
@@ -785,22 +808,27 @@ unsigned long long select_bytes(unsigned long long rows, unsigned long long voca
   return maxima_bytes(rows, vocab) + sizeof(float2) * rows * ((vocab + kLeast - 1) / kLeast);
 }
 
+bool is_whole(const SelectArgs& a) { return a.rounds == 1 && a.beams * a.chunks <= kWholeChunks; }
+
 // As few registers as hold a row's items.
 template <typename T>
 void launch_pick(const SelectArgs& a, hipStream_t stream) {
   const dim3 grid(a.requests), threads(kPickThreads);
   const unsigned int held = (a.items + a.parts * kWave - 1) / (a.parts * kWave);
-  if (held <= 2)
-    hipLaunchKernelGGL((beam_pick<T, 2, kOwnTokens>), grid, threads, 0, stream, a);
+  if (is_whole(a))
+    hipLaunchKernelGGL((beam_pick<T, 2, kOwnTokens, true>), grid, threads, 0, stream, a);
+  else if (held <= 2)
+    hipLaunchKernelGGL((beam_pick<T, 2, kOwnTokens, false>), grid, threads, 0, stream, a);
   else if (held <= 4)
-    hipLaunchKernelGGL((beam_pick<T, 4, kOwnTokens>), grid, threads, 0, stream, a);
+    hipLaunchKernelGGL((beam_pick<T, 4, kOwnTokens, false>), grid, threads, 0, stream, a);
   else if (a.group == 1)
-    hipLaunchKernelGGL((beam_pick<T, kMostItems, kOwnTokens>), grid, threads, 0, stream, a);
+    hipLaunchKernelGGL((beam_pick<T, kMostItems, kOwnTokens, false>), grid, threads, 0, stream, a);
   else if (a.group == 2)
-    hipLaunchKernelGGL((beam_pick<T, kMostItems, 2 * kOwnTokens>), grid, threads, 0, stream, a);
+    hipLaunchKernelGGL((beam_pick<T, kMostItems, 2 * kOwnTokens, false>), grid, threads, 0, stream, a);
   else
-    hipLaunchKernelGGL((beam_pick<T, kMostItems, 8 * kOwnTokens>), grid, threads, 0, stream, a);
+    hipLaunchKernelGGL((beam_pick<T, kMostItems, 8 * kOwnTokens, false>), grid, threads, 0, stream, a);
 }
+static_assert(kWholeChunks * kChunkSegments <= 2 * kWave, "a wave's lanes hold two of a whole row's segments each");
 
 unsigned int chunks_of(unsigned long long width) {
   return (unsigned int)((width + kOrderThreads - 1) / kOrderThreads);
@@ -867,14 +895,17 @@ extern "C" long long kvq_splitzip_beam_select(
   constexpr unsigned int kChunks = kScanThreads / kWave;  // of a workgroup
   const dim3 grid((a.chunks + kChunks - 1) / kChunks, (unsigned int)std::min<unsigned long long>(rows, kGridRows),
                   (unsigned int)((rows + kGridRows - 1) / kGridRows));
-  if (dtype == 0)
-    hipLaunchKernelGGL(beam_scan<Bf16>, grid, dim3(kScanThreads), 0, stream, a);
-  else if (dtype == 1)
-    hipLaunchKernelGGL(beam_scan<Fp16>, grid, dim3(kScanThreads), 0, stream, a);
-  else
-    hipLaunchKernelGGL(beam_scan<Fp32>, grid, dim3(kScanThreads), 0, stream, a);
-  hipError_t st = hipGetLastError();
-  if (st != hipSuccess) return fail("beam_scan", st);
+  hipError_t st = hipSuccess;
+  if (!is_whole(a)) {
+    if (dtype == 0)
+      hipLaunchKernelGGL(beam_scan<Bf16>, grid, dim3(kScanThreads), 0, stream, a);
+    else if (dtype == 1)
+      hipLaunchKernelGGL(beam_scan<Fp16>, grid, dim3(kScanThreads), 0, stream, a);
+    else
+      hipLaunchKernelGGL(beam_scan<Fp32>, grid, dim3(kScanThreads), 0, stream, a);
+    st = hipGetLastError();
+    if (st != hipSuccess) return fail("beam_scan", st);
+  }
   if (dtype == 0)
     launch_pick<Bf16>(a, stream);
   else if (dtype == 1)
