@@ -754,3 +754,25 @@ def test_payload_ready_carries_gpu_times_on_the_gpu(sz, codebooks):
         assert row["payload_elapsed_s"] > 0
         assert row["encoded_bytes"] == sum(p.encoded_bytes for p in payloads)
         codec.release(pending)
+
+
+def test_payload_ready_waits_for_the_encodes_it_times(sz, codebooks):
+    """An encode whose end mark the GPU reaches only after the copies of its payloads."""
+    say("connector late end marks")
+    books = codebooks[2 * 32:3 * 32]
+    rng = np.random.default_rng(32)
+    kv = layer_from_words(words_with_books(rng, books, 48, 0.0), 48)
+    trace = RecordingTrace()
+    codec = SplitzipLayerCodec(CodecConfig(trace_cuda=True), trace=trace, codebooks={2: books})
+    span = codec._gpu_span
+
+    def late(pending, kind, start, stream, torch):
+        torch.cuda._sleep(20_000_000)
+        span(pending, kind, start, stream, torch)
+
+    codec._gpu_span = late
+    pending = codec.save_kv_layer(2, kv, disjoint_tables(rng, 48, [3, 5]))
+    codec.ready(pending)
+    row, = [f for name, f in trace.rows if name == "splitzip_payload_ready"]
+    assert row["encode_gpu_s"] > 1e-3 and row["d2h_gpu_s"] > 0
+    codec.release(pending)

@@ -993,7 +993,9 @@ class SplitzipLayerCodec:
         pending.presence = pending.palette_info = None
         fields = {}
         if self.config.trace_cuda:
-            # the events have completed: every copy above was waited for
+            # every copy above was waited for; an encode's end may lie behind its copies on the stream
+            for _, _, end in pending.timing:
+                end.synchronize()
             fields = {
                 "bits": [p.bits for p in pending.payloads],
                 "fallback": [p.fallback for p in pending.payloads],
