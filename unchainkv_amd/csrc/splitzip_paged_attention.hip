@@ -181,6 +181,7 @@ struct AttendArgs {
   Divider by_block;
   unsigned int tokens, requests, q_heads, kv_heads, group;
   unsigned int few_target, tile_target;   // workgroups to split for, of the two paths
+  unsigned int tile_least;    // steps of a tile's split, at least
   unsigned int fine;          // 1: streamed splits may be shorter than kLeastFewSteps, up to kFineSplits of a request
   unsigned int max_query;     // requests with more new tokens are left out
   unsigned int max_source;    // and, of packed sources, those with more tokens
@@ -337,7 +338,7 @@ struct Work {
       sum += lane_value(wave_scan((unsigned int)min(own, (unsigned long long)kMostSteps)), 63);
     }
     const unsigned int parts = kTiles ? a.tile_target : a.few_target;
-    unsigned int least = kTiles ? (a.causal ? kLeastTileSteps : kLeastSourceTileSteps) : kLeastFewSteps;
+    unsigned int least = kTiles ? a.tile_least : kLeastFewSteps;
     if (!kTiles && a.fine != 0)
       least = (unsigned int)min((unsigned long long)least, sum / (kFineSplits * a.requests) + 1);
     if (!large && a.slots != 0) cap = max(least, share_of(sum, a.kv_heads, parts));
@@ -1515,6 +1516,7 @@ unsigned long long compute_units() {
 // is goes by the longest request's rows alone.
 struct Plan {
   bool tiles, fine;
+  unsigned int tile_least;  // steps of a tile's split, at least
   unsigned long long few_target, tile_target;  // workgroups that splits are made for
   unsigned long long groups, slots;            // workgroups, partial slots
   unsigned long long items;                    // of the tiles
@@ -1530,6 +1532,7 @@ Plan plan_of(unsigned long long tokens, unsigned long long requests, unsigned lo
              unsigned long long max_query, bool paged, bool causal = true) {
   Plan p{};
   p.tiles = !paged || max_query * group > kFewRows;
+  p.tile_least = causal ? kLeastTileSteps : kLeastSourceTileSteps;
   // (streaming: as many as run at once; 64 requests of 128 .. 32000 tokens, 8 / 1 heads of 128: 39.8 us,
   // with three quarters of it 41.3, with half more 44.9)
   // (of 64-dim sources four run on a CU: 64 requests of 128 .. 16000 tokens, 32 / 8 heads 113 us with two, 105
@@ -1805,6 +1808,7 @@ long long attend_paged(
   a.few_target = (unsigned int)plan.few_target;
   a.fine = plan.fine ? 1 : 0;
   a.tile_target = (unsigned int)plan.tile_target;
+  a.tile_least = plan.tile_least;
   a.max_query = (unsigned int)max_query;
   a.causal = causal ? 1 : 0;
   a.slots = (unsigned int)plan.slots;
@@ -1897,6 +1901,7 @@ extern "C" long long kvq_splitzip_prompt_attention(
   a.group = (unsigned int)(q_heads / kv_heads);
   a.few_target = (unsigned int)plan.few_target;
   a.tile_target = (unsigned int)plan.tile_target;
+  a.tile_least = plan.tile_least;
   a.max_query = (unsigned int)max_query;
   a.causal = 1;
   a.slots = (unsigned int)plan.slots;
@@ -1965,6 +1970,7 @@ extern "C" long long kvq_splitzip_cross_attention(
   a.few_target = (unsigned int)plan.few_target;
   a.fine = plan.fine ? 1 : 0;
   a.tile_target = (unsigned int)plan.tile_target;
+  a.tile_least = plan.tile_least;
   a.max_query = (unsigned int)max_query;
   a.max_source = (unsigned int)max_source;
   a.kv_rows = (unsigned int)source_rows;
