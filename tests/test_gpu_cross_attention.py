@@ -122,9 +122,12 @@ def test_matches_float64(sz, rows, source, q_heads, kv_heads, dim, block, dtype)
 
 SPLITS = [
     # short splits of few sources, ends in each of them; as many sources as are taken whole, and one less
-    ([1], [769], 2, 2, 64, 16, "bf16"), ([3, 1], [1025, 130], 4, 2, 64, 16, "fp16"), ([5], [2049], 3, 3, 128, 16, "bf16"),
+    ([1], [769], 2, 2, 64, 16, "bf16"), ([3, 1], [1025, 130], 4, 2, 64, 16, "fp16"),
+    ([5], [2049], 3, 3, 128, 16, "bf16"),
     ([2, 1, 0, 4], [513, 9000, 700, 0], 8, 8, 128, 32, "fp16"), ([1], [16385], 4, 1, 64, 64, "bf16"),
-    ([30], [385], 2, 2, 64, 16, "bf16"), ([70, 3], [1100, 2], 2, 1, 128, 16, "fp16"), ([300, 40], [600, 2049], 4, 1, 128, 24, "bf16"),
+    # and of tiles
+    ([30], [513], 2, 2, 64, 16, "bf16"), ([70, 3], [1100, 2], 2, 1, 128, 16, "fp16"),
+    ([300, 40], [600, 2049], 4, 1, 128, 24, "bf16"),
     ([1] * 192, [1025] + [3, 700] * 95 + [1600], 1, 1, 64, 16, "bf16"),
     ([2] * 191, [1025] + [3, 700] * 95, 2, 1, 128, 16, "fp16")]
 

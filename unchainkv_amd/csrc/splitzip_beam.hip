@@ -158,7 +158,8 @@ __device__ __forceinline__ void scan_chunk(const SelectArgs& a, unsigned int row
       typename T::Raw raw[kLoads];
 #pragma unroll
       for (int n = 0; n < kLoads; ++n)
-        raw[n] = *reinterpret_cast<const typename T::Raw*>(src + min(at + n * T::kLoad, a.vocab - T::kLoad) * T::kBytes);
+        raw[n] = *reinterpret_cast<const typename T::Raw*>(
+            src + min(at + n * T::kLoad, a.vocab - T::kLoad) * T::kBytes);
 #pragma unroll
       for (int i = 0; i < kOwn; ++i) {
         const unsigned int from = at + i / T::kLoad * T::kLoad;

@@ -246,7 +246,9 @@ def _raise_last(lib, default: str):
 
 
 def _is_cuda(tensor) -> bool:
-    return getattr(getattr(tensor, "device", None), "type", "") == "cuda"
+    # (a GPU tensor's is_cuda takes a fourth of the time of its device's type)
+    return getattr(tensor, "is_cuda", None) is True or \
+        getattr(getattr(tensor, "device", None), "type", "") == "cuda"
 
 
 def _stream_handle(device, torch) -> int:
@@ -1261,12 +1263,19 @@ def _step_binding():
     return _BINDING
 
 
-def _entry_address(entry) -> int:
-    """A C entry's address, which the ctypes function keeps."""
-    address = getattr(entry, "address", None)
-    if address is None:
-        address = entry.address = ctypes.cast(entry, ctypes.c_void_p).value
-    return address
+_ENTRY_ADDRESSES: dict = {}
+
+
+def _entry_addresses(lib, *names) -> tuple | None:
+    """The addresses of a call's C entries, ``kvq_splitzip_`` + each name; None where the library
+    does not have them."""
+    kept = _ENTRY_ADDRESSES.get(names)
+    if kept is None or kept[0] is not lib:
+        entries = [getattr(lib, f"kvq_splitzip_{name}", None) for name in names]
+        kept = lib, None if None in entries else tuple(
+            ctypes.cast(entry, ctypes.c_void_p).value for entry in entries)
+        _ENTRY_ADDRESSES[names] = kept
+    return kept[1]
 
 
 # element types of the layers and rows that these calls take, as the C entries number them
@@ -1502,13 +1511,13 @@ def rotate_write_kv_paged(q, k, v, kv_layer, slots, positions, rotation, *,
     Returns the rotated queries (tokens, q_heads, head_dim), or ``None`` when the kernel
     declines."""
     lib = _load()
-    rotate = getattr(lib, "kvq_splitzip_rotate_write_kv_paged", None) if lib else None
-    if rotate is None or not _is_cuda(q):
+    entries = _entry_addresses(lib, "rotate_write_kv_paged")
+    if entries is None or not _is_cuda(q):
         return None
     import torch
 
-    got = _call_on(q.device, torch, _step_binding().rotate_write, _entry_address(rotate), q, k, v,
-                   kv_layer, slots, positions, rotation, interleaved, out)
+    got = _call_on(q.device, torch, _step_binding().rotate_write, *entries, q, k, v, kv_layer, slots,
+                   positions, rotation, interleaved, out)
     if type(got) is int:
         _raise_last(lib, "splitzip rotated K/V write failed")
     return got
@@ -1754,14 +1763,13 @@ def cross_attention_paged(q, kv_layer, tables, query_starts, source_tokens, *,
 
     Returns ``out`` (tokens, q_heads, head_dim), or ``None`` when the kernel declines."""
     lib = _load()
-    attend = getattr(lib, "kvq_splitzip_cross_attention_paged", None) if lib else None
-    if attend is None or not _is_cuda(q):
+    entries = _entry_addresses(lib, "cross_attention_paged", "cross_attention_least_workspace_bytes")
+    if entries is None or not _is_cuda(q):
         return None
     import torch
 
-    got = _call_on(q.device, torch, _step_binding().cross_paged, _entry_address(attend),
-                   _entry_address(lib.kvq_splitzip_cross_attention_least_workspace_bytes), q, kv_layer,
-                   tables, query_starts, source_tokens, max_query, scale, out, lse, workspace)
+    got = _call_on(q.device, torch, _step_binding().cross_paged, *entries, q, kv_layer, tables,
+                   query_starts, source_tokens, max_query, scale, out, lse, workspace)
     if type(got) is int:
         _raise_last(lib, "splitzip cross attention failed")
     return got
@@ -1782,15 +1790,13 @@ def cross_attention(q, k, v, query_starts, source_starts, source_tokens, *,
 
     Returns ``out`` (tokens, q_heads, head_dim), or ``None`` when the kernel declines."""
     lib = _load()
-    attend = getattr(lib, "kvq_splitzip_cross_attention", None) if lib else None
-    if attend is None or not _is_cuda(q):
+    entries = _entry_addresses(lib, "cross_attention", "cross_attention_least_workspace_bytes")
+    if entries is None or not _is_cuda(q):
         return None
     import torch
 
-    got = _call_on(q.device, torch, _step_binding().cross_rows, _entry_address(attend),
-                   _entry_address(lib.kvq_splitzip_cross_attention_least_workspace_bytes), q, k, v,
-                   query_starts, source_starts, source_tokens, max_query, max_source, scale, out, lse,
-                   workspace)
+    got = _call_on(q.device, torch, _step_binding().cross_rows, *entries, q, k, v, query_starts,
+                   source_starts, source_tokens, max_query, max_source, scale, out, lse, workspace)
     if type(got) is int:
         _raise_last(lib, "splitzip cross attention failed")
     return got
@@ -1853,8 +1859,8 @@ def beam_select(logits, scores, *, candidates: int | None = None, ended=None,
 
     Returns a ``BeamChoice``, or ``None`` when the kernel declines."""
     lib = _load()
-    select = getattr(lib, "kvq_splitzip_beam_select", None) if lib else None
-    if select is None or not _is_cuda(logits):
+    entries = _entry_addresses(lib, "beam_select", "beam_select_workspace_bytes")
+    if entries is None or not _is_cuda(logits):
         return None
     import torch
 
@@ -1863,8 +1869,7 @@ def beam_select(logits, scores, *, candidates: int | None = None, ended=None,
     candidates, end_token = int(candidates), -1 if end_token is None else int(end_token)
     if not 0 < candidates <= 64 or (ended is not None and end_token < 0):
         return None
-    got = _call_on(logits.device, torch, _step_binding().beam_select, _entry_address(select),
-                   _entry_address(lib.kvq_splitzip_beam_select_workspace_bytes), logits, scores,
+    got = _call_on(logits.device, torch, _step_binding().beam_select, *entries, logits, scores,
                    candidates, ended, max(end_token, 0), *(choice or (None,) * 3), workspace)
     if type(got) is int:
         _raise_last(lib, "splitzip beam selection failed")
@@ -1940,17 +1945,16 @@ def reorder_beams_paged(layers, tables, parents, context_tokens, free_blocks, fr
 
     Returns a ``BeamOrder``, or ``None`` when the kernel declines."""
     lib = _load()
-    reorder = getattr(lib, "kvq_splitzip_reorder_beams_paged", None) if lib else None
-    if reorder is None or not _is_cuda(tables):
+    entries = _entry_addresses(lib, "reorder_beams_paged", "reorder_beams_workspace_bytes")
+    if entries is None or not _is_cuda(tables):
         return None
     import torch
 
     block_tokens = int(block_tokens)
     if block_tokens <= 0:
         return None
-    got = _call_on(tables.device, torch, _step_binding().reorder_beams, _entry_address(reorder),
-                   _entry_address(lib.kvq_splitzip_reorder_beams_workspace_bytes), tuple(layers),
-                   tables, parents, context_tokens, free_blocks, free_start, block_tokens,
+    got = _call_on(tables.device, torch, _step_binding().reorder_beams, *entries, tuple(layers), tables,
+                   parents, context_tokens, free_blocks, free_start, block_tokens,
                    *(order or (None,) * 5), workspace)
     if type(got) is int:
         _raise_last(lib, "splitzip beam reordering failed")
