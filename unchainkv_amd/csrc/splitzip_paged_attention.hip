@@ -390,17 +390,24 @@ struct Work {
   }
 };
 
-// The last token of a request that its first row sees (negative: none), and how many more each row
-// behind it does.
-__device__ __forceinline__ int first_seen(const AttendArgs& a, const Request& q) {
-  return (int)q.ctx - (int)(a.causal ? q.n : 1u);
+// What a kernel's rows see: their own request's context up to themselves, or all tokens of a source. (Kernels of
+// their own: one for both, told by an argument, took 18 registers more for streamed rows of 64 dims; 3 chunks beside
+// 29 single tokens 293 us and now 288, 4 prompts over 4386 .. 14280 tokens of sources 471 and 463, 16 requests of
+// up to 6 rows 34.4 and 33.9.)
+enum Sight { kOwnContext, kWholeSource };
+
+// The last token of a request that its first row sees (negative: none).
+template <Sight kSight>
+__device__ __forceinline__ int first_seen(const Request& q) {
+  return (int)q.ctx - (int)(kSight == kOwnContext ? q.n : 1u);
 }
 
 // The first row of K and V of a request of packed rows.
-template <bool kPaged>
+template <bool kPaged, Sight kSight>
 __device__ __forceinline__ unsigned int kv_start(const AttendArgs& a, const Request& q) {
   if constexpr (kPaged) return 0;
-  return a.sources == nullptr ? q.start : q.ctx == 0 ? 0u : (unsigned int)a.sources[q.r];
+  if constexpr (kSight == kOwnContext) return q.start;
+  return q.ctx == 0 ? 0u : (unsigned int)a.sources[q.r];
 }
 
 // Row of K and V that token t of a request has: its place in the layer through the block table
@@ -569,7 +576,7 @@ __device__ __forceinline__ void clear_jobs(const AttendArgs& a, unsigned int slo
 // one read spread over the banks: K's piece c of row t at c ^ (t % 16), read 16 bytes a lane by 32
 // rows; V's 64-byte quarters q at q ^ (t % 4), read transposed 8 bytes a lane, 4 tokens by 32 dims
 // per half wave.
-template <typename E, int D, bool kPaged, bool kRuns>
+template <typename E, int D, bool kPaged, bool kRuns, Sight kSight>
 __device__ __forceinline__ void tile_path(const AttendArgs& a, const Request& request,
                                           unsigned int order, unsigned int split, unsigned int most,
                                           unsigned int split_tokens, bool whole, unsigned int slot,
@@ -589,9 +596,10 @@ __device__ __forceinline__ void tile_path(const AttendArgs& a, const Request& re
   const unsigned int tile = tiles_of<kTileRows>(a, request.n) - 1 - order;
   const unsigned int rows = request.n * a.group;
   const unsigned int m0 = tile * kTileRows;
+  constexpr unsigned int kMore = kSight == kOwnContext ? 1 : 0;  // tokens that each row sees beside the one before it
   // last visible token of a row (negative: none)
-  const int shift = first_seen(a, request);
-  const int last_of_tile = shift + (int)(a.causal * ((min(rows, m0 + kTileRows) - 1) / a.group));
+  const int shift = first_seen<kSight>(request);
+  const int last_of_tile = shift + (int)(kMore * ((min(rows, m0 + kTileRows) - 1) / a.group));
   const unsigned int seen = last_of_tile < 0 ? 0u : (unsigned int)last_of_tile + 1;
   const unsigned int splits = most == 1 ? 1u : max(1u, steps_of(seen, split_tokens));  // of this tile
   if (most > 1)
@@ -606,10 +614,10 @@ __device__ __forceinline__ void tile_path(const AttendArgs& a, const Request& re
   const bool valid = m < rows;
   const unsigned int token = valid ? m / a.group : 0u;
   const unsigned int q_head = head * a.group + (valid ? m - token * a.group : 0u);
-  const int limit = valid ? shift + (int)(a.causal * token) : -1;
+  const int limit = valid ? shift + (int)(kMore * token) : -1;
   // the last visible token of the wave's first row
-  const int first_limit = shift + (int)(a.causal * (mw / a.group));
-  const unsigned int source = kv_start<kPaged>(a, request);
+  const int first_limit = shift + (int)(kMore * (mw / a.group));
+  const unsigned int source = kv_start<kPaged, kSight>(a, request);
 
   const int* table = kPaged ? a.tables + request.r * a.table_stride : nullptr;
   const unsigned char* kb = a.k + head * a.k_head;
@@ -1002,7 +1010,7 @@ __device__ __forceinline__ void tile_path(const AttendArgs& a, const Request& re
     const unsigned int at = uniform((unsigned int)__ffs((int)redo) - 1);
     redo &= redo - 1;
     const unsigned int row_m = mw + at, tok = row_m / a.group, qh = head * a.group + row_m % a.group;
-    const unsigned int own = (unsigned int)max(shift + (int)(a.causal * tok) + 1, 0);  // tokens it sees
+    const unsigned int own = (unsigned int)max(shift + (int)(kMore * tok) + 1, 0);  // tokens it sees
     float rm, rl, acc[D / 64];
     slow_row<E, D, kPaged>(a, table, source,
                            a.q + (unsigned long long)(request.start + tok) * a.q_row +
@@ -1031,11 +1039,11 @@ __device__ __forceinline__ void tile_path(const AttendArgs& a, const Request& re
 // no load takes apart 16 rows: 32 requests of 8192 tokens 200 -> 196.6 us, 16 of 1024 19.2 -> 17.6, 64
 // single tokens of 500 .. 16000 and four times 8 354 -> 332. (64 dims: lane l has token l % 16, 16
 // bytes at 16 (l / 16) of every 64, each counting.)
-// Of 64-dim sources (kSource: every row sees all tokens) a load takes eight whole rows: lane l has piece 4 (l
+// Of 64-dim sources (kWholeSource) a load takes eight whole rows: lane l has piece 4 (l
 // % 2) + l / 16 of token 16 u + 4 (l % 16 / 4) + 2 s + l / 2 % 2 for load (u, s); its product with the pieces
 // 0 .. 3 of Q counts in even rows of the result and that with 4 .. 7 in odd ones: 32 requests of 5 rows, 1500
 // tokens, 20 heads 55.5 -> 53.9 us, 64 of one row, 100 .. 16000 tokens, 32 / 8 heads 118 -> 113.
-template <typename E, int D, int kN, int kRows, bool kPaged, bool kSource>
+template <typename E, int D, int kN, int kRows, bool kPaged, Sight kSight>
 __device__ __forceinline__ void few_path(const AttendArgs& a, const Request& request, unsigned int split,
                                          unsigned int splits, unsigned int split_tokens, bool whole,
                                          unsigned int slot, unsigned int head, unsigned char* __restrict__ s0,
@@ -1047,21 +1055,22 @@ __device__ __forceinline__ void few_path(const AttendArgs& a, const Request& req
   constexpr int kStageBytes = kFewStep * kRowBytes;
   constexpr int kSlabs = D / 32, kDimTiles = D / 16;
   constexpr unsigned int kRound = kN * kFewStep;
-  constexpr bool kWhole = D == 128, kHalves = D == 64 && kSource;  // rows of K are loaded whole
+  constexpr bool kWhole = D == 128, kHalves = D == 64 && kSight == kWholeSource;  // rows of K are loaded whole
   static_assert(kStageBytes >= kFewRows * D * 4, "a wave's sums fit its stage");
 
   const unsigned int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
   const unsigned int col = lane % 16, grp = lane / 16;
+  constexpr unsigned int kMore = kSight == kOwnContext ? 1 : 0;  // tokens that each row sees beside the one before it
   store_job(a, slot, head,
-            Job{request.start, 0, first_seen(a, request),
+            Job{request.start, 0, first_seen<kSight>(request),
                 (unsigned short)(request.n * a.group),
                 (unsigned short)(split == 0 && splits > 1 && whole ? splits : 0u)});
   slot = slot * a.kv_heads + head;
   const unsigned int rows = request.n * a.group;
   const unsigned int t_begin = split * split_tokens;
   const unsigned int t_end = splits == 1 ? request.ctx : min(request.ctx, t_begin + split_tokens);
-  const int shift = first_seen(a, request);
-  const unsigned int source = kv_start<kPaged>(a, request);
+  const int shift = first_seen<kSight>(request);
+  const unsigned int source = kv_start<kPaged, kSight>(a, request);
 
   const int* table = kPaged ? a.tables + request.r * a.table_stride : nullptr;
   const unsigned char* kb = a.k + head * a.k_head;
@@ -1071,7 +1080,7 @@ __device__ __forceinline__ void few_path(const AttendArgs& a, const Request& req
   const bool valid = col < rows;
   const unsigned int token = valid ? col / a.group : 0u;
   const unsigned int q_head = head * a.group + (valid ? col - token * a.group : 0u);
-  const int limit = valid ? shift + (int)(a.causal * token) : -1;
+  const int limit = valid ? shift + (int)(kMore * token) : -1;
   x8 q[kSlabs];
   const unsigned char* q_row = a.q + (unsigned long long)(request.start + token) * a.q_row +
                                (unsigned long long)q_head * a.q_head;
@@ -1186,7 +1195,7 @@ __device__ __forceinline__ void few_path(const AttendArgs& a, const Request& req
     }
     const x8 w = pack8<E>(e);
     const unsigned char* bv = stage + v_at;
-    if (!kSource && a.causal) {
+    if constexpr (kSight == kOwnContext) {
 #pragma unroll
       for (int d = 0; d < kDimTiles; ++d) {
         const unsigned char* src = bv + 32 * (d ^ v_x);
@@ -1288,7 +1297,7 @@ __device__ __forceinline__ void few_path(const AttendArgs& a, const Request& req
       for (int i = 0; i < kVals; i += 4)
         *reinterpret_cast<f32x4*>(dst + i) = f32x4{acc[i], acc[i + 1], acc[i + 2], acc[i + 3]};
     } else {
-      const bool none = shift + (int)(a.causal * tok) < 0 && !bad;
+      const bool none = shift + (int)(kMore * tok) < 0 && !bad;
       const float inv = none ? 0.f : 1.f / l;
       uint32_t* dst = reinterpret_cast<uint32_t*>(a.out + out_row * kRowBytes + 2 * d0);
 #pragma unroll
@@ -1302,7 +1311,7 @@ __device__ __forceinline__ void few_path(const AttendArgs& a, const Request& req
   for (unsigned int i = 0; i < kWave / kShare; ++i) {
     if (((flags >> (kShare * i)) & 1) == 0) continue;
     const unsigned int mm = kWave / kShare * wave + i, t = mm / a.group, h = head * a.group + mm % a.group;
-    const unsigned int seen = (unsigned int)max(shift + (int)(a.causal * t) + 1, 0);
+    const unsigned int seen = (unsigned int)max(shift + (int)(kMore * t) + 1, 0);
     float rm, rl, ra[D / 64];
     slow_row<E, D, kPaged>(a, table, source,
                          a.q + (unsigned long long)(request.start + t) * a.q_row +
@@ -1318,7 +1327,7 @@ __device__ __forceinline__ void few_path(const AttendArgs& a, const Request& req
 
 // (a variable for each buffer: the compiler orders a read of one behind the loads into it, and not
 // behind those into the others)
-template <typename E, int D, bool kPaged, bool kRuns>
+template <typename E, int D, bool kPaged, bool kRuns, Sight kSight>
 __global__ __launch_bounds__(kWave * tile_waves(D), D == 128 ? 2 : 3) void attention_tiles(AttendArgs a) {
   constexpr int kN = tile_waves(D), kRows = tile_rows(D);
   constexpr int kBuffer = 2 * kTileTokens * 2 * D;
@@ -1345,15 +1354,14 @@ __global__ __launch_bounds__(kWave * tile_waves(D), D == 128 ? 2 : 3) void atten
   if constexpr (kPaged) {
     if (work.few(request.n)) {
       if (!has_slot) slot = kNoSlot;
-      few_path<E, D, kN, kRows, kPaged, false>(a, request, split, most, split_tokens, whole, slot, head, s0, s1, s2);
+      few_path<E, D, kN, kRows, kPaged, kSight>(a, request, split, most, split_tokens, whole, slot, head, s0, s1, s2);
       return;
     }
   }
-  tile_path<E, D, kPaged, kRuns>(a, request, order, split, most, split_tokens, whole, slot, head, s0, s1,
-                                   s2);
+  tile_path<E, D, kPaged, kRuns, kSight>(a, request, order, split, most, split_tokens, whole, slot, head, s0, s1, s2);
 }
 
-template <typename E, int D, bool kPaged, bool kSource>
+template <typename E, int D, bool kPaged, Sight kSight>
 __global__ __launch_bounds__(kWave * kWaves, 2) void attention_few(AttendArgs a) {
   constexpr int kBuffer = kWaves * kFewStep * 2 * D;
   __shared__ __align__(1024) unsigned char s0[kBuffer];
@@ -1369,8 +1377,8 @@ __global__ __launch_bounds__(kWave * kWaves, 2) void attention_few(AttendArgs a)
     return;
   }
   const unsigned int splits = work.splits(request);
-  few_path<E, D, kWaves, kFewRows, kPaged, kSource>(a, request, split, splits, work.split_tokens(request, splits), true,
-                                   slot, head, s0, s1, s2);
+  few_path<E, D, kWaves, kFewRows, kPaged, kSight>(a, request, split, splits, work.split_tokens(request, splits),
+                                                   true, slot, head, s0, s1, s2);
 }
 
 // ---------------------------------------------------------------------------
@@ -1621,31 +1629,25 @@ hipError_t launch_merge(const AttendArgs& a, hipStream_t stream) {
   return hipGetLastError();
 }
 
-template <typename E, int D, bool kPaged>
+template <typename E, int D, bool kPaged, Sight kSight>
 long long launch(const AttendArgs& a, const Plan& p, hipStream_t stream) {
   const dim3 grid((unsigned int)p.groups);
   hipError_t st = hipSuccess;
   if (p.tiles) {
     const dim3 threads(kWave * tile_waves(D));
     if constexpr (!kPaged)
-      hipLaunchKernelGGL((attention_tiles<E, D, false, true>), grid, threads, 0, stream, a);
+      hipLaunchKernelGGL((attention_tiles<E, D, false, true, kSight>), grid, threads, 0, stream, a);
     else if (a.block_tokens % 8 == 0)
-      hipLaunchKernelGGL((attention_tiles<E, D, true, true>), grid, threads, 0, stream, a);
+      hipLaunchKernelGGL((attention_tiles<E, D, true, true, kSight>), grid, threads, 0, stream, a);
     else
-      hipLaunchKernelGGL((attention_tiles<E, D, true, false>), grid, threads, 0, stream, a);
+      hipLaunchKernelGGL((attention_tiles<E, D, true, false, kSight>), grid, threads, 0, stream, a);
     st = hipGetLastError();
     if (st != hipSuccess) return fail("attention_tiles", st);
     st = launch_merge<E, D, true>(a, stream);
   } else {
-    const dim3 threads(kWave * kWaves);
-    if constexpr (kPaged) {
-      if (a.causal)
-        hipLaunchKernelGGL((attention_few<E, D, true, false>), grid, threads, 0, stream, a);
-      else
-        hipLaunchKernelGGL((attention_few<E, D, true, true>), grid, threads, 0, stream, a);
-    } else {
-      hipLaunchKernelGGL((attention_few<E, D, false, true>), grid, threads, 0, stream, a);
-    }
+    // (prompts always go to attention_tiles)
+    if constexpr (kPaged || kSight == kWholeSource)
+      hipLaunchKernelGGL((attention_few<E, D, kPaged, kSight>), grid, dim3(kWave * kWaves), 0, stream, a);
     st = hipGetLastError();
     if (st != hipSuccess) return fail("attention_few", st);
     st = launch_merge<E, D, false>(a, stream);
@@ -1654,12 +1656,20 @@ long long launch(const AttendArgs& a, const Plan& p, hipStream_t stream) {
   return (long long)((unsigned long long)a.tokens * a.q_heads * D * 2);
 }
 
-template <bool kPaged>
+template <bool kPaged, Sight kSight>
 long long launch_typed(const AttendArgs& a, const Plan& p, unsigned long long head_dim,
                        unsigned long long dtype, hipStream_t stream) {
   if (head_dim == 128)
-    return dtype ? launch<_Float16, 128, kPaged>(a, p, stream) : launch<__bf16, 128, kPaged>(a, p, stream);
-  return dtype ? launch<_Float16, 64, kPaged>(a, p, stream) : launch<__bf16, 64, kPaged>(a, p, stream);
+    return dtype ? launch<_Float16, 128, kPaged, kSight>(a, p, stream)
+                 : launch<__bf16, 128, kPaged, kSight>(a, p, stream);
+  return dtype ? launch<_Float16, 64, kPaged, kSight>(a, p, stream)
+               : launch<__bf16, 64, kPaged, kSight>(a, p, stream);
+}
+template <bool kPaged>
+long long launch_typed(const AttendArgs& a, const Plan& p, unsigned long long head_dim,
+                       unsigned long long dtype, hipStream_t stream) {
+  return a.causal ? launch_typed<kPaged, kOwnContext>(a, p, head_dim, dtype, stream)
+                  : launch_typed<kPaged, kWholeSource>(a, p, head_dim, dtype, stream);
 }
 
 constexpr unsigned long long kMostRows = 0x7FFFFFFFull;
