@@ -1784,10 +1784,10 @@ def cross_attention(q, k, v, query_starts, source_starts, source_tokens, *,
     """``cross_attention_paged`` over sources that are rows of ``k`` and ``v`` (rows, kv_heads,
     head_dim): request r's is the ``source_tokens[r]`` rows from ``source_starts[r]`` on (packed one
     behind the other, padded to one length, or shared between requests; int32, on the device).
-    ``max_source`` bounds a source's tokens (default: all rows of k): a smaller bound, up to 1024,
-    spares a call of few rows the joining of splits (up to 512 where requests * kv_heads is 32 or
-    less). Requests whose source is longer stay as they
-    are, like those with more than ``max_query`` rows; a source that is not inside k makes its
+    ``max_source`` bounds a source's tokens (default: all rows of k): a smaller bound spares a call of few
+    rows the joining of splits, on a GPU of 256 CUs up to 1024 tokens; up to 512 (64-dim heads: 768) where
+    requests * kv_heads is an eighth of the CUs, 32, or less, and up to 2048 from three quarters of them, 192,
+    on. Requests whose source is longer stay as they are, like those with more than ``max_query`` rows; a source that is not inside k makes its
     request's rows NaN. Rows and heads of k and v may be strided by multiples of 16 bytes. The
     workspace is that of ``cross_attention_workspace_bytes``. Softmax weights are rounded to the type
     unless ``max_query`` keeps all requests to 16 rows for each KV head.
