@@ -4,7 +4,7 @@
 // Select. Beam b offers token t at x[b][t] - m - log sum_t exp(x[b][t] - m) + score[b], m = max_t x[b][t]; of all
 // beams and tokens the best n are given, equal ones by their places.
 //   * beam_scan reads every logit once, a wave 4 KB of a row at a time, and keeps the maximum of each 256 of them
-//     and, of each wave's share, (m, sum exp(x - m)): one pass, sums in f32 of at most 64 terms a lane. Bound by
+//     and, of each wave's share, (m, sum exp(x - m)): one pass, sums in f32 of at most 32 terms a lane. Bound by
 //     HBM: 64 requests of 8 beams (one of them finished), 131072 logits in bf16, 117 MB: 22.9 us, 5.1 TB/s (a
 //     large copy: 5.1). A lane takes 64 bytes that follow each other: with 16 a lane, interleaved, a maximum of
 //     256 took five exchanges for each 8 logits and the call 28.5 us.
@@ -65,7 +65,7 @@ struct SelectArgs {
   long long* out_tokens;
   unsigned long long request_stride, beam_stride;
   unsigned int requests, beams, vocab, candidates, end_token;
-  unsigned int segments, chunks, rounds;  // of a row; rounds of a chunk
+  unsigned int segments, chunks;  // of a row
   unsigned int parts;         // waves that search a beam
   unsigned int group, items;  // segments of an item, items of a row
 };
@@ -131,73 +131,66 @@ __device__ __forceinline__ float wave_max(float v) {
   return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
 }
 
-// A row's chunk by a wave: `rounds` times 64 lanes' 64 bytes; a lane's logits follow each other, so that a
-// segment's maximum takes three or four exchanges between lanes for 32 or 16 logits of each. maxima, sums: the row's.
+// A row's chunk by a wave: 64 lanes' 64 bytes; a lane's logits follow each other, so that a segment's maximum
+// takes three or four exchanges between lanes for 32 or 16 logits of each. maxima, sums: the row's.
 template <typename T>
 __device__ __forceinline__ void scan_chunk(const SelectArgs& a, unsigned int row, unsigned int chunk, float* maxima,
                                            float2* sums) {
   constexpr int kOwn = kLaneLogits<T>, kLoads = kOwn / T::kLoad, kLanes = kSegment / kOwn;
   const unsigned int lane = __lane_id();
   const unsigned char* src = row_of<T>(a, row);
-  float top = kLowest, sum = 0.f;
-  const unsigned int first = chunk * a.rounds * (kWave * kOwn);
-  const unsigned int last = min(a.vocab, first + a.rounds * (kWave * kOwn));
-  for (unsigned int base = first; base < last; base += kWave * kOwn) {
-    const unsigned int at = base + lane * kOwn;
-    float x[kOwn];
-    if (base + kWave * kOwn <= a.vocab) {
-      typename T::Raw raw[kLoads];
+  const unsigned int base = chunk * (kWave * kOwn);
+  const unsigned int at = base + lane * kOwn;
+  float x[kOwn];
+  if (base + kWave * kOwn <= a.vocab) {
+    typename T::Raw raw[kLoads];
 #pragma unroll
-      for (int n = 0; n < kLoads; ++n)
-        raw[n] = *reinterpret_cast<const typename T::Raw*>(src + (at + n * T::kLoad) * T::kBytes);
+    for (int n = 0; n < kLoads; ++n)
+      raw[n] = *reinterpret_cast<const typename T::Raw*>(src + (at + n * T::kLoad) * T::kBytes);
 #pragma unroll
-      for (int i = 0; i < kOwn; ++i) x[i] = T::of(raw[i / T::kLoad], i % T::kLoad);
-    } else if (a.vocab >= T::kLoad) {
-      // The row's end: loads that would pass it are of its last logits, of which those count that no load before
-      // has (all go out together; behind a branch for each the call took 1.5 us more).
-      typename T::Raw raw[kLoads];
+    for (int i = 0; i < kOwn; ++i) x[i] = T::of(raw[i / T::kLoad], i % T::kLoad);
+  } else if (a.vocab >= T::kLoad) {
+    // The row's end: loads that would pass it are of its last logits, of which those count that no load before
+    // has (all go out together; behind a branch for each the call took 1.5 us more).
+    typename T::Raw raw[kLoads];
 #pragma unroll
-      for (int n = 0; n < kLoads; ++n)
-        raw[n] = *reinterpret_cast<const typename T::Raw*>(
-            src + min(at + n * T::kLoad, a.vocab - T::kLoad) * T::kBytes);
+    for (int n = 0; n < kLoads; ++n)
+      raw[n] = *reinterpret_cast<const typename T::Raw*>(
+          src + min(at + n * T::kLoad, a.vocab - T::kLoad) * T::kBytes);
 #pragma unroll
-      for (int i = 0; i < kOwn; ++i) {
-        const unsigned int from = at + i / T::kLoad * T::kLoad;
-        x[i] = from + T::kLoad <= a.vocab + i % T::kLoad ? T::of(raw[i / T::kLoad], i % T::kLoad) : -INFINITY;
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < kOwn; ++i) x[i] = at + i < a.vocab ? T::one(src, at + i) : -INFINITY;
+    for (int i = 0; i < kOwn; ++i) {
+      const unsigned int from = at + i / T::kLoad * T::kLoad;
+      x[i] = from + T::kLoad <= a.vocab + i % T::kLoad ? T::of(raw[i / T::kLoad], i % T::kLoad) : -INFINITY;
     }
-    float own = x[0];
+  } else {
 #pragma unroll
-    for (int i = 1; i < kOwn; ++i) own = fmaxf(own, x[i]);
-    const float now = fmaxf(top, own);
-    sum *= __builtin_amdgcn_exp2f((top - now) * kLog2E);
-    top = now;
-    float part = 0.f;
-    if (__all(fabsf(now) < 1e6f)) {
-      // 2^(x log2 e - r) with one rounding, r = now log2 e rounded, and that rounding put right in the sum
-      const float r = now * kLog2E;
-#pragma unroll
-      for (int i = 0; i < kOwn; ++i) part += __builtin_amdgcn_exp2f(fmaf(x[i], kLog2E, -r));
-      part *= __builtin_amdgcn_exp2f(-fmaf(now, kLog2E, -r));
-    } else {
-      // (no logit but -inf, or values whose products with log2 e leave the range or its small steps)
-#pragma unroll
-      for (int i = 0; i < kOwn; ++i) part += __builtin_amdgcn_exp2f((x[i] - now) * kLog2E);
-    }
-    sum += part;
-    // (a NaN, or infinity, which makes the row's sum NaN: every value that is not -inf is then NaN)
-    own = part != part ? INFINITY : own;
-    own = fmaxf(own, shifted<0x111, 0xF>(own));
-    own = fmaxf(own, shifted<0x112, 0xF>(own));
-    own = fmaxf(own, shifted<0x114, 0xF>(own));
-    if constexpr (kLanes == 16) own = fmaxf(own, shifted<0x118, 0xF>(own));
-    const unsigned int segment = at / kSegment;
-    if (lane % kLanes == kLanes - 1 && segment < a.segments)
-      maxima[segment] = own;
+    for (int i = 0; i < kOwn; ++i) x[i] = at + i < a.vocab ? T::one(src, at + i) : -INFINITY;
   }
+  float own = x[0];
+#pragma unroll
+  for (int i = 1; i < kOwn; ++i) own = fmaxf(own, x[i]);
+  const float top = fmaxf(own, kLowest);
+  float sum = 0.f;
+  if (__all(fabsf(top) < 1e6f)) {
+    // 2^(x log2 e - r) with one rounding, r = top log2 e rounded, and that rounding put right in the sum
+    const float r = top * kLog2E;
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i) sum += __builtin_amdgcn_exp2f(fmaf(x[i], kLog2E, -r));
+    sum *= __builtin_amdgcn_exp2f(-fmaf(top, kLog2E, -r));
+  } else {
+    // (no logit but -inf, or values whose products with log2 e leave the range or its small steps)
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i) sum += __builtin_amdgcn_exp2f((x[i] - top) * kLog2E);
+  }
+  // (a NaN, or infinity, which makes the row's sum NaN: every value that is not -inf is then NaN)
+  own = sum != sum ? INFINITY : own;
+  own = fmaxf(own, shifted<0x111, 0xF>(own));
+  own = fmaxf(own, shifted<0x112, 0xF>(own));
+  own = fmaxf(own, shifted<0x114, 0xF>(own));
+  if constexpr (kLanes == 16) own = fmaxf(own, shifted<0x118, 0xF>(own));
+  const unsigned int segment = at / kSegment;
+  if (lane % kLanes == kLanes - 1 && segment < a.segments)
+    maxima[segment] = own;
   const float big = wave_max(top);
   sum *= __builtin_amdgcn_exp2f((top - big) * kLog2E);
 #pragma unroll
@@ -776,14 +769,12 @@ using namespace unchainkv;
 
 namespace {
 
-// Chunks of a row, a wave's each, of one round or, in calls that fill the chip many times over, two (64
-// requests of 8 beams, 131072 logits in bf16: 23.0 us with two, 24.6 with one, 25.8 with four). A row of more
-// segments than a wave's lanes hold is searched by several, as far as there are waves.
-void shape(unsigned long long rows, unsigned long long dtype, SelectArgs& a) {
-  const unsigned int round = kWave * kLaneBytes / (dtype == 2 ? 4 : 2);
-  const unsigned int all = (a.vocab + round - 1) / round;
-  a.rounds = rows * all >= 16384 ? 2 : 1;
-  a.chunks = (all + a.rounds - 1) / a.rounds;
+// Chunks of a row, a wave's each: 4 KB. (Twice that for a wave: 64 requests of 8 beams, 131072 logits in bf16 37.8 us
+// and 36.5, 256 of 4 beams, 50257 logits in fp16 44.1 and 32.7, 1024 of 8, 2500 in bf16 48.3 and 44.2; 2000 of 8, 5000
+// 96.7 and 98.3.) A row of more segments than a wave's lanes hold is searched by several, as far as there are waves.
+void shape(unsigned long long dtype, SelectArgs& a) {
+  const unsigned int chunk = kWave * kLaneBytes / (dtype == 2 ? 4 : 2);
+  a.chunks = (a.vocab + chunk - 1) / chunk;
   a.segments = (a.vocab + kSegment - 1) / kSegment;
   a.parts = 1;
   while (2 * a.parts * a.beams <= kPickThreads / kWave && a.segments > kMostItems * kWave * a.parts) a.parts *= 2;
@@ -799,7 +790,7 @@ bool select_ok(unsigned long long requests, unsigned long long beams, unsigned l
          requests <= 1u << 20;
 }
 
-// Every row's maxima, then sums of as many chunks as it can have (f32, one round each): more for more rows or
+// Every row's maxima, then sums of as many chunks as it can have (those of f32): more for more rows or
 // tokens, whatever their type.
 unsigned long long maxima_bytes(unsigned long long rows, unsigned long long vocab) {
   return (4 * rows * ((vocab + kSegment - 1) / kSegment) + 15) / 16 * 16;
@@ -809,7 +800,7 @@ unsigned long long select_bytes(unsigned long long rows, unsigned long long voca
   return maxima_bytes(rows, vocab) + sizeof(float2) * rows * ((vocab + kLeast - 1) / kLeast);
 }
 
-bool is_whole(const SelectArgs& a) { return a.rounds == 1 && a.beams * a.chunks <= kWholeChunks; }
+bool is_whole(const SelectArgs& a) { return a.beams * a.chunks <= kWholeChunks; }
 
 // As few registers as hold a row's items.
 template <typename T>
@@ -878,7 +869,7 @@ extern "C" long long kvq_splitzip_beam_select(
   SelectArgs a{};
   a.vocab = (unsigned int)vocab;
   a.beams = (unsigned int)beams;
-  shape(rows, dtype, a);
+  shape(dtype, a);
   a.logits = reinterpret_cast<const unsigned char*>(logits_ptr);
   a.scores = reinterpret_cast<const float*>(scores_ptr);
   a.ended = reinterpret_cast<const unsigned char*>(ended_ptr);
