@@ -1854,7 +1854,9 @@ def beam_select(logits, scores, *, candidates: int | None = None, ended=None,
     allowed), whatever else the row holds. A beam whose ``ended`` (requests, beams; bool) is true goes on with
     ``end_token`` alone, at its own score. Where too little else is offered, candidates of -inf follow.
     A NaN or +inf logit makes all that its beam offers NaN, which comes first. Values are formed
-    and compared in 64 bits, with sums of 32-bit exponentials, and scores rounded once.
+    and compared in 64 bits from 32-bit sums of a row's exponentials, and scores rounded once: one beam's
+    tokens come in their exact order, two beams' wherever they differ by more than the sums' roundings
+    (2e-5 at most).
 
     Everything stays on the device, and a captured call follows it (``choice=`` from
     ``new_beam_choice``, ``workspace=`` of ``beam_select_workspace_bytes``); calls that overlap in
