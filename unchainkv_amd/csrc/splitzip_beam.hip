@@ -5,15 +5,15 @@
 // beams and tokens the best n are given, equal ones by their places.
 //   * beam_scan reads every logit once, a wave 4 KB of a row at a time, and keeps the maximum of each 256 of them
 //     and, of each wave's share, (m, sum exp(x - m)): one pass, sums in f32 of at most 32 terms a lane. Bound by
-//     HBM: 64 requests of 8 beams (one of them finished), 131072 logits in bf16, 117 MB: 22.9 us, 5.1 TB/s (a
+//     HBM: 64 requests of 8 beams (one of them finished), 131072 logits in bf16, 117 MB: 24.0 us, 4.9 TB/s (a
 //     large copy: 5.1). A lane takes 64 bytes that follow each other: with 16 a lane, interleaved, a maximum of
 //     256 took five exchanges for each 8 logits and the call 28.5 us.
 //   * beam_pick, a workgroup for each request, joins the sums in 64 bits and searches. The best n values lie in
 //     the n segments with the largest maxima (equal ones: the first), as each of n segments that come before a
 //     value's own holds one that comes before it. So: a bound that n of some wave's lanes reach; the segments above
 //     it, ranked; the logits of the best n of them, read again, that are no less than the n-th maximum; ranked.
-//     Nothing here grows with the vocabulary but the maxima's loads. Bound by latency: 11.9 us for the call above,
-//     6.6 for one request of 4 beams, 32000 logits (loads 1.5 us, twice; log, bound and lists; 49 us when every
+//     Nothing here grows with the vocabulary but the maxima's loads. Bound by latency: 12.0 us for the call above,
+//     6.8 for one request of 4 beams, 32000 logits (loads 1.5 us, twice; log, bound and lists; 49 us when every
 //     list was formed by taking one maximum after another).
 // Values are formed and compared in 64 bits from a row's sum, whose terms and joins within a wave are in 32: a
 // beam's own offers come in their exact order, and those of two beams wherever they differ by more than the
