@@ -14,9 +14,10 @@
 // largest V value (n * 2^-25 without, which 32768 tokens of weight 2^-26 beside one of 1 lost whole).
 // Over sources streamed rows (attention_few, and short requests beside tiles in a layer) lose none of it: what the
 // rounding leaves has a product of its own, on matrix units that wait for memory. Tiles do lose it: bf16 prompts over
-// sources are off by 0.0021 to 0.0022 of their size, and with weights in f32 by 0.0017, the output's own rounding. The
-// second product takes 636 us there in place of 475 (4 prompts over 4386 .. 14280 tokens), 56 in place of 48 (16
-// packed prompts over up to 1912), as the matrix units are what bounds them, and it has no registers to spare.
+// sources are off by 0.0021 to 0.0024 of their size, and with weights in f32 by 0.0017, the output's own rounding. The
+// second product takes 616 us there in place of 455 (4 prompts over 4386 .. 14280 tokens), 53.8 in place of 46.6 (16
+// packed prompts over up to 1912), 14.7 in place of 13.0 (64 rows over 1500), as tiles have neither matrix units that
+// wait nor registers to spare.
 //
 // The query heads of a group read the same K and V, so a request's rows are (token, head of the
 // group) pairs, row m = token * group + head, and a tile of rows serves them together: a single

@@ -1761,8 +1761,8 @@ def cross_attention_paged(q, kv_layer, tables, query_starts, source_tokens, *,
     ``cross_attention_workspace_bytes``), captured calls, gradients. A request without source
     tokens has rows of zero, their lse -inf. Requests of at most 16 rows for each KV head (rows times
     query heads of the group) are off by their output's rounding alone; for longer ones the softmax weights
-    are rounded to the type too, as in ``chunk_attention_paged`` (in bf16 0.0022 of an output's size in
-    all, where the output's rounding alone makes 0.0017).
+    are rounded to the type too, as in ``chunk_attention_paged`` (in bf16 up to 0.0024 of the outputs'
+    size in all, where the outputs' rounding alone makes 0.0017).
 
     Returns ``out`` (tokens, q_heads, head_dim), or ``None`` when the kernel declines."""
     lib = _load()
