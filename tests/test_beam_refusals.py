@@ -300,3 +300,13 @@ def test_calls_that_do_nothing(entered):
     out = torch.full((3, 4, 64), 7.0, dtype=torch.bfloat16)
     assert sz.cross_attention(rows(4), rows(2), rows(2), i32([0]), none, none, out=out) is out
     assert (out == 7).all() and not entered
+
+
+def test_results_given_in_part_are_declined(entered):
+    """Not left as they were, beside results that nobody gets."""
+    choice, into = sz.new_beam_choice(1, 2, "cpu"), sz.new_beam_order(1, 2, 1, "cpu")
+    for name in choice._fields:
+        assert select(choice=choice._replace(**{name: None})) is None
+    for name in into._fields:
+        assert order(order=into._replace(**{name: None})) is None
+    assert not entered and select(choice=choice) is choice and order(order=into) is into

@@ -300,7 +300,7 @@ PyObject* beam_select(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const at::Device device = logits.device();
   const int64_t requests = logits.size(0), beams = logits.size(1), vocab = logits.size(2);
   const std::array<int64_t, 2> rows = {requests, beams}, picked = {requests, (int64_t)candidates};
-  const bool given = best.defined();
+  const bool given = best.defined() || parents.defined() || tokens.defined();  // (all three, or it is declined)
   if ((vocab != 1 && logits.stride(2) != 1) || !matrix_ok(scores, rows, device, at::kFloat) ||
       (ended.defined() && (!matrix_ok(ended, rows, device, at::kBool) || end_token >= (u64)vocab)) ||
       tracked({&logits, &scores, &best}) ||
@@ -365,7 +365,7 @@ PyObject* reorder_beams(PyObject*, PyObject* const* args, Py_ssize_t n) {
     blocks = (u64)layer.size(1);
     row_bytes = 2 * (u64)(layer.size(3) * layer.size(4));
   }
-  const bool given = order[0].defined();
+  const bool given = std::any_of(order.begin(), order.end(), [](const at::Tensor& t) { return t.defined(); });
   const at::TensorOptions ints = at::TensorOptions().dtype(at::kInt).device(device);
   if (!given) {
     order[0] = at::empty({rows, width}, ints);
