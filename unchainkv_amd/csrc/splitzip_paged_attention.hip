@@ -35,8 +35,9 @@
 //     softmax for each product (VALU active 0.74 of the cycles, matrix units 0.44).
 // Over sources the same two: a request's rows, the beams of one token among them, read its source once. 32
 // requests of 5 rows, 1500 tokens, 20 heads of 64 in fp16: 53 us for 247 MB; 4 of 659 .. 862 rows over 4386 ..
-// 14280 tokens, 32 / 8 heads of 128: 462 us, 1.01 PFLOP/s, by card up to 5 % more (384 tiles of 69 to 224 steps on 256 CUs:
-// the longest CU has 259 steps of 227 on average; cut finer, the partials cost more than the balance gives).
+// 14280 tokens, 32 / 8 heads of 128: 455 to 462 us, 1.01 to 1.03 PFLOP/s, on other cards up to 5 % more (384 tiles of
+// 69 to 224 steps on 256 CUs: the longest CU has 259 steps of 227 on average; cut finer, the partials cost more than
+// the balance gives).
 // Both give S^T = K Q^T, so that a row's scores lie in one lane (and its partners 32 or 16 lanes
 // away): the maximum and the sum need one or two lane swaps a step, rescaling is a lane's own
 // product, and the weights are the second product's operand O^T = V^T P^T as they are, with V's
